@@ -300,6 +300,66 @@ int mv_deform_conv_3d(const void *input, const void *offset, const void *weight,
 int mv_deform_conv_2d(const void *input, const void *offset, const void *weight, const void *bias,
                       void *output, const mv_dcn2d_shape *shape, int dtype, int order, void *stream);
 
+/* ---- region decoders ----------------------------------------------------------------------------
+ * What a head does with its regions after pooling; no counterparts in the reference.  Rows are dense unless strides are
+ * given; elements at the alignment of their type suffice.  Types: MV_F32, MV_F16, MV_BF16.
+ *
+ * Cross attention: queries [batch, queries, heads, dim] over keys and values [batch, keys, key_heads, dim] of another
+ * length (heads a multiple of key_heads: consecutive heads share a key head; dim 1..128), with strides in elements for
+ * batch, row and head; elements of a row are neighbours.
+ *   o_i = sum_j p_ij v_j,  p_ij = softmax over the keys that count of scale q_i . k_j
+ * Key j of sample b counts when j < key_lengths[b] (int32, NULL: all; values beyond the keys mean all, below 0 none) and
+ * key_mask[b * mask_stride + j] != 0 (bytes, NULL: all).  What the other keys and values hold is of no effect, not even
+ * NaN.  A query without any key gets zeros, and gives none a gradient.
+ * output [batch, queries, heads, dim] and the gradients are dense; lse [batch, heads, queries] float32 (NULL: not wanted by
+ * the forward pass) holds log2 of the sum of 2^(log2(e) scale q.k), -inf where no key counts.  The backward pass WRITES its
+ * gradients; it wants the workspace, the forward pass splits long rows of keys only if it gets its own. */
+typedef struct {
+  int batch, queries, keys, heads, key_heads, dim;
+  int64_t q_strides[3], k_strides[3], v_strides[3]; /* batch, row, head */
+  int64_t mask_stride;
+} mv_attention_shape;
+size_t mv_cross_attention_forward_workspace_bytes(const mv_attention_shape *shape, int dtype);
+size_t mv_cross_attention_backward_workspace_bytes(const mv_attention_shape *shape, int dtype);
+int mv_cross_attention_forward(const void *query, const void *key, const void *value, const void *key_mask,
+                               const void *key_lengths, void *output, void *lse, const mv_attention_shape *shape,
+                               float scale, int dtype, void *workspace, size_t workspace_bytes, void *stream);
+int mv_cross_attention_backward(const void *query, const void *key, const void *value, const void *key_mask,
+                                const void *key_lengths, const void *output, const void *lse, const void *grad_output,
+                                void *grad_query, void *grad_key, void *grad_value, const mv_attention_shape *shape,
+                                float scale, int dtype, void *workspace, size_t workspace_bytes, void *stream);
+
+/* RMS norm with the residual's addition: h = x + residual, rounded to `dtype` (residual NULL: h = x),
+ * y = h / sqrt(mean(h^2) + eps) * weight, over rows of `columns`.  weight: `weight_dtype`, `dtype` or MV_F32.
+ * sum [rows, columns] receives h (NULL exactly when residual is NULL).
+ * ..._quantized: y in 8 bits (e4m3) instead, as mv_quantize_blocks gives them.
+ * ..._backward: h (x or the sum), grad_y and grad_sum (NULL: none) give grad_x (the residual's gradient is the same) and
+ * grad_weight (of weight_dtype), both written; sums over rows are formed in a fixed order. */
+int mv_add_rms_norm(const void *x, const void *residual, const void *weight, void *y, void *sum, int64_t rows, int columns,
+                    float eps, int dtype, int weight_dtype, void *stream);
+int mv_add_rms_norm_quantized(const void *x, const void *residual, const void *weight, void *q, void *scales, void *sum,
+                              int64_t rows, int columns, float eps, int dtype, int weight_dtype, void *stream);
+size_t mv_add_rms_norm_backward_workspace_bytes(int64_t rows, int columns);
+int mv_add_rms_norm_backward(const void *h, const void *weight, const void *grad_y, const void *grad_sum, void *grad_x,
+                             void *grad_weight, int64_t rows, int columns, float eps, int dtype, int weight_dtype,
+                             void *workspace, size_t workspace_bytes, void *stream);
+
+/* Values in 8 bits with a scale for each block of block_rows (1: activations, 128: weights) x 128 columns:
+ * scale = max(max|x| / 448, 2^-126), q = e4m3(x * (1 / scale)).  q [rows, columns rounded up to 128] (zeros beyond the
+ * columns), scales float32 [ceil(rows / block_rows), ceil(columns / 128)].  A block that holds a NaN or an infinity
+ * has it for a scale, and with it stands for NaN throughout. */
+int mv_quantize_blocks(const void *x, void *q, void *scales, int64_t rows, int columns, int block_rows, int dtype, void *stream);
+
+/* y [rows, outputs] = (q * q_scales) (weight * weight_scales)^T + bias, `dtype` MV_F16 or MV_BF16 (of y and bias; bias may be
+ * NULL): q [rows, inputs] with scales [rows, inputs / 128], weight [outputs, inputs] with scales [ceil(outputs / 128),
+ * inputs / 128], dense, 16-byte aligned; inputs a multiple of 128.  Products of a block are summed by the matrix cores (which
+ * keep about 16 bits below the largest term), blocks in float32.  A workspace smaller than the query's value costs
+ * speed only. */
+size_t mv_block_linear_workspace_bytes(int64_t rows, int inputs, int outputs);
+int mv_block_linear(const void *q, const void *q_scales, const void *weight, const void *weight_scales, const void *bias,
+                    void *y, int64_t rows, int inputs, int outputs, int dtype, void *workspace, size_t workspace_bytes,
+                    void *stream);
+
 /* ---- small host arrays --------------------------------------------------------------------------
  * Copies `bytes` (whole 4-byte words, at most MV_UPLOAD_MAX_BYTES) from host to device memory as
  * kernel arguments: asynchronous on the stream, `host` may be reused as soon as the call returns.

@@ -15,6 +15,7 @@ MV_I32 = 4   # int32 label maps: the displacement warp and the affine engines at
 DTYPES = {torch.float32: MV_F32, torch.float16: MV_F16, torch.bfloat16: MV_BF16,
           torch.float64: MV_F64}
 
+_i64 = ctypes.c_int64
 _i, _f, _p, _sz = ctypes.c_int, ctypes.c_float, ctypes.c_void_p, ctypes.c_size_t
 
 
@@ -33,6 +34,13 @@ class Dcn2dShape(ctypes.Structure):
         "stride_h", "stride_w", "pad_h", "pad_w", "dil_h", "dil_w", "groups", "deformable_groups")]
 
 
+class AttentionShape(ctypes.Structure):
+    """Mirror of ``mv_attention_shape``."""
+    _fields_ = [(n, _i) for n in ("batch", "queries", "keys", "heads", "key_heads", "dim")] + [
+        (n, _i64 * 3) for n in ("q_strides", "k_strides", "v_strides")] + [("mask_stride", _i64)]
+
+
+_ATTENTION_P = ctypes.POINTER(AttentionShape)
 _SHAPE_P = ctypes.POINTER(DcnShape)
 _SHAPE2_P = ctypes.POINTER(Dcn2dShape)
 
@@ -80,6 +88,17 @@ SIGNATURES = {
     "mv_elastic_warp_3d": (_i, [_p, _p, _p] + [_i] * 9 + [ctypes.c_float, _p]),
     "mv_deform_conv_3d": (_i, [_p] * 6 + [_i, _i, _p]),
     "mv_deform_conv_2d": (_i, [_p] * 6 + [_i, _i, _p]),
+    "mv_cross_attention_forward_workspace_bytes": (_sz, [_ATTENTION_P, _i]),
+    "mv_cross_attention_backward_workspace_bytes": (_sz, [_ATTENTION_P, _i]),
+    "mv_cross_attention_forward": (_i, [_p] * 7 + [_ATTENTION_P, _f, _i, _p, _sz, _p]),
+    "mv_cross_attention_backward": (_i, [_p] * 11 + [_ATTENTION_P, _f, _i, _p, _sz, _p]),
+    "mv_add_rms_norm": (_i, [_p] * 5 + [_i64, _i, _f, _i, _i, _p]),
+    "mv_add_rms_norm_quantized": (_i, [_p] * 6 + [_i64, _i, _f, _i, _i, _p]),
+    "mv_add_rms_norm_backward_workspace_bytes": (_sz, [_i64, _i]),
+    "mv_add_rms_norm_backward": (_i, [_p] * 6 + [_i64, _i, _f, _i, _i, _p, _sz, _p]),
+    "mv_quantize_blocks": (_i, [_p] * 3 + [_i64, _i, _i, _i, _p]),
+    "mv_block_linear_workspace_bytes": (_sz, [_i64, _i, _i]),
+    "mv_block_linear": (_i, [_p] * 6 + [_i64, _i, _i, _i, _p, _sz, _p]),
     "mv_upload": (_i, [_p, _p, _sz, _p]),
 }
 

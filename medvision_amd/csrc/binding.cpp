@@ -501,6 +501,366 @@ std::optional<Tensor> elastic_warp(const Tensor &given, const Tensor &grid, doub
   return sample ? out.squeeze(0) : out;
 }
 
+// ---- region decoders: cross attention, RMS norm with residual, 8-bit products -------------------------------------------
+int float_code(const Tensor &t, const char *what) {
+  const auto type = t.scalar_type();
+  MVB_CHECK(type == at::kFloat || type == at::kHalf || type == at::kBFloat16, what, " takes float32, float16 or bfloat16, got ", dtype_name(t));
+  return dtype_code(t);
+}
+
+int to_int(int64_t n, const char *what) {
+  MVB_CHECK(n <= std::numeric_limits<int>::max(), what, " is too large: ", n);
+  return static_cast<int>(n);
+}
+
+bool wants_gradient(std::initializer_list<Tensor> tensors) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const Tensor &t : tensors)
+    if (t.defined() && t.requires_grad()) return true;
+  return false;
+}
+
+// Gradients that cannot be differentiated again: say so when someone tries
+void differentiable_once(const variable_list &grads, variable_list &out) {
+  bool again = false;
+  for (const Tensor &g : grads) again |= g.defined() && g.requires_grad();
+  if (!at::GradMode::is_enabled() || !again) return;
+  for (Tensor &t : out) {
+    if (!t.defined()) continue;
+    auto once = std::make_shared<torch::autograd::DelayedError>(
+        "trying to differentiate twice a function that was marked with @once_differentiable", 1);
+    t.set_requires_grad(true);
+    t = (*once)(variable_list{t})[0];
+  }
+}
+
+// Neighbouring channels of a head; every other stride is the kernels' to follow
+Tensor rows_of_heads(const Tensor &t) { return t.size(3) <= 1 || t.stride(3) == 1 ? t : t.contiguous(); }
+
+struct AttentionCall {
+  Tensor q, k, v, mask, lengths;
+  mv_attention_shape shape;
+  int code;
+};
+
+AttentionCall attention_call(const Tensor &query, const Tensor &key, const Tensor &value, const Tensor &key_mask, const Tensor &key_lengths) {
+  MVB_CHECK(query.is_cuda(), "cross_attention is not implemented on CPU");
+  MVB_CHECK(query.dim() == 4 && key.dim() == 4 && value.dim() == 4, "query, key and value have to be [batch, length, heads, channels]");
+  AttentionCall c;
+  c.code = float_code(query, "cross_attention");
+  MVB_CHECK(key.scalar_type() == query.scalar_type() && value.scalar_type() == query.scalar_type(), "query, key and value must share one dtype");
+  same_device(query, key, "key");
+  same_device(query, value, "value");
+  same_device(query, key_mask, "key_mask");
+  same_device(query, key_lengths, "key_lengths");
+  MVB_CHECK(key.sizes() == value.sizes(), "key has shape ", shape_text(key.sizes()), ", value ", shape_text(value.sizes()));
+  MVB_CHECK(key.size(0) == query.size(0), "key has a batch of ", key.size(0), ", expected ", query.size(0), " like the query");
+  MVB_CHECK(key.size(3) == query.size(3), "key has heads of ", key.size(3), " channels, expected ", query.size(3), " like the query");
+  MVB_CHECK(key.size(2) > 0 && query.size(2) > 0 && query.size(2) % key.size(2) == 0, query.size(2), " heads cannot share ", key.size(2), " heads of keys");
+  MVB_CHECK(query.size(3) >= 1 && query.size(3) <= 128, "heads of ", query.size(3), " channels: 1 to 128 are possible");
+  mv_attention_shape &s = c.shape;
+  s = {to_int(query.size(0), "the batch"), to_int(query.size(1), "the number of queries"), to_int(key.size(1), "the number of keys"),
+       to_int(query.size(2), "the number of heads"), to_int(key.size(2), "the number of heads"), static_cast<int>(query.size(3)), {}, {}, {}, 0};
+  c.q = rows_of_heads(query), c.k = rows_of_heads(key), c.v = rows_of_heads(value);
+  for (int a = 0; a < 3; ++a) s.q_strides[a] = c.q.stride(a), s.k_strides[a] = c.k.stride(a), s.v_strides[a] = c.v.stride(a);
+  if (key_mask.defined()) {
+    MVB_CHECK(key_mask.scalar_type() == at::kBool, "key_mask has to be bool, got ", dtype_name(key_mask));
+    MVB_CHECK(key_mask.dim() == 2 && key_mask.size(0) == s.batch && key_mask.size(1) == s.keys, "key_mask has shape ", shape_text(key_mask.sizes()),
+              ", expected (", s.batch, ", ", s.keys, ")");
+    c.mask = s.keys <= 1 || key_mask.stride(1) == 1 ? key_mask : key_mask.contiguous();
+    s.mask_stride = c.mask.stride(0);
+  }
+  if (key_lengths.defined()) {
+    MVB_CHECK(at::isIntegralType(key_lengths.scalar_type(), false), "key_lengths have to be whole numbers, got ", dtype_name(key_lengths));
+    MVB_CHECK(key_lengths.dim() == 1 && key_lengths.size(0) == s.batch, "key_lengths has shape ", shape_text(key_lengths.sizes()), ", expected (", s.batch, ")");
+    c.lengths = key_lengths.scalar_type() == at::kInt ? key_lengths.contiguous()
+                                                       : key_lengths.clamp(0, s.keys).to(at::kInt).contiguous();
+  }
+  return c;
+}
+
+// output, and the logarithms of the softmax's sums where a backward pass will want them
+std::pair<Tensor, Tensor> attention_forward(const AttentionCall &c, double scale, bool train) {
+  const c10::DeviceGuard guard(c.q.device());
+  const mv_attention_shape &s = c.shape;
+  const Tensor output = at::empty({s.batch, s.queries, s.heads, s.dim}, c.q.options());
+  const Tensor lse = train ? at::empty({s.batch, s.heads, s.queries}, c.q.options().dtype(at::kFloat)) : Tensor();
+  const size_t bytes = mv_cross_attention_forward_workspace_bytes(&s, c.code);
+  const Tensor ws = bytes_on(c.q, bytes);
+  check(mv_cross_attention_forward(ptr(c.q), ptr(c.k), ptr(c.v), ptr(c.mask), ptr(c.lengths), ptr(output), ptr(lse), &s,
+                                   static_cast<float>(scale), c.code, ptr(ws), bytes, stream_of(c.q)));
+  return {output, lse};
+}
+
+variable_list attention_backward(const AttentionCall &c, const Tensor &output, const Tensor &lse, const Tensor &grad_in, double scale) {
+  const c10::DeviceGuard guard(c.q.device());
+  const mv_attention_shape &s = c.shape;
+  same_device(c.q, grad_in, "grad_output");
+  MVB_CHECK(grad_in.sizes() == output.sizes(), "grad_output has shape ", shape_text(grad_in.sizes()), ", expected ", shape_text(output.sizes()));
+  const Tensor grad = grad_in.to(output.scalar_type()).contiguous();
+  const Tensor gq = at::empty({s.batch, s.queries, s.heads, s.dim}, c.q.options());
+  const Tensor gk = at::empty({s.batch, s.keys, s.key_heads, s.dim}, c.q.options()), gv = at::empty_like(gk);
+  const size_t bytes = mv_cross_attention_backward_workspace_bytes(&s, c.code);
+  const Tensor ws = bytes_on(c.q, bytes);
+  check(mv_cross_attention_backward(ptr(c.q), ptr(c.k), ptr(c.v), ptr(c.mask), ptr(c.lengths), ptr(output), ptr(lse), ptr(grad),
+                                    ptr(gq), ptr(gk), ptr(gv), &s, static_cast<float>(scale), c.code, ptr(ws), bytes, stream_of(c.q)));
+  return {gq, gk, gv};
+}
+
+struct CrossAttentionFunction : torch::autograd::Function<CrossAttentionFunction> {
+  static Tensor forward(AutogradContext *ctx, const Tensor &query, const Tensor &key, const Tensor &value,
+                        const std::optional<Tensor> &key_mask, const std::optional<Tensor> &key_lengths, double scale) {
+    const AttentionCall c = attention_call(query, key, value, key_mask.value_or(Tensor()), key_lengths.value_or(Tensor()));
+    const auto [output, lse] = attention_forward(c, scale, true);
+    ctx->save_for_backward({query, key, value, c.mask, c.lengths, output, lse});
+    ctx->saved_data["scale"] = scale;
+    return output;
+  }
+  static variable_list backward(AutogradContext *ctx, const variable_list &grads) {
+    variable_list out(6);
+    if (!grads[0].defined()) return out;
+    {
+      const at::NoGradGuard no_grad;
+      const auto t = ctx->get_saved_variables();
+      const variable_list g = attention_backward(attention_call(t[0], t[1], t[2], t[3], t[4]), t[5], t[6], grads[0],
+                                                 ctx->saved_data["scale"].toDouble());
+      for (int i = 0; i < 3; ++i) out[i] = g[i];
+    }
+    differentiable_once(grads, out);
+    return out;
+  }
+};
+
+double attention_scale(const Tensor &query, const std::optional<double> &scale) {
+  return scale ? *scale : 1.0 / std::sqrt(static_cast<double>(query.dim() == 4 ? query.size(3) : 1));
+}
+
+Tensor cross_attention(const Tensor &query, const Tensor &key, const Tensor &value, const std::optional<Tensor> &key_mask,
+                       const std::optional<Tensor> &key_lengths, const std::optional<double> &scale) {
+  for (const Tensor &t : {query, key, value}) no_forward_mode(t);
+  const py::gil_scoped_release no_gil;
+  if (wants_gradient({query, key, value}))
+    return CrossAttentionFunction::apply(query, key, value, key_mask, key_lengths, attention_scale(query, scale));
+  const at::NoGradGuard no_grad;
+  return attention_forward(attention_call(query, key, value, key_mask.value_or(Tensor()), key_lengths.value_or(Tensor())),
+                           attention_scale(query, scale), false).first;
+}
+
+// The two halves for the Python form of the node
+std::pair<Tensor, Tensor> cross_attention_forward(const Tensor &query, const Tensor &key, const Tensor &value, const std::optional<Tensor> &key_mask,
+                                                  const std::optional<Tensor> &key_lengths, const std::optional<double> &scale) {
+  const py::gil_scoped_release no_gil;
+  const at::NoGradGuard no_grad;
+  return attention_forward(attention_call(query, key, value, key_mask.value_or(Tensor()), key_lengths.value_or(Tensor())),
+                           attention_scale(query, scale), true);
+}
+
+std::tuple<Tensor, Tensor, Tensor> cross_attention_backward(const Tensor &query, const Tensor &key, const Tensor &value,
+                                                            const std::optional<Tensor> &key_mask, const std::optional<Tensor> &key_lengths,
+                                                            const Tensor &output, const Tensor &lse, const Tensor &grad, const std::optional<double> &scale) {
+  const py::gil_scoped_release no_gil;
+  const at::NoGradGuard no_grad;
+  const auto g = attention_backward(attention_call(query, key, value, key_mask.value_or(Tensor()), key_lengths.value_or(Tensor())), output, lse,
+                                    grad, attention_scale(query, scale));
+  return {g[0], g[1], g[2]};
+}
+
+struct NormCall {
+  Tensor x, residual, weight;
+  int64_t rows;
+  int columns, code, weight_code;
+};
+
+NormCall norm_call(const Tensor &x, const Tensor &residual, const Tensor &weight, const char *what) {
+  MVB_CHECK(x.is_cuda(), what, " is not implemented on CPU");
+  NormCall c;
+  c.code = float_code(x, what);
+  MVB_CHECK(x.dim() >= 1 && x.size(-1) >= 1, what, " takes rows of at least one column, got shape ", shape_text(x.sizes()));
+  same_device(x, residual, "residual");
+  same_device(x, weight, "weight");
+  MVB_CHECK(weight.dim() == 1 && weight.size(0) == x.size(-1), "weight has shape ", shape_text(weight.sizes()), ", expected (", x.size(-1), ")");
+  MVB_CHECK(weight.scalar_type() == x.scalar_type() || weight.scalar_type() == at::kFloat, "weight has dtype ", dtype_name(weight),
+            ", expected float32 or that of the input");
+  MVB_CHECK(!residual.defined() || (residual.sizes() == x.sizes() && residual.scalar_type() == x.scalar_type()),
+            "the residual must have the input's shape and dtype");
+  c.weight_code = dtype_code(weight);
+  c.x = x.contiguous();
+  c.residual = residual.defined() ? residual.contiguous() : residual;
+  c.weight = weight.contiguous();
+  c.columns = to_int(x.size(-1), "a row");
+  c.rows = x.numel() / c.columns;
+  return c;
+}
+
+// y, and the sum where there is a residual
+std::pair<Tensor, Tensor> norm_forward(const NormCall &c, double eps) {
+  const c10::DeviceGuard guard(c.x.device());
+  const Tensor y = at::empty_like(c.x);
+  const Tensor sum = c.residual.defined() ? at::empty_like(c.x) : Tensor();
+  check(mv_add_rms_norm(ptr(c.x), ptr(c.residual), ptr(c.weight), ptr(y), ptr(sum), c.rows, c.columns, static_cast<float>(eps), c.code,
+                        c.weight_code, stream_of(c.x)));
+  return {y, sum};
+}
+
+// gradients of the sum and of the weight
+std::pair<Tensor, Tensor> norm_backward(const Tensor &h, const Tensor &weight, const Tensor &grad_y, const Tensor &grad_sum, double eps) {
+  const NormCall c = norm_call(h, Tensor(), weight, "add_rms_norm");
+  const c10::DeviceGuard guard(c.x.device());
+  same_device(c.x, grad_y, "grad_output");
+  same_device(c.x, grad_sum, "grad_output");
+  const Tensor gy = grad_y.defined() ? grad_y.to(h.scalar_type()).contiguous() : at::zeros_like(c.x);
+  const Tensor gs = grad_sum.defined() ? grad_sum.to(h.scalar_type()).contiguous() : grad_sum;
+  MVB_CHECK(gy.sizes() == h.sizes() && (!gs.defined() || gs.sizes() == h.sizes()), "grad_output must have the shape ", shape_text(h.sizes()));
+  const Tensor gx = at::empty_like(c.x), gw = at::empty_like(c.weight);
+  const size_t bytes = mv_add_rms_norm_backward_workspace_bytes(c.rows, c.columns);
+  const Tensor ws = bytes_on(c.x, bytes);
+  check(mv_add_rms_norm_backward(ptr(c.x), ptr(c.weight), ptr(gy), ptr(gs), ptr(gx), ptr(gw), c.rows, c.columns, static_cast<float>(eps),
+                                 c.code, c.weight_code, ptr(ws), bytes, stream_of(c.x)));
+  return {gx, gw};
+}
+
+struct AddRmsNormFunction : torch::autograd::Function<AddRmsNormFunction> {
+  static variable_list forward(AutogradContext *ctx, const Tensor &x, const std::optional<Tensor> &residual, const Tensor &weight, double eps) {
+    const NormCall c = norm_call(x, residual.value_or(Tensor()), weight, "add_rms_norm");
+    const auto [y, sum] = norm_forward(c, eps);
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({sum.defined() ? sum : x, weight});
+    ctx->saved_data["eps"] = eps;
+    if (sum.defined()) return {y, sum};
+    return {y};
+  }
+  static variable_list backward(AutogradContext *ctx, const variable_list &grads) {
+    variable_list out(4);
+    const Tensor none, &gs = grads.size() > 1 ? grads[1] : none;
+    if (!grads[0].defined() && !gs.defined()) return out;
+    {
+      const at::NoGradGuard no_grad;
+      const auto t = ctx->get_saved_variables();
+      const auto [gx, gw] = norm_backward(t[0], t[1], grads[0], gs, ctx->saved_data["eps"].toDouble());
+      out[0] = gx;
+      if (grads.size() > 1) out[1] = gx;
+      out[2] = gw;
+    }
+    differentiable_once(grads, out);
+    return out;
+  }
+};
+
+// (y, sum); without a residual the sum is x itself
+std::pair<Tensor, Tensor> add_rms_norm(const Tensor &x, const std::optional<Tensor> &residual, const Tensor &weight, double eps) {
+  for (const Tensor &t : {x, residual.value_or(Tensor()), weight}) no_forward_mode(t);
+  const py::gil_scoped_release no_gil;
+  if (wants_gradient({x, residual.value_or(Tensor()), weight})) {
+    const variable_list out = AddRmsNormFunction::apply(x, residual, weight, eps);
+    return {out[0], out.size() > 1 ? out[1] : x};
+  }
+  const at::NoGradGuard no_grad;
+  auto out = norm_forward(norm_call(x, residual.value_or(Tensor()), weight, "add_rms_norm"), eps);
+  if (!out.second.defined()) out.second = x;
+  return out;
+}
+
+std::pair<Tensor, std::optional<Tensor>> add_rms_norm_forward(const Tensor &x, const std::optional<Tensor> &residual, const Tensor &weight, double eps) {
+  const py::gil_scoped_release no_gil;
+  const at::NoGradGuard no_grad;
+  const auto out = norm_forward(norm_call(x, residual.value_or(Tensor()), weight, "add_rms_norm"), eps);
+  return {out.first, out.second.defined() ? std::optional<Tensor>(out.second) : std::nullopt};
+}
+
+std::pair<Tensor, Tensor> add_rms_norm_backward(const Tensor &h, const Tensor &weight, const std::optional<Tensor> &grad_y,
+                                                const std::optional<Tensor> &grad_sum, double eps) {
+  const py::gil_scoped_release no_gil;
+  const at::NoGradGuard no_grad;
+  return norm_backward(h, weight, grad_y.value_or(Tensor()), grad_sum.value_or(Tensor()), eps);
+}
+
+// 8-bit values of rows of `columns` and their scales
+std::pair<Tensor, Tensor> empty_blocks(const Tensor &x) {
+  std::vector<int64_t> q = x.sizes().vec(), s = q;
+  s.back() = (q.back() + 127) / 128;
+  q.back() = 128 * s.back();
+  return {at::empty(q, x.options().dtype(at::kFloat8_e4m3fn)), at::empty(s, x.options().dtype(at::kFloat))};
+}
+
+void no_gradient(std::initializer_list<Tensor> tensors, const char *what) {
+  for (const Tensor &t : tensors) no_forward_mode(t);
+  MVB_CHECK(!wants_gradient(tensors), what, " has no gradient: call it under torch.no_grad()");
+}
+
+std::tuple<Tensor, Tensor, Tensor> add_rms_norm_quantized(const Tensor &x, const std::optional<Tensor> &residual, const Tensor &weight, double eps) {
+  no_gradient({x, residual.value_or(Tensor()), weight}, "add_rms_norm_quantized");
+  const py::gil_scoped_release no_gil;
+  const at::NoGradGuard no_grad;
+  const NormCall c = norm_call(x, residual.value_or(Tensor()), weight, "add_rms_norm_quantized");
+  const c10::DeviceGuard guard(c.x.device());
+  const auto [q, scales] = empty_blocks(c.x);
+  const Tensor sum = c.residual.defined() ? at::empty_like(c.x) : Tensor();
+  check(mv_add_rms_norm_quantized(ptr(c.x), ptr(c.residual), ptr(c.weight), ptr(q), ptr(scales), ptr(sum), c.rows, c.columns,
+                                  static_cast<float>(eps), c.code, c.weight_code, stream_of(c.x)));
+  return {q, scales, sum.defined() ? sum : x};
+}
+
+std::pair<Tensor, Tensor> quantize_blocks(const Tensor &given, int64_t block_rows) {
+  no_gradient({given}, "quantize_blocks");
+  const py::gil_scoped_release no_gil;
+  const at::NoGradGuard no_grad;
+  MVB_CHECK(given.is_cuda(), "quantize_blocks is not implemented on CPU");
+  const int code = float_code(given, "quantize_blocks");
+  MVB_CHECK(block_rows == 1 || block_rows == 128, "block_rows ", block_rows, ": 1 or 128 are possible");
+  MVB_CHECK(given.dim() >= 1 && given.size(-1) >= 1, "quantize_blocks takes rows of at least one column, got shape ", shape_text(given.sizes()));
+  MVB_CHECK(block_rows == 1 || given.dim() == 2, "blocks of 128 rows are those of a matrix, got shape ", shape_text(given.sizes()));
+  const c10::DeviceGuard guard(given.device());
+  const Tensor x = given.contiguous();
+  auto [q, scales] = empty_blocks(x);
+  if (block_rows != 1) scales = at::empty({(x.size(0) + 127) / 128, scales.size(1)}, scales.options());
+  const int columns = to_int(x.size(-1), "a row");
+  check(mv_quantize_blocks(ptr(x), ptr(q), ptr(scales), x.numel() / columns, columns, static_cast<int>(block_rows), code, stream_of(x)));
+  return {q, scales};
+}
+
+Tensor aligned_rows(const Tensor &t) {
+  const Tensor c = t.contiguous();
+  return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 == 0 ? c : c.clone();
+}
+
+Tensor block_linear(const Tensor &q_in, const Tensor &q_scales, const Tensor &weight_in, const Tensor &weight_scales,
+                    const std::optional<Tensor> &bias_in, at::ScalarType out_dtype) {
+  const Tensor bias_given = bias_in.value_or(Tensor());
+  no_gradient({q_scales, weight_scales, bias_given}, "block_linear");
+  const py::gil_scoped_release no_gil;
+  const at::NoGradGuard no_grad;
+  MVB_CHECK(q_in.is_cuda(), "block_linear is not implemented on CPU");
+  MVB_CHECK(q_in.scalar_type() == at::kFloat8_e4m3fn && weight_in.scalar_type() == at::kFloat8_e4m3fn, "q and weight have to be float8_e4m3fn, got ",
+            dtype_name(q_in), " and ", dtype_name(weight_in));
+  MVB_CHECK(out_dtype == at::kHalf || out_dtype == at::kBFloat16, "out_dtype has to be float16 or bfloat16");
+  same_device(q_in, q_scales, "q_scales");
+  same_device(q_in, weight_in, "weight");
+  same_device(q_in, weight_scales, "weight_scales");
+  same_device(q_in, bias_given, "bias");
+  MVB_CHECK(q_in.dim() >= 1 && weight_in.dim() == 2 && q_in.size(-1) == weight_in.size(1), "q has shape ", shape_text(q_in.sizes()), ", weight ",
+            shape_text(weight_in.sizes()), ": the last dimensions have to be alike");
+  const int inputs = to_int(weight_in.size(1), "a row"), outputs = to_int(weight_in.size(0), "the number of outputs");
+  MVB_CHECK(inputs > 0 && inputs % 128 == 0, inputs, " inputs: whole blocks of 128 are needed (quantize_blocks pads)");
+  std::vector<int64_t> want = q_in.sizes().vec();
+  want.back() = inputs / 128;
+  MVB_CHECK(q_scales.scalar_type() == at::kFloat && weight_scales.scalar_type() == at::kFloat, "scales have to be float32");
+  MVB_CHECK(q_scales.sizes() == at::IntArrayRef(want), "q_scales has shape ", shape_text(q_scales.sizes()), ", expected ", shape_text(want));
+  const std::vector<int64_t> want_w{(outputs + 127) / 128, inputs / 128};
+  MVB_CHECK(weight_scales.sizes() == at::IntArrayRef(want_w), "weight_scales has shape ", shape_text(weight_scales.sizes()), ", expected ", shape_text(want_w));
+  MVB_CHECK(!bias_given.defined() || (bias_given.dim() == 1 && bias_given.size(0) == outputs), "bias has shape ",
+            bias_given.defined() ? shape_text(bias_given.sizes()) : "", ", expected (", outputs, ")");
+  const c10::DeviceGuard guard(q_in.device());
+  const Tensor q = aligned_rows(q_in), w = aligned_rows(weight_in), qs = q_scales.contiguous(), ws = weight_scales.contiguous();
+  const Tensor bias = bias_given.defined() ? bias_given.to(out_dtype).contiguous() : bias_given;
+  const int64_t rows = q.numel() / inputs;
+  want.back() = outputs;
+  const Tensor y = at::empty(want, q.options().dtype(out_dtype));
+  const size_t bytes = mv_block_linear_workspace_bytes(rows, inputs, outputs);
+  const Tensor work = bytes_on(q, bytes);
+  check(mv_block_linear(ptr(q), ptr(qs), ptr(w), ptr(ws), ptr(bias), ptr(y), rows, inputs, outputs, dtype_code(y), ptr(work), bytes, stream_of(q)));
+  return y;
+}
+
 // ---- helpers of the augmentation stages ----------------------------------------------------------------------------
 // A host array (rois, a control grid) on the device, without waiting for what is queued there.  float64 stays float64,
 // every other type becomes float32.
@@ -563,6 +923,15 @@ PYBIND11_MODULE(_native, m) {
   m.def("deform_conv", &deform_conv);
   m.def("deform_warp", &deform_warp);
   m.def("elastic_warp", &elastic_warp);
+  m.def("cross_attention", &cross_attention);
+  m.def("cross_attention_forward", &cross_attention_forward);
+  m.def("cross_attention_backward", &cross_attention_backward);
+  m.def("add_rms_norm", &add_rms_norm);
+  m.def("add_rms_norm_forward", &add_rms_norm_forward);
+  m.def("add_rms_norm_backward", &add_rms_norm_backward);
+  m.def("add_rms_norm_quantized", &add_rms_norm_quantized);
+  m.def("quantize_blocks", &quantize_blocks);
+  m.def("block_linear", &block_linear);
   m.def("upload", &upload);
   m.def("window_roi", &window_roi);
   m.def("peak_mib", &peak_mib);

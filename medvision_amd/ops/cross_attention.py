@@ -1,0 +1,41 @@
+"""``cross_attention``: queries of a decoder over an encoder's states of another length.  No counterpart in the reference."""
+from torch.autograd.function import once_differentiable
+
+from .._lib import native
+from ._function import NativeFunction
+
+
+class CrossAttentionFunction(NativeFunction):
+    @staticmethod
+    def native(query, key, value, key_mask=None, key_lengths=None, scale=None):
+        return native.cross_attention(query, key, value, key_mask, key_lengths, scale)
+
+    @staticmethod
+    def forward(ctx, query, key, value, key_mask=None, key_lengths=None, scale=None):
+        output, lse = native.cross_attention_forward(query, key, value, key_mask, key_lengths, scale)
+        ctx.save_for_backward(query, key, value, key_mask, key_lengths, output, lse)
+        ctx.scale = scale
+        return output
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_output):
+        query, key, value, key_mask, key_lengths, output, lse = ctx.saved_tensors
+        grads = native.cross_attention_backward(query, key, value, key_mask, key_lengths, output, lse, grad_output, ctx.scale)
+        return (*grads, None, None, None)
+
+
+def cross_attention(query, key, value, key_mask=None, key_lengths=None, scale=None):
+    """Attention of queries over the keys and values of another length, with the gradients of all three.
+
+    Args:
+        query (Tensor): ``[batch, queries, heads, channels]``; float32, float16 or bfloat16, 1 to 128 channels per head
+        key, value (Tensor): ``[batch, keys, key_heads, channels]``; ``heads`` is a multiple of ``key_heads``, consecutive
+            heads of the query share a head of the keys.  Views are read in place as long as a head's channels are neighbours
+        key_mask (Tensor): bool ``[batch, keys]``, False where a key does not count
+        key_lengths (Tensor): whole numbers ``[batch]``: keys from there on do not count
+        scale (float): of the products of queries and keys, ``channels ** -0.5`` by default
+
+    What keys and values that do not count hold has no effect, not even NaN.  A query without any key gets zeros.
+    """
+    return CrossAttentionFunction.apply(query, key, value, key_mask, key_lengths, scale)
