@@ -1,38 +1,328 @@
 // Product of 8-bit floats (e4m3) with a scale for each row and 128 columns of the activations and for each 128 x 128 block
 // of the weights:  y[m, n] = sum over blocks b of  sx[m, b] sw[n / 128, b] sum_k qx[m, 128 b + k] qw[n, 128 b + k]  + bias[n]
+//
+// One v_mfma 16x16x128 takes a whole block of 128: it starts from zero, and its result is added to the sum in 32 bits with
+// the two scales' product.  The weights are its first operand, so that a lane's results lie in one row of y (one scale per
+// tile and lane, four neighbouring results).
 #include "rows.hpp"
+
+#include <algorithm>
 
 namespace mv {
 namespace {
 
-__device__ __forceinline__ float from_e4m3(unsigned word, int byte) {
-  switch (byte) {
-    case 0: return __builtin_amdgcn_cvt_f32_fp8(static_cast<int>(word), 0);
-    case 1: return __builtin_amdgcn_cvt_f32_fp8(static_cast<int>(word), 1);
-    case 2: return __builtin_amdgcn_cvt_f32_fp8(static_cast<int>(word), 2);
-    default: return __builtin_amdgcn_cvt_f32_fp8(static_cast<int>(word), 3);
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ f32x4 block_product(const i32x8 &w, const i32x8 &x) {
+  const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+  // (scales of 0: the instruction without scales)
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, zero, 0, 0, 0, 0, 0, 0);
+}
+
+__device__ __forceinline__ i32x8 join(const i32x4 &a, const i32x4 &b) { return {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]}; }
+
+// Where results go: y itself, or a part of the sums in 32 bits.
+template <typename T> struct Results {
+  T *y;
+  const T *bias;
+  float *part;   // [splits, rows, outputs], NULL: y
+  long rows;
+  int outputs;
+};
+
+// Four neighbouring results of row m
+template <typename T> __device__ __forceinline__ void store4(const Results<T> &to, int split, long m, int n, f32x4 v) {
+  const int left = to.outputs - n;
+  if (m >= to.rows || left <= 0) return;
+  if (to.part) {
+    float *const at = to.part + (split * to.rows + m) * to.outputs + n;
+    if (left >= 4) reinterpret_cast<Loose<f32x4, 4> *>(at)->v = v;
+    else
+      for (int i = 0; i < left; ++i) at[i] = v[i];
+    return;
+  }
+  T *const at = to.y + m * to.outputs + n;
+  if (left >= 4) {
+    if (to.bias) {
+      const u32x2 b = reinterpret_cast<const Loose<u32x2, 2> *>(to.bias + n)->v;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] += Bits<T>::up(static_cast<unsigned short>(b[i / 2] >> (i % 2 * 16)));
+    }
+    u32x2 r;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) r[i] = Bits<T>::down(v[2 * i]) | (static_cast<unsigned>(Bits<T>::down(v[2 * i + 1])) << 16);
+    reinterpret_cast<Loose<u32x2, 2> *>(at)->v = r;
+  } else {
+    for (int i = 0; i < left; ++i) at[i] = store_cast<T>(to.bias ? v[i] + load(to.bias + n + i) : v[i]);
+  }
+}
+
+// ---- tiles ----------------------------------------------------------------------------------------------
+// A workgroup takes BM rows and BN outputs; WM x WN wavefronts share the tile, WK groups of them take every WK-th block of
+// the sum.  Both operands go from memory to LDS without registers (16 bytes per lane, the next blocks while these are
+// multiplied).  A row of a block is 128 bytes, eight pieces of 16; piece c of row r stands at c ^ (r & 7), so that the 16
+// rows of an operand that one instruction reads spread over all banks.
+template <int BM, int BN, int WM, int WN, int WK> struct Tiles {
+  static constexpr int kThreads = 64 * WM * WN * WK, kTM = BM / WM / 16, kTN = BN / WN / 16;
+  static constexpr int kStage = (BM + BN) * kBlock;   // bytes of one block of both operands
+  static constexpr int kLds = 2 * WK * kStage;
+};
+
+template <typename T, int BM, int BN, int WM, int WN, int WK>
+__global__ __launch_bounds__(64 * WM * WN * WK, WM *WN *WK / 4) void product_tiles(
+    const unsigned char *q, const float *qs, const unsigned char *w, const float *ws, const Results<T> to, int rows, int inputs,
+    int outputs, int m_tiles, int n_tiles, int splits) {
+  using S = Tiles<BM, BN, WM, WN, WK>;
+  __shared__ __attribute__((aligned(16))) unsigned char lds[S::kLds];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int group = wave / (WM * WN), in_group = wave % (WM * WN), wm = in_group % WM, wn = in_group / WM;
+  // tiles in an order in which neighbouring workgroups of a die share rows and weights: eight rows of tiles at a time
+  const int tiles = m_tiles * n_tiles;
+  unsigned id = linear_block();
+  if (id >= static_cast<unsigned>(tiles) * splits) return;
+  const int split = id / tiles;
+  id = xcd_contiguous(id % tiles, tiles);
+  const int band = id / (8 * n_tiles), in_band = id % (8 * n_tiles), tall = min(8, m_tiles - 8 * band);
+  const int m0 = (8 * band + in_band % tall) * BM, n0 = in_band / tall * BN;
+  const int blocks = inputs / kBlock, first = static_cast<int>(static_cast<long>(blocks) * split / splits),
+            last = static_cast<int>(static_cast<long>(blocks) * (split + 1) / splits), steps = (last - first + WK - 1) / WK;
+
+  // What this wavefront brings: 8 rows (1024 bytes) per instruction.
+  constexpr int kRows8 = (BM + BN) / 8, kMine = kRows8 / (WM * WN);
+  static_assert(kRows8 % (WM * WN) == 0, "");
+  const int lr = lane >> 3, piece = (lane & 7) ^ lr;
+  const unsigned char *from[kMine];
+#pragma unroll
+  for (int i = 0; i < kMine; ++i) {
+    const int row = (in_group * kMine + i) * 8 + lr;   // of the stage: activations, then weights
+    from[i] = (row < BM ? q + static_cast<long>(min(m0 + row, rows - 1)) * inputs
+                        : w + static_cast<long>(min(n0 + row - BM, outputs - 1)) * inputs) + piece * 16;
+  }
+  auto bring = [&](int step) {
+    const int b = min(first + step * WK + group, last - 1);
+    unsigned char *to = lds + ((step & 1) * WK + group) * S::kStage + in_group * kMine * 1024;
+#pragma unroll
+    for (int i = 0; i < kMine; ++i)
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(from[i] + static_cast<long>(b) * kBlock),
+                                       (__attribute__((address_space(3))) void *)(to + i * 1024), 16, 0, 0);
+  };
+
+  const int r16 = lane & 15, g = lane >> 4;
+  const float *scale_at[S::kTM];
+#pragma unroll
+  for (int t = 0; t < S::kTM; ++t) scale_at[t] = qs + static_cast<long>(min(m0 + (wm * S::kTM + t) * 16 + r16, rows - 1)) * blocks;
+  const float *weight_scale_at = ws + static_cast<long>(min(n0 + wn * S::kTN * 16, outputs - 1) / kBlock) * blocks;
+  float sx[S::kTM], sw;
+  auto scales = [&](int step) {
+    const int b = min(first + step * WK + group, last - 1);
+#pragma unroll
+    for (int t = 0; t < S::kTM; ++t) sx[t] = scale_at[t][b];
+    sw = weight_scale_at[b];
+  };
+
+  f32x4 acc[S::kTN][S::kTM] = {};
+  bring(0);
+  scales(0);
+  for (int step = 0; step < steps; ++step) {
+    __syncthreads();   // this step's operands are there, and nobody reads the place of the next ones
+    if (step + 1 < steps) bring(step + 1);
+    if (WK == 1 || first + step * WK + group < last) {
+      const unsigned char *xs = lds + ((step & 1) * WK + group) * S::kStage, *wsm = xs + BM * kBlock;
+      // piece g and piece g + 4 of the row: any order of k serves, as long as both operands have the same
+      const int p0 = (g ^ (r16 & 7)) * 16, p1 = ((g + 4) ^ (r16 & 7)) * 16;
+      float s[S::kTM];
+#pragma unroll
+      for (int t = 0; t < S::kTM; ++t) s[t] = sx[t] * sw;
+      i32x8 x[S::kTM];
+#pragma unroll
+      for (int t = 0; t < S::kTM; ++t) {
+        const unsigned char *row = xs + ((wm * S::kTM + t) * 16 + r16) * kBlock;
+        x[t] = join(*reinterpret_cast<const i32x4 *>(row + p0), *reinterpret_cast<const i32x4 *>(row + p1));
+      }
+#pragma unroll
+      for (int u = 0; u < S::kTN; ++u) {
+        const unsigned char *row = wsm + ((wn * S::kTN + u) * 16 + r16) * kBlock;
+        const i32x8 v = join(*reinterpret_cast<const i32x4 *>(row + p0), *reinterpret_cast<const i32x4 *>(row + p1));
+#pragma unroll
+        for (int t = 0; t < S::kTM; ++t) {
+          const f32x4 d = block_product(v, x[t]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[u][t][i] = fmaf(d[i], s[t], acc[u][t][i]);
+        }
+      }
+    }
+    scales(step + 1);
+  }
+  if (WK > 1) {   // the groups' sums, in their order
+    f32x4 *const part = reinterpret_cast<f32x4 *>(lds);
+    const int at = in_group * 64 + lane;
+    for (int from_group = 1; from_group < WK; ++from_group) {
+      __syncthreads();
+      if (group == from_group) {
+#pragma unroll
+        for (int u = 0; u < S::kTN; ++u)
+#pragma unroll
+          for (int t = 0; t < S::kTM; ++t) part[(u * S::kTM + t) * (64 * WM * WN) + at] = acc[u][t];
+      }
+      __syncthreads();
+      if (group == 0) {
+#pragma unroll
+        for (int u = 0; u < S::kTN; ++u)
+#pragma unroll
+          for (int t = 0; t < S::kTM; ++t) acc[u][t] += part[(u * S::kTM + t) * (64 * WM * WN) + at];
+      }
+    }
+    if (group) return;
+  }
+#pragma unroll
+  for (int t = 0; t < S::kTM; ++t) {
+    const int m = m0 + (wm * S::kTM + t) * 16 + r16;
+#pragma unroll
+    for (int u = 0; u < S::kTN; ++u) store4(to, split, m, n0 + (wn * S::kTN + u) * 16 + 4 * g, acc[u][t]);
+  }
+}
+
+// ---- few rows -----------------------------------------------------------------------------------------------
+// Bound by reading the weights once: 64 outputs and 16 TM rows per workgroup, straight from memory into the operands'
+// registers, the next block's while this one is multiplied.  The four wavefronts take turns at the blocks of the
+// workgroup's share of the sum and join in LDS.
+template <typename T, int TM>
+__global__ __launch_bounds__(256) void product_rows(const unsigned char *q, const float *qs, const unsigned char *w, const float *ws,
+                                                    const Results<T> to, int rows, int inputs, int outputs, int m_tiles, int n_tiles,
+                                                    int splits) {
+  constexpr int TN = 4;
+  __shared__ f32x4 part[3][TN * TM][64];
+  unsigned id = linear_block();
+  if (id >= static_cast<unsigned>(m_tiles) * n_tiles * splits) return;
+  const int n_tile = id % n_tiles;
+  id /= n_tiles;
+  const int split = id % splits, m0 = id / splits * 16 * TM, n0 = n_tile * 16 * TN;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, g = lane >> 4;
+  const int blocks = inputs / kBlock, first = static_cast<int>(static_cast<long>(blocks) * split / splits),
+            last = static_cast<int>(static_cast<long>(blocks) * (split + 1) / splits);
+  const unsigned char *x_at[TM], *w_at[TN];
+  const float *sx_at[TM];
+#pragma unroll
+  for (int t = 0; t < TM; ++t) {
+    const long m = min(m0 + t * 16 + r16, rows - 1);
+    x_at[t] = q + m * inputs + g * 16;
+    sx_at[t] = qs + m * blocks;
+  }
+#pragma unroll
+  for (int u = 0; u < TN; ++u) w_at[u] = w + static_cast<long>(min(n0 + u * 16 + r16, outputs - 1)) * inputs + g * 16;
+  const float *sw_at = ws + static_cast<long>(n0 / kBlock) * blocks;
+
+  i32x8 x[TM], v[TN];
+  float s[TM];
+  auto bring = [&](int b) {
+    const long k = static_cast<long>(b) * kBlock;
+#pragma unroll
+    for (int u = 0; u < TN; ++u)
+      v[u] = join(*reinterpret_cast<const i32x4 *>(w_at[u] + k), *reinterpret_cast<const i32x4 *>(w_at[u] + k + 64));
+#pragma unroll
+    for (int t = 0; t < TM; ++t)
+      x[t] = join(*reinterpret_cast<const i32x4 *>(x_at[t] + k), *reinterpret_cast<const i32x4 *>(x_at[t] + k + 64));
+#pragma unroll
+    for (int t = 0; t < TM; ++t) s[t] = sx_at[t][b] * sw_at[b];
+  };
+  f32x4 acc[TN][TM] = {};
+  if (first + wave < last) bring(first + wave);
+  for (int b = first + wave; b < last; b += 4) {
+    i32x8 x1[TM], v1[TN];
+    float s1[TM];
+#pragma unroll
+    for (int t = 0; t < TM; ++t) x1[t] = x[t], s1[t] = s[t];
+#pragma unroll
+    for (int u = 0; u < TN; ++u) v1[u] = v[u];
+    if (b + 4 < last) bring(b + 4);
+#pragma unroll
+    for (int u = 0; u < TN; ++u)
+#pragma unroll
+      for (int t = 0; t < TM; ++t) {
+        const f32x4 d = block_product(v1[u], x1[t]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[u][t][i] = fmaf(d[i], s1[t], acc[u][t][i]);
+      }
+  }
+  if (wave) {
+#pragma unroll
+    for (int u = 0; u < TN; ++u)
+#pragma unroll
+      for (int t = 0; t < TM; ++t) part[wave - 1][u * TM + t][lane] = acc[u][t];
+  }
+  __syncthreads();
+  if (wave) return;
+#pragma unroll
+  for (int u = 0; u < TN; ++u)
+#pragma unroll
+    for (int t = 0; t < TM; ++t) {
+#pragma unroll
+      for (int i = 0; i < 3; ++i) acc[u][t] += part[i][u * TM + t][lane];
+      store4(to, split, m0 + t * 16 + r16, n0 + u * 16 + 4 * g, acc[u][t]);
+    }
+}
+
+// The parts' sum, in their order
+template <typename T>
+__global__ __launch_bounds__(256) void join_parts(const float *part, const T *bias, T *y, long count, int outputs, int splits) {
+  const long at = static_cast<long>(linear_block()) * 256 + threadIdx.x;
+  if (at >= count) return;
+  float sum = 0.f;
+  for (int s = 0; s < splits; ++s) sum += part[s * count + at];
+  if (bias) sum += load(bias + at % outputs);
+  y[at] = store_cast<T>(sum);
+}
+
+// ---- which kernel --------------------------------------------------------------------------------------------
+enum Kind { kFew1, kFew2, kFew4, kTile128, kTile256 };
+struct Plan {
+  int kind, m_tiles, n_tiles, splits;
+};
+
+int ceil_div(long a, long b) { return static_cast<int>((a + b - 1) / b); }
+
+Plan plan_of(long rows, int inputs, int outputs) {
+  const int blocks = inputs / kBlock;
+  if (rows <= 64) {
+    const int kind = rows <= 16 ? kFew1 : rows <= 32 ? kFew2 : kFew4;
+    const int n_tiles = ceil_div(outputs, 64);
+    return {kind, 1, n_tiles, std::max(1, std::min(blocks / 8, 512 / n_tiles))};
+  }
+  const long big = static_cast<long>(ceil_div(rows, 256)) * ceil_div(outputs, 256);
+  if (big >= 192) return {kTile256, ceil_div(rows, 256), ceil_div(outputs, 256), 1};
+  const int m = ceil_div(rows, 128), n = ceil_div(outputs, 128);
+  return {kTile128, m, n, std::max(1, std::min(blocks / 8, 256 / (m * n)))};
+}
+
+template <typename T>
+void launch(const Plan &p, const void *q, const void *qs, const void *w, const void *ws, const Results<T> &to, int rows, int inputs,
+            int outputs, hipStream_t s) {
+  const long groups = static_cast<long>(p.m_tiles) * p.n_tiles * p.splits;
+  const auto *q8 = static_cast<const unsigned char *>(q), *w8 = static_cast<const unsigned char *>(w);
+  const auto *qf = static_cast<const float *>(qs), *wf = static_cast<const float *>(ws);
+  switch (p.kind) {
+    case kFew1: product_rows<T, 1><<<linear_grid(groups, 256), 256, 0, s>>>(q8, qf, w8, wf, to, rows, inputs, outputs, p.m_tiles, p.n_tiles, p.splits); break;
+    case kFew2: product_rows<T, 2><<<linear_grid(groups, 256), 256, 0, s>>>(q8, qf, w8, wf, to, rows, inputs, outputs, p.m_tiles, p.n_tiles, p.splits); break;
+    case kFew4: product_rows<T, 4><<<linear_grid(groups, 256), 256, 0, s>>>(q8, qf, w8, wf, to, rows, inputs, outputs, p.m_tiles, p.n_tiles, p.splits); break;
+    case kTile128: product_tiles<T, 128, 128, 2, 2, 2><<<linear_grid(groups, 512), 512, 0, s>>>(q8, qf, w8, wf, to, rows, inputs, outputs, p.m_tiles, p.n_tiles, p.splits); break;
+    default: product_tiles<T, 256, 256, 4, 2, 1><<<linear_grid(groups, 512), 512, 0, s>>>(q8, qf, w8, wf, to, rows, inputs, outputs, p.m_tiles, p.n_tiles, p.splits); break;
   }
 }
 
 template <typename T>
-__global__ __launch_bounds__(256) void product_kernel(const unsigned *q, const float *qs, const unsigned *w, const float *ws,
-                                                      const T *bias, T *y, long rows, int inputs, int outputs) {
-  const long at = static_cast<long>(linear_block()) * 256 + threadIdx.x;
-  if (at >= rows * outputs) return;
-  const long m = at / outputs;
-  const int n = static_cast<int>(at % outputs), blocks = inputs / kBlock;
-  float sum = 0.f;
-  for (int b = 0; b < blocks; ++b) {
-    float part = 0.f;
-    for (int k = 0; k < kBlock / 4; ++k) {
-      const unsigned x = q[m * (inputs / 4) + b * (kBlock / 4) + k], v = w[static_cast<long>(n) * (inputs / 4) + b * (kBlock / 4) + k];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) part += from_e4m3(x, i) * from_e4m3(v, i);
-    }
-    sum += part * (qs[m * blocks + b] * ws[static_cast<long>(n / kBlock) * blocks + b]);
+int product(const void *q, const void *qs, const void *w, const void *ws, const void *bias, void *y, long rows, int inputs, int outputs,
+            void *workspace, size_t workspace_bytes, hipStream_t s) {
+  Plan p = plan_of(rows, inputs, outputs);
+  if (p.splits > 1 && (!workspace || workspace_bytes < sizeof(float) * p.splits * static_cast<size_t>(rows) * outputs)) p.splits = 1;
+  float *const part = p.splits > 1 ? static_cast<float *>(workspace) : nullptr;
+  const Results<T> to{static_cast<T *>(y), static_cast<const T *>(bias), part, rows, outputs};
+  launch(p, q, qs, w, ws, to, static_cast<int>(rows), inputs, outputs, s);
+  if (part) {
+    const long count = rows * outputs;
+    join_parts<T><<<linear_grid((count + 255) / 256, 256), 256, 0, s>>>(part, to.bias, to.y, count, outputs, p.splits);
   }
-  if (bias) sum += load(bias + n);
-  y[at] = store_cast<T>(sum);
+  return check_launch("block_linear");
 }
 
 }  // namespace
@@ -42,27 +332,24 @@ using namespace mv;
 
 extern "C" {
 
-size_t mv_block_linear_workspace_bytes(int64_t rows, int inputs, int outputs) { return 0; }
+size_t mv_block_linear_workspace_bytes(int64_t rows, int inputs, int outputs) {
+  if (rows <= 0 || inputs <= 0 || outputs <= 0 || inputs % kBlock) return 0;
+  const Plan p = plan_of(rows, inputs, outputs);
+  return p.splits > 1 ? sizeof(float) * p.splits * static_cast<size_t>(rows) * outputs : 0;
+}
 
 int mv_block_linear(const void *q, const void *q_scales, const void *weight, const void *weight_scales, const void *bias,
                     void *y, int64_t rows, int inputs, int outputs, int dtype, void *workspace, size_t workspace_bytes,
                     void *stream) {
   MV_REQUIRE(dtype == MV_F16 || dtype == MV_BF16, "dtype %d of the output is not float16 or bfloat16", dtype);
-  MV_REQUIRE(rows >= 0 && inputs > 0 && outputs >= 0 && inputs % kBlock == 0, "wrong sizes: %ld rows, %d inputs (whole blocks of 128), %d outputs",
-             static_cast<long>(rows), inputs, outputs);
+  MV_REQUIRE(rows >= 0 && rows < (1L << 31) - 256 && inputs > 0 && outputs >= 0 && outputs < (1L << 31) - 256 && inputs % kBlock == 0,
+             "wrong sizes: %ld rows, %d inputs (whole blocks of 128), %d outputs", static_cast<long>(rows), inputs, outputs);
   if (rows == 0 || outputs == 0) return MV_OK;
   MV_REQUIRE(q && q_scales && weight && weight_scales && y, "a tensor is missing");
+  MV_REQUIRE(reinterpret_cast<uintptr_t>(q) % 16 == 0 && reinterpret_cast<uintptr_t>(weight) % 16 == 0, "q and weight have to be 16-byte aligned");
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  const dim3 grid = linear_grid((rows * outputs + 255) / 256, 256);
-  if (dtype == MV_F16)
-    product_kernel<__half><<<grid, 256, 0, s>>>(static_cast<const unsigned *>(q), static_cast<const float *>(q_scales),
-        static_cast<const unsigned *>(weight), static_cast<const float *>(weight_scales), static_cast<const __half *>(bias),
-        static_cast<__half *>(y), rows, inputs, outputs);
-  else
-    product_kernel<__hip_bfloat16><<<grid, 256, 0, s>>>(static_cast<const unsigned *>(q), static_cast<const float *>(q_scales),
-        static_cast<const unsigned *>(weight), static_cast<const float *>(weight_scales), static_cast<const __hip_bfloat16 *>(bias),
-        static_cast<__hip_bfloat16 *>(y), rows, inputs, outputs);
-  return check_launch("block_linear");
+  return dtype == MV_F16 ? product<__half>(q, q_scales, weight, weight_scales, bias, y, rows, inputs, outputs, workspace, workspace_bytes, s)
+                         : product<__hip_bfloat16>(q, q_scales, weight, weight_scales, bias, y, rows, inputs, outputs, workspace, workspace_bytes, s);
 }
 
 }  // extern "C"
