@@ -31,30 +31,49 @@ template <typename T> struct Results {
   int outputs;
 };
 
-// Four neighbouring results of row m
-template <typename T> __device__ __forceinline__ void store4(const Results<T> &to, int split, long m, int n, f32x4 v) {
-  const int left = to.outputs - n;
-  if (m >= to.rows || left <= 0) return;
+// Two neighbouring values of 16 bits
+template <typename T> __device__ __forceinline__ unsigned pack2(float a, float b);
+template <> __device__ __forceinline__ unsigned pack2<__half>(float a, float b) {
+  typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(unsigned, h2{static_cast<_Float16>(a), static_cast<_Float16>(b)});
+}
+template <> __device__ __forceinline__ unsigned pack2<__hip_bfloat16>(float a, float b) {
+  typedef float f2 __attribute__((ext_vector_type(2)));
+  typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(unsigned, __builtin_convertvector(f2{a, b}, b2));
+}
+
+// Results of TN tiles along row m, four neighbours of every 16 from n on
+template <typename T, int TN> __device__ __forceinline__ void store_row(const Results<T> &to, int split, long m, int n, const f32x4 (&v)[TN]) {
+  if (m >= to.rows) return;
   if (to.part) {
-    float *const at = to.part + (split * to.rows + m) * to.outputs + n;
-    if (left >= 4) reinterpret_cast<Loose<f32x4, 4> *>(at)->v = v;
-    else
-      for (int i = 0; i < left; ++i) at[i] = v[i];
+    float *const at = to.part + (split * to.rows + m) * to.outputs;
+#pragma unroll
+    for (int u = 0; u < TN; ++u) {
+      const int c = n + 16 * u;
+      if (c + 4 <= to.outputs) reinterpret_cast<Loose<f32x4, 4> *>(at + c)->v = v[u];
+      else
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+          if (c + i < to.outputs) at[c + i] = v[u][i];
+    }
     return;
   }
-  T *const at = to.y + m * to.outputs + n;
-  if (left >= 4) {
+  T *const at = to.y + m * to.outputs;
+#pragma unroll
+  for (int u = 0; u < TN; ++u) {
+    const int c = n + 16 * u;
+    f32x4 r = v[u];
     if (to.bias) {
-      const u32x2 b = reinterpret_cast<const Loose<u32x2, 2> *>(to.bias + n)->v;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] += Bits<T>::up(static_cast<unsigned short>(b[i / 2] >> (i % 2 * 16)));
+      for (int i = 0; i < 4; ++i) r[i] += load(to.bias + min(c + i, to.outputs - 1));
     }
-    u32x2 r;
+    const u32x2 bits = {pack2<T>(r[0], r[1]), pack2<T>(r[2], r[3])};
+    if (c + 4 <= to.outputs) reinterpret_cast<Loose<u32x2, 2> *>(at + c)->v = bits;
+    else
 #pragma unroll
-    for (int i = 0; i < 2; ++i) r[i] = Bits<T>::down(v[2 * i]) | (static_cast<unsigned>(Bits<T>::down(v[2 * i + 1])) << 16);
-    reinterpret_cast<Loose<u32x2, 2> *>(at)->v = r;
-  } else {
-    for (int i = 0; i < left; ++i) at[i] = store_cast<T>(to.bias ? v[i] + load(to.bias + n + i) : v[i]);
+      for (int i = 0; i < 3; ++i)
+        if (c + i < to.outputs) reinterpret_cast<unsigned short *>(at)[c + i] = static_cast<unsigned short>(bits[i / 2] >> (i % 2 * 16));
   }
 }
 
@@ -66,7 +85,7 @@ template <typename T> __device__ __forceinline__ void store4(const Results<T> &t
 template <int BM, int BN, int WM, int WN, int WK> struct Tiles {
   static constexpr int kThreads = 64 * WM * WN * WK, kTM = BM / WM / 16, kTN = BN / WN / 16;
   static constexpr int kStage = (BM + BN) * kBlock;   // bytes of one block of both operands
-  static constexpr int kLds = 2 * WK * kStage;
+  static constexpr int kLds = 2 * WK * kStage, kScales = BM + BN / kBlock;
 };
 
 template <typename T, int BM, int BN, int WM, int WN, int WK>
@@ -75,6 +94,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK, WM *WN *WK / 4) void product_til
     int outputs, int m_tiles, int n_tiles, int splits) {
   using S = Tiles<BM, BN, WM, WN, WK>;
   __shared__ __attribute__((aligned(16))) unsigned char lds[S::kLds];
+  __shared__ float scale[2][4][WK][S::kScales];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int group = wave / (WM * WN), in_group = wave % (WM * WN), wm = in_group % WM, wn = in_group / WM;
   // tiles in an order in which neighbouring workgroups of a die share rows and weights: eight rows of tiles at a time
@@ -109,50 +129,76 @@ __global__ __launch_bounds__(64 * WM * WN * WK, WM *WN *WK / 4) void product_til
   };
 
   const int r16 = lane & 15, g = lane >> 4;
-  const float *scale_at[S::kTM];
+  // The scales of four steps at a time, by one thread for a row (and one for 128 outputs), through LDS: read by every lane
+  // that needs them they would be as many cache lines as the operands.
+  const int mine = threadIdx.x % (64 * WM * WN);
+  const bool brings_scales = mine < S::kScales;
+  const float *const scale_at = mine < BM ? qs + static_cast<long>(min(m0 + mine, rows - 1)) * blocks
+                                          : ws + static_cast<long>(min(n0 + (mine - BM) * kBlock, outputs - 1) / kBlock) * blocks;
+  float ahead[4];
+  auto bring_scales = [&](int step) {
 #pragma unroll
-  for (int t = 0; t < S::kTM; ++t) scale_at[t] = qs + static_cast<long>(min(m0 + (wm * S::kTM + t) * 16 + r16, rows - 1)) * blocks;
-  const float *weight_scale_at = ws + static_cast<long>(min(n0 + wn * S::kTN * 16, outputs - 1) / kBlock) * blocks;
-  float sx[S::kTM], sw;
-  auto scales = [&](int step) {
-    const int b = min(first + step * WK + group, last - 1);
+    for (int i = 0; i < 4; ++i)
+      if (brings_scales) ahead[i] = scale_at[min(first + (step + i) * WK + group, last - 1)];
+  };
+  auto put_scales = [&](int step) {
 #pragma unroll
-    for (int t = 0; t < S::kTM; ++t) sx[t] = scale_at[t][b];
-    sw = weight_scale_at[b];
+    for (int i = 0; i < 4; ++i)
+      if (brings_scales) scale[(step >> 2) & 1][i][group][mine] = ahead[i];
   };
 
-  f32x4 acc[S::kTN][S::kTM] = {};
+  f32x4 acc[S::kTM][S::kTN] = {};
+  bring_scales(0);
   bring(0);
-  scales(0);
+  put_scales(0);
   for (int step = 0; step < steps; ++step) {
     __syncthreads();   // this step's operands are there, and nobody reads the place of the next ones
+    if ((step & 3) == 0) bring_scales(step + 4);
     if (step + 1 < steps) bring(step + 1);
+    if ((step & 3) == 3) put_scales(step + 1);
     if (WK == 1 || first + step * WK + group < last) {
       const unsigned char *xs = lds + ((step & 1) * WK + group) * S::kStage, *wsm = xs + BM * kBlock;
       // piece g and piece g + 4 of the row: any order of k serves, as long as both operands have the same
       const int p0 = (g ^ (r16 & 7)) * 16, p1 = ((g + 4) ^ (r16 & 7)) * 16;
+      const float *const now = scale[(step >> 2) & 1][step & 3][group];
       float s[S::kTM];
 #pragma unroll
-      for (int t = 0; t < S::kTM; ++t) s[t] = sx[t] * sw;
-      i32x8 x[S::kTM];
+      for (int t = 0; t < S::kTM; ++t) s[t] = now[(wm * S::kTM + t) * 16 + r16] * now[BM + wn * S::kTN * 16 / kBlock];
+      auto piece_of = [&](const unsigned char *tile, int row16) {
+        const unsigned char *row = tile + (row16 * 16 + r16) * kBlock;
+        return join(*reinterpret_cast<const i32x4 *>(row + p0), *reinterpret_cast<const i32x4 *>(row + p1));
+      };
+      // The next weights are on their way while these are multiplied, and the last products are added meanwhile.
+      i32x8 x[S::kTM], v = piece_of(wsm, wn * S::kTN);
 #pragma unroll
-      for (int t = 0; t < S::kTM; ++t) {
-        const unsigned char *row = xs + ((wm * S::kTM + t) * 16 + r16) * kBlock;
-        x[t] = join(*reinterpret_cast<const i32x4 *>(row + p0), *reinterpret_cast<const i32x4 *>(row + p1));
-      }
+      for (int t = 0; t < S::kTM; ++t) x[t] = piece_of(xs, wm * S::kTM + t);
+      f32x4 d[2][S::kTM];
 #pragma unroll
-      for (int u = 0; u < S::kTN; ++u) {
-        const unsigned char *row = wsm + ((wn * S::kTN + u) * 16 + r16) * kBlock;
-        const i32x8 v = join(*reinterpret_cast<const i32x4 *>(row + p0), *reinterpret_cast<const i32x4 *>(row + p1));
+      for (int u = 0; u <= S::kTN; ++u) {
+        i32x8 next = v;
+        if (u + 1 < S::kTN) next = piece_of(wsm, wn * S::kTN + u + 1);
+        if (u < S::kTN) {
 #pragma unroll
-        for (int t = 0; t < S::kTM; ++t) {
-          const f32x4 d = block_product(v, x[t]);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) acc[u][t][i] = fmaf(d[i], s[t], acc[u][t][i]);
+          for (int t = 0; t < S::kTM; ++t) d[u & 1][t] = block_product(v, x[t]);
         }
+        if (u) {
+#pragma unroll
+          for (int t = 0; t < S::kTM; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[t][u - 1][i] = fmaf(d[(u - 1) & 1][t][i], s[t], acc[t][u - 1][i]);
+        }
+        v = next;
+        if (u < S::kTN) {
+#pragma unroll
+          for (int t = 0; t < S::kTM; ++t) {
+            __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);   // a matrix instruction
+            if (t == 0) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);   // LDS reads
+            if (u) __builtin_amdgcn_sched_group_barrier(0x2, 4, 0);   // four additions
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
-    scales(step + 1);
   }
   if (WK > 1) {   // the groups' sums, in their order
     f32x4 *const part = reinterpret_cast<f32x4 *>(lds);
@@ -163,23 +209,21 @@ __global__ __launch_bounds__(64 * WM * WN * WK, WM *WN *WK / 4) void product_til
 #pragma unroll
         for (int u = 0; u < S::kTN; ++u)
 #pragma unroll
-          for (int t = 0; t < S::kTM; ++t) part[(u * S::kTM + t) * (64 * WM * WN) + at] = acc[u][t];
+          for (int t = 0; t < S::kTM; ++t) part[(u * S::kTM + t) * (64 * WM * WN) + at] = acc[t][u];
       }
       __syncthreads();
       if (group == 0) {
 #pragma unroll
         for (int u = 0; u < S::kTN; ++u)
 #pragma unroll
-          for (int t = 0; t < S::kTM; ++t) acc[u][t] += part[(u * S::kTM + t) * (64 * WM * WN) + at];
+          for (int t = 0; t < S::kTM; ++t) acc[t][u] += part[(u * S::kTM + t) * (64 * WM * WN) + at];
       }
     }
     if (group) return;
   }
 #pragma unroll
   for (int t = 0; t < S::kTM; ++t) {
-    const int m = m0 + (wm * S::kTM + t) * 16 + r16;
-#pragma unroll
-    for (int u = 0; u < S::kTN; ++u) store4(to, split, m, n0 + (wn * S::kTN + u) * 16 + 4 * g, acc[u][t]);
+    store_row(to, split, m0 + (wm * S::kTM + t) * 16 + r16, n0 + wn * S::kTN * 16 + 4 * g, acc[t]);
   }
 }
 
@@ -226,7 +270,7 @@ __global__ __launch_bounds__(256) void product_rows(const unsigned char *q, cons
 #pragma unroll
     for (int t = 0; t < TM; ++t) s[t] = sx_at[t][b] * sw_at[b];
   };
-  f32x4 acc[TN][TM] = {};
+  f32x4 acc[TM][TN] = {};
   if (first + wave < last) bring(first + wave);
   for (int b = first + wave; b < last; b += 4) {
     i32x8 x1[TM], v1[TN];
@@ -242,14 +286,14 @@ __global__ __launch_bounds__(256) void product_rows(const unsigned char *q, cons
       for (int t = 0; t < TM; ++t) {
         const f32x4 d = block_product(v1[u], x1[t]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[u][t][i] = fmaf(d[i], s1[t], acc[u][t][i]);
+        for (int i = 0; i < 4; ++i) acc[t][u][i] = fmaf(d[i], s1[t], acc[t][u][i]);
       }
   }
   if (wave) {
 #pragma unroll
     for (int u = 0; u < TN; ++u)
 #pragma unroll
-      for (int t = 0; t < TM; ++t) part[wave - 1][u * TM + t][lane] = acc[u][t];
+      for (int t = 0; t < TM; ++t) part[wave - 1][u * TM + t][lane] = acc[t][u];
   }
   __syncthreads();
   if (wave) return;
@@ -258,9 +302,10 @@ __global__ __launch_bounds__(256) void product_rows(const unsigned char *q, cons
 #pragma unroll
     for (int t = 0; t < TM; ++t) {
 #pragma unroll
-      for (int i = 0; i < 3; ++i) acc[u][t] += part[i][u * TM + t][lane];
-      store4(to, split, m0 + t * 16 + r16, n0 + u * 16 + 4 * g, acc[u][t]);
+      for (int i = 0; i < 3; ++i) acc[t][u] += part[i][u * TM + t][lane];
     }
+#pragma unroll
+  for (int t = 0; t < TM; ++t) store_row(to, split, m0 + t * 16 + r16, n0 + 4 * g, acc[t]);
 }
 
 // The parts' sum, in their order
