@@ -31,18 +31,6 @@ template <typename T> struct Results {
   int outputs;
 };
 
-// Two neighbouring values of 16 bits
-template <typename T> __device__ __forceinline__ unsigned pack2(float a, float b);
-template <> __device__ __forceinline__ unsigned pack2<__half>(float a, float b) {
-  typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-  return __builtin_bit_cast(unsigned, h2{static_cast<_Float16>(a), static_cast<_Float16>(b)});
-}
-template <> __device__ __forceinline__ unsigned pack2<__hip_bfloat16>(float a, float b) {
-  typedef float f2 __attribute__((ext_vector_type(2)));
-  typedef __bf16 b2 __attribute__((ext_vector_type(2)));
-  return __builtin_bit_cast(unsigned, __builtin_convertvector(f2{a, b}, b2));
-}
-
 // Results of TN tiles along row m, four neighbours of every 16 from n on
 template <typename T, int TN> __device__ __forceinline__ void store_row(const Results<T> &to, int split, long m, int n, const f32x4 (&v)[TN]) {
   if (m >= to.rows) return;

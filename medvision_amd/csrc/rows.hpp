@@ -15,14 +15,9 @@ template <typename V, int A> struct __attribute__((packed, aligned(A))) Loose { 
 template <typename T> struct Bits;   // element <-> float on raw bits
 template <> struct Bits<__half> {
   static __device__ __forceinline__ float up(unsigned short b) { return __half2float(__ushort_as_half(b)); }
-  static __device__ __forceinline__ unsigned short down(float v) { return __half_as_ushort(__float2half_rn(v)); }
 };
 template <> struct Bits<__hip_bfloat16> {
   static __device__ __forceinline__ float up(unsigned short b) { return __uint_as_float(static_cast<unsigned>(b) << 16); }
-  static __device__ __forceinline__ unsigned short down(float v) {
-    const __bf16 b = static_cast<__bf16>(v);   // to nearest even, NaN stays NaN
-    return __builtin_bit_cast(unsigned short, b);
-  }
 };
 
 // out[0..7] = p[0..7], zeros from `left` on
@@ -53,11 +48,23 @@ template <> __device__ __forceinline__ void load8<float>(const float *p, int lef
   for (int i = 0; i < 8; ++i) out[i] = i < left ? p[i] : 0.f;
 }
 
+// Two neighbouring values of 16 bits
+template <typename T> __device__ __forceinline__ unsigned pack2(float a, float b);
+template <> __device__ __forceinline__ unsigned pack2<__half>(float a, float b) {
+  typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(unsigned, h2{static_cast<_Float16>(a), static_cast<_Float16>(b)});
+}
+template <> __device__ __forceinline__ unsigned pack2<__hip_bfloat16>(float a, float b) {
+  typedef float f2 __attribute__((ext_vector_type(2)));
+  typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(unsigned, __builtin_convertvector(f2{a, b}, b2));
+}
+
 template <typename T> __device__ __forceinline__ void store8(T *p, int left, const float (&v)[8]) {
   if (left >= 8) {
     u32x4 r;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) r[i] = Bits<T>::down(v[2 * i]) | (static_cast<unsigned>(Bits<T>::down(v[2 * i + 1])) << 16);
+    for (int i = 0; i < 4; ++i) r[i] = pack2<T>(v[2 * i], v[2 * i + 1]);
     reinterpret_cast<Loose<u32x4, 2> *>(p)->v = r;
     return;
   }
