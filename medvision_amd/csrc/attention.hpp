@@ -27,6 +27,12 @@ struct AttentionArgs {
   __device__ __forceinline__ float factor() const { return fabsf(scale) * kLog2e; }
 };
 
+// Rows of a head of keys: the queries of all heads that share it, one after the other.
+struct RowOf {
+  int head, query;
+  __device__ __forceinline__ RowOf(const AttentionArgs &a, int g, int row) : head(g * (a.heads / a.key_heads) + row / a.queries), query(row % a.queries) {}
+};
+
 // ---- products of 32 x 32 ---------------------------------------------------------------------------------
 // Row r of a result: lane % 32 is its column, register i holds row 8 (i / 4) + 4 (lane / 32) + i % 4.
 __device__ __forceinline__ constexpr int result_row(int i, int half) { return 8 * (i / 4) + 4 * half + i % 4; }
@@ -120,6 +126,22 @@ template <typename T, int DP> struct Column {
       if (use && d < dim) r[n] = load_piece<T>(row, d, dim);
     }
   }
+  __device__ __forceinline__ float dot(const Column &with) const {
+    float sum = 0.f;
+#pragma unroll
+    for (int n = 0; n < kCount; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const unsigned x = r[n][i], y = with.r[n][i];
+        if constexpr (sizeof(T) == 4) {
+          sum = fmaf(__uint_as_float(x), __uint_as_float(y), sum);
+        } else {
+          sum = fmaf(Bits<T>::up(static_cast<unsigned short>(x & 0xffffu)), Bits<T>::up(static_cast<unsigned short>(y & 0xffffu)), sum);
+          sum = fmaf(Bits<T>::up(static_cast<unsigned short>(x >> 16)), Bits<T>::up(static_cast<unsigned short>(y >> 16)), sum);
+        }
+      }
+    return sum;
+  }
   __device__ __forceinline__ void negate() {
 #pragma unroll
     for (int n = 0; n < kCount; ++n) r[n] ^= sizeof(T) == 2 ? 0x80008000u : 0x80000000u;
@@ -208,6 +230,25 @@ template <typename T> __device__ __forceinline__ void store_quad(T *row, int d, 
     for (int i = 0; i < 3; ++i)
       if (d + i < dim) row[d + i] = store_cast<T>(v[i]);
   }
+}
+
+inline int attention_sizes(const mv_attention_shape *s, int dtype) {
+  MV_REQUIRE(s, "the shape is missing");
+  MV_REQUIRE(dtype == MV_F32 || dtype == MV_F16 || dtype == MV_BF16, "dtype %d is not float32, float16 or bfloat16", dtype);
+  MV_REQUIRE(s->batch >= 0 && s->queries >= 0 && s->keys >= 0, "wrong sizes: batch %d, %d queries, %d keys", s->batch, s->queries, s->keys);
+  MV_REQUIRE(s->key_heads > 0 && s->heads > 0 && s->heads % s->key_heads == 0, "%d heads cannot share %d heads of keys", s->heads, s->key_heads);
+  // (workgroups and rows of a head of keys are counted in 32 bits)
+  const long most = (1L << 31) - 256, heads = static_cast<long>(s->batch) * s->key_heads, rows = static_cast<long>(s->heads / s->key_heads) * s->queries;
+  MV_REQUIRE(rows < most && s->keys < most && heads * (rows / 128 + 1) < most && heads * (s->keys / 128 + 1) < most, "too many heads, queries or keys");
+  MV_REQUIRE(s->dim > 0 && s->dim <= kMostDim, "heads of %d channels: 1 to %d are possible", s->dim, kMostDim);
+  return MV_OK;
+}
+
+inline AttentionArgs attention_arguments(const mv_attention_shape *s, const void *q, const void *k, const void *v, const void *mask, const void *lengths, float scale) {
+  AttentionArgs a{q, k, v, static_cast<const unsigned char *>(mask), static_cast<const int *>(lengths), s->batch, s->queries, s->keys,
+                  s->heads, s->key_heads, s->dim, {}, {}, {}, static_cast<long>(s->mask_stride), scale};
+  for (int i = 0; i < 3; ++i) a.qs[i] = s->q_strides[i], a.ks[i] = s->k_strides[i], a.vs[i] = s->v_strides[i];
+  return a;
 }
 
 }  // namespace mv

@@ -1,0 +1,361 @@
+// Gradients of cross attention.
+//
+//   p_ij = 2^(factor q_i.k_j - L_i)   d_i = do_i.o_i   ds_ij = p_ij (do_i.v_j - d_i)
+//   dq_i = scale sum_j ds_ij k_j   dk_j = scale sum_i ds_ij q_i   dv_j = sum_i p_ij do_i
+//
+// Two kernels form the weights anew, one with a query per lane for dq, one with a key per lane for dk and dv: no atomics,
+// the same results every time.  Long sums with few results are split, and the parts added in their order.
+#include "attention.hpp"
+
+#include <algorithm>
+
+namespace mv {
+namespace {
+
+// float16 has no bits below 2^-24: gradients of weights, which may be far below one, are brought to at most 2^15 by a power
+// of two of their own for each column, which follows the largest so far as a softmax's maximum does.
+template <typename T> struct Raise {
+  static constexpr bool kOn = __is_same(T, __half);
+  float by = 0.f;   // 0: nothing but zeros yet
+  // of 16 values: scales them, and the sums if the power changes
+  template <int N> __device__ __forceinline__ void scale(float (&v)[16], f32x16 (&sum)[N]) {
+    if constexpr (kOn) {
+      float top = 0.f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) top = fmaxf(top, fabsf(v[i]));
+      top = fmaxf(top, other_half(top));
+      if (__ballot(by == 0.f ? top > 0.f : top * by > 32768.f)) {
+        float next = by;
+        if (by == 0.f ? top > 0.f : top * by > 32768.f)   // to 32 .. 64: room for nine more powers
+          next = top < INFINITY ? __builtin_amdgcn_ldexpf(1.f, max(-100, min(100, 6 - __builtin_amdgcn_frexp_expf(top)))) : 1.f;
+        const float keep = by == 0.f ? 1.f : next / by;
+#pragma unroll
+        for (int u = 0; u < N; ++u) sum[u] *= keep;
+        by = next;
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[i] *= by;
+    }
+  }
+  __device__ __forceinline__ float back() const { return kOn && by != 0.f ? 1.f / by : 1.f; }
+};
+
+template <int N> __device__ __forceinline__ void put_sums(const f32x16 (&o)[N], f32x4 *to, int lane) {
+#pragma unroll
+  for (int u = 0; u < N; ++u)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) to[(u * 4 + i) * 64 + lane] = f32x4{o[u][4 * i], o[u][4 * i + 1], o[u][4 * i + 2], o[u][4 * i + 3]};
+}
+template <int N> __device__ __forceinline__ void add_sums(f32x16 (&o)[N], const f32x4 *from, int lane) {
+#pragma unroll
+  for (int u = 0; u < N; ++u)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const f32x4 r = from[(u * 4 + i) * 64 + lane];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[u][4 * i + e] += r[e];
+    }
+}
+// One column of the sums, as a row of `dim` elements
+template <typename O, int N> __device__ __forceinline__ void store_column(O *row, const f32x16 (&o)[N], int dim, int half) {
+#pragma unroll
+  for (int u = 0; u < N; ++u)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) store_quad(row, 32 * u + 8 * i + 4 * half, dim, o[u][4 * i], o[u][4 * i + 1], o[u][4 * i + 2], o[u][4 * i + 3]);
+}
+
+// ---- dq -------------------------------------------------------------------------------------------------------
+// As the forward kernel; leaves d_i for the next one.
+template <typename T, int DP, int WQ>
+__global__ __launch_bounds__(256, DP == 128 || (sizeof(T) == 4 && DP == 64) ? 1 : 2) void attend_grad_query(
+    AttentionArgs a, const T *out, const float *lse, const T *go, T *gq, float *delta, float *part, int row_tiles, int splits) {
+  constexpr int kTiles = WQ == 4 ? 2 : 1, kKeys = WQ == 4 ? 64 : 128, kOut = DP / 32;
+  using L = Tile<T, DP, kKeys>;
+  __shared__ L tiles[2];
+  L &ks = tiles[0], &vs = tiles[1];
+  const int groups = row_tiles * splits * a.batch * a.key_heads;
+  unsigned id = linear_block();
+  if (id >= static_cast<unsigned>(groups)) return;
+  id = xcd_contiguous(id, groups);
+  const int tile = id % row_tiles, split = id / row_tiles % splits, g = id / row_tiles / splits % a.key_heads, b = id / row_tiles / splits / a.key_heads;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
+  const int rows = a.heads / a.key_heads * a.queries, row = tile * 32 * WQ + (WQ == 4 ? wave * 32 : 0) + (lane & 31);
+  const bool live = row < rows;
+  const RowOf at(a, g, live ? row : rows - 1);
+  const long at_row = (static_cast<long>(b) * a.queries + at.query) * a.heads + at.head,
+             at_l = (static_cast<long>(b) * a.heads + at.head) * a.queries + at.query;
+  const float factor = a.factor();
+
+  Column<T, DP> q, d_o;
+  float d_i;
+  {
+    Column<T, DP> o;
+    d_o.load(go + at_row * a.dim, live, a.dim, half);
+    o.load(out + at_row * a.dim, live, a.dim, half);
+    d_i = d_o.dot(o);
+    d_i += other_half(d_i);
+  }
+  q.load(static_cast<const T *>(a.q) + b * a.qs[0] + at.query * a.qs[1] + at.head * a.qs[2], live, a.dim, half);
+  if (a.scale < 0.f) q.negate();
+  float sums_log = live ? lse[at_l] : INFINITY;
+  if (sums_log == -INFINITY) sums_log = INFINITY;   // no key counts: weights of zero
+  if (live && split == 0 && half == 0 && (WQ == 4 || wave == 0)) delta[at_l] = d_i;
+
+  const T *const k = static_cast<const T *>(a.k) + b * a.ks[0] + g * a.ks[2], *const v = static_cast<const T *>(a.v) + b * a.vs[0] + g * a.vs[2];
+  const int length = a.length(b), all_tiles = (length + kKeys - 1) / kKeys;
+  const int first = static_cast<int>(static_cast<long>(all_tiles) * split / splits), last = static_cast<int>(static_cast<long>(all_tiles) * (split + 1) / splits);
+  const int my_key = WQ == 4 ? 0 : 32 * wave;
+  Carry<T, DP, kKeys, 256> next_k, next_v;
+  unsigned long long next_use = 0;
+  auto load = [&](int t) {
+    const auto use = [&](int j) { return a.counts(b, j); };
+    next_k.load(threadIdx.x, t * kKeys, length, a.dim, [&](int j) { return k + j * a.ks[1]; }, use);
+    next_v.load(threadIdx.x, t * kKeys, length, a.dim, [&](int j) { return v + j * a.vs[1]; }, use);
+    const int j = t * kKeys + my_key + lane;
+    next_use = __ballot(j < length && (WQ == 4 || lane < 32) && a.counts(b, min(j, length - 1)));
+  };
+
+  f32x16 sum[kOut] = {};
+  Raise<T> raise;
+  if (first < last) load(first);
+  for (int t = first; t < last; ++t) {
+    if (t > first) __syncthreads();
+    next_k.put(threadIdx.x, ks);
+    next_v.put(threadIdx.x, vs);
+    const unsigned long long use = next_use;
+    __syncthreads();
+    if (t + 1 < last) load(t + 1);
+    if (!use) continue;
+#pragma unroll
+    for (int n = 0; n < kTiles; ++n) {
+      const f32x16 s = times(ks, my_key + 32 * n, q, lane), dp = times(vs, my_key + 32 * n, d_o, lane);
+      float ds[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) ds[i] = __builtin_amdgcn_exp2f(fmaf(s[i], factor, -sums_log)) * (dp[i] - d_i);
+      const unsigned word = static_cast<unsigned>(use >> (32 * n));
+      if (word != ~0u) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) ds[i] = word >> (4 * half) >> result_row(i, 0) & 1 ? ds[i] : 0.f;
+      }
+      raise.scale(ds, sum);
+      add_transposed(ks, my_key + 32 * n, ds, sum, lane);
+    }
+  }
+  const float back = raise.back() * a.scale;
+#pragma unroll
+  for (int u = 0; u < kOut; ++u) sum[u] *= back;
+
+  if constexpr (WQ == 1) {
+    __syncthreads();
+    f32x4 *const sums = reinterpret_cast<f32x4 *>(tiles);
+    static_assert(sizeof(tiles) >= 3 * kOut * 4 * 64 * sizeof(f32x4), "");
+    if (wave) put_sums(sum, sums + (wave - 1) * kOut * 4 * 64, lane);
+    __syncthreads();
+    if (wave) return;
+#pragma unroll
+    for (int w = 0; w < 3; ++w) add_sums(sum, sums + w * kOut * 4 * 64, lane);
+  }
+  if (!live) return;
+  if (splits > 1) store_column(part + (static_cast<long>(split) * a.batch * a.queries * a.heads + at_row) * a.dim, sum, a.dim, half);
+  else store_column(gq + at_row * a.dim, sum, a.dim, half);
+}
+
+// ---- dk, dv -----------------------------------------------------------------------------------------------------
+// A key per lane; rows of queries and of output gradients go through LDS.  WK = 4: 32 keys for each wavefront, the same 32
+// rows; WK = 1 (few keys): the same 32 keys, each wavefront 32 of 128 rows, joined at the end.  A key that does not count
+// spoils nothing but its own column, which is written as zeros.
+template <typename T, int DP, int WK>
+__global__ __launch_bounds__(256, DP == 128 || (sizeof(T) == 4 && DP == 64) ? 1 : 2) void attend_grad_key(
+    AttentionArgs a, const float *lse, const float *delta, const T *go, T *gk, T *gv, float *part, int key_tiles, int splits) {
+  constexpr int kRows = WK == 4 ? 32 : 128, kOut = DP / 32;
+  constexpr float kShift = __is_same(T, __half) ? 15.f : 0.f;   // as in the forward pass
+  using L = Tile<T, DP, kRows>;
+  __shared__ L tiles[2];
+  __shared__ float stats[2][kRows];
+  L &qs = tiles[0], &os = tiles[1];
+  const int groups = key_tiles * splits * a.batch * a.key_heads;
+  unsigned id = linear_block();
+  if (id >= static_cast<unsigned>(groups)) return;
+  id = xcd_contiguous(id, groups);
+  const int tile = id % key_tiles, split = id / key_tiles % splits, g = id / key_tiles / splits % a.key_heads, b = id / key_tiles / splits / a.key_heads;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
+  const int j = tile * 32 * WK + (WK == 4 ? wave * 32 : 0) + (lane & 31), length = a.length(b);
+  const bool live = j < a.keys, use = j < length && a.counts(b, j);
+  const float factor = a.factor();
+  Column<T, DP> k, v;
+  k.load(static_cast<const T *>(a.k) + b * a.ks[0] + j * a.ks[1] + g * a.ks[2], use, a.dim, half);
+  v.load(static_cast<const T *>(a.v) + b * a.vs[0] + j * a.vs[1] + g * a.vs[2], use, a.dim, half);
+  if (a.scale < 0.f) k.negate();
+
+  const int rows = a.heads / a.key_heads * a.queries;
+  // (nothing to sum where none of the workgroup's keys counts by its length)
+  const int all_tiles = tile * 32 * WK < length ? (rows + kRows - 1) / kRows : 0;
+  const int first = static_cast<int>(static_cast<long>(all_tiles) * split / splits), last = static_cast<int>(static_cast<long>(all_tiles) * (split + 1) / splits);
+  const int my_row = WK == 4 ? 0 : 32 * wave;
+  Carry<T, DP, kRows, 256> next_q, next_o;
+  float next_l = INFINITY, next_d = 0.f;
+  auto load = [&](int t) {
+    const auto all = [](int) { return true; };
+    next_q.load(threadIdx.x, t * kRows, rows, a.dim, [&](int r) {
+      const RowOf at(a, g, r);
+      return static_cast<const T *>(a.q) + b * a.qs[0] + at.query * a.qs[1] + at.head * a.qs[2]; }, all);
+    next_o.load(threadIdx.x, t * kRows, rows, a.dim, [&](int r) {
+      const RowOf at(a, g, r);
+      return go + ((static_cast<long>(b) * a.queries + at.query) * a.heads + at.head) * a.dim; }, all);
+    const int r = t * kRows + threadIdx.x;
+    next_l = INFINITY, next_d = 0.f;
+    if (threadIdx.x < kRows && r < rows) {
+      const RowOf at(a, g, r);
+      const long from = (static_cast<long>(b) * a.heads + at.head) * a.queries + at.query;
+      next_l = lse[from], next_d = delta[from];
+      next_l = next_l == -INFINITY ? INFINITY : next_l - kShift;
+    }
+  };
+
+  f32x16 dk[kOut] = {}, dv[kOut] = {};
+  Raise<T> raise;
+  if (first < last) load(first);
+  for (int t = first; t < last; ++t) {
+    if (t > first) __syncthreads();
+    next_q.put(threadIdx.x, qs);
+    next_o.put(threadIdx.x, os);
+    if (threadIdx.x < kRows) stats[0][threadIdx.x] = next_l, stats[1][threadIdx.x] = next_d;
+    __syncthreads();
+    if (t + 1 < last) load(t + 1);
+    const f32x16 s = times(qs, my_row, k, lane), dp = times(os, my_row, v, lane);
+    float p[16], ds[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int r = my_row + result_row(i, 0) + 4 * half;
+      p[i] = __builtin_amdgcn_exp2f(fmaf(s[i], factor, -stats[0][r]));
+      ds[i] = p[i] * (dp[i] - stats[1][r]);
+    }
+    add_transposed(os, my_row, p, dv, lane);
+    raise.scale(ds, dk);
+    add_transposed(qs, my_row, ds, dk, lane);
+  }
+  const float down = kShift ? 1.f / 32768.f : 1.f, back = raise.back() * (a.scale * down);
+#pragma unroll
+  for (int u = 0; u < kOut; ++u) dk[u] *= back, dv[u] *= down;
+
+  if constexpr (WK == 1) {
+    f32x4 *const sums = reinterpret_cast<f32x4 *>(tiles);
+    static_assert(sizeof(tiles) >= 3 * kOut * 4 * 64 * sizeof(f32x4), "");
+    __syncthreads();
+    if (wave) put_sums(dk, sums + (wave - 1) * kOut * 4 * 64, lane);
+    __syncthreads();
+    if (!wave)
+#pragma unroll
+      for (int w = 0; w < 3; ++w) add_sums(dk, sums + w * kOut * 4 * 64, lane);
+    __syncthreads();
+    if (wave) put_sums(dv, sums + (wave - 1) * kOut * 4 * 64, lane);
+    __syncthreads();
+    if (wave) return;
+#pragma unroll
+    for (int w = 0; w < 3; ++w) add_sums(dv, sums + w * kOut * 4 * 64, lane);
+  }
+  if (!live) return;
+  if (!use) {
+#pragma unroll
+    for (int u = 0; u < kOut; ++u) dk[u] = 0.f, dv[u] = 0.f;
+  }
+  const long at_row = (static_cast<long>(b) * a.keys + j) * a.key_heads + g, all = static_cast<long>(a.batch) * a.keys * a.key_heads;
+  if (splits > 1) {
+    store_column(part + (split * all + at_row) * a.dim, dk, a.dim, half);
+    store_column(part + ((splits + split) * all + at_row) * a.dim, dv, a.dim, half);
+  } else {
+    store_column(gk + at_row * a.dim, dk, a.dim, half);
+    store_column(gv + at_row * a.dim, dv, a.dim, half);
+  }
+}
+
+// Sums of the splits, in their order
+template <typename T>
+__global__ __launch_bounds__(256) void add_splits(const float *part, T *out, long count, int splits) {
+  const long at = static_cast<long>(linear_block()) * 256 + threadIdx.x;
+  if (at >= count) return;
+  float sum = 0.f;
+  for (int s = 0; s < splits; ++s) sum += part[s * count + at];
+  out[at] = store_cast<T>(sum);
+}
+
+struct BackwardPlan {
+  bool few_rows, few_keys;
+  int row_tiles, query_splits, key_tiles, key_splits;
+};
+
+BackwardPlan backward_plan(const mv_attention_shape *s) {
+  BackwardPlan p;
+  const long rows = static_cast<long>(s->heads / s->key_heads) * s->queries, heads = std::max(1L, static_cast<long>(s->batch) * s->key_heads);
+  p.few_rows = rows <= 32;
+  p.few_keys = s->keys <= 32;
+  p.row_tiles = static_cast<int>(p.few_rows ? 1 : (rows + 127) / 128);
+  p.key_tiles = static_cast<int>(p.few_keys ? 1 : (s->keys + 127L) / 128);
+  const long key_steps = p.few_rows ? (s->keys + 127L) / 128 : (s->keys + 63L) / 64, row_steps = p.few_keys ? (rows + 127) / 128 : (rows + 31) / 32;
+  p.query_splits = static_cast<int>(std::max(1L, std::min(512 / std::max(1L, p.row_tiles * heads), key_steps / 4)));
+  p.key_splits = static_cast<int>(std::max(1L, std::min(512 / std::max(1L, p.key_tiles * heads), row_steps / 4)));
+  return p;
+}
+
+template <typename T, int DP>
+void launch_backward(const BackwardPlan &p, const AttentionArgs &a, const void *out, const float *lse, const void *go, void *gq, void *gk, void *gv,
+                     float *delta, float *part, hipStream_t s) {
+  const long heads = static_cast<long>(a.batch) * a.key_heads, queries = static_cast<long>(a.batch) * a.queries * a.heads * a.dim,
+             keys = heads * a.keys * a.dim;
+  const T *const o = static_cast<const T *>(out), *const d_o = static_cast<const T *>(go);
+  if (queries) {
+    const dim3 grid = linear_grid(heads * p.row_tiles * p.query_splits, 256);
+    if (p.few_rows) attend_grad_query<T, DP, 1><<<grid, 256, 0, s>>>(a, o, lse, d_o, static_cast<T *>(gq), delta, part, p.row_tiles, p.query_splits);
+    else attend_grad_query<T, DP, 4><<<grid, 256, 0, s>>>(a, o, lse, d_o, static_cast<T *>(gq), delta, part, p.row_tiles, p.query_splits);
+    if (p.query_splits > 1) add_splits<T><<<linear_grid((queries + 255) / 256, 256), 256, 0, s>>>(part, static_cast<T *>(gq), queries, p.query_splits);
+  }
+  if (keys) {
+    const dim3 grid = linear_grid(heads * p.key_tiles * p.key_splits, 256);
+    if (p.few_keys) attend_grad_key<T, DP, 1><<<grid, 256, 0, s>>>(a, lse, delta, d_o, static_cast<T *>(gk), static_cast<T *>(gv), part, p.key_tiles, p.key_splits);
+    else attend_grad_key<T, DP, 4><<<grid, 256, 0, s>>>(a, lse, delta, d_o, static_cast<T *>(gk), static_cast<T *>(gv), part, p.key_tiles, p.key_splits);
+    if (p.key_splits > 1) {
+      const dim3 sums = linear_grid((keys + 255) / 256, 256);
+      add_splits<T><<<sums, 256, 0, s>>>(part, static_cast<T *>(gk), keys, p.key_splits);
+      add_splits<T><<<sums, 256, 0, s>>>(part + p.key_splits * keys, static_cast<T *>(gv), keys, p.key_splits);
+    }
+  }
+}
+
+}  // namespace
+}  // namespace mv
+
+using namespace mv;
+
+extern "C" {
+
+size_t mv_cross_attention_backward_workspace_bytes(const mv_attention_shape *s, int dtype) {
+  if (attention_sizes(s, dtype)) return 0;
+  const BackwardPlan p = backward_plan(s);
+  const size_t queries = static_cast<size_t>(s->batch) * s->queries * s->heads, keys = static_cast<size_t>(s->batch) * s->keys * s->key_heads;
+  const size_t for_queries = p.query_splits > 1 ? p.query_splits * queries * s->dim : 0, for_keys = p.key_splits > 1 ? 2 * p.key_splits * keys * s->dim : 0;
+  return sizeof(float) * (queries + std::max(for_queries, for_keys));
+}
+
+int mv_cross_attention_backward(const void *query, const void *key, const void *value, const void *key_mask,
+                                const void *key_lengths, const void *output, const void *lse, const void *grad_output,
+                                void *grad_query, void *grad_key, void *grad_value, const mv_attention_shape *shape,
+                                float scale, int dtype, void *workspace, size_t workspace_bytes, void *stream) {
+  if (const int status = attention_sizes(shape, dtype)) return status;
+  const AttentionArgs a = attention_arguments(shape, query, key, value, key_mask, key_lengths, scale);
+  const long rows = static_cast<long>(a.batch) * a.queries * a.heads, columns = static_cast<long>(a.batch) * a.keys * a.key_heads;
+  MV_REQUIRE(rows == 0 || (query && output && lse && grad_output && grad_query), "a tensor is missing");
+  MV_REQUIRE(columns == 0 || (key && value && grad_key && grad_value), "a tensor is missing");
+  MV_REQUIRE(rows == 0 || (workspace && workspace_bytes >= mv_cross_attention_backward_workspace_bytes(shape, dtype)), "the workspace is too small");
+  const BackwardPlan p = backward_plan(shape);
+  float *const delta = static_cast<float *>(workspace), *const part = delta + rows;
+  const float *const sums = static_cast<const float *>(lse);
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  MV_FLOATS(dtype, {
+    if (a.dim <= 32) launch_backward<T, 32>(p, a, output, sums, grad_output, grad_query, grad_key, grad_value, delta, part, s);
+    else if (a.dim <= 64) launch_backward<T, 64>(p, a, output, sums, grad_output, grad_query, grad_key, grad_value, delta, part, s);
+    else launch_backward<T, 128>(p, a, output, sums, grad_output, grad_query, grad_key, grad_value, delta, part, s);
+  })
+  return check_launch("cross_attention backward");
+}
+
+}  // extern "C"

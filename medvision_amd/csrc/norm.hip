@@ -228,14 +228,6 @@ __global__ __launch_bounds__(kThreads) void quantize_tiles(const T *x, unsigned 
   if (threadIdx.x == 0) scales[tile] = s;
 }
 
-#define MV_FLOATS(dtype, ...)                                                                                    \
-  switch (dtype) {                                                                                               \
-    case MV_F32: { using T = float; __VA_ARGS__; break; }                                                        \
-    case MV_F16: { using T = __half; __VA_ARGS__; break; }                                                       \
-    case MV_BF16: { using T = __hip_bfloat16; __VA_ARGS__; break; }                                              \
-    default: return ::mv::fail(MV_INVALID_ARGUMENT, "dtype %d is not float32, float16 or bfloat16", (int)(dtype)); \
-  }
-
 int norm_arguments(long rows, int columns, int dtype, int weight_dtype) {
   MV_REQUIRE(dtype == MV_F32 || dtype == MV_F16 || dtype == MV_BF16, "dtype %d is not float32, float16 or bfloat16", dtype);
   MV_REQUIRE(weight_dtype == dtype || weight_dtype == MV_F32, "weight has dtype %d, expected %d or float32", weight_dtype, dtype);

@@ -112,4 +112,13 @@ __device__ __forceinline__ u32x2 to_e4m3(const float (&v)[8]) {
   return r;
 }
 
+// The storage types of the operators on rows
+#define MV_FLOATS(dtype, ...)                                                                                    \
+  switch (dtype) {                                                                                               \
+    case MV_F32: { using T = float; __VA_ARGS__; break; }                                                        \
+    case MV_F16: { using T = __half; __VA_ARGS__; break; }                                                       \
+    case MV_BF16: { using T = __hip_bfloat16; __VA_ARGS__; break; }                                              \
+    default: return ::mv::fail(MV_INVALID_ARGUMENT, "dtype %d is not float32, float16 or bfloat16", (int)(dtype)); \
+  }
+
 }  // namespace mv
