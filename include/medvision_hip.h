@@ -312,8 +312,9 @@ int mv_deform_conv_2d(const void *input, const void *offset, const void *weight,
  * key_mask[b * mask_stride + j] != 0 (bytes, NULL: all).  What the other keys and values hold is of no effect, not even
  * NaN.  A query without any key gets zeros, and gives none a gradient.
  * output [batch, queries, heads, dim] and the gradients are dense; lse [batch, heads, queries] float32 (NULL: not wanted by
- * the forward pass) holds log2 of the sum of 2^(log2(e) scale q.k), -inf where no key counts.  The backward pass WRITES its
- * gradients; it wants the workspace, the forward pass splits long rows of keys only if it gets its own. */
+ * the forward pass) holds log2 of the sum of 2^(log2(e) scale q.k), -inf where no key counts; output_low, like output, what its rounding took
+ * away, for the backward pass of 16-bit types (NULL: not wanted; gradients are then off by up to twice the type's
+ * rounding).  The backward pass WRITES its gradients; it wants the workspace, the forward pass splits long rows of keys only if it gets its own. */
 typedef struct {
   int batch, queries, keys, heads, key_heads, dim;
   int64_t q_strides[3], k_strides[3], v_strides[3]; /* batch, row, head */
@@ -322,10 +323,11 @@ typedef struct {
 size_t mv_cross_attention_forward_workspace_bytes(const mv_attention_shape *shape, int dtype);
 size_t mv_cross_attention_backward_workspace_bytes(const mv_attention_shape *shape, int dtype);
 int mv_cross_attention_forward(const void *query, const void *key, const void *value, const void *key_mask,
-                               const void *key_lengths, void *output, void *lse, const mv_attention_shape *shape,
+                               const void *key_lengths, void *output, void *output_low, void *lse, const mv_attention_shape *shape,
                                float scale, int dtype, void *workspace, size_t workspace_bytes, void *stream);
 int mv_cross_attention_backward(const void *query, const void *key, const void *value, const void *key_mask,
-                                const void *key_lengths, const void *output, const void *lse, const void *grad_output,
+                                const void *key_lengths, const void *output, const void *output_low,
+                                const void *lse, const void *grad_output,
                                 void *grad_query, void *grad_key, void *grad_value, const mv_attention_shape *shape,
                                 float scale, int dtype, void *workspace, size_t workspace_bytes, void *stream);
 

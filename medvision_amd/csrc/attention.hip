@@ -16,8 +16,8 @@ namespace {
 // row are those of a lane and of its other half, and the weights are the second product's operand as they stand.
 // float16: weights are 2^15 times as large (at most 32768), which keeps those below 2^-14 of the largest from losing bits.
 template <typename T, int DP, int WQ>
-__global__ __launch_bounds__(256, sizeof(T) == 4 ? (DP == 128 ? 1 : 2) : DP == 128 ? 2 : DP == 64 ? 3 : 4) void attend_kernel(AttentionArgs a, T *out, float *lse, float *part,
-                                                                                int row_tiles, int splits) {
+__global__ __launch_bounds__(256, sizeof(T) == 4 ? (DP == 128 ? 1 : 2) : DP == 128 ? 2 : DP == 64 ? 3 : 4) void attend_kernel(
+    AttentionArgs a, T *out, T *low, float *lse, float *part, int row_tiles, int splits) {
   constexpr int kTiles = WQ == 4 ? 2 : 1, kKeys = WQ == 4 ? 64 : 128, kOut = DP / 32;
   constexpr float kShift = sizeof(T) == 2 && __is_same(T, __half) ? 15.f : 0.f;
   using L = Tile<T, DP, kKeys>;
@@ -94,7 +94,11 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? (DP == 128 ? 1 : 2) : DP == 1
     for (int n = 0; n < kTiles; ++n) {
       float p[16];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) l += p[i] = __builtin_amdgcn_exp2f(fmaf(s[n][i], factor, shift));
+      for (int i = 0; i < 16; ++i) {
+        // (float32: the difference first, so that the largest weight is one to the last bit)
+        const float x = sizeof(T) == 4 ? (s[n][i] - base) * factor : fmaf(s[n][i], factor, shift);
+        l += p[i] = __builtin_amdgcn_exp2f(x);
+      }
       add_transposed(vs, my_key + 32 * n, p, o, lane);
     }
   }
@@ -155,16 +159,21 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? (DP == 128 ? 1 : 2) : DP == 1
 #pragma unroll
   for (int u = 0; u < kOut; ++u)
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      store_quad(out + at_row * a.dim, 32 * u + 8 * i + 4 * half, a.dim, o[u][4 * i] * inverse, o[u][4 * i + 1] * inverse, o[u][4 * i + 2] * inverse,
-                 o[u][4 * i + 3] * inverse);
+    for (int i = 0; i < 4; ++i) {
+      const int d = 32 * u + 8 * i + 4 * half;
+      float r[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) r[e] = o[u][4 * i + e] * inverse;
+      store_quad(out + at_row * a.dim, d, a.dim, r[0], r[1], r[2], r[3]);
+      if (low) store_quad(low + at_row * a.dim, d, a.dim, rest_of<T>(r[0]), rest_of<T>(r[1]), rest_of<T>(r[2]), rest_of<T>(r[3]));
+    }
   if (lse && half == 0)
     lse[(static_cast<long>(b) * a.heads + at.head) * a.queries + at.query] = l == 0.f ? -INFINITY : fmaf(m, factor, __log2f(l) - kShift);
 }
 
 // The splits' sums of one row: a wavefront.
 template <typename T>
-__global__ __launch_bounds__(256) void join_splits(AttentionArgs a, const float *part, T *out, float *lse, int splits, float shift) {
+__global__ __launch_bounds__(256) void join_splits(AttentionArgs a, const float *part, T *out, T *low, float *lse, int splits, float shift) {
   const long all = static_cast<long>(a.batch) * a.queries * a.heads, row = static_cast<long>(linear_block()) * 4 + (threadIdx.x >> 6);
   if (row >= all) return;
   const int lane = threadIdx.x & 63;
@@ -182,7 +191,11 @@ __global__ __launch_bounds__(256) void join_splits(AttentionArgs a, const float 
   const float inverse = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
   for (int e = 0; e < 2; ++e)
-    if (lane + 64 * e < a.dim) out[row * a.dim + lane + 64 * e] = store_cast<T>(o[e] * inverse);
+    if (lane + 64 * e < a.dim) {
+      const long to = row * a.dim + lane + 64 * e;
+      out[to] = store_cast<T>(o[e] * inverse);
+      if (low) low[to] = store_cast<T>(rest_of<T>(o[e] * inverse));
+    }
   if (lse && lane == 0) {
     const int h = row % a.heads, i = row / a.heads % a.queries, b = row / a.heads / a.queries;
     lse[(static_cast<long>(b) * a.heads + h) * a.queries + i] = l == 0.f ? -INFINITY : fmaf(top, factor, __log2f(l) - shift);
@@ -203,11 +216,11 @@ ForwardPlan forward_plan(const mv_attention_shape *s) {
 }
 
 template <typename T, int DP>
-void launch_forward(const ForwardPlan &p, const AttentionArgs &a, void *out, float *lse, float *part, hipStream_t s) {
+void launch_forward(const ForwardPlan &p, const AttentionArgs &a, void *out, void *low, float *lse, float *part, hipStream_t s) {
   const long groups = static_cast<long>(p.row_tiles) * p.splits * a.batch * a.key_heads;
   const dim3 grid = linear_grid(groups, 256);
-  if (p.few) attend_kernel<T, DP, 1><<<grid, 256, 0, s>>>(a, static_cast<T *>(out), lse, part, p.row_tiles, p.splits);
-  else attend_kernel<T, DP, 4><<<grid, 256, 0, s>>>(a, static_cast<T *>(out), lse, part, p.row_tiles, p.splits);
+  if (p.few) attend_kernel<T, DP, 1><<<grid, 256, 0, s>>>(a, static_cast<T *>(out), static_cast<T *>(low), lse, part, p.row_tiles, p.splits);
+  else attend_kernel<T, DP, 4><<<grid, 256, 0, s>>>(a, static_cast<T *>(out), static_cast<T *>(low), lse, part, p.row_tiles, p.splits);
 }
 
 }  // namespace
@@ -224,7 +237,7 @@ size_t mv_cross_attention_forward_workspace_bytes(const mv_attention_shape *s, i
 }
 
 int mv_cross_attention_forward(const void *query, const void *key, const void *value, const void *key_mask,
-                               const void *key_lengths, void *output, void *lse, const mv_attention_shape *shape,
+                               const void *key_lengths, void *output, void *output_low, void *lse, const mv_attention_shape *shape,
                                float scale, int dtype, void *workspace, size_t workspace_bytes, void *stream) {
   if (const int status = attention_sizes(shape, dtype)) return status;
   const AttentionArgs a = attention_arguments(shape, query, key, value, key_mask, key_lengths, scale);
@@ -236,11 +249,11 @@ int mv_cross_attention_forward(const void *query, const void *key, const void *v
   float *const part = static_cast<float *>(workspace), *const sums = static_cast<float *>(lse);
   const hipStream_t s = static_cast<hipStream_t>(stream);
   MV_FLOATS(dtype, {
-    if (a.dim <= 32) launch_forward<T, 32>(p, a, output, sums, part, s);
-    else if (a.dim <= 64) launch_forward<T, 64>(p, a, output, sums, part, s);
-    else launch_forward<T, 128>(p, a, output, sums, part, s);
+    if (a.dim <= 32) launch_forward<T, 32>(p, a, output, output_low, sums, part, s);
+    else if (a.dim <= 64) launch_forward<T, 64>(p, a, output, output_low, sums, part, s);
+    else launch_forward<T, 128>(p, a, output, output_low, sums, part, s);
     if (p.splits > 1)
-      join_splits<T><<<linear_grid((rows + 3) / 4, 256), 256, 0, s>>>(a, part, static_cast<T *>(output), sums, p.splits, dtype == MV_F16 ? 15.f : 0.f);
+      join_splits<T><<<linear_grid((rows + 3) / 4, 256), 256, 0, s>>>(a, part, static_cast<T *>(output), static_cast<T *>(output_low), sums, p.splits, dtype == MV_F16 ? 15.f : 0.f);
   })
   return check_launch("cross_attention");
 }

@@ -215,6 +215,14 @@ __device__ __forceinline__ void add_transposed(const Tile<T, DP, Rows> &tile, in
 // The other half of the wavefront has the other rows of the same column.
 __device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32); }
 
+// What rounding to T takes away from v (nothing where v is not finite)
+template <typename T> __device__ __forceinline__ float rest_of(float v) {
+  if constexpr (sizeof(T) == 4) return 0.f;
+  const T r = store_cast<T>(v);
+  const float rest = v - mv::load(&r);
+  return rest == rest ? rest : 0.f;
+}
+
 // Four neighbouring elements of a row of `dim` elements
 template <typename T> __device__ __forceinline__ void store_quad(T *row, int d, int dim, float a, float b, float c, float e) {
   const float v[4] = {a, b, c, e};

@@ -68,7 +68,7 @@ template <typename O, int N> __device__ __forceinline__ void store_column(O *row
 // As the forward kernel; leaves d_i for the next one.
 template <typename T, int DP, int WQ>
 __global__ __launch_bounds__(256, DP == 128 || (sizeof(T) == 4 && DP == 64) ? 1 : 2) void attend_grad_query(
-    AttentionArgs a, const T *out, const float *lse, const T *go, T *gq, float *delta, float *part, int row_tiles, int splits) {
+    AttentionArgs a, const T *out, const T *low, const float *lse, const T *go, T *gq, float *delta, float *part, int row_tiles, int splits) {
   constexpr int kTiles = WQ == 4 ? 2 : 1, kKeys = WQ == 4 ? 64 : 128, kOut = DP / 32;
   using L = Tile<T, DP, kKeys>;
   __shared__ L tiles[2];
@@ -93,6 +93,8 @@ __global__ __launch_bounds__(256, DP == 128 || (sizeof(T) == 4 && DP == 64) ? 1 
     d_o.load(go + at_row * a.dim, live, a.dim, half);
     o.load(out + at_row * a.dim, live, a.dim, half);
     d_i = d_o.dot(o);
+    // (o has to be better than its type: with few keys, d_i is as large as the products that it is taken from)
+    if (low) o.load(low + at_row * a.dim, live, a.dim, half), d_i += d_o.dot(o);
     d_i += other_half(d_i);
   }
   q.load(static_cast<const T *>(a.q) + b * a.qs[0] + at.query * a.qs[1] + at.head * a.qs[2], live, a.dim, half);
@@ -298,15 +300,15 @@ BackwardPlan backward_plan(const mv_attention_shape *s) {
 }
 
 template <typename T, int DP>
-void launch_backward(const BackwardPlan &p, const AttentionArgs &a, const void *out, const float *lse, const void *go, void *gq, void *gk, void *gv,
+void launch_backward(const BackwardPlan &p, const AttentionArgs &a, const void *out, const void *low, const float *lse, const void *go, void *gq, void *gk, void *gv,
                      float *delta, float *part, hipStream_t s) {
   const long heads = static_cast<long>(a.batch) * a.key_heads, queries = static_cast<long>(a.batch) * a.queries * a.heads * a.dim,
              keys = heads * a.keys * a.dim;
-  const T *const o = static_cast<const T *>(out), *const d_o = static_cast<const T *>(go);
+  const T *const o = static_cast<const T *>(out), *const ol = static_cast<const T *>(low), *const d_o = static_cast<const T *>(go);
   if (queries) {
     const dim3 grid = linear_grid(heads * p.row_tiles * p.query_splits, 256);
-    if (p.few_rows) attend_grad_query<T, DP, 1><<<grid, 256, 0, s>>>(a, o, lse, d_o, static_cast<T *>(gq), delta, part, p.row_tiles, p.query_splits);
-    else attend_grad_query<T, DP, 4><<<grid, 256, 0, s>>>(a, o, lse, d_o, static_cast<T *>(gq), delta, part, p.row_tiles, p.query_splits);
+    if (p.few_rows) attend_grad_query<T, DP, 1><<<grid, 256, 0, s>>>(a, o, ol, lse, d_o, static_cast<T *>(gq), delta, part, p.row_tiles, p.query_splits);
+    else attend_grad_query<T, DP, 4><<<grid, 256, 0, s>>>(a, o, ol, lse, d_o, static_cast<T *>(gq), delta, part, p.row_tiles, p.query_splits);
     if (p.query_splits > 1) add_splits<T><<<linear_grid((queries + 255) / 256, 256), 256, 0, s>>>(part, static_cast<T *>(gq), queries, p.query_splits);
   }
   if (keys) {
@@ -337,7 +339,7 @@ size_t mv_cross_attention_backward_workspace_bytes(const mv_attention_shape *s, 
 }
 
 int mv_cross_attention_backward(const void *query, const void *key, const void *value, const void *key_mask,
-                                const void *key_lengths, const void *output, const void *lse, const void *grad_output,
+                                const void *key_lengths, const void *output, const void *output_low, const void *lse, const void *grad_output,
                                 void *grad_query, void *grad_key, void *grad_value, const mv_attention_shape *shape,
                                 float scale, int dtype, void *workspace, size_t workspace_bytes, void *stream) {
   if (const int status = attention_sizes(shape, dtype)) return status;
@@ -351,9 +353,9 @@ int mv_cross_attention_backward(const void *query, const void *key, const void *
   const float *const sums = static_cast<const float *>(lse);
   const hipStream_t s = static_cast<hipStream_t>(stream);
   MV_FLOATS(dtype, {
-    if (a.dim <= 32) launch_backward<T, 32>(p, a, output, sums, grad_output, grad_query, grad_key, grad_value, delta, part, s);
-    else if (a.dim <= 64) launch_backward<T, 64>(p, a, output, sums, grad_output, grad_query, grad_key, grad_value, delta, part, s);
-    else launch_backward<T, 128>(p, a, output, sums, grad_output, grad_query, grad_key, grad_value, delta, part, s);
+    if (a.dim <= 32) launch_backward<T, 32>(p, a, output, output_low, sums, grad_output, grad_query, grad_key, grad_value, delta, part, s);
+    else if (a.dim <= 64) launch_backward<T, 64>(p, a, output, output_low, sums, grad_output, grad_query, grad_key, grad_value, delta, part, s);
+    else launch_backward<T, 128>(p, a, output, output_low, sums, grad_output, grad_query, grad_key, grad_value, delta, part, s);
   })
   return check_launch("cross_attention backward");
 }

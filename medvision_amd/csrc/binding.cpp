@@ -579,20 +579,25 @@ AttentionCall attention_call(const Tensor &query, const Tensor &key, const Tenso
   return c;
 }
 
-// output, and the logarithms of the softmax's sums where a backward pass will want them
-std::pair<Tensor, Tensor> attention_forward(const AttentionCall &c, double scale, bool train) {
+// output, and what a backward pass will want: the logarithms of the softmax's sums, and what rounding took from the output
+struct AttentionResult {
+  Tensor output, lse, low;
+};
+
+AttentionResult attention_forward(const AttentionCall &c, double scale, bool train) {
   const c10::DeviceGuard guard(c.q.device());
   const mv_attention_shape &s = c.shape;
   const Tensor output = at::empty({s.batch, s.queries, s.heads, s.dim}, c.q.options());
   const Tensor lse = train ? at::empty({s.batch, s.heads, s.queries}, c.q.options().dtype(at::kFloat)) : Tensor();
+  const Tensor low = train && c.code != MV_F32 ? at::empty_like(output) : Tensor();
   const size_t bytes = mv_cross_attention_forward_workspace_bytes(&s, c.code);
   const Tensor ws = bytes_on(c.q, bytes);
-  check(mv_cross_attention_forward(ptr(c.q), ptr(c.k), ptr(c.v), ptr(c.mask), ptr(c.lengths), ptr(output), ptr(lse), &s,
+  check(mv_cross_attention_forward(ptr(c.q), ptr(c.k), ptr(c.v), ptr(c.mask), ptr(c.lengths), ptr(output), ptr(low), ptr(lse), &s,
                                    static_cast<float>(scale), c.code, ptr(ws), bytes, stream_of(c.q)));
-  return {output, lse};
+  return {output, lse, low};
 }
 
-variable_list attention_backward(const AttentionCall &c, const Tensor &output, const Tensor &lse, const Tensor &grad_in, double scale) {
+variable_list attention_backward(const AttentionCall &c, const Tensor &output, const Tensor &lse, const Tensor &low, const Tensor &grad_in, double scale) {
   const c10::DeviceGuard guard(c.q.device());
   const mv_attention_shape &s = c.shape;
   same_device(c.q, grad_in, "grad_output");
@@ -602,7 +607,7 @@ variable_list attention_backward(const AttentionCall &c, const Tensor &output, c
   const Tensor gk = at::empty({s.batch, s.keys, s.key_heads, s.dim}, c.q.options()), gv = at::empty_like(gk);
   const size_t bytes = mv_cross_attention_backward_workspace_bytes(&s, c.code);
   const Tensor ws = bytes_on(c.q, bytes);
-  check(mv_cross_attention_backward(ptr(c.q), ptr(c.k), ptr(c.v), ptr(c.mask), ptr(c.lengths), ptr(output), ptr(lse), ptr(grad),
+  check(mv_cross_attention_backward(ptr(c.q), ptr(c.k), ptr(c.v), ptr(c.mask), ptr(c.lengths), ptr(output), ptr(low), ptr(lse), ptr(grad),
                                     ptr(gq), ptr(gk), ptr(gv), &s, static_cast<float>(scale), c.code, ptr(ws), bytes, stream_of(c.q)));
   return {gq, gk, gv};
 }
@@ -611,10 +616,10 @@ struct CrossAttentionFunction : torch::autograd::Function<CrossAttentionFunction
   static Tensor forward(AutogradContext *ctx, const Tensor &query, const Tensor &key, const Tensor &value,
                         const std::optional<Tensor> &key_mask, const std::optional<Tensor> &key_lengths, double scale) {
     const AttentionCall c = attention_call(query, key, value, key_mask.value_or(Tensor()), key_lengths.value_or(Tensor()));
-    const auto [output, lse] = attention_forward(c, scale, true);
-    ctx->save_for_backward({query, key, value, c.mask, c.lengths, output, lse});
+    const AttentionResult r = attention_forward(c, scale, true);
+    ctx->save_for_backward({query, key, value, c.mask, c.lengths, r.output, r.lse, r.low});
     ctx->saved_data["scale"] = scale;
-    return output;
+    return r.output;
   }
   static variable_list backward(AutogradContext *ctx, const variable_list &grads) {
     variable_list out(6);
@@ -622,7 +627,7 @@ struct CrossAttentionFunction : torch::autograd::Function<CrossAttentionFunction
     {
       const at::NoGradGuard no_grad;
       const auto t = ctx->get_saved_variables();
-      const variable_list g = attention_backward(attention_call(t[0], t[1], t[2], t[3], t[4]), t[5], t[6], grads[0],
+      const variable_list g = attention_backward(attention_call(t[0], t[1], t[2], t[3], t[4]), t[5], t[6], t[7], grads[0],
                                                  ctx->saved_data["scale"].toDouble());
       for (int i = 0; i < 3; ++i) out[i] = g[i];
     }
@@ -643,25 +648,27 @@ Tensor cross_attention(const Tensor &query, const Tensor &key, const Tensor &val
     return CrossAttentionFunction::apply(query, key, value, key_mask, key_lengths, attention_scale(query, scale));
   const at::NoGradGuard no_grad;
   return attention_forward(attention_call(query, key, value, key_mask.value_or(Tensor()), key_lengths.value_or(Tensor())),
-                           attention_scale(query, scale), false).first;
+                           attention_scale(query, scale), false).output;
 }
 
 // The two halves for the Python form of the node
-std::pair<Tensor, Tensor> cross_attention_forward(const Tensor &query, const Tensor &key, const Tensor &value, const std::optional<Tensor> &key_mask,
+std::tuple<Tensor, Tensor, std::optional<Tensor>> cross_attention_forward(const Tensor &query, const Tensor &key, const Tensor &value, const std::optional<Tensor> &key_mask,
                                                   const std::optional<Tensor> &key_lengths, const std::optional<double> &scale) {
   const py::gil_scoped_release no_gil;
   const at::NoGradGuard no_grad;
-  return attention_forward(attention_call(query, key, value, key_mask.value_or(Tensor()), key_lengths.value_or(Tensor())),
-                           attention_scale(query, scale), true);
+  const AttentionResult r = attention_forward(attention_call(query, key, value, key_mask.value_or(Tensor()), key_lengths.value_or(Tensor())),
+                                              attention_scale(query, scale), true);
+  return {r.output, r.lse, r.low.defined() ? std::optional<Tensor>(r.low) : std::nullopt};
 }
 
 std::tuple<Tensor, Tensor, Tensor> cross_attention_backward(const Tensor &query, const Tensor &key, const Tensor &value,
                                                             const std::optional<Tensor> &key_mask, const std::optional<Tensor> &key_lengths,
-                                                            const Tensor &output, const Tensor &lse, const Tensor &grad, const std::optional<double> &scale) {
+                                                            const Tensor &output, const Tensor &lse, const std::optional<Tensor> &low, const Tensor &grad,
+                                                            const std::optional<double> &scale) {
   const py::gil_scoped_release no_gil;
   const at::NoGradGuard no_grad;
   const auto g = attention_backward(attention_call(query, key, value, key_mask.value_or(Tensor()), key_lengths.value_or(Tensor())), output, lse,
-                                    grad, attention_scale(query, scale));
+                                    low.value_or(Tensor()), grad, attention_scale(query, scale));
   return {g[0], g[1], g[2]};
 }
 

@@ -7,6 +7,9 @@
 // pass needs nothing but that sum.  Statistics and products are in 32 bits, each output is rounded once.
 #include "rows.hpp"
 
+#include <algorithm>
+#include <type_traits>
+
 namespace mv {
 namespace {
 
@@ -71,8 +74,150 @@ __device__ __forceinline__ float lanes_scale(const float (&v)[8]) {
   return block_scale(most);
 }
 
+// Sum over the Lanes threads of a row, the same for each of them
+template <int Lanes> __device__ __forceinline__ float row_sum(float v, float *lds) {
+  if constexpr (Lanes > 64) return block_sum(v, lds);
+#pragma unroll
+  for (int d = Lanes / 2; d; d >>= 1) v += __shfl_xor(v, d);
+  return v;
+}
+
+// Rows that fit into registers: Lanes threads, 8 Chunks columns each.  One pass over memory.
+template <typename T, int Lanes, int Chunks>
+__global__ __launch_bounds__(kThreads) void norm_rows(const T *x, const T *residual, const void *weight, bool wide, T *y, unsigned char *q,
+                                                      float *scales, T *sum, long rows, int columns, float eps) {
+  __shared__ float lds[kThreads / 64];
+  const long row = static_cast<long>(linear_block()) * (kThreads / Lanes) + threadIdx.x / Lanes;
+  if (row >= rows) return;   // (whole rows: nobody of them waits below)
+  const int lane = threadIdx.x % Lanes;
+  const long at = row * columns;
+  float v[Chunks][8], squares = 0.f;
+#pragma unroll
+  for (int k = 0; k < Chunks; ++k) {
+    const int c = (k * Lanes + lane) * 8;
+    load8(x + at + c, columns - c, v[k]);
+  }
+  if (residual) {
+    float r[Chunks][8];
+#pragma unroll
+    for (int k = 0; k < Chunks; ++k) {
+      const int c = (k * Lanes + lane) * 8;
+      load8(residual + at + c, columns - c, r[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < Chunks; ++k) {
+      const int c = (k * Lanes + lane) * 8;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[k][i] += r[k][i];
+      if constexpr (sizeof(T) == 2) {   // what is stored is what is normalised
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const unsigned both = pack2<T>(v[k][2 * i], v[k][2 * i + 1]);
+          v[k][2 * i] = Bits<T>::up(static_cast<unsigned short>(both & 0xffffu));
+          v[k][2 * i + 1] = Bits<T>::up(static_cast<unsigned short>(both >> 16));
+        }
+      }
+      store8(sum + at + c, columns - c, v[k]);
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < Chunks; ++k) squares += dot8(v[k], v[k]);
+  const float n = inverse_root(row_sum<Lanes>(squares, lds) / columns + eps);
+  const int padded = (columns + kBlock - 1) / kBlock * kBlock;
+#pragma unroll
+  for (int k = 0; k < Chunks; ++k) {
+    const int c = (k * Lanes + lane) * 8;
+    float w[8];
+    load_weight(weight, wide, x, c, columns - c, w);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[k][i] = scaled<T>(v[k][i], w[i], n);
+    if (!q) {
+      store8(y + at + c, columns - c, v[k]);
+      continue;
+    }
+    const float s = lanes_scale(v[k]), inverse = 1.f / s;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[k][i] *= inverse;
+    if (c < padded) {
+      *reinterpret_cast<u32x2 *>(q + row * padded + c) = to_e4m3(v[k]);
+      if ((lane & 15) == 0) scales[row * (padded / kBlock) + c / kBlock] = s;
+    }
+  }
+}
+
+// Both gradients in one pass over memory: a workgroup takes every gridDim-th row (or group of rows), and keeps its share of
+// the weight's gradient in registers until the end.
+template <typename T, int Lanes, int Chunks>
+__global__ __launch_bounds__(kThreads) void norm_grad(const T *h, const void *weight, bool wide, const T *gy, const T *gsum, T *gx,
+                                                      float *partial, long rows, int columns, float eps) {
+  constexpr int kGroups = kThreads / Lanes;
+  __shared__ float lds[kThreads / 64];
+  __shared__ float sums[kGroups > 1 ? kGroups - 1 : 1][Lanes * Chunks * 8];
+  const int lane = threadIdx.x % Lanes, group = threadIdx.x / Lanes;
+  float w[Chunks][8], dw[Chunks][8] = {};
+#pragma unroll
+  for (int k = 0; k < Chunks; ++k) {
+    const int c = (k * Lanes + lane) * 8;
+    load_weight(weight, wide, h, c, columns - c, w[k]);
+  }
+  for (long first = static_cast<long>(blockIdx.x) * kGroups; first < rows; first += static_cast<long>(gridDim.x) * kGroups) {
+    const long row = min(first + group, rows - 1), at = row * columns;
+    const bool live = first + group < rows;
+    float v[Chunks][8], g[Chunks][8], s[Chunks][8], squares = 0.f, dot = 0.f;
+#pragma unroll
+    for (int k = 0; k < Chunks; ++k) {
+      const int c = (k * Lanes + lane) * 8, left = live ? columns - c : 0;
+      load8(h + at + c, left, v[k]);
+      load8(gy + at + c, left, g[k]);
+      if (gsum) load8(gsum + at + c, left, s[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < Chunks; ++k) {
+      float gw[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) gw[i] = g[k][i] * w[k][i];
+      squares += dot8(v[k], v[k]);
+      dot += dot8(gw, v[k]);
+    }
+    const float n = inverse_root(row_sum<Lanes>(squares, lds) / columns + eps);
+    const float back = row_sum<Lanes>(dot, lds) / columns * n * n;
+#pragma unroll
+    for (int k = 0; k < Chunks; ++k) {
+      const int c = (k * Lanes + lane) * 8;
+      float d[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        d[i] = n * (g[k][i] * w[k][i] - v[k][i] * back) + (gsum ? s[k][i] : 0.f);
+        dw[k][i] += live ? g[k][i] * (v[k][i] * n) : 0.f;
+      }
+      if (live) store8(gx + at + c, columns - c, d);
+    }
+  }
+  if constexpr (kGroups > 1) {   // the groups' shares, in their order
+    if (group) {
+#pragma unroll
+      for (int k = 0; k < Chunks; ++k)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sums[group - 1][(k * Lanes + lane) * 8 + i] = dw[k][i];
+    }
+    __syncthreads();
+    if (group) return;
+    for (int o = 0; o < kGroups - 1; ++o)
+#pragma unroll
+      for (int k = 0; k < Chunks; ++k)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) dw[k][i] += sums[o][(k * Lanes + lane) * 8 + i];
+  }
+#pragma unroll
+  for (int k = 0; k < Chunks; ++k) {
+    const int c = (k * Lanes + lane) * 8;
+    store8(partial + static_cast<long>(blockIdx.x) * columns + c, columns - c, dw[k]);
+  }
+}
+
+// ---- rows of any length ------------------------------------------------------------------------------------------
 template <typename T>
-__global__ __launch_bounds__(kThreads) void norm_kernel(const T *x, const T *residual, const void *weight, bool wide, T *y,
+__global__ __launch_bounds__(kThreads) void norm_long_rows(const T *x, const T *residual, const void *weight, bool wide, T *y,
                                                         unsigned char *q, float *scales, T *sum, long rows, int columns,
                                                         float eps) {
   __shared__ float lds[kThreads / 64];
@@ -113,7 +258,7 @@ __global__ __launch_bounds__(kThreads) void norm_kernel(const T *x, const T *res
 }
 
 template <typename T>
-__global__ __launch_bounds__(kThreads) void norm_grad_rows(const T *h, const void *weight, bool wide, const T *gy, const T *gsum,
+__global__ __launch_bounds__(kThreads) void norm_grad_long_rows(const T *h, const void *weight, bool wide, const T *gy, const T *gsum,
                                                            T *gx, float *norms, long rows, int columns, float eps) {
   __shared__ float lds[kThreads / 64];
   const long row = linear_block();
@@ -152,7 +297,7 @@ constexpr int kSlices = 64;   // of the rows, for the gradient of the weight
 
 // Thread = eight columns of one slice of rows.
 template <typename T>
-__global__ __launch_bounds__(kThreads) void norm_grad_columns(const T *h, const T *gy, const float *norms, float *partial,
+__global__ __launch_bounds__(kThreads) void norm_grad_long_columns(const T *h, const T *gy, const float *norms, float *partial,
                                                               long rows, int columns) {
   const int c = (blockIdx.x * kThreads + threadIdx.x) * 8;
   if (c >= columns) return;
@@ -168,12 +313,20 @@ __global__ __launch_bounds__(kThreads) void norm_grad_columns(const T *h, const 
   store8(partial + static_cast<long>(blockIdx.y) * columns + c, columns - c, sum);
 }
 
+// Sum of the partial sums, in a fixed order: 16 columns and 16 shares of the parts per workgroup
 template <typename T>
-__global__ __launch_bounds__(kThreads) void norm_grad_weight(const float *partial, void *gw, bool wide, int columns) {
-  const int c = blockIdx.x * kThreads + threadIdx.x;
-  if (c >= columns) return;
+__global__ __launch_bounds__(kThreads) void norm_grad_weight(const float *partial, void *gw, bool wide, int columns, int parts) {
+  __shared__ float sums[16][16];
+  const int in = threadIdx.x & 15, share = threadIdx.x >> 4, c = blockIdx.x * 16 + in;
   float sum = 0.f;
-  for (int s = 0; s < kSlices; ++s) sum += partial[static_cast<long>(s) * columns + c];
+  if (c < columns) {
+#pragma unroll 8
+    for (int p = share; p < parts; p += 16) sum += partial[static_cast<long>(p) * columns + c];
+  }
+  sums[share][in] = sum;
+  __syncthreads();
+  if (share || c >= columns) return;
+  for (int i = 1; i < 16; ++i) sum += sums[i][in];
   if (wide) static_cast<float *>(gw)[c] = sum;
   else static_cast<T *>(gw)[c] = store_cast<T>(sum);
 }
@@ -228,6 +381,26 @@ __global__ __launch_bounds__(kThreads) void quantize_tiles(const T *x, unsigned 
   if (threadIdx.x == 0) scales[tile] = s;
 }
 
+// Calls f with the threads of a row and the pieces of eight columns of each, for rows of up to 8192 columns; false: longer
+template <typename F> bool for_row_shape(int columns, const F &f) {
+  using std::integral_constant;
+  if (columns <= 128) f(integral_constant<int, 16>(), integral_constant<int, 1>());
+  else if (columns <= 256) f(integral_constant<int, 32>(), integral_constant<int, 1>());
+  else if (columns <= 512) f(integral_constant<int, 64>(), integral_constant<int, 1>());
+  else if (columns <= 1024) f(integral_constant<int, 64>(), integral_constant<int, 2>());
+  else if (columns <= 2048) f(integral_constant<int, 256>(), integral_constant<int, 1>());
+  else if (columns <= 4096) f(integral_constant<int, 256>(), integral_constant<int, 2>());
+  else if (columns <= 8192) f(integral_constant<int, 256>(), integral_constant<int, 4>());
+  return columns <= 8192;
+}
+
+constexpr long kGradGroups = 1024;   // workgroups of the gradients' kernel: four per compute unit, and as many partial sums
+// workgroups of it, and partial sums of the weight's gradient
+int grad_parts(long rows, int columns) {
+  const int per = columns <= 128 ? 16 : columns <= 256 ? 8 : columns <= 1024 ? 4 : 1;
+  return columns > 8192 ? kSlices : static_cast<int>(std::max(1L, std::min(kGradGroups, (rows + per - 1) / per)));
+}
+
 int norm_arguments(long rows, int columns, int dtype, int weight_dtype) {
   MV_REQUIRE(dtype == MV_F32 || dtype == MV_F16 || dtype == MV_BF16, "dtype %d is not float32, float16 or bfloat16", dtype);
   MV_REQUIRE(weight_dtype == dtype || weight_dtype == MV_F32, "weight has dtype %d, expected %d or float32", weight_dtype, dtype);
@@ -241,9 +414,21 @@ int norm_forward(const void *x, const void *residual, const void *weight, void *
   if (rows == 0) return MV_OK;
   MV_REQUIRE(x && weight && (y || (q && scales)), "a tensor is missing");
   MV_REQUIRE(!residual == !sum, "the sum goes with a residual");
-  MV_FLOATS(dtype, norm_kernel<T><<<linear_grid(rows, kThreads), kThreads, 0, static_cast<hipStream_t>(stream)>>>(
-      static_cast<const T *>(x), static_cast<const T *>(residual), weight, weight_dtype == MV_F32, static_cast<T *>(y),
-      static_cast<unsigned char *>(q), static_cast<float *>(scales), static_cast<T *>(sum), rows, columns, eps))
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  const bool wide = weight_dtype == MV_F32;
+  auto *const q8 = static_cast<unsigned char *>(q);
+  auto *const sc = static_cast<float *>(scales);
+  MV_FLOATS(dtype, {
+    const T *const xt = static_cast<const T *>(x), *const rt = static_cast<const T *>(residual);
+    T *const yt = static_cast<T *>(y), *const ht = static_cast<T *>(sum);
+    const bool fits = for_row_shape(columns, [&](auto lanes, auto chunks) {
+      constexpr int kRows = kThreads / lanes;
+      norm_rows<T, lanes, chunks><<<linear_grid((rows + kRows - 1) / kRows, kThreads), kThreads, 0, st>>>(xt, rt, weight, wide, yt, q8, sc, ht, rows,
+                                                                                                          columns, eps);
+    });
+    if (!fits)
+      norm_long_rows<T><<<linear_grid(rows, kThreads), kThreads, 0, st>>>(xt, rt, weight, wide, yt, q8, sc, ht, rows, columns, eps);
+  })
   return check_launch("add_rms_norm");
 }
 
@@ -266,7 +451,7 @@ int mv_add_rms_norm_quantized(const void *x, const void *residual, const void *w
 
 size_t mv_add_rms_norm_backward_workspace_bytes(int64_t rows, int columns) {
   if (rows < 0 || columns <= 0) return 0;
-  return 4 * (static_cast<size_t>(rows) + static_cast<size_t>(kSlices) * columns);
+  return 4 * ((columns > 8192 ? static_cast<size_t>(rows) : 0) + static_cast<size_t>(grad_parts(rows, columns)) * columns);
 }
 
 int mv_add_rms_norm_backward(const void *h, const void *weight, const void *grad_y, const void *grad_sum, void *grad_x,
@@ -275,17 +460,21 @@ int mv_add_rms_norm_backward(const void *h, const void *weight, const void *grad
   if (const int status = norm_arguments(rows, columns, dtype, weight_dtype)) return status;
   MV_REQUIRE(weight && grad_weight && (rows == 0 || (h && grad_y && grad_x)), "a tensor is missing");
   MV_REQUIRE(workspace && workspace_bytes >= mv_add_rms_norm_backward_workspace_bytes(rows, columns), "the workspace is too small");
-  float *const norms = static_cast<float *>(workspace), *const partial = norms + rows;
-  const hipStream_t s = static_cast<hipStream_t>(stream);
+  const hipStream_t st = static_cast<hipStream_t>(stream);
   const bool wide = weight_dtype == MV_F32;
+  const int parts = grad_parts(rows, columns);
+  float *const partial = static_cast<float *>(workspace), *const norms = partial + static_cast<long>(parts) * columns;
   MV_FLOATS(dtype, {
-    if (rows > 0)
-      norm_grad_rows<T><<<linear_grid(rows, kThreads), kThreads, 0, s>>>(
-          static_cast<const T *>(h), weight, wide, static_cast<const T *>(grad_y), static_cast<const T *>(grad_sum),
-          static_cast<T *>(grad_x), norms, rows, columns, eps);
-    norm_grad_columns<T><<<dim3((columns + kThreads * 8 - 1) / (kThreads * 8), kSlices), kThreads, 0, s>>>(
-        static_cast<const T *>(h), static_cast<const T *>(grad_y), norms, partial, rows, columns);
-    norm_grad_weight<T><<<(columns + kThreads - 1) / kThreads, kThreads, 0, s>>>(partial, grad_weight, wide, columns);
+    const T *const ht = static_cast<const T *>(h), *const gy = static_cast<const T *>(grad_y), *const gs = static_cast<const T *>(grad_sum);
+    T *const gx = static_cast<T *>(grad_x);
+    const bool fits = for_row_shape(columns, [&](auto lanes, auto chunks) {
+      norm_grad<T, lanes, chunks><<<parts, kThreads, 0, st>>>(ht, weight, wide, gy, gs, gx, partial, rows, columns, eps);
+    });
+    if (!fits) {
+      if (rows > 0) norm_grad_long_rows<T><<<linear_grid(rows, kThreads), kThreads, 0, st>>>(ht, weight, wide, gy, gs, gx, norms, rows, columns, eps);
+      norm_grad_long_columns<T><<<dim3((columns + kThreads * 8 - 1) / (kThreads * 8), kSlices), kThreads, 0, st>>>(ht, gy, norms, partial, rows, columns);
+    }
+    norm_grad_weight<T><<<(columns + 15) / 16, kThreads, 0, st>>>(partial, grad_weight, wide, columns, parts);
   })
   return check_launch("add_rms_norm backward");
 }

@@ -12,16 +12,16 @@ class CrossAttentionFunction(NativeFunction):
 
     @staticmethod
     def forward(ctx, query, key, value, key_mask=None, key_lengths=None, scale=None):
-        output, lse = native.cross_attention_forward(query, key, value, key_mask, key_lengths, scale)
-        ctx.save_for_backward(query, key, value, key_mask, key_lengths, output, lse)
+        output, lse, low = native.cross_attention_forward(query, key, value, key_mask, key_lengths, scale)
+        ctx.save_for_backward(query, key, value, key_mask, key_lengths, output, lse, low)
         ctx.scale = scale
         return output
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_output):
-        query, key, value, key_mask, key_lengths, output, lse = ctx.saved_tensors
-        grads = native.cross_attention_backward(query, key, value, key_mask, key_lengths, output, lse, grad_output, ctx.scale)
+        query, key, value, key_mask, key_lengths, output, lse, low = ctx.saved_tensors
+        grads = native.cross_attention_backward(query, key, value, key_mask, key_lengths, output, lse, low, grad_output, ctx.scale)
         return (*grads, None, None, None)
 
 

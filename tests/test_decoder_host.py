@@ -32,15 +32,15 @@ def test_entry_points_refuse_on_the_host():
     from medvision_amd import _lib
     lib = _lib.load()
     for shape in (_shape(key_heads=3), _shape(dim=129), _shape(dim=0), _shape(batch=-1), _shape(key_heads=0)):
-        assert lib.mv_cross_attention_forward(*[None] * 7, ctypes.byref(shape), 1.0, _lib.MV_F32, None, 0, None) == 1
+        assert lib.mv_cross_attention_forward(*[None] * 8, ctypes.byref(shape), 1.0, _lib.MV_F32, None, 0, None) == 1
         assert lib.mv_last_error()
     good = _shape()
-    assert lib.mv_cross_attention_forward(*[None] * 7, ctypes.byref(good), 1.0, _lib.MV_F64, None, 0, None) == 1
+    assert lib.mv_cross_attention_forward(*[None] * 8, ctypes.byref(good), 1.0, _lib.MV_F64, None, 0, None) == 1
     assert b"float32, float16 or bfloat16" in lib.mv_last_error()
-    assert lib.mv_cross_attention_forward(*[None] * 7, ctypes.byref(good), 1.0, _lib.MV_F32, None, 0, None) == 1
+    assert lib.mv_cross_attention_forward(*[None] * 8, ctypes.byref(good), 1.0, _lib.MV_F32, None, 0, None) == 1
     assert b"missing" in lib.mv_last_error()
-    assert lib.mv_cross_attention_forward(*[None] * 7, None, 1.0, _lib.MV_F32, None, 0, None) == 1
-    assert lib.mv_cross_attention_forward(*[None] * 7, ctypes.byref(_shape(queries=0)), 1.0, _lib.MV_F32, None, 0, None) == 0
+    assert lib.mv_cross_attention_forward(*[None] * 8, None, 1.0, _lib.MV_F32, None, 0, None) == 1
+    assert lib.mv_cross_attention_forward(*[None] * 8, ctypes.byref(_shape(queries=0)), 1.0, _lib.MV_F32, None, 0, None) == 0
     assert lib.mv_add_rms_norm(*[None] * 5, 4, 0, 1e-6, _lib.MV_F32, _lib.MV_F32, None) == 1
     assert lib.mv_add_rms_norm(*[None] * 5, 4, 8, 1e-6, _lib.MV_F16, _lib.MV_BF16, None) == 1
     assert lib.mv_quantize_blocks(*[None] * 3, 4, 8, 2, _lib.MV_F32, None) == 1
