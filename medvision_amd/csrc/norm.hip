@@ -76,7 +76,15 @@ __device__ __forceinline__ float lanes_scale(const float (&v)[8]) {
 
 // Sum over the Lanes threads of a row, the same for each of them
 template <int Lanes> __device__ __forceinline__ float row_sum(float v, float *lds) {
-  if constexpr (Lanes > 64) return block_sum(v, lds);
+  if constexpr (Lanes == kThreads) return block_sum(v, lds);
+  if constexpr (Lanes == 128) {   // two wavefronts
+    v = wave_sum(v);
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = lds[threadIdx.x / 128 * 2] + lds[threadIdx.x / 128 * 2 + 1];
+    __syncthreads();
+    return v;
+  }
 #pragma unroll
   for (int d = Lanes / 2; d; d >>= 1) v += __shfl_xor(v, d);
   return v;
@@ -87,8 +95,9 @@ template <typename T, int Lanes, int Chunks>
 __global__ __launch_bounds__(kThreads) void norm_rows(const T *x, const T *residual, const void *weight, bool wide, T *y, unsigned char *q,
                                                       float *scales, T *sum, long rows, int columns, float eps) {
   __shared__ float lds[kThreads / 64];
-  const long row = static_cast<long>(linear_block()) * (kThreads / Lanes) + threadIdx.x / Lanes;
-  if (row >= rows) return;   // (whole rows: nobody of them waits below)
+  const long mine = static_cast<long>(linear_block()) * (kThreads / Lanes) + threadIdx.x / Lanes;
+  if (mine >= rows && (Lanes != 128 || mine - threadIdx.x / Lanes >= rows)) return;   // (two rows wait for each other)
+  const long row = min(mine, rows - 1);   // (the last one twice, with the same results)
   const int lane = threadIdx.x % Lanes;
   const long at = row * columns;
   float v[Chunks][8], squares = 0.f;
@@ -387,7 +396,7 @@ template <typename F> bool for_row_shape(int columns, const F &f) {
   if (columns <= 128) f(integral_constant<int, 16>(), integral_constant<int, 1>());
   else if (columns <= 256) f(integral_constant<int, 32>(), integral_constant<int, 1>());
   else if (columns <= 512) f(integral_constant<int, 64>(), integral_constant<int, 1>());
-  else if (columns <= 1024) f(integral_constant<int, 64>(), integral_constant<int, 2>());
+  else if (columns <= 1024) f(integral_constant<int, 128>(), integral_constant<int, 1>());
   else if (columns <= 2048) f(integral_constant<int, 256>(), integral_constant<int, 1>());
   else if (columns <= 4096) f(integral_constant<int, 256>(), integral_constant<int, 2>());
   else if (columns <= 8192) f(integral_constant<int, 256>(), integral_constant<int, 4>());
@@ -397,7 +406,7 @@ template <typename F> bool for_row_shape(int columns, const F &f) {
 constexpr long kGradGroups = 1024;   // workgroups of the gradients' kernel: four per compute unit, and as many partial sums
 // workgroups of it, and partial sums of the weight's gradient
 int grad_parts(long rows, int columns) {
-  const int per = columns <= 128 ? 16 : columns <= 256 ? 8 : columns <= 1024 ? 4 : 1;
+  const int per = columns <= 128 ? 16 : columns <= 256 ? 8 : columns <= 512 ? 4 : columns <= 1024 ? 2 : 1;
   return columns > 8192 ? kSlices : static_cast<int>(std::max(1L, std::min(kGradGroups, (rows + per - 1) / per)));
 }
 

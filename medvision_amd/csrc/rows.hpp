@@ -21,6 +21,16 @@ template <> struct Bits<__hip_bfloat16> {
 };
 
 // out[0..7] = p[0..7], zeros from `left` on
+template <typename T> __device__ __forceinline__ void load_tail(const T *p, int left, float (&out)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) out[i] = 0.f;
+  if (left <= 0) return;
+  float v[7];   // (eight addresses that all exist: one wait instead of a branch for each)
+#pragma unroll
+  for (int i = 0; i < 7; ++i) v[i] = load(p + min(i, left - 1));
+#pragma unroll
+  for (int i = 0; i < 7; ++i) out[i] = i < left ? v[i] : 0.f;
+}
 template <typename T> __device__ __forceinline__ void load8(const T *p, int left, float (&out)[8]) {
   if (left >= 8) {
     const u32x4 r = reinterpret_cast<const Loose<u32x4, 2> *>(p)->v;
@@ -31,8 +41,7 @@ template <typename T> __device__ __forceinline__ void load8(const T *p, int left
     }
     return;
   }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) out[i] = i < left ? load(p + i) : 0.f;
+  load_tail(p, left, out);
 }
 template <> __device__ __forceinline__ void load8<float>(const float *p, int left, float (&out)[8]) {
   if (left >= 8) {
@@ -44,8 +53,7 @@ template <> __device__ __forceinline__ void load8<float>(const float *p, int lef
     }
     return;
   }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) out[i] = i < left ? p[i] : 0.f;
+  load_tail(p, left, out);
 }
 
 // Two neighbouring values of 16 bits
