@@ -18,88 +18,98 @@ namespace {
 template <typename T, int DP, int WQ>
 __global__ __launch_bounds__(256, sizeof(T) == 4 ? (DP == 128 ? 1 : 2) : DP == 128 ? 2 : DP == 64 ? 3 : 4) void attend_kernel(
     AttentionArgs a, T *out, T *low, float *lse, float *part, int row_tiles, int splits) {
-  constexpr int kTiles = WQ == 4 ? 2 : 1, kKeys = WQ == 4 ? 64 : 128, kOut = DP / 32;
-  constexpr float kShift = sizeof(T) == 2 && __is_same(T, __half) ? 15.f : 0.f;
+  using S = Staging<T, DP, WQ == 1>;
+  constexpr int kTiles = WQ == 4 && S::kRows >= 64 ? 2 : 1, kKeys = S::kRows, kSteps = WQ == 4 ? kKeys / (32 * kTiles) : 1, kOut = DP / 32;
+  constexpr float kShift = __is_same(T, __half) ? 15.f : 0.f;
   using L = Tile<T, DP, kKeys>;
-  __shared__ L tiles[2];
+  __shared__ L tiles[S::kBuffers][2];
   __shared__ float joined[4][2][32];
-  L &ks = tiles[0], &vs = tiles[1];
-  const int groups = row_tiles * splits * a.batch * a.key_heads;
-  unsigned id = linear_block();
-  if (id >= static_cast<unsigned>(groups)) return;
-  id = xcd_contiguous(id, groups);
-  const int tile = id % row_tiles, split = id / row_tiles % splits, g = id / row_tiles / splits % a.key_heads, b = id / row_tiles / splits / a.key_heads;
+  const Place place(a, row_tiles, splits);
+  if (!place.in) return;
+  const int split = place.split, g = place.g, b = place.b;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
-  const int rows = a.heads / a.key_heads * a.queries, row = tile * 32 * WQ + (WQ == 4 ? wave * 32 : 0) + (lane & 31);
+  const int rows = a.heads / a.key_heads * a.queries, row = place.tile * 32 * WQ + (WQ == 4 ? wave * 32 : 0) + (lane & 31);
   const bool live = row < rows;
   const RowOf at(a, g, live ? row : rows - 1);
   const float factor = a.factor();
 
+  const T *const k = static_cast<const T *>(a.k) + b * a.ks[0] + g * a.ks[2], *const v = static_cast<const T *>(a.v) + b * a.vs[0] + g * a.vs[2];
+  const int length = a.length(b), all_tiles = (length + kKeys - 1) / kKeys;
+  const int first = share(all_tiles, split, splits), last = share(all_tiles, split + 1, splits);
+  const int my_key = WQ == 4 ? 0 : 32 * wave;   // of a tile
+  Pair<T, DP, kKeys> next(a.ks[1], a.vs[1], a.dim);
+  unsigned long long next_use[kSteps] = {};
+  auto load = [&](int t) {
+    next.load(k + t * kKeys * a.ks[1], v + t * kKeys * a.vs[1], length - t * kKeys);
+#pragma unroll
+    for (int n = 0; n < kSteps; ++n) next_use[n] = use_bits(a, b, t * kKeys + my_key + 32 * kTiles * n, 32 * kTiles, length);
+  };
+  auto put = [&](int t) {
+    if (a.mask) next.keep(a.mask + b * a.mask_stride + t * kKeys, length - t * kKeys);
+    next.put(tiles[t % S::kBuffers]);
+  };
+  if (first < last) load(first);
   Column<T, DP> q;
   q.load(static_cast<const T *>(a.q) + b * a.qs[0] + at.query * a.qs[1] + at.head * a.qs[2], live, a.dim, half);
   if (a.scale < 0.f) q.negate();
-
-  const T *const k = static_cast<const T *>(a.k) + b * a.ks[0] + g * a.ks[2], *const v = static_cast<const T *>(a.v) + b * a.vs[0] + g * a.vs[2];
-  const int length = a.length(b), all_tiles = (length + kKeys - 1) / kKeys;
-  const int first = static_cast<int>(static_cast<long>(all_tiles) * split / splits), last = static_cast<int>(static_cast<long>(all_tiles) * (split + 1) / splits);
-  const int my_key = WQ == 4 ? 0 : 32 * wave;   // of a tile
-  Carry<T, DP, kKeys, 256> next_k, next_v;
-  unsigned long long next_use = 0;
-  auto load = [&](int t) {
-    const auto use = [&](int j) { return a.counts(b, j); };
-    next_k.load(threadIdx.x, t * kKeys, length, a.dim, [&](int j) { return k + j * a.ks[1]; }, use);
-    next_v.load(threadIdx.x, t * kKeys, length, a.dim, [&](int j) { return v + j * a.vs[1]; }, use);
-    const int j = t * kKeys + my_key + lane;
-    next_use = __ballot(j < length && (WQ == 4 || lane < 32) && a.counts(b, min(j, length - 1)));
-  };
+  if (first < last) put(first);
 
   float m = -INFINITY, l = 0.f;
   f32x16 o[kOut] = {};
-  if (first < last) load(first);
   for (int t = first; t < last; ++t) {
-    if (t > first) __syncthreads();   // the last tile has been read
-    next_k.put(threadIdx.x, ks);
-    next_v.put(threadIdx.x, vs);
-    const unsigned long long use = next_use;
-    __syncthreads();
-    if (t + 1 < last) load(t + 1);
-    if (!use) continue;
-    f32x16 s[kTiles];
+    unsigned long long use[kSteps];
 #pragma unroll
-    for (int n = 0; n < kTiles; ++n) s[n] = times(ks, my_key + 32 * n, q, lane);
-    if (use != (kTiles == 2 ? ~0ull : 0xffffffffull)) {
+    for (int n = 0; n < kSteps; ++n) use[n] = next_use[n];
+    __syncthreads();   // this tile is there, and the one before it has been read
+    if (t + 1 < last) load(t + 1);
+    const L &ks = tiles[t % S::kBuffers][0], &vs = tiles[t % S::kBuffers][1];
+#pragma unroll
+    for (int step = 0; step < kSteps; ++step) {
+      if (!use[step]) continue;
+      const int key = my_key + 32 * kTiles * step;
+      f32x16 s[kTiles];
+#pragma unroll
+      for (int n = 0; n < kTiles; ++n) s[n] = times(ks, key + 32 * n, q, lane);
+      if (use[step] != (kTiles == 2 ? ~0ull : 0xffffffffull)) {
+#pragma unroll
+        for (int n = 0; n < kTiles; ++n) {
+          const unsigned word = static_cast<unsigned>(use[step] >> (32 * n)) >> (4 * half);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[n][i] = word >> result_row(i, 0) & 1 ? s[n][i] : -INFINITY;
+        }
+      }
+      float top = s[0][0];
+#pragma unroll
+      for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, s[n][i]);
+      top = fmaxf(m, fmaxf(top, other_half(top)));
+      const float base = top == -INFINITY ? 0.f : top;
+      if (__ballot(top > m)) {   // (no row's maximum has grown: nothing to scale)
+        const float keep = __builtin_amdgcn_exp2f((m - base) * factor);
+        l *= keep;
+#pragma unroll
+        for (int u = 0; u < kOut; ++u) o[u] *= keep;
+        m = top;
+      }
+      const float shift = fmaf(base, -factor, kShift);
 #pragma unroll
       for (int n = 0; n < kTiles; ++n) {
-        const unsigned word = static_cast<unsigned>(use >> (32 * n)) >> (4 * half);
+        float p[16], sum[4];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[n][i] = word >> result_row(i, 0) & 1 ? s[n][i] : -INFINITY;
+        for (int i = 0; i < 16; ++i) {
+          // (float32: the difference first, so that the largest weight is one to the last bit)
+          const float x = sizeof(T) == 4 ? (s[n][i] - base) * factor : fmaf(s[n][i], factor, shift);
+          p[i] = __builtin_amdgcn_exp2f(x);
+          sum[i % 4] = i < 4 ? p[i] : sum[i % 4] + p[i];
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        add_transposed(vs, key + 32 * n, p, o, lane);
       }
     }
-    float top = s[0][0];
-#pragma unroll
-    for (int n = 0; n < kTiles; ++n)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) top = fmaxf(top, s[n][i]);
-    top = fmaxf(m, fmaxf(top, other_half(top)));
-    const float base = top == -INFINITY ? 0.f : top;
-    if (__ballot(top > m)) {   // (no row's maximum has grown: nothing to scale)
-      const float keep = __builtin_amdgcn_exp2f((m - base) * factor);
-      l *= keep;
-#pragma unroll
-      for (int u = 0; u < kOut; ++u) o[u] *= keep;
-      m = top;
-    }
-    const float shift = fmaf(base, -factor, kShift);
-#pragma unroll
-    for (int n = 0; n < kTiles; ++n) {
-      float p[16];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        // (float32: the difference first, so that the largest weight is one to the last bit)
-        const float x = sizeof(T) == 4 ? (s[n][i] - base) * factor : fmaf(s[n][i], factor, shift);
-        l += p[i] = __builtin_amdgcn_exp2f(x);
-      }
-      add_transposed(vs, my_key + 32 * n, p, o, lane);
+    if (t + 1 < last) {
+      if constexpr (S::kBuffers == 1) __syncthreads();
+      put(t + 1);
     }
   }
   l += other_half(l);
@@ -171,35 +181,71 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? (DP == 128 ? 1 : 2) : DP == 1
     lse[(static_cast<long>(b) * a.heads + at.head) * a.queries + at.query] = l == 0.f ? -INFINITY : fmaf(m, factor, __log2f(l) - kShift);
 }
 
-// The splits' sums of one row: a wavefront.
+// The splits' sums.  Many splits (few rows): a workgroup for a row, whose wavefronts take turns at the splits.
 template <typename T>
-__global__ __launch_bounds__(256) void join_splits(AttentionArgs a, const float *part, T *out, T *low, float *lse, int splits, float shift) {
-  const long all = static_cast<long>(a.batch) * a.queries * a.heads, row = static_cast<long>(linear_block()) * 4 + (threadIdx.x >> 6);
+__global__ __launch_bounds__(256) void join_many(AttentionArgs a, const float *part, T *out, T *low, float *lse, int splits, float shift) {
+  __shared__ float sums[4][1 + kMostDim];
+  const long all = static_cast<long>(a.batch) * a.queries * a.heads, row = linear_block();
   if (row >= all) return;
-  const int lane = threadIdx.x & 63;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const float *const stats = part + splits * all * a.dim, factor = a.factor();
   float top = -INFINITY, l = 0.f, o[2] = {};
-  for (int s = 0; s < splits; ++s) top = fmaxf(top, stats[(s * all + row) * 2]);
+  for (int s = lane; s < splits; s += 64) top = fmaxf(top, stats[(s * all + row) * 2]);
+#pragma unroll
+  for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
   const float base = top == -INFINITY ? 0.f : top;
-  for (int s = 0; s < splits; ++s) {
+#pragma unroll 4
+  for (int s = wave; s < splits; s += 4) {
     const float keep = __builtin_amdgcn_exp2f((stats[(s * all + row) * 2] - base) * factor);
     l += keep * stats[(s * all + row) * 2 + 1];
 #pragma unroll
-    for (int e = 0; e < 2; ++e)
-      if (lane + 64 * e < a.dim) o[e] += keep * part[(s * all + row) * a.dim + lane + 64 * e];
+    for (int e = 0; e < 2; ++e) o[e] += keep * part[(s * all + row) * a.dim + min(lane + 64 * e, a.dim - 1)];
+  }
+  sums[wave][lane] = o[0], sums[wave][64 + lane] = o[1];
+  if (lane == 0) sums[wave][kMostDim] = l;
+  __syncthreads();
+  l = ((sums[0][kMostDim] + sums[1][kMostDim]) + sums[2][kMostDim]) + sums[3][kMostDim];
+  const float inverse = l == 0.f ? 0.f : 1.f / l;
+  const int d = threadIdx.x;
+  if (d < a.dim) {
+    const float v = (((sums[0][d] + sums[1][d]) + sums[2][d]) + sums[3][d]) * inverse;
+    out[row * a.dim + d] = store_cast<T>(v);
+    if (low) low[row * a.dim + d] = store_cast<T>(rest_of<T>(v));
+  }
+  if (lse && threadIdx.x == 0) lse[a.log_at(row)] = l == 0.f ? -INFINITY : fmaf(top, factor, __log2f(l) - shift);
+}
+
+// Few splits: four neighbouring elements of a row per thread.
+template <typename T>
+__global__ __launch_bounds__(256) void join_few(AttentionArgs a, const float *part, T *out, T *low, float *lse, int splits, float shift) {
+  const int quads = (a.dim + 3) / 4;
+  const long all = static_cast<long>(a.batch) * a.queries * a.heads, at = static_cast<long>(linear_block()) * 256 + threadIdx.x, row = at / quads;
+  if (row >= all) return;
+  const int d = static_cast<int>(at - row * quads) * 4;
+  const float *const stats = part + splits * all * a.dim, factor = a.factor();
+  float top = -INFINITY, l = 0.f, o[4] = {};
+  for (int s = 0; s < splits; ++s) top = fmaxf(top, stats[(s * all + row) * 2]);
+  const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll 4
+  for (int s = 0; s < splits; ++s) {
+    const float keep = __builtin_amdgcn_exp2f((stats[(s * all + row) * 2] - base) * factor);
+    l += keep * stats[(s * all + row) * 2 + 1];
+    const float *const from = part + (s * all + row) * a.dim;
+    if (d + 4 <= a.dim) {
+      const f32x4 r = reinterpret_cast<const Loose<f32x4, 4> *>(from + d)->v;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] += keep * r[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < 3; ++e) o[e] += keep * from[min(d + e, a.dim - 1)];
+    }
   }
   const float inverse = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
-  for (int e = 0; e < 2; ++e)
-    if (lane + 64 * e < a.dim) {
-      const long to = row * a.dim + lane + 64 * e;
-      out[to] = store_cast<T>(o[e] * inverse);
-      if (low) low[to] = store_cast<T>(rest_of<T>(o[e] * inverse));
-    }
-  if (lse && lane == 0) {
-    const int h = row % a.heads, i = row / a.heads % a.queries, b = row / a.heads / a.queries;
-    lse[(static_cast<long>(b) * a.heads + h) * a.queries + i] = l == 0.f ? -INFINITY : fmaf(top, factor, __log2f(l) - shift);
-  }
+  for (int e = 0; e < 4; ++e) o[e] *= inverse;
+  store_quad(out + row * a.dim, d, a.dim, o[0], o[1], o[2], o[3]);
+  if (low) store_quad(low + row * a.dim, d, a.dim, rest_of<T>(o[0]), rest_of<T>(o[1]), rest_of<T>(o[2]), rest_of<T>(o[3]));
+  if (lse && d == 0) lse[a.log_at(row)] = l == 0.f ? -INFINITY : fmaf(top, factor, __log2f(l) - shift);
 }
 
 struct ForwardPlan {
@@ -207,20 +253,24 @@ struct ForwardPlan {
   int row_tiles, splits;
 };
 
-ForwardPlan forward_plan(const mv_attention_shape *s) {
+ForwardPlan forward_plan(const mv_attention_shape *s, int dtype) {
   const long rows = static_cast<long>(s->heads / s->key_heads) * s->queries;
-  const bool few = rows <= 32;
+  const bool few = rows <= 32 && has_few(dtype, s->dim);
   const long row_tiles = few ? 1 : (rows + 127) / 128, groups = std::max(1L, row_tiles * s->batch * s->key_heads);
-  const long tiles = few ? (s->keys + 127L) / 128 : (s->keys + 63L) / 64;
-  return {few, static_cast<int>(row_tiles), static_cast<int>(std::max(1L, std::min(512 / groups, tiles / 4)))};
+  const long shares = dtype == MV_F32 ? (s->keys + 63L) / 64 : (s->keys + 511L) / 512;   // the least worth a split
+  return {few, static_cast<int>(row_tiles), static_cast<int>(std::max(1L, std::min((s->dim <= 32 ? 1024 : s->dim <= 64 && !few ? 768 : 512) / groups, shares)))};
 }
 
 template <typename T, int DP>
 void launch_forward(const ForwardPlan &p, const AttentionArgs &a, void *out, void *low, float *lse, float *part, hipStream_t s) {
   const long groups = static_cast<long>(p.row_tiles) * p.splits * a.batch * a.key_heads;
   const dim3 grid = linear_grid(groups, 256);
-  if (p.few) attend_kernel<T, DP, 1><<<grid, 256, 0, s>>>(a, static_cast<T *>(out), static_cast<T *>(low), lse, part, p.row_tiles, p.splits);
-  else attend_kernel<T, DP, 4><<<grid, 256, 0, s>>>(a, static_cast<T *>(out), static_cast<T *>(low), lse, part, p.row_tiles, p.splits);
+  if constexpr (kHasFew<T, DP>)
+    if (p.few) {
+      attend_kernel<T, DP, 1><<<grid, 256, 0, s>>>(a, static_cast<T *>(out), static_cast<T *>(low), lse, part, p.row_tiles, p.splits);
+      return;
+    }
+  attend_kernel<T, DP, 4><<<grid, 256, 0, s>>>(a, static_cast<T *>(out), static_cast<T *>(low), lse, part, p.row_tiles, p.splits);
 }
 
 }  // namespace
@@ -232,7 +282,7 @@ extern "C" {
 
 size_t mv_cross_attention_forward_workspace_bytes(const mv_attention_shape *s, int dtype) {
   if (attention_sizes(s, dtype)) return 0;
-  const ForwardPlan p = forward_plan(s);
+  const ForwardPlan p = forward_plan(s, dtype);
   return p.splits > 1 ? sizeof(float) * p.splits * s->batch * static_cast<size_t>(s->queries) * s->heads * (s->dim + 2) : 0;
 }
 
@@ -244,7 +294,7 @@ int mv_cross_attention_forward(const void *query, const void *key, const void *v
   const long rows = static_cast<long>(a.batch) * a.queries * a.heads;
   if (rows == 0) return MV_OK;
   MV_REQUIRE(query && output && (a.keys == 0 || (key && value)), "a tensor is missing");
-  ForwardPlan p = forward_plan(shape);
+  ForwardPlan p = forward_plan(shape, dtype);
   if (p.splits > 1 && (!workspace || workspace_bytes < mv_cross_attention_forward_workspace_bytes(shape, dtype))) p.splits = 1;
   float *const part = static_cast<float *>(workspace), *const sums = static_cast<float *>(lse);
   const hipStream_t s = static_cast<hipStream_t>(stream);
@@ -252,8 +302,10 @@ int mv_cross_attention_forward(const void *query, const void *key, const void *v
     if (a.dim <= 32) launch_forward<T, 32>(p, a, output, output_low, sums, part, s);
     else if (a.dim <= 64) launch_forward<T, 64>(p, a, output, output_low, sums, part, s);
     else launch_forward<T, 128>(p, a, output, output_low, sums, part, s);
-    if (p.splits > 1)
-      join_splits<T><<<linear_grid((rows + 3) / 4, 256), 256, 0, s>>>(a, part, static_cast<T *>(output), static_cast<T *>(output_low), sums, p.splits, dtype == MV_F16 ? 15.f : 0.f);
+    const float shift = dtype == MV_F16 ? 15.f : 0.f;
+    T *const o = static_cast<T *>(output), *const ol = static_cast<T *>(output_low);
+    if (p.splits > 8) join_many<T><<<linear_grid(rows, 256), 256, 0, s>>>(a, part, o, ol, sums, p.splits, shift);
+    else if (p.splits > 1) join_few<T><<<linear_grid((rows * ((a.dim + 3) / 4) + 255) / 256, 256), 256, 0, s>>>(a, part, o, ol, sums, p.splits, shift);
   })
   return check_launch("cross_attention");
 }

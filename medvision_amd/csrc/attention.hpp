@@ -24,14 +24,51 @@ struct AttentionArgs {
   float scale;   // of the results; its magnitude times log2(e) scales the products, its sign goes into the queries
   __device__ __forceinline__ int length(int b) const { return lengths ? min(max(lengths[b], 0), keys) : keys; }
   __device__ __forceinline__ bool counts(int b, int j) const { return !mask || mask[b * mask_stride + j]; }
+  // of the logarithms [batch, heads, queries], for a row of the output [batch, queries, heads]
+  __device__ __forceinline__ long log_at(long row) const {
+    const long i = row / heads, b = i / queries;
+    return (b * heads + (row - i * heads)) * queries + (i - b * queries);
+  }
   __device__ __forceinline__ float factor() const { return fabsf(scale) * kLog2e; }
 };
 
 // Rows of a head of keys: the queries of all heads that share it, one after the other.
 struct RowOf {
   int head, query;
-  __device__ __forceinline__ RowOf(const AttentionArgs &a, int g, int row) : head(g * (a.heads / a.key_heads) + row / a.queries), query(row % a.queries) {}
+  __device__ __forceinline__ RowOf(const AttentionArgs &a, int g, int row) : head(g), query(row) {
+    if (a.heads != a.key_heads) {
+      head = row / a.queries;
+      query = row - head * a.queries;
+      head += g * (a.heads / a.key_heads);
+    }
+  }
 };
+
+// A workgroup's place: tiles first, then splits, heads of keys and samples, so that neighbours share what they read.
+struct Place {
+  int tile, split, g, b;
+  bool in;
+  __device__ __forceinline__ Place(const AttentionArgs &a, int tiles, int splits) {
+    const unsigned all = static_cast<unsigned>(tiles) * splits * a.batch * a.key_heads;
+    unsigned id = linear_block();
+    in = id < all;
+    if (!in) return;
+    id = xcd_contiguous(id, all);
+    unsigned rest = id / tiles;
+    tile = id - rest * tiles;
+    split = 0;
+    if (splits > 1) {
+      split = rest % splits;
+      rest /= splits;
+    }
+    b = rest / a.key_heads;
+    g = rest - b * a.key_heads;
+  }
+};
+// The share of `all` steps that a split does
+__device__ __forceinline__ int share(int all, int split, int splits) {
+  return splits == 1 ? (split ? all : 0) : static_cast<int>(static_cast<long>(all) * split / splits);
+}
 
 // ---- products of 32 x 32 ---------------------------------------------------------------------------------
 // Row r of a result: lane % 32 is its column, register i holds row 8 (i / 4) + 4 (lane / 32) + i % 4.
@@ -62,14 +99,14 @@ template <> struct Mma<__hip_bfloat16> {
 };
 
 // ---- tiles in LDS -------------------------------------------------------------------------------------------
-// `Rows` rows of DP elements in pieces of 16 bytes.  Pieces of a row are exchanged by its number, so that eight rows of one
-// column of pieces lie in different banks.
+// `Rows` rows of DP elements in pieces of 16 bytes.  Pieces of a row are exchanged by its number: eight rows of one column of
+// pieces lie in different banks (whole rows are read so), and so do four rows of one pair of pieces (transposed ones).
 template <typename T, int DP, int Rows> struct Tile {
   static constexpr int kPer = 16 / sizeof(T), kPieces = DP / kPer, kCount = Rows * kPieces;
   u32x4 at[kCount];
   static __device__ __forceinline__ int place(int row, int piece) {
-    if constexpr (kPieces == 4) return row * 4 + (piece ^ ((row >> 1) & 3));
-    else return row * kPieces + (piece ^ (row & 7));
+    if constexpr (kPieces == 4) return row * 4 + (piece ^ ((row & 2) | ((row >> 2) & 1)));
+    else return row * kPieces + (piece ^ ((row & 3) << 1 | ((row >> 2) & 1)));
   }
 };
 
@@ -90,29 +127,80 @@ template <typename T> __device__ __forceinline__ u32x4 load_piece(const T *row, 
   return r;
 }
 
-// What a thread of `Threads` brings of a tile: loaded ahead into registers, put into LDS later.
-template <typename T, int DP, int Rows, int Threads> struct Carry {
+// Two tiles of the same rows (keys and values, queries and gradients) on their way into LDS: each of 256 threads has one
+// column of pieces, and every kStep-th row of it.
+template <typename T, int DP, int Rows> struct Pair {
   using L = Tile<T, DP, Rows>;
-  static constexpr int kMine = (L::kCount + Threads - 1) / Threads;
-  u32x4 r[kMine];
-  // rows `first` + 0 .. Rows - 1 of those below `last`; `row(i)` gives the address of one, `use(i)` whether it counts
-  template <typename Row, typename Use>
-  __device__ __forceinline__ void load(int thread, int first, int last, int dim, const Row &row, const Use &use) {
+  static constexpr int kStep = 256 / L::kPieces, kMine = Rows / kStep;
+  static_assert(Rows % kStep == 0, "");
+  u32x4 a[kMine], b[kMine];
+  int row, d, dim;
+  long stride_a, stride_b, at_a, at_b;   // of this thread's first piece
+  __device__ __forceinline__ Pair(long stride_a, long stride_b, int dim)
+      : row(threadIdx.x / L::kPieces), d(threadIdx.x % L::kPieces * L::kPer), dim(dim), stride_a(stride_a), stride_b(stride_b) {
+    at_a = row * stride_a + (d < dim ? d : 0), at_b = row * stride_b + (d < dim ? d : 0);
+  }
+  // Rows 0 .. left - 1 from two addresses on.  Whole tiles without a branch; what stands for elements that do not exist is
+  // any value, to be replaced by put().
+  __device__ __forceinline__ void load(const T *from_a, const T *from_b, int left) {
+    if (left >= Rows && dim % L::kPer == 0) {
+#pragma unroll
+      for (int n = 0; n < kMine; ++n) {
+        a[n] = reinterpret_cast<const Loose<u32x4, sizeof(T)> *>(from_a + n * kStep * stride_a + at_a)->v;
+        b[n] = reinterpret_cast<const Loose<u32x4, sizeof(T)> *>(from_b + n * kStep * stride_b + at_b)->v;
+      }
+      return;
+    }
 #pragma unroll
     for (int n = 0; n < kMine; ++n) {
-      const int at = thread + n * Threads, i = first + at / L::kPieces, d = at % L::kPieces * L::kPer;
-      r[n] = u32x4{0, 0, 0, 0};
-      if (i < last && d < dim && use(i)) r[n] = load_piece<T>(row(i), d, dim);
+      a[n] = b[n] = u32x4{0, 0, 0, 0};
+      if (row + n * kStep < left && d < dim) {
+        a[n] = load_piece<T>(from_a + (row + n * kStep) * stride_a, d, dim);
+        b[n] = load_piece<T>(from_b + (row + n * kStep) * stride_b, d, dim);
+      }
     }
   }
-  __device__ __forceinline__ void put(int thread, L &to) const {
+  // zeros in the rows that a mask leaves out (they may hold anything, and NaN times a weight of zero is NaN)
+  __device__ __forceinline__ void keep(const unsigned char *mask, int left) {
+    bool use[kMine];
+#pragma unroll
+    for (int n = 0; n < kMine; ++n) use[n] = mask[min(row + n * kStep, left - 1)];
 #pragma unroll
     for (int n = 0; n < kMine; ++n) {
-      const int at = thread + n * Threads;
-      if (L::kCount % Threads == 0 || at < L::kCount) to.at[L::place(at / L::kPieces, at % L::kPieces)] = r[n];
+      a[n] = use[n] ? a[n] : u32x4{0, 0, 0, 0};
+      b[n] = use[n] ? b[n] : u32x4{0, 0, 0, 0};
+    }
+  }
+  __device__ __forceinline__ void put(L (&to)[2]) {
+    if (dim < DP && d >= dim) {
+#pragma unroll
+      for (int n = 0; n < kMine; ++n) a[n] = b[n] = u32x4{0, 0, 0, 0};
+    }
+#pragma unroll
+    for (int n = 0; n < kMine; ++n) {
+      const int at = L::place(row + n * kStep, d / L::kPer);
+      to[0].at[at] = a[n], to[1].at[at] = b[n];
     }
   }
 };
+
+// Keys (or rows) that a workgroup has in LDS at a time, and whether twice: the next ones are written while these are read.
+template <typename T, int DP, bool Few> struct Staging {
+  static constexpr int kRows = Few || (sizeof(T) == 2 && DP == 32) ? 128 : sizeof(T) == 4 && DP == 128 ? 32 : 64;
+  static constexpr int kBytes = 2 * kRows * DP * static_cast<int>(sizeof(T));
+  static constexpr int kBuffers = kBytes <= 32768 ? 2 : 1;
+};
+
+// Whether the kernels for few rows or keys take this type and width: float32 heads of more than 64 channels would not fit
+// into the registers.
+template <typename T, int DP> constexpr bool kHasFew = sizeof(T) == 2 || DP <= 64;
+inline bool has_few(int dtype, int dim) { return dtype != MV_F32 || dim <= 64; }
+
+// Which of 64 keys count: bits for lanes' keys
+__device__ __forceinline__ unsigned long long use_bits(const AttentionArgs &a, int b, int first, int count, int length) {
+  const int lane = threadIdx.x & 63, j = first + lane;
+  return __ballot(lane < count && j < length && a.counts(b, j));
+}
 
 // One column (a query, a key) per lane % 32, all DP elements: the second operand of products over the elements.
 template <typename T, int DP> struct Column {
@@ -210,6 +298,33 @@ __device__ __forceinline__ void add_transposed(const Tile<T, DP, Rows> &tile, in
       }
     }
   }
+}
+
+// Sums of parts, in their order: `Slices` threads share the parts of one element of the first `count` (or of the second ones,
+// which lie `splits` times `count` behind and go to `second`).
+template <typename T, int Slices>
+__global__ __launch_bounds__(256) void add_parts(const float *part, T *out, T *second, long count, int splits) {
+  constexpr int kWide = 256 / Slices;
+  __shared__ float sums[Slices][kWide];
+  const int in = threadIdx.x % kWide, slice = threadIdx.x / kWide;
+  long at = static_cast<long>(linear_block()) * kWide + in;
+  const bool live = at < (second ? 2 : 1) * count, other = at >= count;
+  if (other) at += (splits - 1) * count;   // (the first part of the second ones)
+  float sum = 0.f;
+  if (live) {
+#pragma unroll 8
+    for (int s = slice; s < splits; s += Slices) sum += part[s * count + at];
+  }
+  if constexpr (Slices > 1) {
+    sums[slice][in] = sum;
+    __syncthreads();
+    if (slice) return;
+#pragma unroll
+    for (int i = 1; i < Slices; ++i) sum += sums[i][in];
+  }
+  if (!live) return;
+  if (other) second[at - splits * count] = store_cast<T>(sum);
+  else out[at] = store_cast<T>(sum);
 }
 
 // The other half of the wavefront has the other rows of the same column.

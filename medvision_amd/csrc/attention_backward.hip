@@ -67,24 +67,39 @@ template <typename O, int N> __device__ __forceinline__ void store_column(O *row
 // ---- dq -------------------------------------------------------------------------------------------------------
 // As the forward kernel; leaves d_i for the next one.
 template <typename T, int DP, int WQ>
-__global__ __launch_bounds__(256, DP == 128 || (sizeof(T) == 4 && DP == 64) ? 1 : 2) void attend_grad_query(
+__global__ __launch_bounds__(256, DP == 128 || (sizeof(T) == 4 && DP == 64) ? 1 : DP == 64 || sizeof(T) == 4 ? 2 : 3) void attend_grad_query(
     AttentionArgs a, const T *out, const T *low, const float *lse, const T *go, T *gq, float *delta, float *part, int row_tiles, int splits) {
-  constexpr int kTiles = WQ == 4 ? 2 : 1, kKeys = WQ == 4 ? 64 : 128, kOut = DP / 32;
+  using S = Staging<T, DP, WQ == 1>;
+  constexpr int kKeys = S::kRows, kSteps = WQ == 4 ? kKeys / 32 : 1, kOut = DP / 32;
   using L = Tile<T, DP, kKeys>;
-  __shared__ L tiles[2];
-  L &ks = tiles[0], &vs = tiles[1];
-  const int groups = row_tiles * splits * a.batch * a.key_heads;
-  unsigned id = linear_block();
-  if (id >= static_cast<unsigned>(groups)) return;
-  id = xcd_contiguous(id, groups);
-  const int tile = id % row_tiles, split = id / row_tiles % splits, g = id / row_tiles / splits % a.key_heads, b = id / row_tiles / splits / a.key_heads;
+  __shared__ L tiles[S::kBuffers][2];
+  const Place place(a, row_tiles, splits);
+  if (!place.in) return;
+  const int split = place.split, g = place.g, b = place.b;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
-  const int rows = a.heads / a.key_heads * a.queries, row = tile * 32 * WQ + (WQ == 4 ? wave * 32 : 0) + (lane & 31);
+  const int rows = a.heads / a.key_heads * a.queries, row = place.tile * 32 * WQ + (WQ == 4 ? wave * 32 : 0) + (lane & 31);
   const bool live = row < rows;
   const RowOf at(a, g, live ? row : rows - 1);
   const long at_row = (static_cast<long>(b) * a.queries + at.query) * a.heads + at.head,
              at_l = (static_cast<long>(b) * a.heads + at.head) * a.queries + at.query;
   const float factor = a.factor();
+
+  const T *const k = static_cast<const T *>(a.k) + b * a.ks[0] + g * a.ks[2], *const v = static_cast<const T *>(a.v) + b * a.vs[0] + g * a.vs[2];
+  const int length = a.length(b), all_tiles = (length + kKeys - 1) / kKeys;
+  const int first = share(all_tiles, split, splits), last = share(all_tiles, split + 1, splits);
+  const int my_key = WQ == 4 ? 0 : 32 * wave;
+  Pair<T, DP, kKeys> next(a.ks[1], a.vs[1], a.dim);
+  unsigned long long next_use[(kSteps + 1) / 2] = {};
+  auto load = [&](int t) {
+    next.load(k + t * kKeys * a.ks[1], v + t * kKeys * a.vs[1], length - t * kKeys);
+#pragma unroll
+    for (int n = 0; n < (kSteps + 1) / 2; ++n) next_use[n] = use_bits(a, b, t * kKeys + my_key + 64 * n, kSteps == 1 ? 32 : 64, length);
+  };
+  auto put = [&](int t) {
+    if (a.mask) next.keep(a.mask + b * a.mask_stride + t * kKeys, length - t * kKeys);
+    next.put(tiles[t % S::kBuffers]);
+  };
+  if (first < last) load(first);
 
   Column<T, DP> q, d_o;
   float d_i;
@@ -102,45 +117,36 @@ __global__ __launch_bounds__(256, DP == 128 || (sizeof(T) == 4 && DP == 64) ? 1 
   float sums_log = live ? lse[at_l] : INFINITY;
   if (sums_log == -INFINITY) sums_log = INFINITY;   // no key counts: weights of zero
   if (live && split == 0 && half == 0 && (WQ == 4 || wave == 0)) delta[at_l] = d_i;
-
-  const T *const k = static_cast<const T *>(a.k) + b * a.ks[0] + g * a.ks[2], *const v = static_cast<const T *>(a.v) + b * a.vs[0] + g * a.vs[2];
-  const int length = a.length(b), all_tiles = (length + kKeys - 1) / kKeys;
-  const int first = static_cast<int>(static_cast<long>(all_tiles) * split / splits), last = static_cast<int>(static_cast<long>(all_tiles) * (split + 1) / splits);
-  const int my_key = WQ == 4 ? 0 : 32 * wave;
-  Carry<T, DP, kKeys, 256> next_k, next_v;
-  unsigned long long next_use = 0;
-  auto load = [&](int t) {
-    const auto use = [&](int j) { return a.counts(b, j); };
-    next_k.load(threadIdx.x, t * kKeys, length, a.dim, [&](int j) { return k + j * a.ks[1]; }, use);
-    next_v.load(threadIdx.x, t * kKeys, length, a.dim, [&](int j) { return v + j * a.vs[1]; }, use);
-    const int j = t * kKeys + my_key + lane;
-    next_use = __ballot(j < length && (WQ == 4 || lane < 32) && a.counts(b, min(j, length - 1)));
-  };
+  if (first < last) put(first);
 
   f32x16 sum[kOut] = {};
   Raise<T> raise;
-  if (first < last) load(first);
   for (int t = first; t < last; ++t) {
-    if (t > first) __syncthreads();
-    next_k.put(threadIdx.x, ks);
-    next_v.put(threadIdx.x, vs);
-    const unsigned long long use = next_use;
+    unsigned long long use[(kSteps + 1) / 2];
+#pragma unroll
+    for (int n = 0; n < (kSteps + 1) / 2; ++n) use[n] = next_use[n];
     __syncthreads();
     if (t + 1 < last) load(t + 1);
-    if (!use) continue;
+    const L &ks = tiles[t % S::kBuffers][0], &vs = tiles[t % S::kBuffers][1];
 #pragma unroll
-    for (int n = 0; n < kTiles; ++n) {
-      const f32x16 s = times(ks, my_key + 32 * n, q, lane), dp = times(vs, my_key + 32 * n, d_o, lane);
+    for (int n = 0; n < kSteps; ++n) {
+      const unsigned word = static_cast<unsigned>(use[n / 2] >> (32 * (n % 2)));
+      if (!word) continue;
+      const int key = my_key + 32 * n;
+      const f32x16 s = times(ks, key, q, lane), dp = times(vs, key, d_o, lane);
       float ds[16];
 #pragma unroll
       for (int i = 0; i < 16; ++i) ds[i] = __builtin_amdgcn_exp2f(fmaf(s[i], factor, -sums_log)) * (dp[i] - d_i);
-      const unsigned word = static_cast<unsigned>(use >> (32 * n));
       if (word != ~0u) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) ds[i] = word >> (4 * half) >> result_row(i, 0) & 1 ? ds[i] : 0.f;
       }
       raise.scale(ds, sum);
-      add_transposed(ks, my_key + 32 * n, ds, sum, lane);
+      add_transposed(ks, key, ds, sum, lane);
+    }
+    if (t + 1 < last) {
+      if constexpr (S::kBuffers == 1) __syncthreads();
+      put(t + 1);
     }
   }
   const float back = raise.back() * a.scale;
@@ -167,74 +173,83 @@ __global__ __launch_bounds__(256, DP == 128 || (sizeof(T) == 4 && DP == 64) ? 1 
 // rows; WK = 1 (few keys): the same 32 keys, each wavefront 32 of 128 rows, joined at the end.  A key that does not count
 // spoils nothing but its own column, which is written as zeros.
 template <typename T, int DP, int WK>
-__global__ __launch_bounds__(256, DP == 128 || (sizeof(T) == 4 && DP == 64) ? 1 : 2) void attend_grad_key(
+__global__ __launch_bounds__(256, DP == 128 || (sizeof(T) == 4 && DP == 64) ? 1 : DP == 64 || sizeof(T) == 4 ? 2 : 3) void attend_grad_key(
     AttentionArgs a, const float *lse, const float *delta, const T *go, T *gk, T *gv, float *part, int key_tiles, int splits) {
-  constexpr int kRows = WK == 4 ? 32 : 128, kOut = DP / 32;
+  using S = Staging<T, DP, WK == 1>;
+  constexpr int kRows = S::kRows, kSteps = WK == 4 ? kRows / 32 : 1, kOut = DP / 32;
   constexpr float kShift = __is_same(T, __half) ? 15.f : 0.f;   // as in the forward pass
   using L = Tile<T, DP, kRows>;
-  __shared__ L tiles[2];
-  __shared__ float stats[2][kRows];
-  L &qs = tiles[0], &os = tiles[1];
-  const int groups = key_tiles * splits * a.batch * a.key_heads;
-  unsigned id = linear_block();
-  if (id >= static_cast<unsigned>(groups)) return;
-  id = xcd_contiguous(id, groups);
-  const int tile = id % key_tiles, split = id / key_tiles % splits, g = id / key_tiles / splits % a.key_heads, b = id / key_tiles / splits / a.key_heads;
+  __shared__ L tiles[S::kBuffers][2];
+  __shared__ float stats[S::kBuffers][2][kRows];
+  const Place place(a, key_tiles, splits);
+  if (!place.in) return;
+  const int split = place.split, g = place.g, b = place.b;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
-  const int j = tile * 32 * WK + (WK == 4 ? wave * 32 : 0) + (lane & 31), length = a.length(b);
+  const int j = place.tile * 32 * WK + (WK == 4 ? wave * 32 : 0) + (lane & 31), length = a.length(b);
   const bool live = j < a.keys, use = j < length && a.counts(b, j);
   const float factor = a.factor();
+
+  // rows of one head after the other; nothing to sum where none of the workgroup's keys counts by its length
+  const int group = a.heads / a.key_heads, per_head = (a.queries + kRows - 1) / kRows;
+  const int all_tiles = place.tile * 32 * WK < length ? group * per_head : 0;
+  const int first = share(all_tiles, split, splits), last = share(all_tiles, split + 1, splits);
+  const int my_row = WK == 4 ? 0 : 32 * wave;
+  float next_l = INFINITY, next_d = 0.f;
+  const long go_row = static_cast<long>(a.heads) * a.dim;
+  Pair<T, DP, kRows> next(a.qs[1], go_row, a.dim);
+  auto load = [&](int t) {
+    const int in_group = group > 1 ? t / per_head : 0, row = (t - in_group * per_head) * kRows, h = g * group + in_group, left = a.queries - row;
+    next.load(static_cast<const T *>(a.q) + b * a.qs[0] + row * a.qs[1] + h * a.qs[2],
+              go + (static_cast<long>(b) * a.queries + row) * go_row + static_cast<long>(h) * a.dim, left);
+    next_l = INFINITY, next_d = 0.f;
+    if (threadIdx.x < min(kRows, left)) {
+      const long from = (static_cast<long>(b) * a.heads + h) * a.queries + row + threadIdx.x;
+      next_l = lse[from], next_d = delta[from];
+    }
+  };
+  auto put = [&](int t) {
+    next.put(tiles[t % S::kBuffers]);
+    if (threadIdx.x < kRows) {
+      stats[t % S::kBuffers][0][threadIdx.x] = next_l == -INFINITY ? INFINITY : next_l - kShift;
+      stats[t % S::kBuffers][1][threadIdx.x] = next_d;
+    }
+  };
+  if (first < last) load(first);
   Column<T, DP> k, v;
   k.load(static_cast<const T *>(a.k) + b * a.ks[0] + j * a.ks[1] + g * a.ks[2], use, a.dim, half);
   v.load(static_cast<const T *>(a.v) + b * a.vs[0] + j * a.vs[1] + g * a.vs[2], use, a.dim, half);
   if (a.scale < 0.f) k.negate();
-
-  const int rows = a.heads / a.key_heads * a.queries;
-  // (nothing to sum where none of the workgroup's keys counts by its length)
-  const int all_tiles = tile * 32 * WK < length ? (rows + kRows - 1) / kRows : 0;
-  const int first = static_cast<int>(static_cast<long>(all_tiles) * split / splits), last = static_cast<int>(static_cast<long>(all_tiles) * (split + 1) / splits);
-  const int my_row = WK == 4 ? 0 : 32 * wave;
-  Carry<T, DP, kRows, 256> next_q, next_o;
-  float next_l = INFINITY, next_d = 0.f;
-  auto load = [&](int t) {
-    const auto all = [](int) { return true; };
-    next_q.load(threadIdx.x, t * kRows, rows, a.dim, [&](int r) {
-      const RowOf at(a, g, r);
-      return static_cast<const T *>(a.q) + b * a.qs[0] + at.query * a.qs[1] + at.head * a.qs[2]; }, all);
-    next_o.load(threadIdx.x, t * kRows, rows, a.dim, [&](int r) {
-      const RowOf at(a, g, r);
-      return go + ((static_cast<long>(b) * a.queries + at.query) * a.heads + at.head) * a.dim; }, all);
-    const int r = t * kRows + threadIdx.x;
-    next_l = INFINITY, next_d = 0.f;
-    if (threadIdx.x < kRows && r < rows) {
-      const RowOf at(a, g, r);
-      const long from = (static_cast<long>(b) * a.heads + at.head) * a.queries + at.query;
-      next_l = lse[from], next_d = delta[from];
-      next_l = next_l == -INFINITY ? INFINITY : next_l - kShift;
-    }
-  };
+  if (first < last) put(first);
 
   f32x16 dk[kOut] = {}, dv[kOut] = {};
   Raise<T> raise;
-  if (first < last) load(first);
   for (int t = first; t < last; ++t) {
-    if (t > first) __syncthreads();
-    next_q.put(threadIdx.x, qs);
-    next_o.put(threadIdx.x, os);
-    if (threadIdx.x < kRows) stats[0][threadIdx.x] = next_l, stats[1][threadIdx.x] = next_d;
     __syncthreads();
     if (t + 1 < last) load(t + 1);
-    const f32x16 s = times(qs, my_row, k, lane), dp = times(os, my_row, v, lane);
-    float p[16], ds[16];
+    const L &qs = tiles[t % S::kBuffers][0], &os = tiles[t % S::kBuffers][1];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int r = my_row + result_row(i, 0) + 4 * half;
-      p[i] = __builtin_amdgcn_exp2f(fmaf(s[i], factor, -stats[0][r]));
-      ds[i] = p[i] * (dp[i] - stats[1][r]);
+    for (int n = 0; n < kSteps; ++n) {
+      const int row = my_row + 32 * n;
+      const f32x16 s = times(qs, row, k, lane), dp = times(os, row, v, lane);
+      float p[16], ds[16];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const f32x4 l4 = *reinterpret_cast<const f32x4 *>(&stats[t % S::kBuffers][0][row + 8 * i + 4 * half]),
+                    d4 = *reinterpret_cast<const f32x4 *>(&stats[t % S::kBuffers][1][row + 8 * i + 4 * half]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          p[4 * i + e] = __builtin_amdgcn_exp2f(fmaf(s[4 * i + e], factor, -l4[e]));
+          ds[4 * i + e] = p[4 * i + e] * (dp[4 * i + e] - d4[e]);
+        }
+      }
+      add_transposed(os, row, p, dv, lane);
+      raise.scale(ds, dk);
+      add_transposed(qs, row, ds, dk, lane);
     }
-    add_transposed(os, my_row, p, dv, lane);
-    raise.scale(ds, dk);
-    add_transposed(qs, my_row, ds, dk, lane);
+    if (t + 1 < last) {
+      if constexpr (S::kBuffers == 1) __syncthreads();
+      put(t + 1);
+    }
   }
   const float down = kShift ? 1.f / 32768.f : 1.f, back = raise.back() * (a.scale * down);
 #pragma unroll
@@ -271,14 +286,10 @@ __global__ __launch_bounds__(256, DP == 128 || (sizeof(T) == 4 && DP == 64) ? 1 
   }
 }
 
-// Sums of the splits, in their order
-template <typename T>
-__global__ __launch_bounds__(256) void add_splits(const float *part, T *out, long count, int splits) {
-  const long at = static_cast<long>(linear_block()) * 256 + threadIdx.x;
-  if (at >= count) return;
-  float sum = 0.f;
-  for (int s = 0; s < splits; ++s) sum += part[s * count + at];
-  out[at] = store_cast<T>(sum);
+template <typename T> void sum_parts(const float *part, T *out, T *second, long count, int splits, hipStream_t s) {
+  const long all = (second ? 2 : 1) * count;
+  if (splits >= 16) add_parts<T, 16><<<linear_grid((all + 15) / 16, 256), 256, 0, s>>>(part, out, second, count, splits);
+  else add_parts<T, 1><<<linear_grid((all + 255) / 256, 256), 256, 0, s>>>(part, out, second, count, splits);
 }
 
 struct BackwardPlan {
@@ -286,16 +297,17 @@ struct BackwardPlan {
   int row_tiles, query_splits, key_tiles, key_splits;
 };
 
-BackwardPlan backward_plan(const mv_attention_shape *s) {
+BackwardPlan backward_plan(const mv_attention_shape *s, int dtype) {
   BackwardPlan p;
   const long rows = static_cast<long>(s->heads / s->key_heads) * s->queries, heads = std::max(1L, static_cast<long>(s->batch) * s->key_heads);
-  p.few_rows = rows <= 32;
-  p.few_keys = s->keys <= 32;
+  p.few_rows = rows <= 32 && has_few(dtype, s->dim);
+  p.few_keys = s->keys <= 32 && has_few(dtype, s->dim);
   p.row_tiles = static_cast<int>(p.few_rows ? 1 : (rows + 127) / 128);
   p.key_tiles = static_cast<int>(p.few_keys ? 1 : (s->keys + 127L) / 128);
-  const long key_steps = p.few_rows ? (s->keys + 127L) / 128 : (s->keys + 63L) / 64, row_steps = p.few_keys ? (rows + 127) / 128 : (rows + 31) / 32;
-  p.query_splits = static_cast<int>(std::max(1L, std::min(512 / std::max(1L, p.row_tiles * heads), key_steps / 4)));
-  p.key_splits = static_cast<int>(std::max(1L, std::min(512 / std::max(1L, p.key_tiles * heads), row_steps / 4)));
+  const long least = dtype == MV_F32 ? 64 : 512;   // keys, or rows, that are worth a split
+  const long key_steps = (s->keys + least - 1) / least, row_steps = s->heads / s->key_heads * ((s->queries + least - 1) / least);
+  p.query_splits = static_cast<int>(std::max(1L, std::min(512 / std::max(1L, p.row_tiles * heads), key_steps)));
+  p.key_splits = static_cast<int>(std::max(1L, std::min(512 / std::max(1L, p.key_tiles * heads), row_steps)));
   return p;
 }
 
@@ -307,19 +319,25 @@ void launch_backward(const BackwardPlan &p, const AttentionArgs &a, const void *
   const T *const o = static_cast<const T *>(out), *const ol = static_cast<const T *>(low), *const d_o = static_cast<const T *>(go);
   if (queries) {
     const dim3 grid = linear_grid(heads * p.row_tiles * p.query_splits, 256);
-    if (p.few_rows) attend_grad_query<T, DP, 1><<<grid, 256, 0, s>>>(a, o, ol, lse, d_o, static_cast<T *>(gq), delta, part, p.row_tiles, p.query_splits);
-    else attend_grad_query<T, DP, 4><<<grid, 256, 0, s>>>(a, o, ol, lse, d_o, static_cast<T *>(gq), delta, part, p.row_tiles, p.query_splits);
-    if (p.query_splits > 1) add_splits<T><<<linear_grid((queries + 255) / 256, 256), 256, 0, s>>>(part, static_cast<T *>(gq), queries, p.query_splits);
+    bool done = false;
+    if constexpr (kHasFew<T, DP>)
+      if (p.few_rows) {
+        attend_grad_query<T, DP, 1><<<grid, 256, 0, s>>>(a, o, ol, lse, d_o, static_cast<T *>(gq), delta, part, p.row_tiles, p.query_splits);
+        done = true;
+      }
+    if (!done) attend_grad_query<T, DP, 4><<<grid, 256, 0, s>>>(a, o, ol, lse, d_o, static_cast<T *>(gq), delta, part, p.row_tiles, p.query_splits);
+    if (p.query_splits > 1) sum_parts<T>(part, static_cast<T *>(gq), nullptr, queries, p.query_splits, s);
   }
   if (keys) {
     const dim3 grid = linear_grid(heads * p.key_tiles * p.key_splits, 256);
-    if (p.few_keys) attend_grad_key<T, DP, 1><<<grid, 256, 0, s>>>(a, lse, delta, d_o, static_cast<T *>(gk), static_cast<T *>(gv), part, p.key_tiles, p.key_splits);
-    else attend_grad_key<T, DP, 4><<<grid, 256, 0, s>>>(a, lse, delta, d_o, static_cast<T *>(gk), static_cast<T *>(gv), part, p.key_tiles, p.key_splits);
-    if (p.key_splits > 1) {
-      const dim3 sums = linear_grid((keys + 255) / 256, 256);
-      add_splits<T><<<sums, 256, 0, s>>>(part, static_cast<T *>(gk), keys, p.key_splits);
-      add_splits<T><<<sums, 256, 0, s>>>(part + p.key_splits * keys, static_cast<T *>(gv), keys, p.key_splits);
-    }
+    bool done = false;
+    if constexpr (kHasFew<T, DP>)
+      if (p.few_keys) {
+        attend_grad_key<T, DP, 1><<<grid, 256, 0, s>>>(a, lse, delta, d_o, static_cast<T *>(gk), static_cast<T *>(gv), part, p.key_tiles, p.key_splits);
+        done = true;
+      }
+    if (!done) attend_grad_key<T, DP, 4><<<grid, 256, 0, s>>>(a, lse, delta, d_o, static_cast<T *>(gk), static_cast<T *>(gv), part, p.key_tiles, p.key_splits);
+    if (p.key_splits > 1) sum_parts<T>(part, static_cast<T *>(gk), static_cast<T *>(gv), keys, p.key_splits, s);
   }
 }
 
@@ -332,7 +350,7 @@ extern "C" {
 
 size_t mv_cross_attention_backward_workspace_bytes(const mv_attention_shape *s, int dtype) {
   if (attention_sizes(s, dtype)) return 0;
-  const BackwardPlan p = backward_plan(s);
+  const BackwardPlan p = backward_plan(s, dtype);
   const size_t queries = static_cast<size_t>(s->batch) * s->queries * s->heads, keys = static_cast<size_t>(s->batch) * s->keys * s->key_heads;
   const size_t for_queries = p.query_splits > 1 ? p.query_splits * queries * s->dim : 0, for_keys = p.key_splits > 1 ? 2 * p.key_splits * keys * s->dim : 0;
   return sizeof(float) * (queries + std::max(for_queries, for_keys));
@@ -348,7 +366,7 @@ int mv_cross_attention_backward(const void *query, const void *key, const void *
   MV_REQUIRE(rows == 0 || (query && output && lse && grad_output && grad_query), "a tensor is missing");
   MV_REQUIRE(columns == 0 || (key && value && grad_key && grad_value), "a tensor is missing");
   MV_REQUIRE(rows == 0 || (workspace && workspace_bytes >= mv_cross_attention_backward_workspace_bytes(shape, dtype)), "the workspace is too small");
-  const BackwardPlan p = backward_plan(shape);
+  const BackwardPlan p = backward_plan(shape, dtype);
   float *const delta = static_cast<float *>(workspace), *const part = delta + rows;
   const float *const sums = static_cast<const float *>(lse);
   const hipStream_t s = static_cast<hipStream_t>(stream);
