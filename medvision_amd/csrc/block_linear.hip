@@ -139,54 +139,93 @@ __global__ __launch_bounds__(64 * WM * WN * WK, WM *WN *WK / 4) void product_til
   bring_scales(0);
   bring(0);
   put_scales(0);
-  for (int step = 0; step < steps; ++step) {
+  // The next weights are on their way while these are multiplied, and the last products are added meanwhile.  Where there are
+  // registers for it, the last weights of a step are multiplied in the next one, while its first operands come from LDS
+  // (4000 x 12544 x 1024: LATER us with, 73.6 without; tiles of 256 x 256 would spill 210 registers).
+  constexpr bool kLater = S::kTM * S::kTN <= 16;
+  i32x8 x0[S::kTM] = {}, x1[S::kTM] = {}, v = {};
+  float scale_before[S::kTM] = {};
+  const int p0 = (g ^ (r16 & 7)) * 16, p1 = ((g + 4) ^ (r16 & 7)) * 16;
+  auto piece_of = [&](const unsigned char *tile, int row16) {
+    // piece g and piece g + 4 of the row: any order of k serves, as long as both operands have the same
+    const unsigned char *row = tile + (row16 * 16 + r16) * kBlock;
+    return join(*reinterpret_cast<const i32x4 *>(row + p0), *reinterpret_cast<const i32x4 *>(row + p1));
+  };
+  auto add = [&](int u, const f32x4 (&d)[S::kTM], const float (&s)[S::kTM]) {
+#pragma unroll
+    for (int t = 0; t < S::kTM; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[t][u][i] = fmaf(d[t][i], s[t], acc[t][u][i]);
+  };
+  auto one_step = [&](int step, i32x8 (&now)[S::kTM], const i32x8 (&before)[S::kTM]) {
     __syncthreads();   // this step's operands are there, and nobody reads the place of the next ones
     if ((step & 3) == 0) bring_scales(step + 4);
     if (step + 1 < steps) bring(step + 1);
     if ((step & 3) == 3) put_scales(step + 1);
-    if (WK == 1 || first + step * WK + group < last) {
-      const unsigned char *xs = lds + ((step & 1) * WK + group) * S::kStage, *wsm = xs + BM * kBlock;
-      // piece g and piece g + 4 of the row: any order of k serves, as long as both operands have the same
-      const int p0 = (g ^ (r16 & 7)) * 16, p1 = ((g + 4) ^ (r16 & 7)) * 16;
-      const float *const now = scale[(step >> 2) & 1][step & 3][group];
-      float s[S::kTM];
+    if (WK > 1 && first + step * WK + group >= last) {   // (the last step of a group that has no block left)
 #pragma unroll
-      for (int t = 0; t < S::kTM; ++t) s[t] = now[(wm * S::kTM + t) * 16 + r16] * now[BM + wn * S::kTN * 16 / kBlock];
-      auto piece_of = [&](const unsigned char *tile, int row16) {
-        const unsigned char *row = tile + (row16 * 16 + r16) * kBlock;
-        return join(*reinterpret_cast<const i32x4 *>(row + p0), *reinterpret_cast<const i32x4 *>(row + p1));
-      };
-      // The next weights are on their way while these are multiplied, and the last products are added meanwhile.
-      i32x8 x[S::kTM], v = piece_of(wsm, wn * S::kTN);
-#pragma unroll
-      for (int t = 0; t < S::kTM; ++t) x[t] = piece_of(xs, wm * S::kTM + t);
-      f32x4 d[2][S::kTM];
-#pragma unroll
-      for (int u = 0; u <= S::kTN; ++u) {
-        i32x8 next = v;
-        if (u + 1 < S::kTN) next = piece_of(wsm, wn * S::kTN + u + 1);
-        if (u < S::kTN) {
-#pragma unroll
-          for (int t = 0; t < S::kTM; ++t) d[u & 1][t] = block_product(v, x[t]);
-        }
-        if (u) {
-#pragma unroll
-          for (int t = 0; t < S::kTM; ++t)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc[t][u - 1][i] = fmaf(d[(u - 1) & 1][t][i], s[t], acc[t][u - 1][i]);
-        }
-        v = next;
-        if (u < S::kTN) {
-#pragma unroll
-          for (int t = 0; t < S::kTM; ++t) {
-            __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);   // a matrix instruction
-            if (t == 0) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);   // LDS reads
-            if (u) __builtin_amdgcn_sched_group_barrier(0x2, 4, 0);   // four additions
-          }
-        }
-        __builtin_amdgcn_sched_barrier(0);
-      }
+      for (int t = 0; t < S::kTM; ++t)
+        if (kLater) now[t] = before[t];
+      return;
     }
+    const unsigned char *xs = lds + ((step & 1) * WK + group) * S::kStage, *wsm = xs + BM * kBlock;
+    const float *const factors = scale[(step >> 2) & 1][step & 3][group];
+    float s[S::kTM];
+    i32x8 next = piece_of(wsm, wn * S::kTN);
+#pragma unroll
+    for (int t = 0; t < S::kTM; ++t) now[t] = piece_of(xs, wm * S::kTM + t);
+#pragma unroll
+    for (int t = 0; t < S::kTM; ++t) s[t] = factors[(wm * S::kTM + t) * 16 + r16] * factors[BM + wn * S::kTN * 16 / kBlock];
+    __builtin_amdgcn_sched_barrier(0);
+    f32x4 d[2][S::kTM];
+    if constexpr (kLater) {
+#pragma unroll
+      for (int t = 0; t < S::kTM; ++t) d[1][t] = block_product(v, before[t]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    v = next;
+    static_assert(S::kTN % 2 == 0, "");
+#pragma unroll
+    for (int u = 0; u < (kLater ? S::kTN - 1 : S::kTN); ++u) {
+      if (u + 1 < S::kTN) next = piece_of(wsm, wn * S::kTN + u + 1);
+#pragma unroll
+      for (int t = 0; t < S::kTM; ++t) d[u & 1][t] = block_product(v, now[t]);
+      if (u) add(u - 1, d[(u - 1) & 1], s);
+      else if (kLater) add(S::kTN - 1, d[1], scale_before);
+      v = next;
+#pragma unroll
+      for (int t = 0; t < S::kTM; ++t) {
+        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);   // a matrix instruction
+        if (t == 0) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);   // LDS reads
+        if (u || kLater) __builtin_amdgcn_sched_group_barrier(0x2, 4, 0);   // four additions
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if constexpr (kLater) {
+      add(S::kTN - 2, d[0], s);
+#pragma unroll
+      for (int t = 0; t < S::kTM; ++t) scale_before[t] = s[t];
+    } else {
+      add(S::kTN - 1, d[1], s);
+    }
+  };
+  if constexpr (kLater) {
+    for (int step = 0; step < steps; step += 2) {
+      one_step(step, x0, x1);
+      if (step + 1 < steps) one_step(step + 1, x1, x0);
+    }
+  } else {
+    for (int step = 0; step < steps; ++step) one_step(step, x0, x0);
+  }
+  auto finish = [&](const i32x8 (&before)[S::kTM]) {
+    f32x4 d[S::kTM];
+#pragma unroll
+    for (int t = 0; t < S::kTM; ++t) d[t] = block_product(v, before[t]);
+    add(S::kTN - 1, d, scale_before);
+  };
+  if constexpr (kLater) {
+    if (steps & 1) finish(x0);
+    else finish(x1);
   }
   if (WK > 1) {   // the groups' sums, in their order
     f32x4 *const part = reinterpret_cast<f32x4 *>(lds);
@@ -296,13 +335,26 @@ __global__ __launch_bounds__(256) void product_rows(const unsigned char *q, cons
   for (int t = 0; t < TM; ++t) store_row(to, split, m0 + t * 16 + r16, n0 + 4 * g, acc[t]);
 }
 
-// The parts' sum, in their order
-template <typename T>
+// The parts' sum, in a fixed order: `Slices` threads share the parts of a result.
+template <typename T, int Slices>
 __global__ __launch_bounds__(256) void join_parts(const float *part, const T *bias, T *y, long count, int outputs, int splits) {
-  const long at = static_cast<long>(linear_block()) * 256 + threadIdx.x;
-  if (at >= count) return;
+  constexpr int kWide = 256 / Slices;
+  __shared__ float sums[Slices][kWide];
+  const int in = threadIdx.x % kWide, slice = threadIdx.x / kWide;
+  const long at = static_cast<long>(linear_block()) * kWide + in;
   float sum = 0.f;
-  for (int s = 0; s < splits; ++s) sum += part[s * count + at];
+  if (at < count) {
+#pragma unroll 4
+    for (int s = slice; s < splits; s += Slices) sum += part[s * count + at];
+  }
+  if constexpr (Slices > 1) {
+    sums[slice][in] = sum;
+    __syncthreads();
+    if (slice) return;
+#pragma unroll
+    for (int i = 1; i < Slices; ++i) sum += sums[i][in];
+  }
+  if (at >= count) return;
   if (bias) sum += load(bias + at % outputs);
   y[at] = store_cast<T>(sum);
 }
@@ -353,7 +405,8 @@ int product(const void *q, const void *qs, const void *w, const void *ws, const 
   launch(p, q, qs, w, ws, to, static_cast<int>(rows), inputs, outputs, s);
   if (part) {
     const long count = rows * outputs;
-    join_parts<T><<<linear_grid((count + 255) / 256, 256), 256, 0, s>>>(part, to.bias, to.y, count, outputs, p.splits);
+    if (p.splits > 8) join_parts<T, 8><<<linear_grid((count + 31) / 32, 256), 256, 0, s>>>(part, to.bias, to.y, count, outputs, p.splits);
+    else join_parts<T, 1><<<linear_grid((count + 255) / 256, 256), 256, 0, s>>>(part, to.bias, to.y, count, outputs, p.splits);
   }
   return check_launch("block_linear");
 }
