@@ -11,6 +11,7 @@ from .cuda_fun_tools import affine_2d, affine_3d, apply_offset_2d, apply_offset_
 from .cross_attention import cross_attention
 from .rms_norm import AddRMSNorm, add_rms_norm, add_rms_norm_quantized
 from .block_linear import BlockScaledLinear, block_linear, quantize_blocks
+from .region_decoder import RegionDecoderLayer, map_tokens
 
 __all__ = [
     'RoIAlign',
@@ -28,4 +29,5 @@ __all__ = [
     'cross_attention',
     'AddRMSNorm', 'add_rms_norm', 'add_rms_norm_quantized',
     'BlockScaledLinear', 'block_linear', 'quantize_blocks',
+    'RegionDecoderLayer', 'map_tokens',
 ]
