@@ -32,19 +32,20 @@ struct AttentionArgs {
   __device__ __forceinline__ float factor() const { return fabsf(scale) * kLog2e; }
 };
 
-// Rows of a head of keys: the queries of all heads that share it, one after the other.
+// Rows of a head of keys: the heads that share it, query after query (neighbours in memory).
 struct RowOf {
   int head, query;
   __device__ __forceinline__ RowOf(const AttentionArgs &a, int g, int row) : head(g), query(row) {
     if (a.heads != a.key_heads) {
-      head = row / a.queries;
-      query = row - head * a.queries;
-      head += g * (a.heads / a.key_heads);
+      const unsigned group = a.heads / a.key_heads;
+      query = static_cast<unsigned>(row) / group;
+      head = g * group + (row - query * group);
     }
   }
 };
 
-// A workgroup's place: tiles first, then splits, heads of keys and samples, so that neighbours share what they read.
+// A workgroup's place.  Neighbours share what they read: tiles of the same keys where those are the longer side, heads of the
+// same queries (of which two or four lie in a cache line) otherwise.
 struct Place {
   int tile, split, g, b;
   bool in;
@@ -54,15 +55,18 @@ struct Place {
     in = id < all;
     if (!in) return;
     id = xcd_contiguous(id, all);
-    unsigned rest = id / tiles;
-    tile = id - rest * tiles;
+    const unsigned inner = a.queries > a.keys ? a.key_heads : tiles, outer = a.queries > a.keys ? tiles : a.key_heads;
+    unsigned rest = id / inner;
+    const int in_inner = id - rest * inner;
     split = 0;
     if (splits > 1) {
       split = rest % splits;
       rest /= splits;
     }
-    b = rest / a.key_heads;
-    g = rest - b * a.key_heads;
+    b = rest / outer;
+    const int in_outer = rest - b * outer;
+    g = a.queries > a.keys ? in_inner : in_outer;
+    tile = a.queries > a.keys ? in_outer : in_inner;
   }
 };
 // The share of `all` steps that a split does
@@ -136,18 +140,32 @@ template <typename T, int DP, int Rows> struct Pair {
   u32x4 a[kMine], b[kMine];
   int row, d, dim;
   long stride_a, stride_b, at_a, at_b;   // of this thread's first piece
+  int per = 1;   // heads of a query that follow each other
+  long head_a = 0, head_b = 0;
   __device__ __forceinline__ Pair(long stride_a, long stride_b, int dim)
       : row(threadIdx.x / L::kPieces), d(threadIdx.x % L::kPieces * L::kPer), dim(dim), stride_a(stride_a), stride_b(stride_b) {
     at_a = row * stride_a + (d < dim ? d : 0), at_b = row * stride_b + (d < dim ? d : 0);
   }
+  // rows that are `inner` heads (a divisor of Rows) of each of Rows / inner queries
+  __device__ __forceinline__ void heads(int inner, long head_a, long head_b) {
+    per = inner;
+    at_a = row_at(0, stride_a, head_a) + (d < dim ? d : 0), at_b = row_at(0, stride_b, head_b) + (d < dim ? d : 0);
+    this->head_a = head_a, this->head_b = head_b;
+  }
+  __device__ __forceinline__ long row_at(int n, long stride, long head) const {
+    const int r = row + n * kStep;
+    if (per == 1) return r * stride;
+    const int query = static_cast<unsigned>(r) / static_cast<unsigned>(per);
+    return query * stride + (r - query * per) * head;
+  }
   // Rows 0 .. left - 1 from two addresses on.  Whole tiles without a branch; what stands for elements that do not exist is
   // any value, to be replaced by put().
   __device__ __forceinline__ void load(const T *from_a, const T *from_b, int left) {
-    if (left >= Rows && dim % L::kPer == 0) {
+    if (left >= Rows && dim % L::kPer == 0 && kStep % per == 0) {
 #pragma unroll
       for (int n = 0; n < kMine; ++n) {
-        a[n] = reinterpret_cast<const Loose<u32x4, sizeof(T)> *>(from_a + n * kStep * stride_a + at_a)->v;
-        b[n] = reinterpret_cast<const Loose<u32x4, sizeof(T)> *>(from_b + n * kStep * stride_b + at_b)->v;
+        a[n] = reinterpret_cast<const Loose<u32x4, sizeof(T)> *>(from_a + n * (kStep / per) * stride_a + at_a)->v;
+        b[n] = reinterpret_cast<const Loose<u32x4, sizeof(T)> *>(from_b + n * (kStep / per) * stride_b + at_b)->v;
       }
       return;
     }
@@ -155,8 +173,8 @@ template <typename T, int DP, int Rows> struct Pair {
     for (int n = 0; n < kMine; ++n) {
       a[n] = b[n] = u32x4{0, 0, 0, 0};
       if (row + n * kStep < left && d < dim) {
-        a[n] = load_piece<T>(from_a + (row + n * kStep) * stride_a, d, dim);
-        b[n] = load_piece<T>(from_b + (row + n * kStep) * stride_b, d, dim);
+        a[n] = load_piece<T>(from_a + row_at(n, stride_a, head_a), d, dim);
+        b[n] = load_piece<T>(from_b + row_at(n, stride_b, head_b), d, dim);
       }
     }
   }

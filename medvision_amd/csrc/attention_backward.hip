@@ -67,7 +67,7 @@ template <typename O, int N> __device__ __forceinline__ void store_column(O *row
 // ---- dq -------------------------------------------------------------------------------------------------------
 // As the forward kernel; leaves d_i for the next one.
 template <typename T, int DP, int WQ>
-__global__ __launch_bounds__(256, DP == 128 || (sizeof(T) == 4 && DP == 64) ? 1 : DP == 64 || sizeof(T) == 4 ? 2 : 3) void attend_grad_query(
+__global__ __launch_bounds__(256, DP == 128 || (sizeof(T) == 4 && DP == 64) ? 1 : sizeof(T) == 4 ? 2 : 3) void attend_grad_query(
     AttentionArgs a, const T *out, const T *low, const float *lse, const T *go, T *gq, float *delta, float *part, int row_tiles, int splits) {
   using S = Staging<T, DP, WQ == 1>;
   constexpr int kKeys = S::kRows, kSteps = WQ == 4 ? kKeys / 32 : 1, kOut = DP / 32;
@@ -189,21 +189,26 @@ __global__ __launch_bounds__(256, DP == 128 || (sizeof(T) == 4 && DP == 64) ? 1 
   const bool live = j < a.keys, use = j < length && a.counts(b, j);
   const float factor = a.factor();
 
-  // rows of one head after the other; nothing to sum where none of the workgroup's keys counts by its length
-  const int group = a.heads / a.key_heads, per_head = (a.queries + kRows - 1) / kRows;
-  const int all_tiles = place.tile * 32 * WK < length ? group * per_head : 0;
+  // Rows: all heads of the group, query after query, where a tile holds whole queries; one head after the other where not.
+  // Nothing to sum where none of the workgroup's keys counts by its length.
+  const int group = a.heads / a.key_heads, inner = kRows % group == 0 ? group : 1, outer = group / inner;
+  const int rows = a.queries * inner, per_head = (rows + kRows - 1) / kRows;
+  const int all_tiles = place.tile * 32 * WK < length ? outer * per_head : 0;
   const int first = share(all_tiles, split, splits), last = share(all_tiles, split + 1, splits);
   const int my_row = WK == 4 ? 0 : 32 * wave;
   float next_l = INFINITY, next_d = 0.f;
   const long go_row = static_cast<long>(a.heads) * a.dim;
   Pair<T, DP, kRows> next(a.qs[1], go_row, a.dim);
+  if (inner > 1) next.heads(inner, a.qs[2], a.dim);
+  const int my_stat_query = static_cast<unsigned>(threadIdx.x) / static_cast<unsigned>(inner), my_stat_head = threadIdx.x - my_stat_query * inner;
   auto load = [&](int t) {
-    const int in_group = group > 1 ? t / per_head : 0, row = (t - in_group * per_head) * kRows, h = g * group + in_group, left = a.queries - row;
-    next.load(static_cast<const T *>(a.q) + b * a.qs[0] + row * a.qs[1] + h * a.qs[2],
-              go + (static_cast<long>(b) * a.queries + row) * go_row + static_cast<long>(h) * a.dim, left);
+    const int round = outer > 1 ? t / per_head : 0, row = (t - round * per_head) * kRows, h = g * group + round, left = rows - row;
+    const int query = row / inner;
+    next.load(static_cast<const T *>(a.q) + b * a.qs[0] + query * a.qs[1] + h * a.qs[2],
+              go + (static_cast<long>(b) * a.queries + query) * go_row + static_cast<long>(h) * a.dim, left);
     next_l = INFINITY, next_d = 0.f;
-    if (threadIdx.x < min(kRows, left)) {
-      const long from = (static_cast<long>(b) * a.heads + h) * a.queries + row + threadIdx.x;
+    if (static_cast<int>(threadIdx.x) < min(kRows, left)) {
+      const long from = (static_cast<long>(b) * a.heads + h + my_stat_head) * a.queries + query + my_stat_query;
       next_l = lse[from], next_d = delta[from];
     }
   };
