@@ -15,11 +15,12 @@ namespace {
 // time (few rows: their sums are joined at the end).  Scores are formed transposed, a query per lane: maximum and sum of a
 // row are those of a lane and of its other half, and the weights are the second product's operand as they stand.
 // float16: weights are 2^15 times as large (at most 32768), which keeps those below 2^-14 of the largest from losing bits.
-template <typename T, int DP, int WQ>
-__global__ __launch_bounds__(256, sizeof(T) == 4 ? (DP == 128 ? 1 : 2) : DP == 128 ? 2 : DP == 64 ? 3 : 4) void attend_kernel(
+template <typename T, int W, int WQ>
+__global__ __launch_bounds__(256, sizeof(T) == 4 ? (W > 64 ? 1 : 2) : W > 64 ? 2 : W == 64 ? 3 : 4) void attend_kernel(
     AttentionArgs a, T *out, T *low, float *lse, float *part, int row_tiles, int splits) {
+  constexpr int DP = stored(W);
   using S = Staging<T, DP, WQ == 1>;
-  constexpr int kTiles = WQ == 4 && S::kRows >= 64 ? 2 : 1, kKeys = S::kRows, kSteps = WQ == 4 ? kKeys / (32 * kTiles) : 1, kOut = DP / 32;
+  constexpr int kTiles = WQ == 4 && S::kRows >= 64 ? 2 : 1, kKeys = S::kRows, kSteps = WQ == 4 ? kKeys / (32 * kTiles) : 1, kOut = W / 32;
   constexpr float kShift = __is_same(T, __half) ? 15.f : 0.f;
   using L = Tile<T, DP, kKeys>;
   __shared__ L tiles[S::kBuffers][2];
@@ -49,7 +50,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? (DP == 128 ? 1 : 2) : DP == 1
     next.put(tiles[t % S::kBuffers]);
   };
   if (first < last) load(first);
-  Column<T, DP> q;
+  Column<T, W> q;
   q.load(static_cast<const T *>(a.q) + b * a.qs[0] + at.query * a.qs[1] + at.head * a.qs[2], live, a.dim, half);
   if (a.scale < 0.f) q.negate();
   if (first < last) put(first);
@@ -261,16 +262,16 @@ ForwardPlan forward_plan(const mv_attention_shape *s, int dtype) {
   return {few, static_cast<int>(row_tiles), static_cast<int>(std::max(1L, std::min((s->dim <= 32 ? 1024 : s->dim <= 64 && !few ? 768 : 512) / groups, shares)))};
 }
 
-template <typename T, int DP>
+template <typename T, int W>
 void launch_forward(const ForwardPlan &p, const AttentionArgs &a, void *out, void *low, float *lse, float *part, hipStream_t s) {
   const long groups = static_cast<long>(p.row_tiles) * p.splits * a.batch * a.key_heads;
   const dim3 grid = linear_grid(groups, 256);
-  if constexpr (kHasFew<T, DP>)
+  if constexpr (kHasFew<T, W>)
     if (p.few) {
-      attend_kernel<T, DP, 1><<<grid, 256, 0, s>>>(a, static_cast<T *>(out), static_cast<T *>(low), lse, part, p.row_tiles, p.splits);
+      attend_kernel<T, W, 1><<<grid, 256, 0, s>>>(a, static_cast<T *>(out), static_cast<T *>(low), lse, part, p.row_tiles, p.splits);
       return;
     }
-  attend_kernel<T, DP, 4><<<grid, 256, 0, s>>>(a, static_cast<T *>(out), static_cast<T *>(low), lse, part, p.row_tiles, p.splits);
+  attend_kernel<T, W, 4><<<grid, 256, 0, s>>>(a, static_cast<T *>(out), static_cast<T *>(low), lse, part, p.row_tiles, p.splits);
 }
 
 }  // namespace
@@ -301,6 +302,7 @@ int mv_cross_attention_forward(const void *query, const void *key, const void *v
   MV_FLOATS(dtype, {
     if (a.dim <= 32) launch_forward<T, 32>(p, a, output, output_low, sums, part, s);
     else if (a.dim <= 64) launch_forward<T, 64>(p, a, output, output_low, sums, part, s);
+    else if (a.dim <= 96) launch_forward<T, 96>(p, a, output, output_low, sums, part, s);
     else launch_forward<T, 128>(p, a, output, output_low, sums, part, s);
     const float shift = dtype == MV_F16 ? 15.f : 0.f;
     T *const o = static_cast<T *>(output), *const ol = static_cast<T *>(output_low);

@@ -102,6 +102,10 @@ template <> struct Mma<__hip_bfloat16> {
   }
 };
 
+// ---- widths ----
+// Kernels work on heads of W = 32, 64, 96 or 128 channels (zeros beyond the real ones); a tile's rows are powers of two.
+constexpr int stored(int w) { return w == 96 ? 128 : w; }
+
 // ---- tiles in LDS -------------------------------------------------------------------------------------------
 // `Rows` rows of DP elements in pieces of 16 bytes.  Pieces of a row are exchanged by its number: eight rows of one column of
 // pieces lie in different banks (whole rows are read so), and so do four rows of one pair of pieces (transposed ones).
@@ -211,7 +215,7 @@ template <typename T, int DP, bool Few> struct Staging {
 
 // Whether the kernels for few rows or keys take this type and width: float32 heads of more than 64 channels would not fit
 // into the registers.
-template <typename T, int DP> constexpr bool kHasFew = sizeof(T) == 2 || DP <= 64;
+template <typename T, int W> constexpr bool kHasFew = sizeof(T) == 2 || W <= 64;
 inline bool has_few(int dtype, int dim) { return dtype != MV_F32 || dim <= 64; }
 
 // Which of 64 keys count: bits for lanes' keys
@@ -220,9 +224,9 @@ __device__ __forceinline__ unsigned long long use_bits(const AttentionArgs &a, i
   return __ballot(lane < count && j < length && a.counts(b, j));
 }
 
-// One column (a query, a key) per lane % 32, all DP elements: the second operand of products over the elements.
-template <typename T, int DP> struct Column {
-  static constexpr int kPer = 16 / sizeof(T), kCount = DP / kPer / 2;
+// One column (a query, a key) per lane % 32, all W elements: the second operand of products over the elements.
+template <typename T, int W> struct Column {
+  static constexpr int kPer = 16 / sizeof(T), kCount = W / kPer / 2;
   u32x4 r[kCount];   // piece 2 n + lane / 32
   __device__ __forceinline__ void load(const T *row, bool use, int dim, int half) {
 #pragma unroll
@@ -255,12 +259,12 @@ template <typename T, int DP> struct Column {
 };
 
 // 32 rows of a tile times the columns: over the elements of a row
-template <typename T, int DP, int Rows>
-__device__ __forceinline__ f32x16 times(const Tile<T, DP, Rows> &tile, int first_row, const Column<T, DP> &c, int lane) {
+template <typename T, int W, int DP, int Rows>
+__device__ __forceinline__ f32x16 times(const Tile<T, DP, Rows> &tile, int first_row, const Column<T, W> &c, int lane) {
   f32x16 s = {};
   const int row = first_row + (lane & 31), half = lane >> 5;
 #pragma unroll
-  for (int n = 0; n < Column<T, DP>::kCount; ++n) {
+  for (int n = 0; n < Column<T, W>::kCount; ++n) {
     const u32x4 a = tile.at[Tile<T, DP, Rows>::place(row, 2 * n + half)];
     if constexpr (sizeof(T) == 2) {
       using P = typename Mma<T>::piece;
@@ -277,8 +281,8 @@ __device__ __forceinline__ f32x16 times(const Tile<T, DP, Rows> &tile, int first
 // sum[t] += (32 rows of a tile)^T weights, elements 32 t .. 32 t + 31 by the weights' columns: over the rows.  `w` is a
 // result of times() (or what was made of it).  16 bits: the transposing load gives a lane four rows of its element, in the
 // order in which the weights stand.
-template <typename T, int DP, int Rows>
-__device__ __forceinline__ void add_transposed(const Tile<T, DP, Rows> &tile, int first_row, const float (&w)[16], f32x16 (&sum)[DP / 32],
+template <typename T, int Tiles, int DP, int Rows>
+__device__ __forceinline__ void add_transposed(const Tile<T, DP, Rows> &tile, int first_row, const float (&w)[16], f32x16 (&sum)[Tiles],
                                                int lane) {
   using L = Tile<T, DP, Rows>;
   const int half = lane >> 5;
@@ -292,7 +296,7 @@ __device__ __forceinline__ void add_transposed(const Tile<T, DP, Rows> &tile, in
     for (int s = 0; s < 2; ++s) {
       const P b = Mma<T>::pack(w + 8 * s);
 #pragma unroll
-      for (int t = 0; t < DP / 32; ++t) {
+      for (int t = 0; t < Tiles; ++t) {
         s16x4 part[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
@@ -309,7 +313,7 @@ __device__ __forceinline__ void add_transposed(const Tile<T, DP, Rows> &tile, in
     for (int i = 0; i < 16; ++i) {
       const int row = first_row + result_row(i, 0) + 4 * half;
 #pragma unroll
-      for (int t = 0; t < DP / 32; ++t) {
+      for (int t = 0; t < Tiles; ++t) {
         const int d = 32 * t + (lane & 31);
         const float a = reinterpret_cast<const float *>(&tile.at[L::place(row, d / 4)])[d % 4];
         sum[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, w[i], sum[t], 0, 0, 0);

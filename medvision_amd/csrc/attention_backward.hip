@@ -66,11 +66,12 @@ template <typename O, int N> __device__ __forceinline__ void store_column(O *row
 
 // ---- dq -------------------------------------------------------------------------------------------------------
 // As the forward kernel; leaves d_i for the next one.
-template <typename T, int DP, int WQ>
-__global__ __launch_bounds__(256, DP == 128 || (sizeof(T) == 4 && DP == 64) ? 1 : sizeof(T) == 4 ? 2 : 3) void attend_grad_query(
+template <typename T, int W, int WQ>
+__global__ __launch_bounds__(256, W > 64 || (sizeof(T) == 4 && W == 64) ? 1 : sizeof(T) == 4 ? 2 : 3) void attend_grad_query(
     AttentionArgs a, const T *out, const T *low, const float *lse, const T *go, T *gq, float *delta, float *part, int row_tiles, int splits) {
+  constexpr int DP = stored(W);
   using S = Staging<T, DP, WQ == 1>;
-  constexpr int kKeys = S::kRows, kSteps = WQ == 4 ? kKeys / 32 : 1, kOut = DP / 32;
+  constexpr int kKeys = S::kRows, kSteps = WQ == 4 ? kKeys / 32 : 1, kOut = W / 32;
   using L = Tile<T, DP, kKeys>;
   __shared__ L tiles[S::kBuffers][2];
   const Place place(a, row_tiles, splits);
@@ -101,10 +102,10 @@ __global__ __launch_bounds__(256, DP == 128 || (sizeof(T) == 4 && DP == 64) ? 1 
   };
   if (first < last) load(first);
 
-  Column<T, DP> q, d_o;
+  Column<T, W> q, d_o;
   float d_i;
   {
-    Column<T, DP> o;
+    Column<T, W> o;
     d_o.load(go + at_row * a.dim, live, a.dim, half);
     o.load(out + at_row * a.dim, live, a.dim, half);
     d_i = d_o.dot(o);
@@ -172,11 +173,12 @@ __global__ __launch_bounds__(256, DP == 128 || (sizeof(T) == 4 && DP == 64) ? 1 
 // A key per lane; rows of queries and of output gradients go through LDS.  WK = 4: 32 keys for each wavefront, the same 32
 // rows; WK = 1 (few keys): the same 32 keys, each wavefront 32 of 128 rows, joined at the end.  A key that does not count
 // spoils nothing but its own column, which is written as zeros.
-template <typename T, int DP, int WK>
-__global__ __launch_bounds__(256, DP == 128 || (sizeof(T) == 4 && DP == 64) ? 1 : DP == 64 || sizeof(T) == 4 ? 2 : 3) void attend_grad_key(
+template <typename T, int W, int WK>
+__global__ __launch_bounds__(256, W > 64 || (sizeof(T) == 4 && W == 64) ? 1 : W == 64 || sizeof(T) == 4 ? 2 : 3) void attend_grad_key(
     AttentionArgs a, const float *lse, const float *delta, const T *go, T *gk, T *gv, float *part, int key_tiles, int splits) {
+  constexpr int DP = stored(W);
   using S = Staging<T, DP, WK == 1>;
-  constexpr int kRows = S::kRows, kSteps = WK == 4 ? kRows / 32 : 1, kOut = DP / 32;
+  constexpr int kRows = S::kRows, kSteps = WK == 4 ? kRows / 32 : 1, kOut = W / 32;
   constexpr float kShift = __is_same(T, __half) ? 15.f : 0.f;   // as in the forward pass
   using L = Tile<T, DP, kRows>;
   __shared__ L tiles[S::kBuffers][2];
@@ -220,7 +222,7 @@ __global__ __launch_bounds__(256, DP == 128 || (sizeof(T) == 4 && DP == 64) ? 1 
     }
   };
   if (first < last) load(first);
-  Column<T, DP> k, v;
+  Column<T, W> k, v;
   k.load(static_cast<const T *>(a.k) + b * a.ks[0] + j * a.ks[1] + g * a.ks[2], use, a.dim, half);
   v.load(static_cast<const T *>(a.v) + b * a.vs[0] + j * a.vs[1] + g * a.vs[2], use, a.dim, half);
   if (a.scale < 0.f) k.negate();
@@ -311,12 +313,14 @@ BackwardPlan backward_plan(const mv_attention_shape *s, int dtype) {
   p.key_tiles = static_cast<int>(p.few_keys ? 1 : (s->keys + 127L) / 128);
   const long least = dtype == MV_F32 ? 64 : 512;   // keys, or rows, that are worth a split
   const long key_steps = (s->keys + least - 1) / least, row_steps = s->heads / s->key_heads * ((s->queries + least - 1) / least);
-  p.query_splits = static_cast<int>(std::max(1L, std::min(512 / std::max(1L, p.row_tiles * heads), key_steps)));
-  p.key_splits = static_cast<int>(std::max(1L, std::min(512 / std::max(1L, p.key_tiles * heads), row_steps)));
+  // as many workgroups as are resident at a time
+  const long for_queries = s->dim <= 64 ? 768 : 256, for_keys = s->dim <= 32 ? 768 : s->dim <= 64 ? 512 : 256;
+  p.query_splits = static_cast<int>(std::max(1L, std::min(for_queries / std::max(1L, p.row_tiles * heads), key_steps)));
+  p.key_splits = static_cast<int>(std::max(1L, std::min(for_keys / std::max(1L, p.key_tiles * heads), row_steps)));
   return p;
 }
 
-template <typename T, int DP>
+template <typename T, int W>
 void launch_backward(const BackwardPlan &p, const AttentionArgs &a, const void *out, const void *low, const float *lse, const void *go, void *gq, void *gk, void *gv,
                      float *delta, float *part, hipStream_t s) {
   const long heads = static_cast<long>(a.batch) * a.key_heads, queries = static_cast<long>(a.batch) * a.queries * a.heads * a.dim,
@@ -325,23 +329,23 @@ void launch_backward(const BackwardPlan &p, const AttentionArgs &a, const void *
   if (queries) {
     const dim3 grid = linear_grid(heads * p.row_tiles * p.query_splits, 256);
     bool done = false;
-    if constexpr (kHasFew<T, DP>)
+    if constexpr (kHasFew<T, W>)
       if (p.few_rows) {
-        attend_grad_query<T, DP, 1><<<grid, 256, 0, s>>>(a, o, ol, lse, d_o, static_cast<T *>(gq), delta, part, p.row_tiles, p.query_splits);
+        attend_grad_query<T, W, 1><<<grid, 256, 0, s>>>(a, o, ol, lse, d_o, static_cast<T *>(gq), delta, part, p.row_tiles, p.query_splits);
         done = true;
       }
-    if (!done) attend_grad_query<T, DP, 4><<<grid, 256, 0, s>>>(a, o, ol, lse, d_o, static_cast<T *>(gq), delta, part, p.row_tiles, p.query_splits);
+    if (!done) attend_grad_query<T, W, 4><<<grid, 256, 0, s>>>(a, o, ol, lse, d_o, static_cast<T *>(gq), delta, part, p.row_tiles, p.query_splits);
     if (p.query_splits > 1) sum_parts<T>(part, static_cast<T *>(gq), nullptr, queries, p.query_splits, s);
   }
   if (keys) {
     const dim3 grid = linear_grid(heads * p.key_tiles * p.key_splits, 256);
     bool done = false;
-    if constexpr (kHasFew<T, DP>)
+    if constexpr (kHasFew<T, W>)
       if (p.few_keys) {
-        attend_grad_key<T, DP, 1><<<grid, 256, 0, s>>>(a, lse, delta, d_o, static_cast<T *>(gk), static_cast<T *>(gv), part, p.key_tiles, p.key_splits);
+        attend_grad_key<T, W, 1><<<grid, 256, 0, s>>>(a, lse, delta, d_o, static_cast<T *>(gk), static_cast<T *>(gv), part, p.key_tiles, p.key_splits);
         done = true;
       }
-    if (!done) attend_grad_key<T, DP, 4><<<grid, 256, 0, s>>>(a, lse, delta, d_o, static_cast<T *>(gk), static_cast<T *>(gv), part, p.key_tiles, p.key_splits);
+    if (!done) attend_grad_key<T, W, 4><<<grid, 256, 0, s>>>(a, lse, delta, d_o, static_cast<T *>(gk), static_cast<T *>(gv), part, p.key_tiles, p.key_splits);
     if (p.key_splits > 1) sum_parts<T>(part, static_cast<T *>(gk), static_cast<T *>(gv), keys, p.key_splits, s);
   }
 }
@@ -378,6 +382,7 @@ int mv_cross_attention_backward(const void *query, const void *key, const void *
   MV_FLOATS(dtype, {
     if (a.dim <= 32) launch_backward<T, 32>(p, a, output, output_low, sums, grad_output, grad_query, grad_key, grad_value, delta, part, s);
     else if (a.dim <= 64) launch_backward<T, 64>(p, a, output, output_low, sums, grad_output, grad_query, grad_key, grad_value, delta, part, s);
+    else if (a.dim <= 96) launch_backward<T, 96>(p, a, output, output_low, sums, grad_output, grad_query, grad_key, grad_value, delta, part, s);
     else launch_backward<T, 128>(p, a, output, output_low, sums, grad_output, grad_query, grad_key, grad_value, delta, part, s);
   })
   return check_launch("cross_attention backward");
