@@ -207,8 +207,8 @@ template <typename T, int DP, int Rows> struct Pair {
 };
 
 // Keys (or rows) that a workgroup has in LDS at a time, and whether twice: the next ones are written while these are read.
-template <typename T, int DP, bool Few> struct Staging {
-  static constexpr int kRows = Few || (sizeof(T) == 2 && DP == 32) ? 128 : sizeof(T) == 4 && DP == 128 ? 32 : 64;
+template <typename T, int DP, bool Few, bool Room = true> struct Staging {
+  static constexpr int kRows = !Few && !Room ? 32 : Few || (sizeof(T) == 2 && DP == 32) ? 128 : sizeof(T) == 4 && DP == 128 ? 32 : 64;
   static constexpr int kBytes = 2 * kRows * DP * static_cast<int>(sizeof(T));
   static constexpr int kBuffers = kBytes <= 32768 ? 2 : 1;
 };

@@ -174,10 +174,10 @@ __global__ __launch_bounds__(256, W > 64 || (sizeof(T) == 4 && W == 64) ? 1 : si
 // rows; WK = 1 (few keys): the same 32 keys, each wavefront 32 of 128 rows, joined at the end.  A key that does not count
 // spoils nothing but its own column, which is written as zeros.
 template <typename T, int W, int WK>
-__global__ __launch_bounds__(256, W > 64 || (sizeof(T) == 4 && W == 64) ? 1 : W == 64 || sizeof(T) == 4 ? 2 : 3) void attend_grad_key(
+__global__ __launch_bounds__(256, W == 128 || (sizeof(T) == 4 && W > 32) || (W == 96 && WK == 1) ? 1 : W == 32 && sizeof(T) == 2 ? 3 : 2) void attend_grad_key(
     AttentionArgs a, const float *lse, const float *delta, const T *go, T *gk, T *gv, float *part, int key_tiles, int splits) {
   constexpr int DP = stored(W);
-  using S = Staging<T, DP, WK == 1>;
+  using S = Staging<T, DP, WK == 1, W != 96>;   // (96: two wavefronts per SIMD, 130 -> 83 us at 1000 x 4000 x 8 heads of 80; 128 would spill)
   constexpr int kRows = S::kRows, kSteps = WK == 4 ? kRows / 32 : 1, kOut = W / 32;
   constexpr float kShift = __is_same(T, __half) ? 15.f : 0.f;   // as in the forward pass
   using L = Tile<T, DP, kRows>;
@@ -314,7 +314,7 @@ BackwardPlan backward_plan(const mv_attention_shape *s, int dtype) {
   const long least = dtype == MV_F32 ? 64 : 512;   // keys, or rows, that are worth a split
   const long key_steps = (s->keys + least - 1) / least, row_steps = s->heads / s->key_heads * ((s->queries + least - 1) / least);
   // as many workgroups as are resident at a time
-  const long for_queries = s->dim <= 64 ? 768 : 256, for_keys = s->dim <= 32 ? 768 : s->dim <= 64 ? 512 : 256;
+  const long for_queries = s->dim <= 64 ? 768 : 256, for_keys = s->dim <= 32 ? 768 : s->dim <= 96 ? 512 : 256;
   p.query_splits = static_cast<int>(std::max(1L, std::min(for_queries / std::max(1L, p.row_tiles * heads), key_steps)));
   p.key_splits = static_cast<int>(std::max(1L, std::min(for_keys / std::max(1L, p.key_tiles * heads), row_steps)));
   return p;
