@@ -281,7 +281,8 @@ __device__ __forceinline__ f32x16 times(const Tile<T, DP, Rows> &tile, int first
 // sum[t] += (32 rows of a tile)^T weights, elements 32 t .. 32 t + 31 by the weights' columns: over the rows.  `w` is a
 // result of times() (or what was made of it).  16 bits: the transposing load gives a lane four rows of its element, in the
 // order in which the weights stand.
-template <typename T, int Tiles, int DP, int Rows>
+// Fine: what rounding takes from the weights is multiplied too (a second product with the same first operand).
+template <bool Fine = false, typename T, int Tiles, int DP, int Rows>
 __device__ __forceinline__ void add_transposed(const Tile<T, DP, Rows> &tile, int first_row, const float (&w)[16], f32x16 (&sum)[Tiles],
                                                int lane) {
   using L = Tile<T, DP, Rows>;
@@ -295,6 +296,13 @@ __device__ __forceinline__ void add_transposed(const Tile<T, DP, Rows> &tile, in
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       const P b = Mma<T>::pack(w + 8 * s);
+      P b_low = {};
+      if constexpr (Fine) {
+        float rest[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) rest[i] = w[8 * s + i] - static_cast<float>(b[i]);
+        b_low = Mma<T>::pack(rest);
+      }
 #pragma unroll
       for (int t = 0; t < Tiles; ++t) {
         s16x4 part[2];
@@ -306,6 +314,7 @@ __device__ __forceinline__ void add_transposed(const Tile<T, DP, Rows> &tile, in
         }
         const s16x8 a = __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7);
         sum[t] = Mma<T>::mul(__builtin_bit_cast(P, a), b, sum[t]);
+        if constexpr (Fine) sum[t] = Mma<T>::mul(__builtin_bit_cast(P, a), b_low, sum[t]);
       }
     }
   } else {

@@ -143,7 +143,7 @@ __global__ __launch_bounds__(256, W > 64 || (sizeof(T) == 4 && W == 64) ? 1 : si
         for (int i = 0; i < 16; ++i) ds[i] = word >> (4 * half) >> result_row(i, 0) & 1 ? ds[i] : 0.f;
       }
       raise.scale(ds, sum);
-      add_transposed(ks, key, ds, sum, lane);
+      add_transposed<true>(ks, key, ds, sum, lane);
     }
     if (t + 1 < last) {
       if constexpr (S::kBuffers == 1) __syncthreads();
