@@ -246,7 +246,39 @@ __global__ __launch_bounds__(64 * WM * WN * WK, WM *WN *WK / 4) void product_til
           for (int t = 0; t < S::kTM; ++t) acc[t][u] += part[(u * S::kTM + t) * (64 * WM * WN) + at];
       }
     }
-    if (group) return;
+  }
+  __syncthreads();   // the operands, and the groups' sums, have been read: their place is free
+  if (group) return;
+  // Whole tiles of results in 16 bits: through LDS, so that 256 (128) neighbouring bytes of a row are written at a time; as
+  // they stand, 32 bytes of each of 16 rows.
+  constexpr int kCols = S::kTN * 16, kUnits = kCols / 8;   // pieces of 16 bytes of a row of this wavefront
+  const int m_first = m0 + wm * S::kTM * 16, n_first = n0 + wn * kCols;
+  if (!to.part && m_first + S::kTM * 16 <= rows && n_first + kCols <= outputs && outputs % 8 == 0 && reinterpret_cast<unsigned long>(to.y) % 16 == 0) {
+    unsigned char *const mine = lds + in_group * (S::kTM * 16 * kCols * 2);
+    static_assert(WM * WN * S::kTM * 16 * kCols * 2 <= S::kLds, "");
+#pragma unroll
+    for (int u = 0; u < S::kTN; ++u) {
+      float add[4] = {};
+      if (to.bias) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) add[i] = load(to.bias + n_first + u * 16 + 4 * g + i);
+      }
+#pragma unroll
+      for (int t = 0; t < S::kTM; ++t) {
+        const f32x4 v = acc[t][u];
+        const int row = t * 16 + r16, unit = (u * 2 + g / 2) ^ (row % kUnits);
+        *reinterpret_cast<u32x2 *>(mine + (row * kUnits + unit) * 16 + g % 2 * 8) =
+            u32x2{pack2<T>(v[0] + add[0], v[1] + add[1]), pack2<T>(v[2] + add[2], v[3] + add[3])};
+      }
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // (a wavefront reads only what it wrote)
+#pragma unroll
+    for (int i = 0; i < S::kTM * 16 * kUnits / 64; ++i) {
+      const int at = i * 64 + lane, row = at / kUnits, unit = at % kUnits;
+      *reinterpret_cast<u32x4 *>(to.y + static_cast<long>(m_first + row) * outputs + n_first + unit * 8) =
+          *reinterpret_cast<const u32x4 *>(mine + (row * kUnits + (unit ^ (row % kUnits))) * 16);
+    }
+    return;
   }
 #pragma unroll
   for (int t = 0; t < S::kTM; ++t) {
