@@ -29,7 +29,11 @@ struct AttentionArgs {
     const long i = row / heads, b = i / queries;
     return (b * heads + (row - i * heads)) * queries + (i - b * queries);
   }
-  __device__ __forceinline__ float factor() const { return fabsf(scale) * kLog2e; }
+  // (not zero: a key that does not count has a score of minus infinity, which has to stay that)
+  __device__ __forceinline__ float factor() const {
+    const float f = fabsf(scale) * kLog2e;
+    return f == 0.f ? 1.17549435e-38f : f;
+  }
 };
 
 // Rows of a head of keys: the heads that share it, query after query (neighbours in memory).

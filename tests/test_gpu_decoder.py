@@ -446,3 +446,31 @@ def test_block_refusals():
                        ((x, None, one.half()), "weight has dtype"), ((x.double(), None, one.double()), "float32, float16 or bfloat16")):
         with pytest.raises(RuntimeError, match=text):
             ops.add_rms_norm(*args)
+
+
+@pytest.mark.parametrize("rows,inputs,outputs", [(3300, 300, 3850), (3584, 128, 3848)])
+def test_block_linear_on_large_tiles(rows, inputs, outputs):
+    """More than 192 tiles of 256 x 256: whole ones and ragged ones, rows of results at any alignment."""
+    import medvision_amd.ops as ops
+    g = gen(rows)
+    q, s = ops.quantize_blocks(randn(g, rows, inputs) * torch.exp(randn(g, rows, 1)))
+    wq, ws = ops.quantize_blocks(randn(g, outputs, inputs) / math.sqrt(inputs), 128)
+    b = randn(g, outputs, dtype=torch.float16)
+    y = ops.block_linear(q, s, wq, ws, b, out_dtype=torch.float16)
+    ref.check(y, *ref.block_linear(q, s, wq, ws, b, torch.float16), "y")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("scale", [-0.25, 0.0, 3.0])
+def test_attention_with_any_scale(dtype, scale):
+    case = attention_case(17, dtype, 2, 45, 90, 3, 1, 48, "mask")
+    compare_attention(run_attention(*case, scale), *case, scale)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,key_heads", [(12, 2), (5, 1), (16, 2), (130, 1)])
+def test_groups_of_heads_of_any_size(dtype, heads, key_heads):
+    """Groups that divide a tile's rows and groups that do not, more queries than keys and the reverse."""
+    for Lq, Lk in ((70, 20), (20, 70)):
+        case = attention_case(heads + Lq, dtype, 1, Lq, Lk, heads, key_heads, 24, "both")
+        compare_attention(run_attention(*case), *case)
