@@ -69,7 +69,15 @@ template <typename T, int TN> __device__ __forceinline__ void store_row(const Re
 // A workgroup takes BM rows and BN outputs; WM x WN wavefronts share the tile, WK groups of them take every WK-th block of
 // the sum.  Both operands go from memory to LDS without registers (16 bytes per lane, the next blocks while these are
 // multiplied).  A row of a block is 128 bytes, eight pieces of 16; piece c of row r stands at c ^ (r & 7), so that the 16
-// rows of an operand that one instruction reads spread over all banks.
+// rows of an operand that one instruction reads spread over all banks (no conflicts).
+//
+// 256 x 256 with eight wavefronts of 64 x 128: 16384 x 4096 x 4096 276 us = 1.99 PFLOP/s (a plain product of the library:
+// 2.34), 8192^3 2.06.  Of 490 us for the latter 380 are left without the loads, 406 without the products, 400 without the
+// additions of the scaled products to the sums: loads into LDS, reads from it (96 bytes per clock and compute unit at the
+// matrix units' full rate), matrix and vector instructions take about as long each and overlap less than whole.
+// 128 x 128 with twice four wavefronts of 64 x 64, where there are fewer than 192 of the large tiles (4000 x 12544 x 1024: 72 us = 1.42 PFLOP/s; 160 with
+// the large ones, 80 with those split in four): the loads alone take 52 us (803 MB from the L2s, 15.6 TB/s), reads and products
+// 48, and both share the LDS.
 template <int BM, int BN, int WM, int WN, int WK> struct Tiles {
   static constexpr int kThreads = 64 * WM * WN * WK, kTM = BM / WM / 16, kTN = BN / WN / 16;
   static constexpr int kStage = (BM + BN) * kBlock;   // bytes of one block of both operands
@@ -289,7 +297,8 @@ __global__ __launch_bounds__(64 * WM * WN * WK, WM *WN *WK / 4) void product_til
 // ---- few rows -----------------------------------------------------------------------------------------------
 // Bound by reading the weights once: 64 outputs and 16 TM rows per workgroup, straight from memory into the operands'
 // registers, the next block's while this one is multiplied.  The four wavefronts take turns at the blocks of the
-// workgroup's share of the sum and join in LDS.
+// workgroup's share of the sum and join in LDS.  8 x 87808 x 1024: 17 us and 3 us for the join of 32 splits (90 MB of
+// weights: 4.5 TB/s in all).
 template <typename T, int TM>
 __global__ __launch_bounds__(256) void product_rows(const unsigned char *q, const float *qs, const unsigned char *w, const float *ws,
                                                     const Results<T> to, int rows, int inputs, int outputs, int m_tiles, int n_tiles,
@@ -399,6 +408,9 @@ struct Plan {
 
 int ceil_div(long a, long b) { return static_cast<int>((a + b - 1) / b); }
 
+// Few rows up to 64 (of 128 x 12544 x 1024, which tiles take, 19 us).  Sums are split where there are fewer workgroups than compute units (512 for few rows), into shares of
+// eight blocks at least; a split costs the parts' way through memory (4000 x 1024 x 4096 in one piece 25 us, in two 77), so
+// that no more are made than fill the chip once (1000 x 4096 x 1024: 30.0 us in one piece, 21.0 in four, 30.7 in eight).
 Plan plan_of(long rows, int inputs, int outputs) {
   const int blocks = inputs / kBlock;
   if (rows <= 64) {

@@ -90,7 +90,11 @@ template <int Lanes> __device__ __forceinline__ float row_sum(float v, float *ld
   return v;
 }
 
-// Rows that fit into registers: Lanes threads, 8 Chunks columns each.  One pass over memory.
+// Rows that fit into registers: Lanes threads, 8 Chunks columns each.  One pass over memory, which bounds it: 55296 x 256 in
+// bf16 with residual 19 us (5.9 TB/s for four bytes in and four out of an element), 55296 x 1000 79 us (5.6 TB/s), in 8 bits
+// 72 us (5.4 TB/s).  Rows of 1003 columns start at any byte: 97 us.  A wavefront or less takes a row as long as there
+// are 512 columns (no barrier); 513 to 1024 columns run on two wavefronts with eight columns per thread (on one with sixteen, the
+// gradients below took 150 instead of 105 us: half as many loads in flight).
 template <typename T, int Lanes, int Chunks>
 __global__ __launch_bounds__(kThreads) void norm_rows(const T *x, const T *residual, const void *weight, bool wide, T *y, unsigned char *q,
                                                       float *scales, T *sum, long rows, int columns, float eps) {
@@ -155,7 +159,8 @@ __global__ __launch_bounds__(kThreads) void norm_rows(const T *x, const T *resid
 }
 
 // Both gradients in one pass over memory: a workgroup takes every gridDim-th row (or group of rows), and keeps its share of
-// the weight's gradient in registers until the end.
+// the weight's gradient in registers until the end.  Bound by memory: 55296 x 256 in bf16 with both incoming gradients 29 us
+// (3.9 TB/s), 55296 x 1000 105 us (4.2 TB/s), with the join of 1024 partial sums.
 template <typename T, int Lanes, int Chunks>
 __global__ __launch_bounds__(kThreads) void norm_grad(const T *h, const void *weight, bool wide, const T *gy, const T *gsum, T *gx,
                                                       float *partial, long rows, int columns, float eps) {
@@ -340,7 +345,7 @@ __global__ __launch_bounds__(kThreads) void norm_grad_weight(const float *partia
   else static_cast<T *>(gw)[c] = store_cast<T>(sum);
 }
 
-// One wavefront for four blocks of one row and 128 columns.
+// 16 threads for a block of one row and 128 columns.  Bound by memory: 4000 x 12544 in bf16 33 us (150 MB, 4.6 TB/s).
 template <typename T>
 __global__ __launch_bounds__(kThreads) void quantize_rows(const T *x, unsigned char *q, float *scales, long blocks, int columns) {
   const int per_row = (columns + kBlock - 1) / kBlock;
@@ -357,7 +362,8 @@ __global__ __launch_bounds__(kThreads) void quantize_rows(const T *x, unsigned c
   if ((threadIdx.x & 15) == 0) scales[block] = s;
 }
 
-// One workgroup for a block of 128 x 128: 16 rows at a time, twice.
+// One workgroup for a block of 128 x 128: 16 rows at a time, twice (weights, once when a layer is built: 1024 x 87808 from
+// float32 123 us).
 template <typename T>
 __global__ __launch_bounds__(kThreads) void quantize_tiles(const T *x, unsigned char *q, float *scales, long rows, int columns) {
   __shared__ float lds[kThreads / 64];
