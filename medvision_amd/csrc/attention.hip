@@ -85,7 +85,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? (W > 64 ? 1 : 2) : W > 64 ? 2
         for (int n = 0; n < kTiles; ++n) {
           const unsigned word = static_cast<unsigned>(use[step] >> (32 * n)) >> (4 * half);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) s[n][i] = word >> result_row(i, 0) & 1 ? s[n][i] : -INFINITY;
+          for (int i = 0; i < 16; ++i) s[n][i] = where_bit(word, result_row(i, 0), s[n][i], -INFINITY);
         }
       }
       float top = s[0][0];
@@ -177,16 +177,17 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? (W > 64 ? 1 : 2) : W > 64 ? 2
   }
   const float inverse = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
-  for (int u = 0; u < kOut; ++u)
+  for (int u = 0; u < kOut; ++u) {
+    float r[16];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int d = 32 * u + 8 * i + 4 * half;
-      float r[4];
+    for (int i = 0; i < 16; ++i) r[i] = o[u][i] * inverse;
+    store_results(out + at_row * a.dim, 32 * u, a.dim, half, r);
+    if (low) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) r[e] = o[u][4 * i + e] * inverse;
-      store_quad(out + at_row * a.dim, d, a.dim, r[0], r[1], r[2], r[3]);
-      if (low) store_quad(low + at_row * a.dim, d, a.dim, rest_of<T>(r[0]), rest_of<T>(r[1]), rest_of<T>(r[2]), rest_of<T>(r[3]));
+      for (int i = 0; i < 16; ++i) r[i] = rest_of<T>(r[i]);
+      store_results(low + at_row * a.dim, 32 * u, a.dim, half, r);
     }
+  }
   if (lse && half == 0)
     lse[(static_cast<long>(b) * a.heads + at.head) * a.queries + at.query] = l == 0.f ? -INFINITY : fmaf(m, factor, __log2f(l) - kShift);
 }

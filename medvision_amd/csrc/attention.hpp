@@ -222,6 +222,12 @@ template <typename T, int DP, bool Few, bool Room = true> struct Staging {
 template <typename T, int W> constexpr bool kHasFew = sizeof(T) == 2 || W <= 64;
 inline bool has_few(int dtype, int dim) { return dtype != MV_F32 || dim <= 64; }
 
+// v where bit `row` of the word is set, `other` where not (a field and a merge: two instructions)
+__device__ __forceinline__ float where_bit(unsigned word, int row, float v, float other) {
+  const unsigned all = static_cast<unsigned>(__builtin_amdgcn_sbfe(static_cast<int>(word), row, 1));
+  return __uint_as_float((all & __float_as_uint(v)) | (~all & __float_as_uint(other)));
+}
+
 // Which of 64 keys count: bits for lanes' keys
 __device__ __forceinline__ unsigned long long use_bits(const AttentionArgs &a, int b, int first, int count, int length) {
   const int lane = threadIdx.x & 63, j = first + lane;
@@ -387,6 +393,38 @@ template <typename T> __device__ __forceinline__ void store_quad(T *row, int d, 
 #pragma unroll
     for (int i = 0; i < 3; ++i)
       if (d + i < dim) row[d + i] = store_cast<T>(v[i]);
+  }
+}
+
+// 32 elements of a column's results (as product results stand) to a row from element `first` on.  16 bits: the halves of the
+// wavefront exchange what they have, so that each lane writes eight neighbours.
+template <typename T> __device__ __forceinline__ void store_results(T *row, int first, int dim, int half, const float (&v)[16]) {
+  if constexpr (sizeof(T) == 2) {
+#pragma unroll
+    for (int a = 0; a < 2; ++a) {
+      unsigned w[2][2];   // [register group 2 a + .][pair]
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) w[i][e] = pack2<T>(v[4 * (2 * a + i) + 2 * e], v[4 * (2 * a + i) + 2 * e + 1]);
+      u32x4 r;   // lower half: elements 16 a .. + 7, upper half: 16 a + 8 .. + 15
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const auto both = __builtin_amdgcn_permlane32_swap(w[0][e], w[1][e], false, false);
+        r[e] = both[0], r[2 + e] = both[1];
+      }
+      const int d = first + 16 * a + 8 * half;
+      if (d + 8 <= dim) {
+        reinterpret_cast<Loose<u32x4, 2> *>(row + d)->v = r;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 7; ++i)
+          if (d + i < dim) reinterpret_cast<unsigned short *>(row)[d + i] = static_cast<unsigned short>(r[i / 2] >> (i % 2 * 16));
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) store_quad(row, first + 8 * i + 4 * half, dim, v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
   }
 }
 

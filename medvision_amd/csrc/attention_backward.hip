@@ -66,9 +66,12 @@ template <int N> __device__ __forceinline__ void add_sums(f32x16 (&o)[N], const 
 // One column of the sums, as a row of `dim` elements
 template <typename O, int N> __device__ __forceinline__ void store_column(O *row, const f32x16 (&o)[N], int dim, int half) {
 #pragma unroll
-  for (int u = 0; u < N; ++u)
+  for (int u = 0; u < N; ++u) {
+    float r[16];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) store_quad(row, 32 * u + 8 * i + 4 * half, dim, o[u][4 * i], o[u][4 * i + 1], o[u][4 * i + 2], o[u][4 * i + 3]);
+    for (int i = 0; i < 16; ++i) r[i] = o[u][i];
+    store_results(row, 32 * u, dim, half, r);
+  }
 }
 
 // Rounding of the weights' gradients to 16 bits for the second product would leave dq with 1.45 - 1.7 times the error of its
@@ -152,7 +155,7 @@ __global__ __launch_bounds__(256, W > 64 || (sizeof(T) == 4 && W == 64) ? 1 : si
       for (int i = 0; i < 16; ++i) ds[i] = __builtin_amdgcn_exp2f(fmaf(s[i], factor, -sums_log)) * (dp[i] - d_i);
       if (word != ~0u) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) ds[i] = word >> (4 * half) >> result_row(i, 0) & 1 ? ds[i] : 0.f;
+        for (int i = 0; i < 16; ++i) ds[i] = where_bit(word >> (4 * half), result_row(i, 0), ds[i], 0.f);
       }
       raise.scale(ds, sum);
       add_transposed<true>(ks, key, ds, sum, lane);
