@@ -474,3 +474,66 @@ def test_groups_of_heads_of_any_size(dtype, heads, key_heads):
     for Lq, Lk in ((70, 20), (20, 70)):
         case = attention_case(heads + Lq, dtype, 1, Lq, Lk, heads, key_heads, 24, "both")
         compare_attention(run_attention(*case), *case)
+
+
+# ---- offsets of more than 32 bits -----------------------------------------------------------------------------------
+def far_apart(t, stride, start):
+    """The values of ``t [1, rows, heads, channels]`` in memory where rows are ``stride`` elements apart."""
+    storage = torch.empty(start + t.shape[1] * stride, dtype=t.dtype, device=t.device)
+    view = storage.as_strided(t.shape, (storage.numel(), stride, t.shape[3], 1), start)
+    view.copy_(t)
+    return view
+
+
+@pytest.mark.parametrize("sizes", [(3, 700, 4, 2, 64), (700, 700, 2, 2, 32), (700, 40, 2, 1, 128)])
+def test_attention_on_rows_far_apart(sizes):
+    """Rows 2^22 elements apart: the last ones are behind 2^31 elements.  The same bits as from dense copies."""
+    Lq, Lk, H, Hk, D = sizes
+    q, k, v, go, mask, lengths = attention_case(Lq, torch.float16, 1, Lq, Lk, H, Hk, D, "mask")
+    near = run_attention(q, k, v, go, mask, lengths)
+    far = run_attention(far_apart(q, 2 ** 22, 8), far_apart(k, 2 ** 22, 16), far_apart(v, 2 ** 22, 24), go, mask, lengths)
+    for a, b in zip(near, far):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("rows,columns", [(2 ** 18 + 40, 8192), (2 ** 28 + 40, 8)])
+def test_norm_of_more_than_2_31_elements(rows, columns):
+    """The last rows give what they give alone."""
+    import medvision_amd.ops as ops
+    g = gen(columns)
+    x, r = (torch.empty(rows, columns, dtype=torch.float16, device=DEV) for _ in range(2))
+    last = slice(rows - 100, rows)
+    for t in (x, r):
+        t[:-100] = 1
+        t[last] = randn(g, 100, columns, dtype=torch.float16)
+    w = randn(g, columns, dtype=torch.float16)
+    gy = torch.ones_like(x)
+
+    def grads(x, r, gy):
+        x, r = x.detach().requires_grad_(True), r.detach().requires_grad_(True)
+        y, h = ops.add_rms_norm(x, r, w)
+        return (y, h, torch.autograd.grad((y, h), x, (gy, gy))[0])
+
+    whole = [t[last].clone() for t in grads(x, r, gy)]
+    for a, b in zip(whole, grads(x[last], r[last], gy[last])):
+        assert torch.equal(a, b)
+    if columns >= 128:
+        del whole, gy
+        whole = [t[last].clone() for t in ops.add_rms_norm_quantized(x, r, w)]
+        for a, b in zip(whole, ops.add_rms_norm_quantized(x[last], r[last], w)):
+            assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+@pytest.mark.parametrize("rows,inputs,outputs", [(25000, 87808, 64), (2 ** 19 + 1000, 128, 4096)])
+def test_block_linear_of_more_than_2_31_elements(rows, inputs, outputs):
+    import medvision_amd.ops as ops
+    g = gen(rows)
+    x = torch.ones(rows, inputs, dtype=torch.float16, device=DEV)
+    last = slice(rows - 70, rows)
+    x[last] = randn(g, 70, inputs, dtype=torch.float16)
+    q, s = ops.quantize_blocks(x)
+    q1, s1 = ops.quantize_blocks(x[last])
+    assert torch.equal(q[last].view(torch.uint8), q1.view(torch.uint8)) and torch.equal(s[last], s1)
+    wq, ws = ops.quantize_blocks(randn(g, outputs, inputs) / math.sqrt(inputs), 128)
+    y = ops.block_linear(q, s, wq, ws, out_dtype=torch.float16)
+    ref.check(y[last], *ref.block_linear(q1, s1, wq, ws, None, torch.float16), "y")
