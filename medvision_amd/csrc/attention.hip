@@ -21,9 +21,11 @@ namespace {
 // Bound by vector issue for heads of 32: of a score, seven issue slots are vector instructions (four of them the
 // exponential), two matrix instructions.  2 x 2000 queries x 8 heads over 27648 keys of 32, float16: 218 us with the join of
 // four splits = 4.05e12 scores/s, vector units 76 % and matrix units 23 % busy.  Heads of 64 (2 x 1000 over 6912, bf16): 52 us,
-// of 128 (2 x 2000 over 8192): 186 us = 720 TFLOP/s, two wavefronts per SIMD and LDS 45 %.  One query per sample reads the
+// of 128 (2 x 2000 over 8192): 184 us = 730 TFLOP/s, two wavefronts per SIMD and LDS 45 %.  One query per sample reads the
 // keys once: 4 samples of 32768 keys, 16 heads over 4 of 64 channels: 27 us + 4 us for the join of 32 splits (134 MB at full
-// length: 5.0 TB/s).  float32 on its own matrix instructions: 2 x 2000 over 4096, 8 heads of 64: 329 us = 102 of 154 TFLOP/s.
+// length: 5.0 TB/s).  float32 on its own matrix instructions: 2 x 2000 over 4096, 8 heads of 64: 338 us = 99 of 154 TFLOP/s.
+// 2 x 32768 queries over 100 keys, 8 heads sharing 2 of 32, float16, with the output's low bits: 35 us, 102 MB (keys held in LDS
+// over several tiles of rows, with the next queries on their way: 39 us, for that takes 167 registers instead of 121).
 template <typename T, int W, int WQ>
 __global__ __launch_bounds__(256, sizeof(T) == 4 ? (W > 64 ? 1 : 2) : W > 64 ? 2 : W == 64 ? 3 : 4) void attend_kernel(
     AttentionArgs a, T *out, T *low, float *lse, float *part, int row_tiles, int splits) {

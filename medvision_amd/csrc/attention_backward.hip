@@ -9,9 +9,9 @@
 // Forming the weights twice costs two of seven products, and saves what dq by atomics would: 64 times the scores' count over
 // the head's width in additions to memory.  Both kernels are bound by the chain from LDS through products, exponential and
 // products again, with two or three wavefronts per SIMD to hide it (registers: sums and operands of a 32 x W tile twice).
-// 2 x 1000 queries over 6912 keys, 8 heads of 64, bf16: dq 76 us, dk and dv 94 us, matrix units 41 and 26 %, vector issue 52
+// 2 x 1000 queries over 6912 keys, 8 heads of 64, bf16: dq 77 us, dk and dv 91 us, matrix units 41 and 26 %, vector issue 52
 // and 31 % busy.  2 x 32768 queries over 100 keys, 8 heads sharing 2 of 32, float16: 55 and 39 us (+ 7 us for the sums of 128
-// splits); 170 MB are read and written for dq.  2 x 2000 over 8192, 8 heads of 128, bf16: 366 and 517 us, one wavefront per SIMD.
+// splits); 170 MB are read and written for dq.  2 x 2000 over 8192, 8 heads of 128, bf16: 358 and 500 us, one wavefront per SIMD.
 #include "attention.hpp"
 
 #include <algorithm>
@@ -76,7 +76,7 @@ template <typename O, int N> __device__ __forceinline__ void store_column(O *row
 
 // Rounding of the weights' gradients to 16 bits for the second product would leave dq with 1.45 - 1.7 times the error of its
 // own rounding (they sum to zero over a row, their roundings do not); what it takes away is multiplied too: 1.01 - 1.1 times,
-// for a fourth of the kernel's matrix instructions more (62 -> 76 us at 1000 x 6912).  dk and dv sum over queries and keep the
+// for a fourth of the kernel's matrix instructions more (62 -> 77 us at 1000 x 6912).  dk and dv sum over queries and keep the
 // single product: 1.4 times.
 //
 // ---- dq -------------------------------------------------------------------------------------------------------

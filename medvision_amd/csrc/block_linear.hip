@@ -71,13 +71,13 @@ template <typename T, int TN> __device__ __forceinline__ void store_row(const Re
 // multiplied).  A row of a block is 128 bytes, eight pieces of 16; piece c of row r stands at c ^ (r & 7), so that the 16
 // rows of an operand that one instruction reads spread over all banks (no conflicts).
 //
-// 256 x 256 with eight wavefronts of 64 x 128: 16384 x 4096 x 4096 276 us = 1.99 PFLOP/s (a plain product of the library:
-// 2.34), 8192^3 2.06.  Of 490 us for the latter 380 are left without the loads, 406 without the products, 400 without the
+// 256 x 256 with eight wavefronts of 64 x 128: 16384 x 4096 x 4096 257 us = 2.14 PFLOP/s (a plain product of the library:
+// 2.34), 8192^3 2.11.  Of 490 us for the latter 380 are left without the loads, 406 without the products, 400 without the
 // additions of the scaled products to the sums: loads into LDS, reads from it (96 bytes per clock and compute unit at the
 // matrix units' full rate), matrix and vector instructions take about as long each and overlap less than whole.
-// 128 x 128 with twice four wavefronts of 64 x 64, where there are fewer than 192 of the large tiles (4000 x 12544 x 1024: 72 us = 1.42 PFLOP/s; 160 with
-// the large ones, 80 with those split in four): the loads alone take 52 us (803 MB from the L2s, 15.6 TB/s), reads and products
-// 48, and both share the LDS.
+// 128 x 128 with twice four wavefronts of 64 x 64, where there are fewer than 192 of the large tiles (4000 x 12544 x 1024:
+// 72 us = 1.42 PFLOP/s; 160 with the large ones, 80 with those split in four): the loads alone take 52 us (803 MB from the
+// L2s, 15.6 TB/s), reads and products 48, and both share the LDS.
 template <int BM, int BN, int WM, int WN, int WK> struct Tiles {
   static constexpr int kThreads = 64 * WM * WN * WK, kTM = BM / WM / 16, kTN = BN / WN / 16;
   static constexpr int kStage = (BM + BN) * kBlock;   // bytes of one block of both operands
@@ -408,8 +408,8 @@ struct Plan {
 
 int ceil_div(long a, long b) { return static_cast<int>((a + b - 1) / b); }
 
-// Few rows up to 64 (of 128 x 12544 x 1024, which tiles take, 19 us).  Sums are split where there are fewer workgroups than compute units (512 for few rows), into shares of
-// eight blocks at least; a split costs the parts' way through memory (4000 x 1024 x 4096 in one piece 25 us, in two 77), so
+// Few rows up to 64 (64 x 12544 x 1024 14.6 us; of 128, which tiles take, 19.4).  Sums are split where there are fewer
+// workgroups than compute units (512 for few rows), into shares of eight blocks at least; a split costs the parts' way through memory (4000 x 1024 x 4096 in one piece 25 us, in two 77), so
 // that no more are made than fill the chip once (1000 x 4096 x 1024: 30.0 us in one piece, 21.0 in four, 30.7 in eight).
 Plan plan_of(long rows, int inputs, int outputs) {
   const int blocks = inputs / kBlock;

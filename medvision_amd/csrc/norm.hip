@@ -91,8 +91,8 @@ template <int Lanes> __device__ __forceinline__ float row_sum(float v, float *ld
 }
 
 // Rows that fit into registers: Lanes threads, 8 Chunks columns each.  One pass over memory, which bounds it: 55296 x 256 in
-// bf16 with residual 19 us (5.9 TB/s for four bytes in and four out of an element), 55296 x 1000 79 us (5.6 TB/s), in 8 bits
-// 72 us (5.4 TB/s).  Rows of 1003 columns start at any byte: 97 us.  A wavefront or less takes a row as long as there
+// bf16 with residual 19 us (5.9 TB/s for four bytes in and four out of an element), 55296 x 1000 78 us (5.6 TB/s), in 8 bits
+// 75 us (5.2 TB/s).  Rows of 1003 columns start at any byte: 97 us.  A wavefront or less takes a row as long as there
 // are 512 columns (no barrier); 513 to 1024 columns run on two wavefronts with eight columns per thread (on one with sixteen, the
 // gradients below took 150 instead of 105 us: half as many loads in flight).
 template <typename T, int Lanes, int Chunks>
@@ -160,7 +160,7 @@ __global__ __launch_bounds__(kThreads) void norm_rows(const T *x, const T *resid
 
 // Both gradients in one pass over memory: a workgroup takes every gridDim-th row (or group of rows), and keeps its share of
 // the weight's gradient in registers until the end.  Bound by memory: 55296 x 256 in bf16 with both incoming gradients 29 us
-// (3.9 TB/s), 55296 x 1000 105 us (4.2 TB/s), with the join of 1024 partial sums.
+// (3.9 TB/s), 55296 x 1000 104 us (4.2 TB/s), with the join of 1024 partial sums.
 template <typename T, int Lanes, int Chunks>
 __global__ __launch_bounds__(kThreads) void norm_grad(const T *h, const void *weight, bool wide, const T *gy, const T *gsum, T *gx,
                                                       float *partial, long rows, int columns, float eps) {
@@ -345,7 +345,8 @@ __global__ __launch_bounds__(kThreads) void norm_grad_weight(const float *partia
   else static_cast<T *>(gw)[c] = store_cast<T>(sum);
 }
 
-// 16 threads for a block of one row and 128 columns.  Bound by memory: 4000 x 12544 in bf16 33 us (150 MB, 4.6 TB/s).
+// 16 threads for a block of one row and 128 columns.  Bound by memory: 4000 x 12544 in bf16 33 us (150 MB, 4.6 TB/s);
+// 8 x 87808, the first of two kernels of a call, 4 us.
 constexpr int kAtOnce = 2;   // blocks of 16 threads, the loads of all before the first is used
 template <typename T>
 __global__ __launch_bounds__(kThreads) void quantize_rows(const T *x, unsigned char *q, float *scales, long blocks, int columns) {
