@@ -76,8 +76,11 @@ template <typename O, int N> __device__ __forceinline__ void store_column(O *row
 
 // Rounding of the weights' gradients to 16 bits for the second product would leave dq with 1.45 - 1.7 times the error of its
 // own rounding (they sum to zero over a row, their roundings do not); what it takes away is multiplied too: 1.01 - 1.1 times,
-// for a fourth of the kernel's matrix instructions more (62 -> 77 us at 1000 x 6912).  dk and dv sum over queries and keep the
-// single product: 1.4 times.
+// for a fourth of the kernel's matrix instructions more (62 -> 77 us at 1000 x 6912).  dk and dv sum over queries; theirs is 1.4
+// times with the single product, and up to 1.9 where there are few keys (the gradients of two weights are each other's
+// negative), few rows, or so few weights that those of a few large ones show: up to 32 keys, 64 rows for a head of keys or 2^20
+// weights are multiplied twice as well (1.0 - 1.1 times).  There that costs little (bf16, 8 heads of 64: 6674 queries x 14 keys 19.8 -> 20.1 us,
+// 60 x 9000 15.6 -> 17.4; float16, 8 of 32, 32768 x 30 20.8 -> 24.1); it would take 1000 x 6912 from 91 to 126 us.
 //
 // ---- dq -------------------------------------------------------------------------------------------------------
 // As the forward kernel; leaves d_i for the next one.
@@ -188,8 +191,8 @@ __global__ __launch_bounds__(256, W > 64 || (sizeof(T) == 4 && W == 64) ? 1 : si
 // A key per lane; rows of queries and of output gradients go through LDS.  WK = 4: 32 keys for each wavefront, the same 32
 // rows; WK = 1 (few keys): the same 32 keys, each wavefront 32 of 128 rows, joined at the end.  A key that does not count
 // spoils nothing but its own column, which is written as zeros.
-template <typename T, int W, int WK>
-__global__ __launch_bounds__(256, W == 128 || (sizeof(T) == 4 && W > 32) || (W == 96 && WK == 1) ? 1 : W == 32 && sizeof(T) == 2 ? 3 : 2) void attend_grad_key(
+template <typename T, int W, int WK, bool Fine>
+__global__ __launch_bounds__(256, W == 128 || (sizeof(T) == 4 && W > 32) || (W == 96 && Fine) ? 1 : W == 32 && sizeof(T) == 2 ? 3 : 2) void attend_grad_key(
     AttentionArgs a, const float *lse, const float *delta, const T *go, T *gk, T *gv, float *part, int key_tiles, int splits) {
   constexpr int DP = stored(W);
   using S = Staging<T, DP, WK == 1, W != 96>;   // (96: two wavefronts per SIMD, 130 -> 83 us at 1000 x 4000 x 8 heads of 80; 128 would spill)
@@ -264,9 +267,9 @@ __global__ __launch_bounds__(256, W == 128 || (sizeof(T) == 4 && W > 32) || (W =
           ds[4 * i + e] = p[4 * i + e] * (dp[4 * i + e] - d4[e]);
         }
       }
-      add_transposed(os, row, p, dv, lane);
+      add_transposed<Fine>(os, row, p, dv, lane);
       raise.scale(ds, dk);
-      add_transposed(qs, row, ds, dk, lane);
+      add_transposed<Fine>(qs, row, ds, dk, lane);
     }
     if (t + 1 < last) {
       if constexpr (S::kBuffers == 1) __syncthreads();
@@ -315,7 +318,7 @@ template <typename T> void sum_parts(const float *part, T *out, T *second, long 
 }
 
 struct BackwardPlan {
-  bool few_rows, few_keys;
+  bool few_rows, few_keys, fine;
   int row_tiles, query_splits, key_tiles, key_splits;
 };
 
@@ -324,6 +327,7 @@ BackwardPlan backward_plan(const mv_attention_shape *s, int dtype) {
   const long rows = static_cast<long>(s->heads / s->key_heads) * s->queries, heads = std::max(1L, static_cast<long>(s->batch) * s->key_heads);
   p.few_rows = rows <= 32 && has_few(dtype, s->dim);
   p.few_keys = s->keys <= 32 && has_few(dtype, s->dim);
+  p.fine = rows <= 64 || heads * rows * s->keys <= 1 << 20;
   p.row_tiles = static_cast<int>(p.few_rows ? 1 : (rows + 127) / 128);
   p.key_tiles = static_cast<int>(p.few_keys ? 1 : (s->keys + 127L) / 128);
   const long least = dtype == MV_F32 ? 64 : 512;   // keys, or rows, that are worth a split
@@ -357,10 +361,15 @@ void launch_backward(const BackwardPlan &p, const AttentionArgs &a, const void *
     bool done = false;
     if constexpr (kHasFew<T, W>)
       if (p.few_keys) {
-        attend_grad_key<T, W, 1><<<grid, 256, 0, s>>>(a, lse, delta, d_o, static_cast<T *>(gk), static_cast<T *>(gv), part, p.key_tiles, p.key_splits);
+        attend_grad_key<T, W, 1, sizeof(T) == 2><<<grid, 256, 0, s>>>(a, lse, delta, d_o, static_cast<T *>(gk), static_cast<T *>(gv), part, p.key_tiles, p.key_splits);
         done = true;
       }
-    if (!done) attend_grad_key<T, W, 4><<<grid, 256, 0, s>>>(a, lse, delta, d_o, static_cast<T *>(gk), static_cast<T *>(gv), part, p.key_tiles, p.key_splits);
+    if constexpr (sizeof(T) == 2)
+      if (!done && p.fine) {
+        attend_grad_key<T, W, 4, true><<<grid, 256, 0, s>>>(a, lse, delta, d_o, static_cast<T *>(gk), static_cast<T *>(gv), part, p.key_tiles, p.key_splits);
+        done = true;
+      }
+    if (!done) attend_grad_key<T, W, 4, false><<<grid, 256, 0, s>>>(a, lse, delta, d_o, static_cast<T *>(gk), static_cast<T *>(gv), part, p.key_tiles, p.key_splits);
     if (p.key_splits > 1) sum_parts<T>(part, static_cast<T *>(gk), static_cast<T *>(gv), keys, p.key_splits, s);
   }
 }

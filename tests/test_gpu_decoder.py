@@ -537,3 +537,14 @@ def test_block_linear_of_more_than_2_31_elements(rows, inputs, outputs):
     wq, ws = ops.quantize_blocks(randn(g, outputs, inputs) / math.sqrt(inputs), 128)
     y = ops.block_linear(q, s, wq, ws, out_dtype=torch.float16)
     ref.check(y[last], *ref.block_linear(q1, s1, wq, ws, None, torch.float16), "y")
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("sizes", [(1, 17, 206, 4, 4, 80), (2, 300, 2, 8, 8, 32), (1, 3000, 14, 2, 1, 64), (1, 12, 5000, 4, 4, 32)])
+def test_gradients_of_few_weights_are_off_by_little_more_than_their_rounding(dtype, sizes):
+    """Weights rounded once would add an error as large as the result's own: a factor of the root of two."""
+    q, k, v, go, mask, lengths = attention_case(sizes[1], dtype, *sizes, "none")
+    got = run_attention(q, k, v, go, mask, lengths)
+    for name, t, (w, _) in zip(("output", "dq", "dk", "dv"), got, ref.attention(q, k, v, mask, lengths, None, go)):
+        w = w.double().to(t.device)
+        assert (t.double() - w).norm() <= math.sqrt(2) * (w.to(dtype).double() - w).norm(), name
