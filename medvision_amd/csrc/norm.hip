@@ -14,20 +14,21 @@ namespace mv {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kMostColumns = 16384;   // of a row in registers
 
-__device__ __forceinline__ float wave_sum(float v) {
+template <typename V> __device__ __forceinline__ V wave_sum(V v) {
 #pragma unroll
   for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
   return v;
 }
 // Sum over the workgroup, the same for every thread.
-__device__ __forceinline__ float block_sum(float v, float *lds) {
+template <int Threads = kThreads, typename V> __device__ __forceinline__ V block_sum(V v, V *lds) {
   v = wave_sum(v);
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
   __syncthreads();
-  v = 0.f;
+  v = 0;
 #pragma unroll
-  for (int i = 0; i < kThreads / 64; ++i) v += lds[i];
+  for (int i = 0; i < Threads / 64; ++i) v += lds[i];
   __syncthreads();
   return v;
 }
@@ -40,19 +41,40 @@ __device__ __forceinline__ float dot8(const float (&a)[8], const float (&b)[8]) 
   return (s[0] + s[1]) + (s[2] + s[3]);
 }
 
-// v w n: 16-bit factors v, w have an exact product; of others the rest goes into the second one.
-template <typename T> __device__ __forceinline__ float scaled(float v, float w, float n) {
-  const float p = v * w;
-  if constexpr (sizeof(T) == 2) return p * n;
-  const float most = fmaf(p, n, fmaf(v, w, -p) * n);
-  return most == most ? most : p * n;   // (an infinite product has no rest)
-}
-
 // 1 / sqrt(a) to the last bit but one: the hardware's value (1 ulp), corrected by what a r^2 is off from 1, in two parts.
 __device__ __forceinline__ float inverse_root(float a) {
   const float r = __builtin_amdgcn_rsqf(a), t = a * r, rest = fmaf(a, r, -t);
   const float e = fmaf(-t, r, 1.f) - rest * r, better = fmaf(0.5f * r, e, r);
   return better == better ? better : r;   // (0, infinity, NaN, and numbers so small that a r is none)
+}
+
+// 1 / sqrt(a) of a row in two parts, corrected in the same way: results in front of a scale of 8-bit values are then off by their
+// own roundings alone (16-bit rows, 55296 x 1000 in 8 bits: 74 -> 75 us).  float32 rows sum their squares over lanes in 64
+// bits too, memory leaves the time for it; 16-bit rows would take 78 us with that.
+template <typename T> using SumOf = std::conditional_t<sizeof(T) == 4, double, float>;
+struct Root {
+  float high, low = 0.f;
+  __device__ __forceinline__ explicit Root(float a) {
+    const float r = __builtin_amdgcn_rsqf(a), t = a * r, rest = fmaf(a, r, -t);
+    const float step = 0.5f * r * (fmaf(-t, r, 1.f) - rest * r);
+    high = r + step, low = (r - high) + step;
+    if (high != high) high = r;   // (0, infinity, NaN, and numbers so small that a r is none)
+    if (low != low) low = 0.f;
+  }
+  __device__ __forceinline__ explicit Root(double a) {
+    double r = __builtin_amdgcn_rsq(a);
+    const double better = fma(0.5 * r, fma(-a * r, r, 1.), r);
+    if (better == better) r = better;   // (0, infinity, NaN)
+    high = static_cast<float>(r), low = static_cast<float>(r - high);
+    if (low != low) low = 0.f;
+  }
+};
+
+// v w n: 16-bit factors v, w have an exact product; of others the rest goes into the second one.
+template <typename T> __device__ __forceinline__ float scaled(float v, float w, const Root &n) {
+  const float p = v * w;
+  const float most = fmaf(p, n.high, sizeof(T) == 2 ? p * n.low : fmaf(p, n.low, fmaf(v, w, -p) * n.high));
+  return most == most ? most : p * n.high;   // (an infinite product has no rest)
 }
 
 __device__ __forceinline__ void load_weight(const void *w, bool wide, const float *, int col, int left, float (&out)[8]) {
@@ -75,8 +97,8 @@ __device__ __forceinline__ float lanes_scale(const float (&v)[8]) {
 }
 
 // Sum over the Lanes threads of a row, the same for each of them
-template <int Lanes> __device__ __forceinline__ float row_sum(float v, float *lds) {
-  if constexpr (Lanes == kThreads) return block_sum(v, lds);
+template <int Lanes, typename V> __device__ __forceinline__ V row_sum(V v, V *lds) {
+  if constexpr (Lanes >= kThreads) return block_sum<Lanes>(v, lds);
   if constexpr (Lanes == 128) {   // two wavefronts
     v = wave_sum(v);
     if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
@@ -90,16 +112,19 @@ template <int Lanes> __device__ __forceinline__ float row_sum(float v, float *ld
   return v;
 }
 
+constexpr int threads_of(int lanes) { return lanes > kThreads ? lanes : kThreads; }
+
 // Rows that fit into registers: Lanes threads, 8 Chunks columns each.  One pass over memory, which bounds it: 55296 x 256 in
 // bf16 with residual 19 us (5.9 TB/s for four bytes in and four out of an element), 55296 x 1000 78 us (5.6 TB/s), in 8 bits
 // 75 us (5.2 TB/s).  Rows of 1003 columns start at any byte: 97 us.  A wavefront or less takes a row as long as there
-// are 512 columns (no barrier); 513 to 1024 columns run on two wavefronts with eight columns per thread (on one with sixteen, the
-// gradients below took 150 instead of 105 us: half as many loads in flight).
+// are 512 columns (no barrier); 513 to 1024 columns run on two wavefronts with eight columns per thread (on one with sixteen,
+// the gradients below took 150 instead of 105 us: half as many loads in flight), more than 4096 on 512 or 1024 threads with
+// sixteen (5000 x 8192 61 us; with 32 on 256 threads 65).  10000 columns 62 us of 4000 rows (72 in two passes).
 template <typename T, int Lanes, int Chunks>
-__global__ __launch_bounds__(kThreads) void norm_rows(const T *x, const T *residual, const void *weight, bool wide, T *y, unsigned char *q,
+__global__ __launch_bounds__(threads_of(Lanes)) void norm_rows(const T *x, const T *residual, const void *weight, bool wide, T *y, unsigned char *q,
                                                       float *scales, T *sum, long rows, int columns, float eps) {
-  __shared__ float lds[kThreads / 64];
-  const long mine = static_cast<long>(linear_block()) * (kThreads / Lanes) + threadIdx.x / Lanes;
+  __shared__ SumOf<T> lds[threads_of(Lanes) / 64];
+  const long mine = static_cast<long>(linear_block()) * (threads_of(Lanes) / Lanes) + threadIdx.x / Lanes;
   if (mine >= rows && (Lanes != 128 || mine - threadIdx.x / Lanes >= rows)) return;   // (two rows wait for each other)
   const long row = min(mine, rows - 1);   // (the last one twice, with the same results)
   const int lane = threadIdx.x % Lanes;
@@ -135,7 +160,7 @@ __global__ __launch_bounds__(kThreads) void norm_rows(const T *x, const T *resid
   }
 #pragma unroll
   for (int k = 0; k < Chunks; ++k) squares += dot8(v[k], v[k]);
-  const float n = inverse_root(row_sum<Lanes>(squares, lds) / columns + eps);
+  const Root n(row_sum<Lanes>(static_cast<SumOf<T>>(squares), lds) / columns + eps);
   const int padded = (columns + kBlock - 1) / kBlock * kBlock;
 #pragma unroll
   for (int k = 0; k < Chunks; ++k) {
@@ -160,12 +185,15 @@ __global__ __launch_bounds__(kThreads) void norm_rows(const T *x, const T *resid
 
 // Both gradients in one pass over memory: a workgroup takes every gridDim-th row (or group of rows), and keeps its share of
 // the weight's gradient in registers until the end.  Bound by memory: 55296 x 256 in bf16 with both incoming gradients 29 us
-// (3.9 TB/s), 55296 x 1000 104 us (4.2 TB/s), with the join of 1024 partial sums.
+// (3.9 TB/s), 55296 x 1000 100 us (4.4 TB/s), with the join of 1024 partial sums (1536: 32 and 125 us, 512: 35 and 164).
+// Longer rows have fewer workgroups, and as many fewer partial sums: 5000 x 8192 on 512 of 512 threads 76 us (115 on 1024 of
+// 256, 108 on 512 of those); beyond 8192 columns on 512 threads with 32 columns each (3000 x 16384 127 us; two passes 164, 1024
+// threads with sixteen spill 275 registers: 338).
 template <typename T, int Lanes, int Chunks>
-__global__ __launch_bounds__(kThreads) void norm_grad(const T *h, const void *weight, bool wide, const T *gy, const T *gsum, T *gx,
+__global__ __launch_bounds__(threads_of(Lanes)) void norm_grad(const T *h, const void *weight, bool wide, const T *gy, const T *gsum, T *gx,
                                                       float *partial, long rows, int columns, float eps) {
-  constexpr int kGroups = kThreads / Lanes;
-  __shared__ float lds[kThreads / 64];
+  constexpr int kGroups = threads_of(Lanes) / Lanes;
+  __shared__ float lds[threads_of(Lanes) / 64];
   __shared__ float sums[kGroups > 1 ? kGroups - 1 : 1][Lanes * Chunks * 8];
   const int lane = threadIdx.x % Lanes, group = threadIdx.x / Lanes;
   float w[Chunks][8], dw[Chunks][8] = {};
@@ -234,11 +262,11 @@ template <typename T>
 __global__ __launch_bounds__(kThreads) void norm_long_rows(const T *x, const T *residual, const void *weight, bool wide, T *y,
                                                         unsigned char *q, float *scales, T *sum, long rows, int columns,
                                                         float eps) {
-  __shared__ float lds[kThreads / 64];
+  __shared__ SumOf<T> lds[kThreads / 64];
   const long row = linear_block();
   if (row >= rows) return;
   const T *xr = x + row * columns;
-  float squares = 0.f;
+  SumOf<T> squares = 0;
   for (int c = threadIdx.x * 8; c < columns; c += kThreads * 8) {
     float v[8], r[8];
     load8(xr + c, columns - c, v);
@@ -250,7 +278,7 @@ __global__ __launch_bounds__(kThreads) void norm_long_rows(const T *x, const T *
     }
     squares += dot8(v, v);
   }
-  const float n = inverse_root(block_sum(squares, lds) / columns + eps);
+  const Root n(block_sum(squares, lds) / columns + eps);
   const T *hr = residual ? sum + row * columns : xr;
   const int padded = (columns + kBlock - 1) / kBlock * kBlock;
   for (int c = threadIdx.x * 8; c < (q ? padded : columns); c += kThreads * 8) {
@@ -407,8 +435,8 @@ __global__ __launch_bounds__(kThreads) void quantize_tiles(const T *x, unsigned 
   if (threadIdx.x == 0) scales[tile] = s;
 }
 
-// Calls f with the threads of a row and the pieces of eight columns of each, for rows of up to 8192 columns; false: longer
-template <typename F> bool for_row_shape(int columns, const F &f) {
+// Calls f with the threads of a row and the pieces of eight columns of each, for rows of up to kMostColumns; false: longer
+template <bool Gradients, typename F> bool for_row_shape(int columns, const F &f) {
   using std::integral_constant;
   if (columns <= 128) f(integral_constant<int, 16>(), integral_constant<int, 1>());
   else if (columns <= 256) f(integral_constant<int, 32>(), integral_constant<int, 1>());
@@ -416,15 +444,17 @@ template <typename F> bool for_row_shape(int columns, const F &f) {
   else if (columns <= 1024) f(integral_constant<int, 128>(), integral_constant<int, 1>());
   else if (columns <= 2048) f(integral_constant<int, 256>(), integral_constant<int, 1>());
   else if (columns <= 4096) f(integral_constant<int, 256>(), integral_constant<int, 2>());
-  else if (columns <= 8192) f(integral_constant<int, 256>(), integral_constant<int, 4>());
-  return columns <= 8192;
+  else if (columns <= 8192) f(integral_constant<int, 512>(), integral_constant<int, 2>());
+  else if (columns <= kMostColumns) f(integral_constant<int, Gradients ? 512 : 1024>(), integral_constant<int, Gradients ? 4 : 2>());
+  return columns <= kMostColumns;
 }
 
-constexpr long kGradGroups = 1024;   // workgroups of the gradients' kernel: four per compute unit, and as many partial sums
+constexpr long kGradGroups = 1024;   // workgroups of 256 threads of the gradients' kernel: four per compute unit
 // workgroups of it, and partial sums of the weight's gradient
 int grad_parts(long rows, int columns) {
   const int per = columns <= 128 ? 16 : columns <= 256 ? 8 : columns <= 512 ? 4 : columns <= 1024 ? 2 : 1;
-  return columns > 8192 ? kSlices : static_cast<int>(std::max(1L, std::min(kGradGroups, (rows + per - 1) / per)));
+  const long most = columns <= 4096 ? kGradGroups : columns <= 8192 ? kGradGroups / 2 : kGradGroups / 4;
+  return columns > kMostColumns ? kSlices : static_cast<int>(std::max(1L, std::min(most, (rows + per - 1) / per)));
 }
 
 int norm_arguments(long rows, int columns, int dtype, int weight_dtype) {
@@ -447,10 +477,9 @@ int norm_forward(const void *x, const void *residual, const void *weight, void *
   MV_FLOATS(dtype, {
     const T *const xt = static_cast<const T *>(x), *const rt = static_cast<const T *>(residual);
     T *const yt = static_cast<T *>(y), *const ht = static_cast<T *>(sum);
-    const bool fits = for_row_shape(columns, [&](auto lanes, auto chunks) {
-      constexpr int kRows = kThreads / lanes;
-      norm_rows<T, lanes, chunks><<<linear_grid((rows + kRows - 1) / kRows, kThreads), kThreads, 0, st>>>(xt, rt, weight, wide, yt, q8, sc, ht, rows,
-                                                                                                          columns, eps);
+    const bool fits = for_row_shape<false>(columns, [&](auto lanes, auto chunks) {
+      constexpr int kAll = threads_of(lanes), kRows = kAll / lanes;
+      norm_rows<T, lanes, chunks><<<linear_grid((rows + kRows - 1) / kRows, kAll), kAll, 0, st>>>(xt, rt, weight, wide, yt, q8, sc, ht, rows, columns, eps);
     });
     if (!fits)
       norm_long_rows<T><<<linear_grid(rows, kThreads), kThreads, 0, st>>>(xt, rt, weight, wide, yt, q8, sc, ht, rows, columns, eps);
@@ -477,7 +506,7 @@ int mv_add_rms_norm_quantized(const void *x, const void *residual, const void *w
 
 size_t mv_add_rms_norm_backward_workspace_bytes(int64_t rows, int columns) {
   if (rows < 0 || columns <= 0) return 0;
-  return 4 * ((columns > 8192 ? static_cast<size_t>(rows) : 0) + static_cast<size_t>(grad_parts(rows, columns)) * columns);
+  return 4 * ((columns > kMostColumns ? static_cast<size_t>(rows) : 0) + static_cast<size_t>(grad_parts(rows, columns)) * columns);
 }
 
 int mv_add_rms_norm_backward(const void *h, const void *weight, const void *grad_y, const void *grad_sum, void *grad_x,
@@ -493,8 +522,8 @@ int mv_add_rms_norm_backward(const void *h, const void *weight, const void *grad
   MV_FLOATS(dtype, {
     const T *const ht = static_cast<const T *>(h), *const gy = static_cast<const T *>(grad_y), *const gs = static_cast<const T *>(grad_sum);
     T *const gx = static_cast<T *>(grad_x);
-    const bool fits = for_row_shape(columns, [&](auto lanes, auto chunks) {
-      norm_grad<T, lanes, chunks><<<parts, kThreads, 0, st>>>(ht, weight, wide, gy, gs, gx, partial, rows, columns, eps);
+    const bool fits = for_row_shape<true>(columns, [&](auto lanes, auto chunks) {
+      norm_grad<T, lanes, chunks><<<parts, threads_of(lanes), 0, st>>>(ht, weight, wide, gy, gs, gx, partial, rows, columns, eps);
     });
     if (!fits) {
       if (rows > 0) norm_grad_long_rows<T><<<linear_grid(rows, kThreads), kThreads, 0, st>>>(ht, weight, wide, gy, gs, gx, norms, rows, columns, eps);

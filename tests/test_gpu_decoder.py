@@ -548,3 +548,22 @@ def test_gradients_of_few_weights_are_off_by_little_more_than_their_rounding(dty
     for name, t, (w, _) in zip(("output", "dq", "dk", "dv"), got, ref.attention(q, k, v, mask, lengths, None, go)):
         w = w.double().to(t.device)
         assert (t.double() - w).norm() <= math.sqrt(2) * (w.to(dtype).double() - w).norm(), name
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,columns", [(1100, 4100), (600, 8200), (300, 16384), (70, 16392)])
+def test_norm_of_long_rows(dtype, rows, columns):
+    """More rows than workgroups, on both sides of the longest row that is kept in registers; in 8 bits too."""
+    import medvision_amd.ops as ops
+    g = gen(columns)
+    x, r, gy, gs = (randn(g, rows, columns, dtype=dtype) for _ in range(4))
+    w = randn(g, columns, dtype=dtype)
+    ins = [t.detach().requires_grad_(True) for t in (x, r, w)]
+    y, h = ops.add_rms_norm(*ins, eps=1e-5)
+    grads = torch.autograd.grad((y, h), ins, (gy, gs))
+    want = ref.add_rms_norm(x, r, w, 1e-5, gy, gs)
+    for name, t, (value, bound) in zip(("y", "sum", "dx", "dweight"), (y, h, grads[0], grads[2]), want):
+        ref.check(t, value, bound, name)
+    q, s, h2 = ops.add_rms_norm_quantized(x[:70], r[:70], w, eps=1e-5)
+    assert torch.equal(h2, h[:70])
+    same_blocks((q, s), ref.blocks(want[0][0][:70].float(), 1))
