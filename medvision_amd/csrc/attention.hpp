@@ -122,10 +122,28 @@ template <typename T, int DP, int Rows> struct Tile {
   }
 };
 
-// 16 bytes of a row from element d on, zeros beyond dim
-template <typename T> __device__ __forceinline__ u32x4 load_piece(const T *row, int d, int dim) {
+// The last piece of a row whose elements do not fill it: 16 bytes up to the row's end, moved down by the `over` elements that
+// stand in front of the piece, with zeros behind.  One load and a few instructions: 2 x 1000 queries over 6912 keys, 4 heads of
+// 100 channels, bf16: forward 52 us, dq 93, dk and dv 143 (an element at a time 100, 197 and 263).
+template <typename T> __device__ __forceinline__ u32x4 moved_down(u32x4 r, int over) {
+  const int bits = over * 8 * static_cast<int>(sizeof(T));   // 16 .. 112
+  const unsigned long long low = r[0] | static_cast<unsigned long long>(r[1]) << 32, high = r[2] | static_cast<unsigned long long>(r[3]) << 32;
+  const unsigned long long down = bits < 64 ? low >> bits | high << (64 - bits) : high >> (bits - 64), rest = bits < 64 ? high >> bits : 0;
+  return u32x4{static_cast<unsigned>(down), static_cast<unsigned>(down >> 32), static_cast<unsigned>(rest), static_cast<unsigned>(rest >> 32)};
+}
+
+// 16 bytes of a row from element d < dim on, zeros beyond dim.  Ends: a piece that the row does not fill is read so; Raw: left to
+// be moved down.  Otherwise it is read an element at a time.
+template <typename T, bool Ends = true, bool Raw = false> __device__ __forceinline__ u32x4 load_piece(const T *row, int d, int dim) {
   constexpr int kPer = 16 / sizeof(T);
-  if (d + kPer <= dim) return reinterpret_cast<const Loose<u32x4, sizeof(T)> *>(row + d)->v;
+  if constexpr (Ends) {
+    if (dim >= kPer) {
+      const u32x4 r = reinterpret_cast<const Loose<u32x4, sizeof(T)> *>(row + min(d, dim - kPer))->v;
+      return Raw || d + kPer <= dim ? r : moved_down<T>(r, d + kPer - dim);
+    }
+  } else if (d + kPer <= dim) {
+    return reinterpret_cast<const Loose<u32x4, sizeof(T)> *>(row + d)->v;
+  }
   u32x4 r = {0, 0, 0, 0};
   if constexpr (sizeof(T) == 2) {
 #pragma unroll
@@ -141,7 +159,7 @@ template <typename T> __device__ __forceinline__ u32x4 load_piece(const T *row, 
 
 // Two tiles of the same rows (keys and values, queries and gradients) on their way into LDS: each of 256 threads has one
 // column of pieces, and every kStep-th row of it.
-template <typename T, int DP, int Rows> struct Pair {
+template <typename T, int DP, int Rows, bool Ends = true> struct Pair {
   using L = Tile<T, DP, Rows>;
   static constexpr int kStep = 256 / L::kPieces, kMine = Rows / kStep;
   static_assert(Rows % kStep == 0, "");
@@ -152,12 +170,15 @@ template <typename T, int DP, int Rows> struct Pair {
   long head_a = 0, head_b = 0;
   __device__ __forceinline__ Pair(long stride_a, long stride_b, int dim)
       : row(threadIdx.x / L::kPieces), d(threadIdx.x % L::kPieces * L::kPer), dim(dim), stride_a(stride_a), stride_b(stride_b) {
-    at_a = row * stride_a + (d < dim ? d : 0), at_b = row * stride_b + (d < dim ? d : 0);
+    const int from = first_element();
+    at_a = row * stride_a + from, at_b = row * stride_b + from;
   }
+  __device__ __forceinline__ int first_element() const { return Ends ? max(0, min(d, dim - L::kPer)) : d < dim ? d : 0; }
   // rows that are `inner` heads (a divisor of Rows) of each of Rows / inner queries
   __device__ __forceinline__ void heads(int inner, long head_a, long head_b) {
     per = inner;
-    at_a = row_at(0, stride_a, head_a) + (d < dim ? d : 0), at_b = row_at(0, stride_b, head_b) + (d < dim ? d : 0);
+    const int from = first_element();
+    at_a = row_at(0, stride_a, head_a) + from, at_b = row_at(0, stride_b, head_b) + from;
     this->head_a = head_a, this->head_b = head_b;
   }
   __device__ __forceinline__ long row_at(int n, long stride, long head) const {
@@ -169,7 +190,7 @@ template <typename T, int DP, int Rows> struct Pair {
   // Rows 0 .. left - 1 from two addresses on.  Whole tiles without a branch; what stands for elements that do not exist is
   // any value, to be replaced by put().
   __device__ __forceinline__ void load(const T *from_a, const T *from_b, int left) {
-    if (left >= Rows && dim % L::kPer == 0 && kStep % per == 0) {
+    if (left >= Rows && (Ends ? dim >= L::kPer : dim % L::kPer == 0) && kStep % per == 0) {
 #pragma unroll
       for (int n = 0; n < kMine; ++n) {
         a[n] = reinterpret_cast<const Loose<u32x4, sizeof(T)> *>(from_a + n * (kStep / per) * stride_a + at_a)->v;
@@ -181,8 +202,8 @@ template <typename T, int DP, int Rows> struct Pair {
     for (int n = 0; n < kMine; ++n) {
       a[n] = b[n] = u32x4{0, 0, 0, 0};
       if (row + n * kStep < left && d < dim) {
-        a[n] = load_piece<T>(from_a + row_at(n, stride_a, head_a), d, dim);
-        b[n] = load_piece<T>(from_b + row_at(n, stride_b, head_b), d, dim);
+        a[n] = load_piece<T, Ends, Ends>(from_a + row_at(n, stride_a, head_a), d, dim);
+        b[n] = load_piece<T, Ends, Ends>(from_b + row_at(n, stride_b, head_b), d, dim);
       }
     }
   }
@@ -201,6 +222,13 @@ template <typename T, int DP, int Rows> struct Pair {
     if (dim < DP && d >= dim) {
 #pragma unroll
       for (int n = 0; n < kMine; ++n) a[n] = b[n] = u32x4{0, 0, 0, 0};
+    }
+    if (Ends && dim % L::kPer && dim >= L::kPer) {
+      if (d < dim && d + L::kPer > dim) {
+        const int over = L::kPer - dim % L::kPer;
+#pragma unroll
+        for (int n = 0; n < kMine; ++n) a[n] = moved_down<T>(a[n], over), b[n] = moved_down<T>(b[n], over);
+      }
     }
 #pragma unroll
     for (int n = 0; n < kMine; ++n) {
@@ -235,7 +263,7 @@ __device__ __forceinline__ unsigned long long use_bits(const AttentionArgs &a, i
 }
 
 // One column (a query, a key) per lane % 32, all W elements: the second operand of products over the elements.
-template <typename T, int W> struct Column {
+template <typename T, int W, bool Ends = true> struct Column {
   static constexpr int kPer = 16 / sizeof(T), kCount = W / kPer / 2;
   u32x4 r[kCount];   // piece 2 n + lane / 32
   __device__ __forceinline__ void load(const T *row, bool use, int dim, int half) {
@@ -243,7 +271,7 @@ template <typename T, int W> struct Column {
     for (int n = 0; n < kCount; ++n) {
       const int d = (2 * n + half) * kPer;
       r[n] = u32x4{0, 0, 0, 0};
-      if (use && d < dim) r[n] = load_piece<T>(row, d, dim);
+      if (use && d < dim) r[n] = load_piece<T, Ends>(row, d, dim);
     }
   }
   __device__ __forceinline__ float dot(const Column &with) const {
@@ -269,8 +297,8 @@ template <typename T, int W> struct Column {
 };
 
 // 32 rows of a tile times the columns: over the elements of a row
-template <typename T, int W, int DP, int Rows>
-__device__ __forceinline__ f32x16 times(const Tile<T, DP, Rows> &tile, int first_row, const Column<T, W> &c, int lane) {
+template <typename T, int W, bool Ends, int DP, int Rows>
+__device__ __forceinline__ f32x16 times(const Tile<T, DP, Rows> &tile, int first_row, const Column<T, W, Ends> &c, int lane) {
   f32x16 s = {};
   const int row = first_row + (lane & 31), half = lane >> 5;
 #pragma unroll

@@ -199,6 +199,9 @@ __global__ __launch_bounds__(256, W == 128 || (sizeof(T) == 4 && W > 32) || (W =
   using S = Staging<T, DP, WK == 1, W != 96>;   // (96: two wavefronts per SIMD, 130 -> 83 us at 1000 x 4000 x 8 heads of 80; 128 would spill)
   constexpr int kRows = S::kRows, kSteps = WK == 4 ? kRows / 32 : 1, kOut = W / 32;
   constexpr float kShift = __is_same(T, __half) ? 15.f : 0.f;   // as in the forward pass
+  // Ends of rows at once, but for heads of 33 to 64 channels in 16 bits: with it the compiler keeps 25 registers fewer in use
+  // there, and heads of 64 take 100 instead of 90 us (1000 x 6912).
+  constexpr bool kEnds = sizeof(T) == 4 || W != 64;
   using L = Tile<T, DP, kRows>;
   __shared__ L tiles[S::kBuffers][2];
   __shared__ float stats[S::kBuffers][2][kRows];
@@ -219,7 +222,7 @@ __global__ __launch_bounds__(256, W == 128 || (sizeof(T) == 4 && W > 32) || (W =
   const int my_row = WK == 4 ? 0 : 32 * wave;
   float next_l = INFINITY, next_d = 0.f;
   const long go_row = static_cast<long>(a.heads) * a.dim;
-  Pair<T, DP, kRows> next(a.qs[1], go_row, a.dim);
+  Pair<T, DP, kRows, kEnds> next(a.qs[1], go_row, a.dim);
   if (inner > 1) next.heads(inner, a.qs[2], a.dim);
   const int my_stat_query = static_cast<unsigned>(threadIdx.x) / static_cast<unsigned>(inner), my_stat_head = threadIdx.x - my_stat_query * inner;
   auto load = [&](int t) {
@@ -241,7 +244,7 @@ __global__ __launch_bounds__(256, W == 128 || (sizeof(T) == 4 && W > 32) || (W =
     }
   };
   if (first < last) load(first);
-  Column<T, W> k, v;
+  Column<T, W, kEnds> k, v;
   k.load(static_cast<const T *>(a.k) + b * a.ks[0] + j * a.ks[1] + g * a.ks[2], use, a.dim, half);
   v.load(static_cast<const T *>(a.v) + b * a.vs[0] + j * a.vs[1] + g * a.vs[2], use, a.dim, half);
   if (a.scale < 0.f) k.negate();
