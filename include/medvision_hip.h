@@ -311,8 +311,9 @@ int mv_deform_conv_2d(const void *input, const void *offset, const void *weight,
  * Key j of sample b counts when j < key_lengths[b] (int32, NULL: all; values beyond the keys mean all, below 0 none) and
  * key_mask[b * mask_stride + j] != 0 (bytes, NULL: all).  What the other keys and values hold is of no effect, not even
  * NaN.  A query without any key gets zeros, and gives none a gradient.
- * output [batch, queries, heads, dim] and the gradients are dense; lse [batch, heads, queries] float32 (NULL: not wanted by
- * the forward pass) holds log2 of the sum of 2^(log2(e) scale q.k), -inf where no key counts; output_low, like output, what
+ * output [batch, queries, heads, dim] and the gradients are dense; lse [2, batch, heads, queries] float32 (NULL: not wanted by
+ * the forward pass) holds log2 of the sum of 2^(log2(e) (scale q.k - |scale| m)), -inf where no key counts, and then m, the
+ * largest q.k (-q.k where the scale is negative) of a row; output_low, like output, what
  * its rounding took away, for the backward pass of 16-bit types (NULL: not wanted; gradients are then off by up to twice the
  * type's rounding).  The backward pass WRITES its gradients; it wants the workspace, the forward pass splits long rows of
  * keys only if it gets its own. */

@@ -10,6 +10,12 @@
 namespace mv {
 namespace {
 
+// log2 of a row's sum of weights beside the largest one, and the largest score (RowLog takes them)
+__device__ __forceinline__ void put_log(const AttentionArgs &a, float *lse, long at, float m, float l, float shift) {
+  lse[at] = l == 0.f ? -INFINITY : __log2f(l) - shift;
+  lse[static_cast<long>(a.batch) * a.heads * a.queries + at] = l == 0.f ? 0.f : m;
+}
+
 // ---- forward -------------------------------------------------------------------------------------------------
 // Four wavefronts: WQ = 4, 32 rows each over the same 64 keys at a time; WQ = 1, the same 32 rows, each 32 of 128 keys at a
 // time (few rows: their sums are joined at the end).  Scores are formed transposed, a query per lane: maximum and sum of a
@@ -68,6 +74,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? (W > 64 ? 1 : 2) : W > 64 ? 2
   if (first < last) put(first);
 
   float m = -INFINITY, l = 0.f;
+  bool far = false;
   f32x16 o[kOut] = {};
   for (int t = first; t < last; ++t) {
     unsigned long long use[kSteps];
@@ -97,13 +104,19 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? (W > 64 ? 1 : 2) : W > 64 ? 2
 #pragma unroll
         for (int i = 0; i < 16; ++i) top = fmaxf(top, s[n][i]);
       top = fmaxf(m, fmaxf(top, other_half(top)));
-      const float base = top == -INFINITY ? 0.f : top;
+      float base = top == -INFINITY ? 0.f : top;
       if (__ballot(top > m)) {   // (no row's maximum has grown: nothing to scale)
+        far = sizeof(T) == 2 && __ballot(fabsf(base) * factor > kFar);
         const float keep = __builtin_amdgcn_exp2f((m - base) * factor);
         l *= keep;
 #pragma unroll
         for (int u = 0; u < kOut; ++u) o[u] *= keep;
         m = top;
+      }
+      if (__builtin_expect(far, false)) {   // (the difference first)
+#pragma unroll
+        for (int n = 0; n < kTiles; ++n) s[n] -= base;
+        base = 0.f;
       }
       const float shift = fmaf(base, -factor, kShift);
 #pragma unroll
@@ -191,8 +204,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? (W > 64 ? 1 : 2) : W > 64 ? 2
       store_results(low + at_row * a.dim, 32 * u, a.dim, half, r);
     }
   }
-  if (lse && half == 0)
-    lse[(static_cast<long>(b) * a.heads + at.head) * a.queries + at.query] = l == 0.f ? -INFINITY : fmaf(m, factor, __log2f(l) - kShift);
+  if (lse && half == 0) put_log(a, lse, (static_cast<long>(b) * a.heads + at.head) * a.queries + at.query, m, l, kShift);
 }
 
 // The splits' sums.  Many splits (few rows): a workgroup for a row, whose wavefronts take turns at the splits.
@@ -226,7 +238,7 @@ __global__ __launch_bounds__(256) void join_many(AttentionArgs a, const float *p
     out[row * a.dim + d] = store_cast<T>(v);
     if (low) low[row * a.dim + d] = store_cast<T>(rest_of<T>(v));
   }
-  if (lse && threadIdx.x == 0) lse[a.log_at(row)] = l == 0.f ? -INFINITY : fmaf(top, factor, __log2f(l) - shift);
+  if (lse && threadIdx.x == 0) put_log(a, lse, a.log_at(row), top, l, shift);
 }
 
 // Few splits: four neighbouring elements of a row per thread.
@@ -259,7 +271,7 @@ __global__ __launch_bounds__(256) void join_few(AttentionArgs a, const float *pa
   for (int e = 0; e < 4; ++e) o[e] *= inverse;
   store_quad(out + row * a.dim, d, a.dim, o[0], o[1], o[2], o[3]);
   if (low) store_quad(low + row * a.dim, d, a.dim, rest_of<T>(o[0]), rest_of<T>(o[1]), rest_of<T>(o[2]), rest_of<T>(o[3]));
-  if (lse && d == 0) lse[a.log_at(row)] = l == 0.f ? -INFINITY : fmaf(top, factor, __log2f(l) - shift);
+  if (lse && d == 0) put_log(a, lse, a.log_at(row), top, l, shift);
 }
 
 // Four wavefronts have 128 rows, or the 32 rows that there are.  Keys are split until every resident workgroup has work

@@ -14,6 +14,10 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kMostDim = 128;
 constexpr float kLog2e = 1.44269504088896f;
+// Scores beyond this (in powers of two) have their row's largest one taken off before they are scaled.  Otherwise scaling and
+// the difference are one instruction, which rounds the largest one's product by up to 2^-24 of it: 2^-14 here, less than the
+// weights' rounding to 16 bits; from 2^24 on whole powers of two, with which weights of 2^15 overflow float16.
+constexpr float kFar = 1024.f;
 
 struct AttentionArgs {
   const void *q, *k, *v;
@@ -249,6 +253,21 @@ template <typename T, int DP, bool Few, bool Room = true> struct Staging {
 // into the registers.
 template <typename T, int W> constexpr bool kHasFew = sizeof(T) == 2 || W <= 64;
 inline bool has_few(int dtype, int dim) { return dtype != MV_F32 || dim <= 64; }
+
+// What the backward pass takes from a score, `base` before scaling and `log` after it: the logarithm of the row's sum in one
+// part, or the largest score first (float32: always, weights are then good to their last bits).  The difference is taken from the
+// product as it was rounded in the forward pass too: a product that started from -most would not round it.
+template <typename T> struct RowLog {
+  float rest = -INFINITY, most = 0.f;   // (rows that do not exist are like those without a key)
+  __device__ __forceinline__ void load(const AttentionArgs &a, const float *lse, long at) {
+    rest = lse[at], most = lse[static_cast<long>(a.batch) * a.heads * a.queries + at];
+  }
+  __device__ __forceinline__ bool far(float factor) const { return sizeof(T) == 4 || fabsf(most) * factor > kFar; }
+  __device__ __forceinline__ float base(float factor) const { return far(factor) ? most : 0.f; }
+  __device__ __forceinline__ float log(float factor) const {
+    return rest == -INFINITY ? INFINITY : far(factor) ? rest : fmaf(most, factor, rest);   // (weights of zero where no key counts)
+  }
+};
 
 // v where bit `row` of the word is set, `other` where not (a field and a merge: two instructions)
 __device__ __forceinline__ float where_bit(unsigned word, int row, float v, float other) {

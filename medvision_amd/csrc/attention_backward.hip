@@ -1,6 +1,6 @@
 // Gradients of cross attention.
 //
-//   p_ij = 2^(factor q_i.k_j - L_i)   d_i = do_i.o_i   ds_ij = p_ij (do_i.v_j - d_i)
+//   p_ij = 2^(factor q_i.k_j - L_i) = 2^(factor (q_i.k_j - m_i) - l_i)   d_i = do_i.o_i   ds_ij = p_ij (do_i.v_j - d_i)
 //   dq_i = scale sum_j ds_ij k_j   dk_j = scale sum_i ds_ij q_i   dv_j = sum_i p_ij do_i
 //
 // Two kernels form the weights anew, one with a query per lane for dq, one with a key per lane for dk and dv: no atomics,
@@ -134,8 +134,9 @@ __global__ __launch_bounds__(256, W > 64 || (sizeof(T) == 4 && W == 64) ? 1 : si
   }
   q.load(static_cast<const T *>(a.q) + b * a.qs[0] + at.query * a.qs[1] + at.head * a.qs[2], live, a.dim, half);
   if (a.scale < 0.f) q.negate();
-  float sums_log = live ? lse[at_l] : INFINITY;
-  if (sums_log == -INFINITY) sums_log = INFINITY;   // no key counts: weights of zero
+  RowLog<T> sums;
+  if (live) sums.load(a, lse, at_l);
+  const float sums_log = sums.log(factor), base = sums.base(factor);
   if (live && split == 0 && half == 0 && (WQ == 4 || wave == 0)) delta[at_l] = d_i;
   if (first < last) put(first);
 
@@ -153,7 +154,10 @@ __global__ __launch_bounds__(256, W > 64 || (sizeof(T) == 4 && W == 64) ? 1 : si
       const unsigned word = static_cast<unsigned>(use[n / 2] >> (32 * (n % 2)));
       if (!word) continue;
       const int key = my_key + 32 * n;
-      const f32x16 s = times(ks, key, q, lane), dp = times(vs, key, d_o, lane);
+      f32x16 s = times(ks, key, q, lane);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[i] -= base;
+      const f32x16 dp = times(vs, key, d_o, lane);
       float ds[16];
 #pragma unroll
       for (int i = 0; i < 16; ++i) ds[i] = __builtin_amdgcn_exp2f(fmaf(s[i], factor, -sums_log)) * (dp[i] - d_i);
@@ -175,13 +179,13 @@ __global__ __launch_bounds__(256, W > 64 || (sizeof(T) == 4 && W == 64) ? 1 : si
 
   if constexpr (WQ == 1) {
     __syncthreads();
-    f32x4 *const sums = reinterpret_cast<f32x4 *>(tiles);
+    f32x4 *const parts = reinterpret_cast<f32x4 *>(tiles);
     static_assert(sizeof(tiles) >= 3 * kOut * 4 * 64 * sizeof(f32x4), "");
-    if (wave) put_sums(sum, sums + (wave - 1) * kOut * 4 * 64, lane);
+    if (wave) put_sums(sum, parts + (wave - 1) * kOut * 4 * 64, lane);
     __syncthreads();
     if (wave) return;
 #pragma unroll
-    for (int w = 0; w < 3; ++w) add_sums(sum, sums + w * kOut * 4 * 64, lane);
+    for (int w = 0; w < 3; ++w) add_sums(sum, parts + w * kOut * 4 * 64, lane);
   }
   if (!live) return;
   if (splits > 1) store_column(part + (static_cast<long>(split) * a.batch * a.queries * a.heads + at_row) * a.dim, sum, a.dim, half);
@@ -202,9 +206,14 @@ __global__ __launch_bounds__(256, W == 128 || (sizeof(T) == 4 && W > 32) || (W =
   // Ends of rows at once, but for heads of 33 to 64 channels in 16 bits: with it the compiler keeps 25 registers fewer in use
   // there, and heads of 64 take 100 instead of 90 us (1000 x 6912).
   constexpr bool kEnds = sizeof(T) == 4 || W != 64;
+  // Whether rows' largest scores are taken off where there is one to take off, or always (RowLog): zeros are taken off faster, in the
+  // shade of the next product, than a branch lets the compiler schedule (2 x 2000 over 8192, heads of 128, bf16: 437 and 512 us), but
+  // for heads of 32 (2 x 2000 over 27648 434 and 402 us).
+  constexpr bool kAsk = sizeof(T) == 2 && W == 32;
   using L = Tile<T, DP, kRows>;
   __shared__ L tiles[S::kBuffers][2];
-  __shared__ float stats[S::kBuffers][2][kRows];
+  __shared__ float stats[S::kBuffers][3][kRows];   // logarithms, delta, what is taken off the scores first
+  __shared__ int far_rows[S::kBuffers][kAsk ? kRows / 32 : 1];
   const Place place(a, key_tiles, splits);
   if (!place.in) return;
   const int split = place.split, g = place.g, b = place.b;
@@ -220,7 +229,8 @@ __global__ __launch_bounds__(256, W == 128 || (sizeof(T) == 4 && W > 32) || (W =
   const int all_tiles = place.tile * 32 * WK < length ? outer * per_head : 0;
   const int first = share(all_tiles, split, splits), last = share(all_tiles, split + 1, splits);
   const int my_row = WK == 4 ? 0 : 32 * wave;
-  float next_l = INFINITY, next_d = 0.f;
+  RowLog<T> next_log;
+  float next_d = 0.f;
   const long go_row = static_cast<long>(a.heads) * a.dim;
   Pair<T, DP, kRows, kEnds> next(a.qs[1], go_row, a.dim);
   if (inner > 1) next.heads(inner, a.qs[2], a.dim);
@@ -230,17 +240,22 @@ __global__ __launch_bounds__(256, W == 128 || (sizeof(T) == 4 && W > 32) || (W =
     const int query = row / inner;
     next.load(static_cast<const T *>(a.q) + b * a.qs[0] + query * a.qs[1] + h * a.qs[2],
               go + (static_cast<long>(b) * a.queries + query) * go_row + static_cast<long>(h) * a.dim, left);
-    next_l = INFINITY, next_d = 0.f;
+    next_log = RowLog<T>(), next_d = 0.f;
     if (static_cast<int>(threadIdx.x) < min(kRows, left)) {
       const long from = (static_cast<long>(b) * a.heads + h + my_stat_head) * a.queries + query + my_stat_query;
-      next_l = lse[from], next_d = delta[from];
+      next_log.load(a, lse, from), next_d = delta[from];
     }
   };
   auto put = [&](int t) {
     next.put(tiles[t % S::kBuffers]);
     if (threadIdx.x < kRows) {
-      stats[t % S::kBuffers][0][threadIdx.x] = next_l == -INFINITY ? INFINITY : next_l - kShift;
+      stats[t % S::kBuffers][0][threadIdx.x] = next_log.log(factor) - kShift;
       stats[t % S::kBuffers][1][threadIdx.x] = next_d;
+      stats[t % S::kBuffers][2][threadIdx.x] = next_log.base(factor);
+      if constexpr (kAsk) {
+        const unsigned long long far = __ballot(next_log.far(factor));
+        if ((lane & 31) == 0) far_rows[t % S::kBuffers][threadIdx.x / 32] = static_cast<int>(lane ? far >> 32 : far);
+      }
     }
   };
   if (first < last) load(first);
@@ -259,7 +274,26 @@ __global__ __launch_bounds__(256, W == 128 || (sizeof(T) == 4 && W > 32) || (W =
 #pragma unroll
     for (int n = 0; n < kSteps; ++n) {
       const int row = my_row + 32 * n;
-      const f32x16 s = times(qs, row, k, lane), dp = times(os, row, v, lane);
+      f32x16 s = times(qs, row, k, lane);
+      if constexpr (!kAsk) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const f32x4 base = *reinterpret_cast<const f32x4 *>(&stats[t % S::kBuffers][2][row + 8 * i + 4 * half]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[4 * i + e] -= base[e];
+        }
+      }
+      const f32x16 dp = times(os, row, v, lane);
+      if constexpr (kAsk) {
+        if (__builtin_expect(__builtin_amdgcn_readfirstlane(far_rows[t % S::kBuffers][row / 32]), 0)) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const f32x4 base = *reinterpret_cast<const f32x4 *>(&stats[t % S::kBuffers][2][row + 8 * i + 4 * half]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[4 * i + e] -= base[e];
+          }
+        }
+      }
       float p[16], ds[16];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {

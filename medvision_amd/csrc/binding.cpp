@@ -588,7 +588,7 @@ AttentionResult attention_forward(const AttentionCall &c, double scale, bool tra
   const c10::DeviceGuard guard(c.q.device());
   const mv_attention_shape &s = c.shape;
   const Tensor output = at::empty({s.batch, s.queries, s.heads, s.dim}, c.q.options());
-  const Tensor lse = train ? at::empty({s.batch, s.heads, s.queries}, c.q.options().dtype(at::kFloat)) : Tensor();
+  const Tensor lse = train ? at::empty({2, s.batch, s.heads, s.queries}, c.q.options().dtype(at::kFloat)) : Tensor();
   const Tensor low = train && c.code != MV_F32 ? at::empty_like(output) : Tensor();
   const size_t bytes = mv_cross_attention_forward_workspace_bytes(&s, c.code);
   const Tensor ws = bytes_on(c.q, bytes);
