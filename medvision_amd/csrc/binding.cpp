@@ -573,8 +573,11 @@ AttentionCall attention_call(const Tensor &query, const Tensor &key, const Tenso
   if (key_lengths.defined()) {
     MVB_CHECK(at::isIntegralType(key_lengths.scalar_type(), false), "key_lengths have to be whole numbers, got ", dtype_name(key_lengths));
     MVB_CHECK(key_lengths.dim() == 1 && key_lengths.size(0) == s.batch, "key_lengths has shape ", shape_text(key_lengths.sizes()), ", expected (", s.batch, ")");
-    c.lengths = key_lengths.scalar_type() == at::kInt ? key_lengths.contiguous()
-                                                       : key_lengths.clamp(0, s.keys).to(at::kInt).contiguous();
+    // (the kernels clamp; types that 32 bits do not hold are clamped first, and none in a type that may not hold the keys' number)
+    const auto type = key_lengths.scalar_type();
+    MVB_CHECK(type != at::kUInt64, "key_lengths have to fit into int64, got ", dtype_name(key_lengths));
+    c.lengths = type == at::kLong || type == at::kUInt32 ? key_lengths.to(at::kLong).clamp(0, s.keys) : key_lengths;
+    c.lengths = c.lengths.to(at::kInt).contiguous();
   }
   return c;
 }
