@@ -43,16 +43,19 @@ class RegionDecoderLayer(nn.Module):
         self.up, self.down = nn.Linear(channels, hidden), nn.Linear(hidden, channels)
 
     def for_inference(self, dtype=torch.bfloat16):
-        """This layer, on the GPU, for inference: linear layers in 8 bits, results and the rest in ``dtype``."""
+        """This layer, on the GPU, for inference: linear layers in 8 bits, their results in ``dtype``.  The norms' weights are
+        float32, which goes with regions of any type."""
         layer = copy.copy(self)
         layer._modules = dict(self._modules)
         for name in ("query", "key_value", "out", "up", "down"):
             layer._modules[name] = BlockScaledLinear.from_linear(getattr(self, name), dtype)
         for name in ("norm_query", "norm_hidden"):
-            layer._modules[name] = copy.deepcopy(getattr(self, name)).to(dtype).requires_grad_(False)
+            layer._modules[name] = copy.deepcopy(getattr(self, name)).float().requires_grad_(False)
         return layer.eval()
 
     def _normed(self, norm, x, residual):
+        if residual is not None:   # the sum that is carried keeps its type: float32 regions under autocast, or in front of 8-bit layers
+            x = x.to(residual.dtype)
         if isinstance(self.query, BlockScaledLinear):   # straight to 8 bits
             return norm.quantized(x, residual)
         return norm(x, residual)
@@ -60,7 +63,7 @@ class RegionDecoderLayer(nn.Module):
     def forward(self, regions, tokens, residual=None, key_mask=None, key_lengths=None):
         """``regions [batch, regions, channels]``, ``residual`` like them or None, ``tokens [batch, cells, channels]`` of
         which ``key_mask`` and ``key_lengths`` may leave some out: ``(regions, residual)`` for the next layer.  After the last
-        one the result is their sum."""
+        one the result is their sum.  The residual has the type of the one that was given, or of the regions."""
         y, residual = self._normed(self.norm_query, regions, residual)
         q = self.query(y).unflatten(-1, (self.heads, self.head_channels))
         k, v = self.key_value(tokens).unflatten(-1, (2, self.key_heads, self.head_channels)).unbind(2)
