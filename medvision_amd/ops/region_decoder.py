@@ -46,7 +46,9 @@ class RegionDecoderLayer(nn.Module):
         """This layer, on the GPU, for inference: linear layers in 8 bits, their results in ``dtype``.  The norms' weights are
         float32, which goes with regions of any type."""
         layer = copy.copy(self)
-        layer._modules = dict(self._modules)
+        for name, value in vars(self).items():   # hooks, parameters, buffers and modules of its own
+            if isinstance(value, (dict, set)):
+                setattr(layer, name, value.copy())
         for name in ("query", "key_value", "out", "up", "down"):
             layer._modules[name] = BlockScaledLinear.from_linear(getattr(self, name), dtype)
         for name in ("norm_query", "norm_hidden"):

@@ -58,3 +58,21 @@ def test_layers_of_16_bits_are_served():
         out = whole.for_inference(torch.bfloat16)(*(t.to(DEV).bfloat16() for t in (regions, tokens, residual)), key_lengths=lengths.to(DEV))
     assert all(t.dtype == torch.bfloat16 and torch.isfinite(t).all() for t in out)
     assert whole.norm_query.weight.dtype == torch.bfloat16
+
+
+def test_hooks_stay_with_their_layer():
+    """Hooks that are registered on the layer or on its form for inference run for that one alone; buffers are each one's own."""
+    layer, regions, tokens, *_ = case(torch.float32)
+    layer = layer.to(DEV)
+    before, after = [], []
+    layer.register_forward_hook(lambda *_: before.append(1))
+    with torch.no_grad():
+        fast = layer.for_inference(torch.float16)
+        fast.register_forward_hook(lambda *_: after.append("fast"))
+        layer.register_forward_pre_hook(lambda *_: after.append("layer"))
+        fast.register_buffer("extra", torch.zeros(1))
+        layer(regions.to(DEV), tokens.to(DEV))
+        assert after == ["layer"]
+        fast(regions.to(DEV).half(), tokens.to(DEV).half())
+        assert after == ["layer", "fast"] and len(before) == 2   # (what was registered before goes along)
+    assert "extra" not in dict(layer.named_buffers()) and layer.training and not fast.training
