@@ -51,11 +51,12 @@ class BlockScaledLinear(nn.Module):
 
     def _apply(self, fn, recurse=True):
         # .half() and its like leave what is in 8 bits, and its scales, as they are; moves between devices take all
-        kept = self.weight, self.weight_scales
+        kept = {name: getattr(self, name) for name in ('weight', 'weight_scales')}
         super()._apply(fn, recurse)
-        if self.weight.dtype != torch.float8_e4m3fn:
-            self.weight = kept[0].to(self.weight.device)
-        self.weight_scales = kept[1].to(self.weight.device)
+        for name, tensor in kept.items():
+            now = getattr(self, name)
+            if now.dtype != tensor.dtype:
+                setattr(self, name, tensor.to(now.device))
         return self
 
     def forward(self, x):

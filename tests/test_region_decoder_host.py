@@ -20,3 +20,20 @@ def test_tokens_of_a_map():
     x = torch.arange(2 * 3 * 2 * 2 * 2).view(2, 3, 2, 2, 2)
     t = ops.map_tokens(x)
     assert t.shape == (2, 8, 3) and torch.equal(t[1, 5], x[1, :, 1, 0, 1])
+
+
+def test_8_bit_layers_are_made_on_the_meta_device():
+    """Allocated later, as large models are loaded; other moves and casts keep types and, from a device with values, those."""
+    import medvision_amd.ops as ops
+    layer = ops.BlockScaledLinear(200, 130, device="meta").to_empty(device="cpu")
+    assert layer.weight.device.type == layer.weight_scales.device.type == layer.bias.device.type == "cpu"
+    assert layer.weight.dtype == torch.float8_e4m3fn and layer.weight_scales.dtype == torch.float32
+    given = ops.BlockScaledLinear(200, 130)
+    given.weight.copy_(torch.randn(130, 256).to(torch.float8_e4m3fn))
+    given.weight_scales.copy_(torch.rand(2, 2) + 1e-6)
+    layer.load_state_dict(given.state_dict())
+    for cast in (lambda m: m.half(), lambda m: m.double(), lambda m: m.to(torch.bfloat16), lambda m: m.to("cpu")):
+        moved = cast(layer)
+        assert torch.equal(moved.weight.view(torch.uint8), given.weight.view(torch.uint8)) and torch.equal(moved.weight_scales, given.weight_scales)
+    assert ops.BlockScaledLinear(200, 130, device="meta").half().weight.dtype == torch.float8_e4m3fn
+    assert layer.to("meta").weight.is_meta
