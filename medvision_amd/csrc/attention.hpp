@@ -243,8 +243,11 @@ template <typename T, int DP, int Rows, bool Ends = true> struct Pair {
 };
 
 // Keys (or rows) that a workgroup has in LDS at a time, and whether twice: the next ones are written while these are read.
+constexpr int staged_rows(int bytes, int dp, bool few, bool room) {
+  return !few && !room ? 32 : few || (bytes == 2 && dp == 32) ? 128 : bytes == 4 && dp == 128 ? 32 : 64;
+}
 template <typename T, int DP, bool Few, bool Room = true> struct Staging {
-  static constexpr int kRows = !Few && !Room ? 32 : Few || (sizeof(T) == 2 && DP == 32) ? 128 : sizeof(T) == 4 && DP == 128 ? 32 : 64;
+  static constexpr int kRows = staged_rows(sizeof(T), DP, Few, Room);
   static constexpr int kBytes = 2 * kRows * DP * static_cast<int>(sizeof(T));
   static constexpr int kBuffers = kBytes <= 32768 ? 2 : 1;
 };
@@ -474,6 +477,13 @@ template <typename T> __device__ __forceinline__ void store_results(T *row, int 
     for (int i = 0; i < 4; ++i) store_quad(row, first + 8 * i + 4 * half, dim, v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
   }
 }
+
+// The same for a head of `dim` channels, for the plans: no more splits than there are tiles.  `few` and `room` as the kernels give
+// them to Staging.
+inline int tile_rows(int dtype, int dim, bool few, bool room = true) {
+  return staged_rows(dtype == MV_F32 ? 4 : 2, stored(dim <= 32 ? 32 : dim <= 64 ? 64 : dim <= 96 ? 96 : 128), few, room);
+}
+inline long parts_of(long count, long each) { return (count + each - 1) / each; }
 
 inline int attention_sizes(const mv_attention_shape *s, int dtype) {
   MV_REQUIRE(s, "the shape is missing");

@@ -368,8 +368,11 @@ BackwardPlan backward_plan(const mv_attention_shape *s, int dtype) {
   p.fine = rows <= 64 || heads * rows * s->keys <= 1 << 20;
   p.row_tiles = static_cast<int>(p.few_rows ? 1 : (rows + 127) / 128);
   p.key_tiles = static_cast<int>(p.few_keys ? 1 : (s->keys + 127L) / 128);
-  const long least = dtype == MV_F32 ? 64 : 512;   // keys, or rows, that are worth a split
-  const long key_steps = (s->keys + least - 1) / least, row_steps = s->heads / s->key_heads * ((s->queries + least - 1) / least);
+  const int least = dtype == MV_F32 ? 64 : 512;   // keys, or rows, that are worth a split
+  const long key_steps = parts_of(s->keys, std::max(least, tile_rows(dtype, s->dim, p.few_rows)));
+  // rows as the kernel takes them: those of a group's heads together, or one head after the other
+  const int tile = tile_rows(dtype, s->dim, p.few_keys, s->dim <= 64 || s->dim > 96), group = s->heads / s->key_heads, inner = tile % group == 0 ? group : 1;
+  const long row_steps = group / inner * parts_of(static_cast<long>(s->queries) * inner, std::max(least, tile));
   // as many workgroups as are resident at a time
   const long for_queries = s->dim <= 64 ? 768 : 256, for_keys = s->dim <= 32 ? 768 : s->dim <= 96 ? 512 : 256;
   p.query_splits = static_cast<int>(std::max(1L, std::min(for_queries / std::max(1L, p.row_tiles * heads), key_steps)));

@@ -107,3 +107,20 @@ def test_modules_keep_their_8_bit_weights():
     with pytest.raises(RuntimeError, match="rows of 100, expected 200"):
         m(torch.zeros(3, 100))
     assert "BlockScaledLinear(200, 130" in repr(m) and "AddRMSNorm(8" in repr(ops.AddRMSNorm(8))
+
+
+@pytest.mark.parametrize("dtype,sizes,forward,queries,keys", [
+    # (batch, queries, keys, heads, key_heads, channels), splits of the forward pass, of dq, and of dk and dv
+    ("MV_F16", (1, 1, 1000, 64, 1, 32), 2, 2, 1), ("MV_F16", (1, 10, 200, 16, 4, 32), 1, 1, 1), ("MV_F32", (1, 2, 1000, 64, 2, 64), 16, 16, 1),
+    ("MV_BF16", (2, 7, 500, 64, 1, 128), 1, 1, 1), ("MV_F32", (1, 4, 20, 32, 1, 32), 1, 1, 1), ("MV_F32", (1, 1, 100, 1, 1, 32), 1, 1, 1),
+    ("MV_F16", (1, 600, 64, 4, 2, 64), 1, 1, 3), ("MV_F32", (1, 100, 1000, 2, 2, 64), 16, 16, 2)])
+def test_no_more_splits_than_there_is_work_for(dtype, sizes, forward, queries, keys):
+    """A split has 512 keys or rows (float32: 64) at least, and a tile of them.  Rows of heads that share keys follow each other:
+    few queries of many heads are one tile, with nothing to split.  Read from the workspaces, whose parts are the splits'."""
+    from medvision_amd import _lib
+    lib, kind = _lib.load(), getattr(_lib, dtype)
+    B, Lq, Lk, H, Hk, D = sizes
+    shape = ctypes.byref(_shape(*sizes))
+    assert lib.mv_cross_attention_forward_workspace_bytes(shape, kind) == (4 * forward * B * Lq * H * (D + 2) if forward > 1 else 0)
+    parts = max(queries * B * Lq * H * D if queries > 1 else 0, 2 * keys * B * Lk * Hk * D if keys > 1 else 0)
+    assert lib.mv_cross_attention_backward_workspace_bytes(shape, kind) == 4 * (B * Lq * H + parts)
