@@ -315,8 +315,9 @@ int mv_deform_conv_2d(const void *input, const void *offset, const void *weight,
  * the forward pass) holds log2 of the sum of 2^(log2(e) (scale q.k - |scale| m)), -inf where no key counts, and then m, the
  * largest q.k (-q.k where the scale is negative) of a row; output_low, like output, what
  * its rounding took away, for the backward pass of 16-bit types (NULL: not wanted; gradients are then off by up to twice the
- * type's rounding).  The backward pass WRITES its gradients; it wants the workspace, the forward pass splits long rows of
- * keys only if it gets its own. */
+ * type's rounding).  The backward pass WRITES its gradients: grad_query, or the pair of grad_key and grad_value, may be NULL
+ * where nobody wants them, and then cost nothing.  It wants the workspace (..._for: of the gradients that are wanted, each 0
+ * or 1); the forward pass splits long rows of keys only if it gets its own. */
 typedef struct {
   int batch, queries, keys, heads, key_heads, dim;
   int64_t q_strides[3], k_strides[3], v_strides[3]; /* batch, row, head */
@@ -324,6 +325,7 @@ typedef struct {
 } mv_attention_shape;
 size_t mv_cross_attention_forward_workspace_bytes(const mv_attention_shape *shape, int dtype);
 size_t mv_cross_attention_backward_workspace_bytes(const mv_attention_shape *shape, int dtype);
+size_t mv_cross_attention_backward_workspace_bytes_for(const mv_attention_shape *shape, int dtype, int for_query, int for_keys);
 int mv_cross_attention_forward(const void *query, const void *key, const void *value, const void *key_mask,
                                const void *key_lengths, void *output, void *output_low, void *lse, const mv_attention_shape *shape,
                                float scale, int dtype, void *workspace, size_t workspace_bytes, void *stream);

@@ -90,6 +90,7 @@ SIGNATURES = {
     "mv_deform_conv_2d": (_i, [_p] * 6 + [_i, _i, _p]),
     "mv_cross_attention_forward_workspace_bytes": (_sz, [_ATTENTION_P, _i]),
     "mv_cross_attention_backward_workspace_bytes": (_sz, [_ATTENTION_P, _i]),
+    "mv_cross_attention_backward_workspace_bytes_for": (_sz, [_ATTENTION_P, _i, _i, _i]),
     "mv_cross_attention_forward": (_i, [_p] * 8 + [_ATTENTION_P, _f, _i, _p, _sz, _p]),
     "mv_cross_attention_backward": (_i, [_p] * 12 + [_ATTENTION_P, _f, _i, _p, _sz, _p]),
     "mv_add_rms_norm": (_i, [_p] * 5 + [_i64, _i, _f, _i, _i, _p]),

@@ -83,7 +83,7 @@ template <typename O, int N> __device__ __forceinline__ void store_column(O *row
 // 60 x 9000 15.6 -> 17.4; float16, 8 of 32, 32768 x 30 20.8 -> 24.1); it would take 1000 x 6912 from 91 to 126 us.
 //
 // ---- dq -------------------------------------------------------------------------------------------------------
-// As the forward kernel; leaves d_i for the next one.
+// As the forward kernel; leaves d_i for the next one.  Without gq that is all.
 template <typename T, int W, int WQ>
 __global__ __launch_bounds__(256, W > 64 || (sizeof(T) == 4 && W == 64) ? 1 : sizeof(T) == 4 ? 2 : 3) void attend_grad_query(
     AttentionArgs a, const T *out, const T *low, const float *lse, const T *go, T *gq, float *delta, float *part, int row_tiles, int splits) {
@@ -105,7 +105,7 @@ __global__ __launch_bounds__(256, W > 64 || (sizeof(T) == 4 && W == 64) ? 1 : si
   const float factor = a.factor();
 
   const T *const k = static_cast<const T *>(a.k) + b * a.ks[0] + g * a.ks[2], *const v = static_cast<const T *>(a.v) + b * a.vs[0] + g * a.vs[2];
-  const int length = a.length(b), all_tiles = (length + kKeys - 1) / kKeys;
+  const int length = a.length(b), all_tiles = gq ? (length + kKeys - 1) / kKeys : 0;
   const int first = share(all_tiles, split, splits), last = share(all_tiles, split + 1, splits);
   const int my_key = WQ == 4 ? 0 : 32 * wave;
   Pair<T, DP, kKeys> next(a.ks[1], a.vs[1], a.dim);
@@ -187,7 +187,7 @@ __global__ __launch_bounds__(256, W > 64 || (sizeof(T) == 4 && W == 64) ? 1 : si
 #pragma unroll
     for (int w = 0; w < 3; ++w) add_sums(sum, parts + w * kOut * 4 * 64, lane);
   }
-  if (!live) return;
+  if (!live || !gq) return;
   if (splits > 1) store_column(part + (static_cast<long>(split) * a.batch * a.queries * a.heads + at_row) * a.dim, sum, a.dim, half);
   else store_column(gq + at_row * a.dim, sum, a.dim, half);
 }
@@ -360,7 +360,7 @@ struct BackwardPlan {
   int row_tiles, query_splits, key_tiles, key_splits;
 };
 
-BackwardPlan backward_plan(const mv_attention_shape *s, int dtype) {
+BackwardPlan backward_plan(const mv_attention_shape *s, int dtype, bool for_query = true) {
   BackwardPlan p;
   const long rows = static_cast<long>(s->heads / s->key_heads) * s->queries, heads = std::max(1L, static_cast<long>(s->batch) * s->key_heads);
   p.few_rows = rows <= 32 && has_few(dtype, s->dim);
@@ -375,7 +375,7 @@ BackwardPlan backward_plan(const mv_attention_shape *s, int dtype) {
   const long row_steps = group / inner * parts_of(static_cast<long>(s->queries) * inner, std::max(least, tile));
   // as many workgroups as are resident at a time
   const long for_queries = s->dim <= 64 ? 768 : 256, for_keys = s->dim <= 32 ? 768 : s->dim <= 96 ? 512 : 256;
-  p.query_splits = static_cast<int>(std::max(1L, std::min(for_queries / std::max(1L, p.row_tiles * heads), key_steps)));
+  p.query_splits = !for_query ? 1 : static_cast<int>(std::max(1L, std::min(for_queries / std::max(1L, p.row_tiles * heads), key_steps)));
   p.key_splits = static_cast<int>(std::max(1L, std::min(for_keys / std::max(1L, p.key_tiles * heads), row_steps)));
   return p;
 }
@@ -397,7 +397,7 @@ void launch_backward(const BackwardPlan &p, const AttentionArgs &a, const void *
     if (!done) attend_grad_query<T, W, 4><<<grid, 256, 0, s>>>(a, o, ol, lse, d_o, static_cast<T *>(gq), delta, part, p.row_tiles, p.query_splits);
     if (p.query_splits > 1) sum_parts<T>(part, static_cast<T *>(gq), nullptr, queries, p.query_splits, s);
   }
-  if (keys) {
+  if (keys && gk) {
     const dim3 grid = linear_grid(heads * p.key_tiles * p.key_splits, 256);
     bool done = false;
     if constexpr (kHasFew<T, W>)
@@ -423,11 +423,16 @@ using namespace mv;
 extern "C" {
 
 size_t mv_cross_attention_backward_workspace_bytes(const mv_attention_shape *s, int dtype) {
+  return mv_cross_attention_backward_workspace_bytes_for(s, dtype, 1, 1);
+}
+
+size_t mv_cross_attention_backward_workspace_bytes_for(const mv_attention_shape *s, int dtype, int for_query, int for_keys) {
   if (attention_sizes(s, dtype)) return 0;
-  const BackwardPlan p = backward_plan(s, dtype);
+  const BackwardPlan p = backward_plan(s, dtype, for_query);
   const size_t queries = static_cast<size_t>(s->batch) * s->queries * s->heads, keys = static_cast<size_t>(s->batch) * s->keys * s->key_heads;
-  const size_t for_queries = p.query_splits > 1 ? p.query_splits * queries * s->dim : 0, for_keys = p.key_splits > 1 ? 2 * p.key_splits * keys * s->dim : 0;
-  return sizeof(float) * (queries + std::max(for_queries, for_keys));
+  const size_t query_parts = p.query_splits > 1 ? p.query_splits * queries * s->dim : 0,
+               key_parts = for_keys && p.key_splits > 1 ? 2 * p.key_splits * keys * s->dim : 0;
+  return sizeof(float) * (queries + std::max(query_parts, key_parts));
 }
 
 int mv_cross_attention_backward(const void *query, const void *key, const void *value, const void *key_mask,
@@ -437,10 +442,15 @@ int mv_cross_attention_backward(const void *query, const void *key, const void *
   if (const int status = attention_sizes(shape, dtype)) return status;
   const AttentionArgs a = attention_arguments(shape, query, key, value, key_mask, key_lengths, scale);
   const long rows = static_cast<long>(a.batch) * a.queries * a.heads, columns = static_cast<long>(a.batch) * a.keys * a.key_heads;
-  MV_REQUIRE(rows == 0 || (query && output && lse && grad_output && grad_query), "a tensor is missing");
-  MV_REQUIRE(columns == 0 || (key && value && grad_key && grad_value), "a tensor is missing");
-  MV_REQUIRE(rows == 0 || (workspace && workspace_bytes >= mv_cross_attention_backward_workspace_bytes(shape, dtype)), "the workspace is too small");
-  const BackwardPlan p = backward_plan(shape, dtype);
+  // (a tensor without elements may have any address)
+  const bool for_query = rows != 0 && grad_query, for_keys = columns != 0 && (grad_key || grad_value);
+  MV_REQUIRE(!for_keys || (grad_key && grad_value), "grad_key and grad_value are wanted as a pair");
+  if (!for_query && !for_keys) return MV_OK;
+  MV_REQUIRE(rows == 0 || (query && output && lse && grad_output), "a tensor is missing");
+  MV_REQUIRE(columns == 0 || (key && value), "a tensor is missing");
+  MV_REQUIRE(rows == 0 || (workspace && workspace_bytes >= mv_cross_attention_backward_workspace_bytes_for(shape, dtype, for_query, for_keys)),
+             "the workspace is too small");
+  const BackwardPlan p = backward_plan(shape, dtype, for_query);
   float *const delta = static_cast<float *>(workspace), *const part = delta + rows;
   const float *const sums = static_cast<const float *>(lse);
   const hipStream_t s = static_cast<hipStream_t>(stream);

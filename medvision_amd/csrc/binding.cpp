@@ -534,6 +534,8 @@ void differentiable_once(const variable_list &grads, variable_list &out) {
   }
 }
 
+std::optional<Tensor> maybe(const Tensor &t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; }
+
 // Neighbouring channels of a head; every other stride is the kernels' to follow
 Tensor rows_of_heads(const Tensor &t) { return t.size(3) <= 1 || t.stride(3) == 1 ? t : t.contiguous(); }
 
@@ -600,15 +602,18 @@ AttentionResult attention_forward(const AttentionCall &c, double scale, bool tra
   return {output, lse, low};
 }
 
-variable_list attention_backward(const AttentionCall &c, const Tensor &output, const Tensor &lse, const Tensor &low, const Tensor &grad_in, double scale) {
+// Gradients of the query, and of key and value, as far as they are wanted
+variable_list attention_backward(const AttentionCall &c, const Tensor &output, const Tensor &lse, const Tensor &low, const Tensor &grad_in, double scale,
+                                 bool for_query, bool for_keys) {
   const c10::DeviceGuard guard(c.q.device());
   const mv_attention_shape &s = c.shape;
   same_device(c.q, grad_in, "grad_output");
   MVB_CHECK(grad_in.sizes() == output.sizes(), "grad_output has shape ", shape_text(grad_in.sizes()), ", expected ", shape_text(output.sizes()));
   const Tensor grad = grad_in.to(output.scalar_type()).contiguous();
-  const Tensor gq = at::empty({s.batch, s.queries, s.heads, s.dim}, c.q.options());
-  const Tensor gk = at::empty({s.batch, s.keys, s.key_heads, s.dim}, c.q.options()), gv = at::empty_like(gk);
-  const size_t bytes = mv_cross_attention_backward_workspace_bytes(&s, c.code);
+  Tensor gq, gk, gv;
+  if (for_query) gq = at::empty({s.batch, s.queries, s.heads, s.dim}, c.q.options());
+  if (for_keys) gk = at::empty({s.batch, s.keys, s.key_heads, s.dim}, c.q.options()), gv = at::empty_like(gk);
+  const size_t bytes = mv_cross_attention_backward_workspace_bytes_for(&s, c.code, for_query, for_keys);
   const Tensor ws = bytes_on(c.q, bytes);
   check(mv_cross_attention_backward(ptr(c.q), ptr(c.k), ptr(c.v), ptr(c.mask), ptr(c.lengths), ptr(output), ptr(low), ptr(lse), ptr(grad),
                                     ptr(gq), ptr(gk), ptr(gv), &s, static_cast<float>(scale), c.code, ptr(ws), bytes, stream_of(c.q)));
@@ -630,9 +635,11 @@ struct CrossAttentionFunction : torch::autograd::Function<CrossAttentionFunction
     {
       const at::NoGradGuard no_grad;
       const auto t = ctx->get_saved_variables();
+      const bool wanted[3] = {ctx->needs_input_grad(0), ctx->needs_input_grad(1), ctx->needs_input_grad(2)};
       const variable_list g = attention_backward(attention_call(t[0], t[1], t[2], t[3], t[4]), t[5], t[6], t[7], grads[0],
-                                                 ctx->saved_data["scale"].toDouble());
-      for (int i = 0; i < 3; ++i) out[i] = g[i];
+                                                 ctx->saved_data["scale"].toDouble(), wanted[0], wanted[1] || wanted[2]);
+      for (int i = 0; i < 3; ++i)
+        if (wanted[i]) out[i] = g[i];
     }
     differentiable_once(grads, out);
     return out;
@@ -664,15 +671,15 @@ std::tuple<Tensor, Tensor, std::optional<Tensor>> cross_attention_forward(const 
   return {r.output, r.lse, r.low.defined() ? std::optional<Tensor>(r.low) : std::nullopt};
 }
 
-std::tuple<Tensor, Tensor, Tensor> cross_attention_backward(const Tensor &query, const Tensor &key, const Tensor &value,
+std::vector<std::optional<Tensor>> cross_attention_backward(const Tensor &query, const Tensor &key, const Tensor &value,
                                                             const std::optional<Tensor> &key_mask, const std::optional<Tensor> &key_lengths,
                                                             const Tensor &output, const Tensor &lse, const std::optional<Tensor> &low, const Tensor &grad,
-                                                            const std::optional<double> &scale) {
+                                                            const std::optional<double> &scale, bool for_query, bool for_keys) {
   const py::gil_scoped_release no_gil;
   const at::NoGradGuard no_grad;
   const auto g = attention_backward(attention_call(query, key, value, key_mask.value_or(Tensor()), key_lengths.value_or(Tensor())), output, lse,
-                                    low.value_or(Tensor()), grad, attention_scale(query, scale));
-  return {g[0], g[1], g[2]};
+                                    low.value_or(Tensor()), grad, attention_scale(query, scale), for_query, for_keys);
+  return {maybe(g[0]), maybe(g[1]), maybe(g[2])};
 }
 
 struct NormCall {

@@ -21,8 +21,10 @@ class CrossAttentionFunction(NativeFunction):
     @once_differentiable
     def backward(ctx, grad_output):
         query, key, value, key_mask, key_lengths, output, lse, low = ctx.saved_tensors
-        grads = native.cross_attention_backward(query, key, value, key_mask, key_lengths, output, lse, low, grad_output, ctx.scale)
-        return (*grads, None, None, None)
+        wanted = ctx.needs_input_grad[:3]
+        grads = native.cross_attention_backward(query, key, value, key_mask, key_lengths, output, lse, low, grad_output, ctx.scale,
+                                                wanted[0], wanted[1] or wanted[2])
+        return (*(g if w else None for g, w in zip(grads, wanted)), None, None, None)
 
 
 def cross_attention(query, key, value, key_mask=None, key_lengths=None, scale=None):

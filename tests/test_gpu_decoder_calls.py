@@ -29,3 +29,80 @@ def test_lengths_beyond_int64_are_refused():
     q = rand(1, 2, 5, 2, 16)
     with pytest.raises(RuntimeError, match="fit into int64"):
         ops.cross_attention(q, q, q, key_lengths=torch.tensor([1, 2], device=DEV).to(torch.uint64))
+
+
+# ---- gradients that are wanted -------------------------------------------------------------------------------
+SUBSETS = [(True, False, False), (False, True, False), (False, False, True), (True, True, False), (True, False, True), (False, True, True)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("sizes", [(2, 3, 700, 4, 2, 32), (1, 300, 20, 2, 1, 64), (2, 150, 260, 2, 2, 96)])
+def test_attention_gradients_of_some_inputs(dtype, sizes):
+    """The same bits as all three together, in both forms of the node."""
+    from medvision_amd.ops.cross_attention import CrossAttentionFunction
+
+    class Python(CrossAttentionFunction):
+        @staticmethod
+        def backward(ctx, grad):
+            return CrossAttentionFunction.backward(ctx, grad)
+
+    B, Lq, Lk, H, Hk, D = sizes
+    tensors = rand(1, B, Lq, H, D, dtype=dtype), rand(2, B, Lk, Hk, D, dtype=dtype), rand(3, B, Lk, Hk, D, dtype=dtype)
+    go = rand(4, B, Lq, H, D, dtype=dtype)
+    lengths = torch.full((B,), Lk - 3, device=DEV)
+
+    def grads(function, wanted):
+        ins = [t.clone().requires_grad_(w) for t, w in zip(tensors, wanted)]
+        function.apply(*ins, None, lengths, None).backward(go)
+        return [t.grad for t in ins]
+
+    want = grads(CrossAttentionFunction, (True, True, True))
+    for function in (CrossAttentionFunction, Python):
+        for wanted in SUBSETS:
+            for got, all_of_them, w in zip(grads(function, wanted), want, wanted):
+                assert torch.equal(got, all_of_them) if w else got is None
+
+
+def test_gradients_that_nobody_wants_take_no_memory():
+    """Queries over a frozen encoder: no gradients of the keys and values, and no parts of them, are formed."""
+    import medvision_amd.ops as ops
+    q, k = rand(1, 1, 2000, 8, 64, dtype=torch.float16).requires_grad_(True), rand(2, 1, 100000, 8, 64, dtype=torch.float16)
+    out = ops.cross_attention(q, k, k)
+    go = torch.ones_like(out)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    out.backward(go)
+    assert torch.cuda.max_memory_allocated() - before < k.numel() * k.element_size()
+
+
+def test_entry_points_without_some_gradients():
+    """Null pointers for gradients that are not wanted; what is wanted is the same."""
+    from medvision_amd import _lib
+    lib = _lib.load()
+    B, Lq, Lk, H, D = 1, 9, 50, 2, 32
+    q, go = rand(1, B, Lq, H, D), rand(2, B, Lq, H, D)
+    k, v = rand(3, B, Lk, H, D), rand(4, B, Lk, H, D)
+    s = _lib.AttentionShape(B, Lq, Lk, H, H, D)
+    for strides, t in ((s.q_strides, q), (s.k_strides, k), (s.v_strides, v)):
+        for i in range(3):
+            strides[i] = t.stride(i)
+    from medvision_amd._lib import native
+    out, lse, _ = native.cross_attention_forward(q, k, v, None, None, 0.25)
+    p = lambda t: None if t is None else t.data_ptr()   # noqa: E731
+
+    def call(gq, gk, gv):
+        bytes_ = lib.mv_cross_attention_backward_workspace_bytes(ctypes.byref(s), _lib.MV_F32)
+        ws = torch.empty(bytes_, dtype=torch.uint8, device=DEV)
+        status = lib.mv_cross_attention_backward(p(q), p(k), p(v), None, None, p(out), None, p(lse), p(go), p(gq), p(gk), p(gv), ctypes.byref(s),
+                                                 0.25, _lib.MV_F32, p(ws), bytes_, torch.cuda.current_stream().cuda_stream)
+        torch.cuda.synchronize()
+        return status
+
+    new = lambda: [torch.full_like(t, 7.0) for t in (q, k, v)]   # noqa: E731
+    full, only_q, only_kv = new(), new(), new()
+    assert call(*full) == 0
+    assert call(only_q[0], None, None) == 0 and torch.equal(only_q[0], full[0])
+    assert call(None, *only_kv[1:]) == 0 and torch.equal(only_kv[1], full[1]) and torch.equal(only_kv[2], full[2])
+    assert call(None, None, None) == 0
+    assert call(full[0], full[1], None) == 1 and b"pair" in lib.mv_last_error()
