@@ -340,7 +340,8 @@ int mv_cross_attention_backward(const void *query, const void *key, const void *
  * sum [rows, columns] receives h (NULL exactly when residual is NULL).
  * ..._quantized: y in 8 bits (e4m3) instead, as mv_quantize_blocks gives them.
  * ..._backward: h (x or the sum), grad_y and grad_sum (NULL: none) give grad_x (the residual's gradient is the same) and
- * grad_weight (of weight_dtype), both written; sums over rows are formed in a fixed order. */
+ * grad_weight (of weight_dtype), both written; sums over rows are formed in a fixed order.  Either may be NULL where nobody
+ * wants it; the workspace is for grad_weight. */
 int mv_add_rms_norm(const void *x, const void *residual, const void *weight, void *y, void *sum, int64_t rows, int columns,
                     float eps, int dtype, int weight_dtype, void *stream);
 int mv_add_rms_norm_quantized(const void *x, const void *residual, const void *weight, void *q, void *scales, void *sum,

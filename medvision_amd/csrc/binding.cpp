@@ -719,8 +719,9 @@ std::pair<Tensor, Tensor> norm_forward(const NormCall &c, double eps) {
   return {y, sum};
 }
 
-// gradients of the sum and of the weight
-std::pair<Tensor, Tensor> norm_backward(const Tensor &h, const Tensor &weight, const Tensor &grad_y, const Tensor &grad_sum, double eps) {
+// gradients of the sum and of the weight, as far as they are wanted
+std::pair<Tensor, Tensor> norm_backward(const Tensor &h, const Tensor &weight, const Tensor &grad_y, const Tensor &grad_sum, double eps,
+                                        bool for_sum, bool for_weight) {
   const NormCall c = norm_call(h, Tensor(), weight, "add_rms_norm");
   const c10::DeviceGuard guard(c.x.device());
   same_device(c.x, grad_y, "grad_output");
@@ -728,8 +729,10 @@ std::pair<Tensor, Tensor> norm_backward(const Tensor &h, const Tensor &weight, c
   const Tensor gy = grad_y.defined() ? grad_y.to(h.scalar_type()).contiguous() : at::zeros_like(c.x);
   const Tensor gs = grad_sum.defined() ? grad_sum.to(h.scalar_type()).contiguous() : grad_sum;
   MVB_CHECK(gy.sizes() == h.sizes() && (!gs.defined() || gs.sizes() == h.sizes()), "grad_output must have the shape ", shape_text(h.sizes()));
-  const Tensor gx = at::empty_like(c.x), gw = at::empty_like(c.weight);
-  const size_t bytes = mv_add_rms_norm_backward_workspace_bytes(c.rows, c.columns);
+  Tensor gx, gw;
+  if (for_sum) gx = at::empty_like(c.x);
+  if (for_weight) gw = at::empty_like(c.weight);
+  const size_t bytes = for_weight ? mv_add_rms_norm_backward_workspace_bytes(c.rows, c.columns) : 0;
   const Tensor ws = bytes_on(c.x, bytes);
   check(mv_add_rms_norm_backward(ptr(c.x), ptr(c.weight), ptr(gy), ptr(gs), ptr(gx), ptr(gw), c.rows, c.columns, static_cast<float>(eps),
                                  c.code, c.weight_code, ptr(ws), bytes, stream_of(c.x)));
@@ -753,9 +756,12 @@ struct AddRmsNormFunction : torch::autograd::Function<AddRmsNormFunction> {
     {
       const at::NoGradGuard no_grad;
       const auto t = ctx->get_saved_variables();
-      const auto [gx, gw] = norm_backward(t[0], t[1], grads[0], gs, ctx->saved_data["eps"].toDouble());
-      out[0] = gx;
-      if (grads.size() > 1) out[1] = gx;
+      // (inputs that are tensors: x, the residual where there is one, the weight)
+      const bool added = grads.size() > 1, for_x = ctx->needs_input_grad(0), for_residual = added && ctx->needs_input_grad(1);
+      const auto [gx, gw] = norm_backward(t[0], t[1], grads[0], gs, ctx->saved_data["eps"].toDouble(), for_x || for_residual,
+                                          ctx->needs_input_grad(added ? 2 : 1));
+      if (for_x) out[0] = gx;
+      if (for_residual) out[1] = gx;
       out[2] = gw;
     }
     differentiable_once(grads, out);
@@ -784,11 +790,13 @@ std::pair<Tensor, std::optional<Tensor>> add_rms_norm_forward(const Tensor &x, c
   return {out.first, out.second.defined() ? std::optional<Tensor>(out.second) : std::nullopt};
 }
 
-std::pair<Tensor, Tensor> add_rms_norm_backward(const Tensor &h, const Tensor &weight, const std::optional<Tensor> &grad_y,
-                                                const std::optional<Tensor> &grad_sum, double eps) {
+std::pair<std::optional<Tensor>, std::optional<Tensor>> add_rms_norm_backward(const Tensor &h, const Tensor &weight, const std::optional<Tensor> &grad_y,
+                                                                             const std::optional<Tensor> &grad_sum, double eps, bool for_sum,
+                                                                             bool for_weight) {
   const py::gil_scoped_release no_gil;
   const at::NoGradGuard no_grad;
-  return norm_backward(h, weight, grad_y.value_or(Tensor()), grad_sum.value_or(Tensor()), eps);
+  const auto [gx, gw] = norm_backward(h, weight, grad_y.value_or(Tensor()), grad_sum.value_or(Tensor()), eps, for_sum, for_weight);
+  return {maybe(gx), maybe(gw)};
 }
 
 // 8-bit values of rows of `columns` and their scales

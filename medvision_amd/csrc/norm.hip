@@ -232,9 +232,10 @@ __global__ __launch_bounds__(threads_of(Lanes)) void norm_grad(const T *h, const
         d[i] = n * (g[k][i] * w[k][i] - v[k][i] * back) + (gsum ? s[k][i] : 0.f);
         dw[k][i] += live ? g[k][i] * (v[k][i] * n) : 0.f;
       }
-      if (live) store8(gx + at + c, columns - c, d);
+      if (live && gx) store8(gx + at + c, columns - c, d);
     }
   }
+  if (!partial) return;
   if constexpr (kGroups > 1) {   // the groups' shares, in their order
     if (group) {
 #pragma unroll
@@ -318,7 +319,8 @@ __global__ __launch_bounds__(kThreads) void norm_grad_long_rows(const T *h, cons
   }
   const float n = inverse_root(block_sum(squares, lds) / columns + eps);
   const float back = block_sum(dot, lds) / columns * n * n;
-  if (threadIdx.x == 0) norms[row] = n;
+  if (threadIdx.x == 0 && norms) norms[row] = n;
+  if (!gx) return;
   for (int c = threadIdx.x * 8; c < columns; c += kThreads * 8) {
     float v[8], g[8], w[8], s[8];
     load8(h + row * columns + c, columns - c, v);
@@ -513,12 +515,14 @@ int mv_add_rms_norm_backward(const void *h, const void *weight, const void *grad
                              void *grad_weight, int64_t rows, int columns, float eps, int dtype, int weight_dtype,
                              void *workspace, size_t workspace_bytes, void *stream) {
   if (const int status = norm_arguments(rows, columns, dtype, weight_dtype)) return status;
-  MV_REQUIRE(weight && grad_weight && (rows == 0 || (h && grad_y && grad_x)), "a tensor is missing");
-  MV_REQUIRE(workspace && workspace_bytes >= mv_add_rms_norm_backward_workspace_bytes(rows, columns), "the workspace is too small");
+  if ((rows == 0 || !grad_x) && !grad_weight) return MV_OK;
+  MV_REQUIRE(weight && (rows == 0 || (h && grad_y)), "a tensor is missing");
+  MV_REQUIRE(!grad_weight || (workspace && workspace_bytes >= mv_add_rms_norm_backward_workspace_bytes(rows, columns)), "the workspace is too small");
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const bool wide = weight_dtype == MV_F32;
   const int parts = grad_parts(rows, columns);
-  float *const partial = static_cast<float *>(workspace), *const norms = partial + static_cast<long>(parts) * columns;
+  float *const partial = grad_weight ? static_cast<float *>(workspace) : nullptr;
+  float *const norms = grad_weight ? partial + static_cast<long>(parts) * columns : nullptr;
   MV_FLOATS(dtype, {
     const T *const ht = static_cast<const T *>(h), *const gy = static_cast<const T *>(grad_y), *const gs = static_cast<const T *>(grad_sum);
     T *const gx = static_cast<T *>(grad_x);
@@ -527,9 +531,10 @@ int mv_add_rms_norm_backward(const void *h, const void *weight, const void *grad
     });
     if (!fits) {
       if (rows > 0) norm_grad_long_rows<T><<<linear_grid(rows, kThreads), kThreads, 0, st>>>(ht, weight, wide, gy, gs, gx, norms, rows, columns, eps);
-      norm_grad_long_columns<T><<<dim3((columns + kThreads * 8 - 1) / (kThreads * 8), kSlices), kThreads, 0, st>>>(ht, gy, norms, partial, rows, columns);
+      if (grad_weight)
+        norm_grad_long_columns<T><<<dim3((columns + kThreads * 8 - 1) / (kThreads * 8), kSlices), kThreads, 0, st>>>(ht, gy, norms, partial, rows, columns);
     }
-    norm_grad_weight<T><<<(columns + 15) / 16, kThreads, 0, st>>>(partial, grad_weight, wide, columns, parts);
+    if (grad_weight) norm_grad_weight<T><<<(columns + 15) / 16, kThreads, 0, st>>>(partial, grad_weight, wide, columns, parts);
   })
   return check_launch("add_rms_norm backward");
 }

@@ -27,8 +27,9 @@ class AddRMSNormFunction(NativeFunction):
         if grad_y is None and grad_sum is None:
             return None, None, None, None
         h, weight = ctx.saved_tensors
-        grad_x, grad_weight = native.add_rms_norm_backward(h, weight, grad_y, grad_sum, ctx.eps)
-        return grad_x, grad_x if ctx.added else None, grad_weight, None
+        for_x, for_residual, for_weight = ctx.needs_input_grad[:3]
+        grad_h, grad_weight = native.add_rms_norm_backward(h, weight, grad_y, grad_sum, ctx.eps, for_x or for_residual, for_weight)
+        return grad_h if for_x else None, grad_h if for_residual else None, grad_weight, None
 
 
 def add_rms_norm(x, residual, weight, eps=1e-6):

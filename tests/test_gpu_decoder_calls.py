@@ -106,3 +106,53 @@ def test_entry_points_without_some_gradients():
     assert call(None, *only_kv[1:]) == 0 and torch.equal(only_kv[1], full[1]) and torch.equal(only_kv[2], full[2])
     assert call(None, None, None) == 0
     assert call(full[0], full[1], None) == 1 and b"pair" in lib.mv_last_error()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("rows,columns", [(70, 40), (33, 1000), (5, 20000)])
+@pytest.mark.parametrize("added", [True, False])
+def test_norm_gradients_of_some_inputs(dtype, rows, columns, added):
+    from medvision_amd.ops.rms_norm import AddRMSNormFunction
+
+    class Python(AddRMSNormFunction):
+        @staticmethod
+        def backward(ctx, grad_y, grad_sum):
+            return AddRMSNormFunction.backward(ctx, grad_y, grad_sum)
+
+    tensors = rand(1, rows, columns, dtype=dtype), rand(2, rows, columns, dtype=dtype) if added else None, rand(3, columns, dtype=dtype)
+    gy, gs = rand(4, rows, columns, dtype=dtype), rand(5, rows, columns, dtype=dtype)
+
+    def grads(function, wanted):
+        ins = [None if t is None else t.clone().requires_grad_(w) for t, w in zip(tensors, wanted)]
+        y, h = function.apply(*ins, 1e-6)
+        torch.autograd.backward((y, h) if added else (y,), (gy, gs) if added else (gy,))
+        return [None if t is None else t.grad for t in ins]
+
+    want = grads(AddRMSNormFunction, (True, True, True))
+    alone = grads(AddRMSNormFunction, (False, False, True))
+    assert alone[0] is None and alone[1] is None and torch.equal(alone[2], want[2])
+    for function in (AddRMSNormFunction, Python):
+        for wanted in SUBSETS:
+            if not any(w for w, t in zip(wanted, tensors) if t is not None):
+                continue
+            for got, all_of_them, w, t in zip(grads(function, wanted), want, wanted, tensors):
+                assert torch.equal(got, all_of_them) if w and t is not None else got is None
+
+
+def test_norm_entry_point_without_some_gradients():
+    from medvision_amd import _lib
+    lib = _lib.load()
+    p = lambda t: None if t is None else t.data_ptr()   # noqa: E731
+    for rows, columns in ((30, 200), (3, 20000)):
+        x, w, gy = rand(5, rows, columns), rand(6, columns), rand(7, rows, columns)
+        bytes_ = lib.mv_add_rms_norm_backward_workspace_bytes(rows, columns)
+        ws = torch.empty(bytes_, dtype=torch.uint8, device=DEV)
+
+        def call(gx, gw, given=True):
+            return lib.mv_add_rms_norm_backward(p(x), p(w), p(gy), None, p(gx), p(gw), rows, columns, 1e-6, _lib.MV_F32, _lib.MV_F32,
+                                                p(ws) if given else None, bytes_ if given else 0, torch.cuda.current_stream().cuda_stream)
+
+        gx, gw, gx1, gw1 = (torch.full_like(t, 7.0) for t in (x, w, x, w))
+        assert call(gx, gw) == 0 and call(gx1, None, given=False) == 0 and call(None, gw1) == 0 and call(None, None, given=False) == 0
+        assert torch.equal(gx, gx1) and torch.equal(gw, gw1)
+        assert call(None, gw1, given=False) == 1 and b"workspace" in lib.mv_last_error()
