@@ -166,6 +166,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK, WM *WN *WK / 4) void product_til
       for (int i = 0; i < 4; ++i) acc[t][u][i] = fmaf(d[t][i], s[t], acc[t][u][i]);
   };
   auto one_step = [&](int step, i32x8 (&now)[S::kTM], const i32x8 (&before)[S::kTM]) {
+    __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0): what this wavefront brought has arrived (a barrier alone does not promise that)
     __syncthreads();   // this step's operands are there, and nobody reads the place of the next ones
     if ((step & 3) == 0) bring_scales(step + 4);
     if (step + 1 < steps) bring(step + 1);
