@@ -156,3 +156,105 @@ def test_norm_entry_point_without_some_gradients():
         assert call(gx, gw) == 0 and call(gx1, None, given=False) == 0 and call(None, gw1) == 0 and call(None, None, given=False) == 0
         assert torch.equal(gx, gx1) and torch.equal(gw, gw1)
         assert call(None, gw1, given=False) == 1 and b"workspace" in lib.mv_last_error()
+
+
+# ---- subclasses, traces, transforms, hooks -----------------------------------------------------------------------
+def functions():
+    from medvision_amd.ops.cross_attention import CrossAttentionFunction
+    from medvision_amd.ops.rms_norm import AddRMSNormFunction
+    q, k, v = rand(1, 2, 7, 4, 24), rand(2, 2, 40, 2, 24), rand(3, 2, 40, 2, 24)
+    mask = torch.rand(2, 40, generator=torch.Generator().manual_seed(4)).to(DEV) < 0.6
+    lengths = torch.tensor([40, 13], device=DEV)
+    x, r, w = rand(5, 6, 100), rand(6, 6, 100), rand(7, 100)
+    return [(CrossAttentionFunction, lambda f, *t: f.apply(*t, None, None, None), [q, k, v]),
+            (CrossAttentionFunction, lambda f, *t: f.apply(*t, mask, lengths, 0.3), [q, k, v]),
+            (AddRMSNormFunction, lambda f, *t: f.apply(*t, 1e-6), [x, r, w]),
+            (AddRMSNormFunction, lambda f, x, w: f.apply(x, None, w, 1e-6), [x, w])]
+
+
+def as_tuple(t):
+    return t if isinstance(t, tuple) else (t,)
+
+
+@pytest.mark.parametrize("index", range(4))
+def test_the_python_form_of_the_nodes_agrees(index):
+    """``forward`` and ``backward`` as a subclass of the function runs them, against the native node: the same bits."""
+    base, run, leaves = functions()[index]
+
+    class Counted(base):
+        calls = 0
+
+        @staticmethod
+        def backward(ctx, *grads):
+            Counted.calls += 1
+            return base.backward(ctx, *grads)
+
+    results = []
+    for function in (base, Counted):
+        ins = [t.clone().requires_grad_() for t in leaves]
+        out = as_tuple(run(function, *ins))
+        # (without a residual the native node hands the input through, and its gradient does not pass the node)
+        out = out[:1] if len(leaves) == 2 else out
+        results.append([*out, *torch.autograd.grad(out, ins, [torch.ones_like(o) for o in out])])
+    assert Counted.calls == 1
+    for got, want in zip(*results):
+        assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("index", range(4))
+def test_traced_calls_run_their_operator(index):
+    function, run, leaves = functions()[index]
+    with torch.no_grad():
+        traced = torch.jit.trace(lambda *t: as_tuple(run(function, *t)), tuple(leaves))
+        other = (leaves[0] * 2 + 1, *leaves[1:])
+        for a, b in zip(traced(*other), as_tuple(run(function, *other))):
+            torch.testing.assert_close(a, b)
+        assert not torch.equal(traced(*other)[0], traced(*leaves)[0])
+
+
+@pytest.mark.parametrize("index", range(4))
+def test_transforms_of_functions_are_refused(index):
+    function, run, leaves = functions()[index]
+    first = lambda t: as_tuple(run(function, t, *leaves[1:]))[0]   # noqa: E731
+    with pytest.raises((NotImplementedError, RuntimeError)):
+        torch.func.jvp(first, (leaves[0],), (torch.ones_like(leaves[0]),))
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(first)(leaves[0].unsqueeze(0))
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda t: first(t).sum())(leaves[0])
+    assert torch.isfinite(first(leaves[0])).all()
+
+
+def test_8_bit_operators_refuse_transforms():
+    import medvision_amd.ops as ops
+    x, w = rand(1, 3, 256), rand(2, 256)
+    q, s = ops.quantize_blocks(x)
+    weight, scales = ops.quantize_blocks(rand(3, 40, 256), 128)
+    for call, t in ((lambda t: ops.quantize_blocks(t)[1], x), (lambda t: ops.add_rms_norm_quantized(t, None, w)[1], x),
+                    (lambda t: ops.block_linear(q, t, weight, scales), s)):
+        with pytest.raises(RuntimeError):
+            torch.func.vmap(call)(t.unsqueeze(0))
+        with pytest.raises((NotImplementedError, RuntimeError)):
+            torch.func.jvp(call, (t,), (torch.ones_like(t),))
+
+
+@pytest.mark.parametrize("index", range(4))
+def test_hooks_see_the_gradients(index):
+    function, run, leaves = functions()[index]
+    ins = [t.clone().requires_grad_() for t in leaves]
+    moved = [t * 1.0 for t in ins]
+    seen = {}
+    for i, t in enumerate(moved):
+        t.retain_grad()
+        t.register_hook(lambda g, i=i: seen.__setitem__(i, g.clone()))
+    out = as_tuple(run(function, *moved))
+    nodes = []
+    out[0].grad_fn.register_hook(lambda inputs, outputs: nodes.append(inputs))
+    out[0].register_hook(lambda g: 2 * g)
+    go = torch.ones_like(out[0])
+    out[0].backward(go)
+    plain = [t.clone().requires_grad_() for t in leaves]
+    want = torch.autograd.grad(as_tuple(run(function, *plain))[0], plain, 2 * go)
+    assert len(nodes) == 1
+    for i, w in enumerate(want):
+        assert torch.equal(seen[i], w) and torch.equal(ins[i].grad, w) and torch.equal(moved[i].grad, w)
