@@ -24,14 +24,19 @@ __device__ __forceinline__ void put_log(const AttentionArgs &a, float *lse, long
 // The weights are rounded to the values' type for the second product (a matrix instruction has one type), maximum, sum and
 // output stay in 32 bits: the error against 64 bits is 1.1 - 1.3 times that of rounding the output alone.
 //
-// Bound by vector issue for heads of 32: of a score, seven issue slots are vector instructions (four of them the
-// exponential), two matrix instructions.  2 x 2000 queries x 8 heads over 27648 keys of 32, float16: 218 us with the join of
-// four splits = 4.05e12 scores/s, vector units 76 % and matrix units 23 % busy.  Heads of 64 (2 x 1000 over 6912, bf16): 52 us,
-// of 128 (2 x 2000 over 8192): 184 us = 730 TFLOP/s, two wavefronts per SIMD and LDS 45 %.  One query per sample reads the
-// keys once: 4 samples of 32768 keys, 16 heads over 4 of 64 channels: 27 us + 4 us for the join of 32 splits (134 MB at full
-// length: 5.0 TB/s).  float32 on its own matrix instructions: 2 x 2000 over 4096, 8 heads of 64: 338 us = 99 of 154 TFLOP/s.
-// 2 x 32768 queries over 100 keys, 8 heads sharing 2 of 32, float16, with the output's low bits: 35 us, 102 MB (keys held in LDS
-// over several tiles of rows, with the next queries on their way: 39 us, for that takes 167 registers instead of 121).
+// Heads of 32: of a score, 6.6 issue slots are vector instructions (two of them the exponential), two matrix instructions.  2 x 2000
+// queries x 8 heads over 27648 keys of 32, float16: 221 us with the join of four splits = 4.0e12 scores/s, vector units 73 % and
+// matrix units 22 % busy.  The rest is waiting: the columns' loads may be outstanding where the loop starts, so the compiler waits for
+// all loads in front of each tile's first product, the next tile's among them, and only other wavefronts cover those.  Heads of 64
+// (2 x 1000 over 6912, bf16): 50 us, vector units 46 %, matrix units 23 %; of 128 (2 x 2000 over 8192): 163 us = 820 TFLOP/s,
+// two wavefronts per SIMD, LDS 45 %, matrix units 35 %.  One query per sample reads the keys once: 4 samples of 32768 keys, 16 heads over 4 of
+// 64 channels: 25 us + 5 us for the join of 32 splits (134 MB at full length: 5.3 TB/s).  float32 on its own matrix instructions:
+// 2 x 2000 over 4096, 8 heads of 64: 297 us = 113 of 154 TFLOP/s, matrix units 71 % busy.  2 x 32768 queries over 100 keys, 8 heads sharing
+// 2 of 32, float16, with the output's low bits: 39 us, 102 MB (keys held in LDS over several tiles of rows, with the next queries
+// on their way, were a tenth slower: that takes 167 registers instead of 128).
+// Few rows: 128 keys at a time, with heads of more than 64 channels in all 256 registers of two wavefronts per SIMD, and 17 (96) or
+// 40 (128) of them in memory; 13 in float32 with 64 (heads of 64 in 16 bits run on two wavefronts too, not on three).  2 x 8 queries
+// over 32768 keys, 8 heads of 64 26 us, of 96 44, of 128 63 to 68: 134, 201 and 268 MB, 5.1, 4.6 and 4.2 TB/s.
 template <typename T, int W, int WQ>
 __global__ __launch_bounds__(256, sizeof(T) == 4 ? (W > 64 ? 1 : 2) : W > 64 ? 2 : W == 64 ? 3 : 4) void attend_kernel(
     AttentionArgs a, T *out, T *low, float *lse, float *part, int row_tiles, int splits) {

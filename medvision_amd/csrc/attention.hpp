@@ -272,7 +272,8 @@ template <typename T> struct RowLog {
   }
 };
 
-// v where bit `row` of the word is set, `other` where not (a field and a merge: two instructions)
+// v where bit `row` of the word is set, `other` where not (a field and a merge: two instructions in the forward pass; for
+// `other` zero the compiler makes an and, a comparison and a selection of them)
 __device__ __forceinline__ float where_bit(unsigned word, int row, float v, float other) {
   const unsigned all = static_cast<unsigned>(__builtin_amdgcn_sbfe(static_cast<int>(word), row, 1));
   return __uint_as_float((all & __float_as_uint(v)) | (~all & __float_as_uint(other)));

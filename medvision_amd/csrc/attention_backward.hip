@@ -8,10 +8,15 @@
 //
 // Forming the weights twice costs two of seven products, and saves what dq by atomics would: 64 times the scores' count over
 // the head's width in additions to memory.  Both kernels are bound by the chain from LDS through products, exponential and
-// products again, with two or three wavefronts per SIMD to hide it (registers: sums and operands of a 32 x W tile twice).
-// 2 x 1000 queries over 6912 keys, 8 heads of 64, bf16: dq 77 us, dk and dv 91 us, matrix units 41 and 26 %, vector issue 52
-// and 31 % busy.  2 x 32768 queries over 100 keys, 8 heads sharing 2 of 32, float16: 55 and 39 us (+ 7 us for the sums of 128
-// splits); 170 MB are read and written for dq.  2 x 2000 over 8192, 8 heads of 128, bf16: 358 and 500 us, one wavefront per SIMD.
+// products again, with two or three wavefronts per SIMD to hide it (registers: sums and operands of a 32 x W tile twice).  In the kernel of
+// dk and dv a tile also waits twice for memory, with nothing of its own in between: for the next rows' elements before their
+// logarithms are asked for, and for those before the first product (the compiler waits for all loads at both places).
+// 2 x 1000 queries over 6912 keys, 8 heads of 64, bf16: dq 77 us, dk and dv 90 us, matrix units 32 and 26 %, vector issue 53
+// and 35 % busy.  2 x 32768 queries over 100 keys, 8 heads sharing 2 of 32, float16: 61 and 40 us (+ 7 us for the sums of 128
+// splits); 170 MB are read and written for dq.  2 x 2000 over 8192, 8 heads of 128, bf16: 300 and 437 us (four products: 614 TFLOP/s),
+// one wavefront per SIMD.
+// Registers in memory: 42 of 256 for dk and dv of heads of 96 in 16 bits with the single product, 18 of 168 for those of 32 in bf16 with the
+// rest's, up to 32 where there are few keys; 13 of 512 in float32 with 128; 8 of 168 for dq of heads of 64.
 #include "attention.hpp"
 
 #include <algorithm>
@@ -206,9 +211,9 @@ __global__ __launch_bounds__(256, W == 128 || (sizeof(T) == 4 && W > 32) || (W =
   // Ends of rows at once, but for heads of 33 to 64 channels in 16 bits: with it the compiler keeps 25 registers fewer in use
   // there, and heads of 64 take 100 instead of 90 us (1000 x 6912).
   constexpr bool kEnds = sizeof(T) == 4 || W != 64;
-  // Whether rows' largest scores are taken off where there is one to take off, or always (RowLog): zeros are taken off faster, in the
-  // shade of the next product, than a branch lets the compiler schedule (2 x 2000 over 8192, heads of 128, bf16: 437 and 512 us), but
-  // for heads of 32 (2 x 2000 over 27648 434 and 402 us).
+  // Whether rows' largest scores are taken off where there is one to take off, or always (RowLog): taking off zeros, in the shade of the
+  // next product, is faster than a branch that the compiler does not schedule across (2 x 2000 over 8192, heads of 128, bf16: 437 and
+  // 512 us), but for heads of 32 (2 x 2000 over 27648, float16: 434 and 401 us).
   constexpr bool kAsk = sizeof(T) == 2 && W == 32;
   using L = Tile<T, DP, kRows>;
   __shared__ L tiles[S::kBuffers][2];

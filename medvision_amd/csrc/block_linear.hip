@@ -71,13 +71,14 @@ template <typename T, int TN> __device__ __forceinline__ void store_row(const Re
 // multiplied).  A row of a block is 128 bytes, eight pieces of 16; piece c of row r stands at c ^ (r & 7), so that the 16
 // rows of an operand that one instruction reads spread over all banks (no conflicts).
 //
-// 256 x 256 with eight wavefronts of 64 x 128: 16384 x 4096 x 4096 257 us = 2.14 PFLOP/s (a plain product of the library:
-// 2.34), 8192^3 2.11.  Of 490 us for the latter 380 are left without the loads, 406 without the products, 400 without the
-// additions of the scaled products to the sums: loads into LDS, reads from it (96 bytes per clock and compute unit at the
-// matrix units' full rate), matrix and vector instructions take about as long each and overlap less than whole.
+// 256 x 256 with eight wavefronts of 64 x 128: 16384 x 4096 x 4096 253 - 261 us = 2.1 - 2.2 PFLOP/s (a plain product of the
+// library: 2.34), 8192^3 479 us = 2.30 (the same inputs each time).  Matrix units 46 % busy, vector units 37 % (the additions of the
+// scaled products to the sums), LDS reads 21 %; they overlap less than whole, and every fourth step the five wavefronts that put scales
+// into LDS wait for the next block first (a store to LDS behind loads into LDS).
 // 128 x 128 with twice four wavefronts of 64 x 64, where there are fewer than 192 of the large tiles (4000 x 12544 x 1024:
-// 72 us = 1.42 PFLOP/s; 160 with the large ones, 80 with those split in four): the loads alone take 52 us (803 MB from the
-// L2s, 15.6 TB/s), reads and products 48, and both share the LDS.
+// 68 - 72 us = 1.4 - 1.5 PFLOP/s; 160 with the large ones, 80 with those split in four): the loads alone take 52 us (803 MB from the
+// L2s, 15.6 TB/s), reads and products 48, and both share the LDS; all wavefronts wait for the next blocks in every second step, for the
+// scales' sake.  Matrix units and vector units 29 % busy each.
 template <int BM, int BN, int WM, int WN, int WK> struct Tiles {
   static constexpr int kThreads = 64 * WM * WN * WK, kTM = BM / WM / 16, kTN = BN / WN / 16;
   static constexpr int kStage = (BM + BN) * kBlock;   // bytes of one block of both operands

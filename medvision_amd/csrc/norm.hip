@@ -185,7 +185,8 @@ __global__ __launch_bounds__(threads_of(Lanes)) void norm_rows(const T *x, const
 
 // Both gradients in one pass over memory: a workgroup takes every gridDim-th row (or group of rows), and keeps its share of
 // the weight's gradient in registers until the end.  Bound by memory: 55296 x 256 in bf16 with both incoming gradients 29 us
-// (3.9 TB/s), 55296 x 1000 100 us (4.4 TB/s), with the join of 1024 partial sums (1536: 32 and 125 us, 512: 35 and 164).
+// (3.9 TB/s), 55296 x 1000 100 us (4.4 TB/s), with the join of 1024 partial sums (1536: 32 and 125 us, 512: 35 and 164); float32
+// 6000 x 4096 82 us (4.8 TB/s) and 7 for the join.
 // Longer rows have fewer workgroups, and as many fewer partial sums: 5000 x 8192 on 512 of 512 threads 76 us (115 on 1024 of
 // 256, 108 on 512 of those); beyond 8192 columns on 512 threads with 32 columns each (3000 x 16384 127 us; two passes 164, 1024
 // threads with sixteen spill 275 registers: 338).

@@ -38,6 +38,9 @@ def cross_attention(query, key, value, key_mask=None, key_lengths=None, scale=No
         key_lengths (Tensor): whole numbers ``[batch]``: keys from there on do not count
         scale (float): of the products of queries and keys, ``channels ** -0.5`` by default
 
-    What keys and values that do not count hold has no effect, not even NaN.  A query without any key gets zeros.
+    What keys and values that do not count hold has no effect, not even NaN.  A query without any key gets zeros.  Gradients
+    are formed for the inputs that want one.  Scores, their softmax and all sums are in 32 bits; of float16 and bfloat16 the
+    softmax's weights are rounded to that type before they meet the values, and in the gradients of keys and values (with
+    their own gradients) from 2 ** 20 weights on, unless there are no more than 32 keys or 64 rows for a head of keys.
     """
     return CrossAttentionFunction.apply(query, key, value, key_mask, key_lengths, scale)
