@@ -31,7 +31,7 @@ typedef enum { MV_F32 = 0, MV_F16 = 1, MV_BF16 = 2, MV_F64 = 3,
 typedef enum { MV_OK = 0, MV_INVALID_ARGUMENT = 1, MV_HIP_ERROR = 2 } mv_status;
 
 const char *mv_last_error(void);
-int mv_version(void);
+int mv_version(void);   /* 2: the lse of mv_cross_attention_* holds two numbers for each row */
 
 /* ---- RoIAlign, plain boxes --------------------------------------------------------------
  * replaces roi_align_2d_forward / roi_align_2d_backward   csrc/roi_align_2d.h (vision.cpp:31-34)

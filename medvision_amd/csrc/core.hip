@@ -25,5 +25,5 @@ dim3 linear_grid(long workgroups, int threads) {
 
 extern "C" {
 const char *mv_last_error(void) { return mv::last_error_buffer(); }
-int mv_version(void) { return 1; }
+int mv_version(void) { return 2; }
 }
