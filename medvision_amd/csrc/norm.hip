@@ -70,7 +70,8 @@ struct Root {
   }
 };
 
-// v w n: 16-bit factors v, w have an exact product; of others the rest goes into the second one.
+// v w n: 16-bit factors v, w have an exact product (16-bit rows with float32 weights: to 2^-24); of others the rest goes into the
+// second one.
 template <typename T> __device__ __forceinline__ float scaled(float v, float w, const Root &n) {
   const float p = v * w;
   const float most = fmaf(p, n.high, sizeof(T) == 2 ? p * n.low : fmaf(p, n.low, fmaf(v, w, -p) * n.high));
