@@ -367,6 +367,51 @@ int mv_block_linear(const void *q, const void *q_scales, const void *weight, con
                     void *y, int64_t rows, int inputs, int outputs, int dtype, void *workspace, size_t workspace_bytes,
                     void *stream);
 
+/* Group norm of cells in channels-last order with an activation, over x [batch, cells, channels]:
+ *   h = (x - mean) / sqrt(var + eps) over the cells of a sample and the channels / groups channels of a group,
+ *   y = a(h * weight + bias)
+ * weight, bias: [channels] of `weight_dtype`, `dtype` or MV_F32 (NULL: ones, zeros).  low: the slope of MV_LEAKY_RELU below
+ * zero.  MV_GELU is z times the normal distribution's value.  stats [3, batch, groups] float32 receives each group's mean,
+ * what rounding took from it, and 1 / sqrt(var + eps).
+ * ..._backward WRITES grad_x, grad_weight and grad_bias (of weight_dtype); each may be NULL where nobody wants it.  At the
+ * border of two branches the derivative is the lower one's.  Sums are formed in a fixed order. */
+typedef enum { MV_NO_ACTIVATION = 0, MV_RELU = 1, MV_LEAKY_RELU = 2, MV_SILU = 3, MV_GELU = 4 } mv_activation;
+size_t mv_group_norm_workspace_bytes(int batch, int64_t cells, int channels, int groups);
+int mv_group_norm(const void *x, const void *weight, const void *bias, void *y, void *stats, int batch, int64_t cells, int channels,
+                  int groups, float eps, int activation, float low, int dtype, int weight_dtype, void *workspace,
+                  size_t workspace_bytes, void *stream);
+size_t mv_group_norm_backward_workspace_bytes(int batch, int64_t cells, int channels, int groups);
+int mv_group_norm_backward(const void *x, const void *weight, const void *bias, const void *stats, const void *grad_y, void *grad_x,
+                           void *grad_weight, void *grad_bias, int batch, int64_t cells, int channels, int groups, int activation,
+                           float low, int dtype, int weight_dtype, void *workspace, size_t workspace_bytes, void *stream);
+
+/* Rotary positions on several axes: in each row and head of x, pair p of the channels is turned by the angle
+ * sum over a of places[batch, row, a] * frequencies[a, p] (radians; formed in 64 bits).  A pair is (p, pairs + p), or
+ * (2p, 2p + 1) where `neighbours` is not 0; channels behind 2 * pairs stay.  back != 0 turns the other way, which is the
+ * gradient.  x is read through strides (elements; the channels of a head are neighbours; dim 1..1024), places (`place_dtype`
+ * MV_F32, MV_F64 or MV_I32; axes 1..8) too (0: shared by a batch); frequencies [axes, pairs] are float64 and dense, y is dense. */
+typedef struct {
+  int batch, rows, heads, dim, axes, pairs;
+  int64_t x_strides[3];     /* batch, row, head */
+  int64_t place_strides[3]; /* batch, row, axis */
+} mv_rotary_shape;
+int mv_rotary_positions(const void *x, const void *places, const void *frequencies, void *y, const mv_rotary_shape *shape,
+                        int neighbours, int back, int dtype, int place_dtype, void *stream);
+
+/* Linear layers with weights in 4 bits (e2m1: 0, 1/2, 1, 3/2, 2, 3, 4, 6; codes 8..15 negative) and a float32 scale for each
+ * `group` (32, 64 or 128) columns of a row: scale = max(max|w| / 6, 2^-126), code = e2m1(w * (1 / scale)), halves to even.
+ * weight [outputs, 64 * ceil(inputs / 128)] bytes, rows of blocks of 128 columns (zeros beyond the inputs): the four bytes of
+ * eight neighbouring columns together, two codes a byte, the first one low; piece 4 s + g of a block at place 4 g + s.
+ * scales [outputs, 128 / group * ceil(inputs / 128)].  A group that holds a NaN or an infinity has it for a scale, and with it
+ * stands for NaN throughout.
+ * mv_group_linear: y [rows, outputs] = x [rows, inputs] times the values' transpose + bias, `dtype` MV_F16 or MV_BF16 (of x, y
+ * and bias; bias may be NULL), dense; weight 16-byte aligned.  Sums are in 32 bits, products exact.  A workspace smaller than
+ * the query's value costs speed only. */
+int mv_quantize_groups(const void *weight, void *q, void *scales, int64_t rows, int columns, int group, int dtype, void *stream);
+size_t mv_group_linear_workspace_bytes(int64_t rows, int inputs, int outputs);
+int mv_group_linear(const void *x, const void *weight, const void *scales, const void *bias, void *y, int64_t rows, int inputs,
+                    int outputs, int group, int dtype, void *workspace, size_t workspace_bytes, void *stream);
+
 /* ---- small host arrays --------------------------------------------------------------------------
  * Copies `bytes` (whole 4-byte words, at most MV_UPLOAD_MAX_BYTES) from host to device memory as
  * kernel arguments: asynchronous on the stream, `host` may be reused as soon as the call returns.

@@ -40,7 +40,14 @@ class AttentionShape(ctypes.Structure):
         (n, _i64 * 3) for n in ("q_strides", "k_strides", "v_strides")] + [("mask_stride", _i64)]
 
 
+class RotaryShape(ctypes.Structure):
+    """Mirror of ``mv_rotary_shape``."""
+    _fields_ = [(n, _i) for n in ("batch", "rows", "heads", "dim", "axes", "pairs")] + [
+        (n, _i64 * 3) for n in ("x_strides", "place_strides")]
+
+
 _ATTENTION_P = ctypes.POINTER(AttentionShape)
+_ROTARY_P = ctypes.POINTER(RotaryShape)
 _SHAPE_P = ctypes.POINTER(DcnShape)
 _SHAPE2_P = ctypes.POINTER(Dcn2dShape)
 
@@ -100,6 +107,14 @@ SIGNATURES = {
     "mv_quantize_blocks": (_i, [_p] * 3 + [_i64, _i, _i, _i, _p]),
     "mv_block_linear_workspace_bytes": (_sz, [_i64, _i, _i]),
     "mv_block_linear": (_i, [_p] * 6 + [_i64, _i, _i, _i, _p, _sz, _p]),
+    "mv_group_norm_workspace_bytes": (_sz, [_i, _i64, _i, _i]),
+    "mv_group_norm": (_i, [_p] * 5 + [_i, _i64, _i, _i, _f, _i, _f, _i, _i, _p, _sz, _p]),
+    "mv_group_norm_backward_workspace_bytes": (_sz, [_i, _i64, _i, _i]),
+    "mv_group_norm_backward": (_i, [_p] * 8 + [_i, _i64, _i, _i, _i, _f, _i, _i, _p, _sz, _p]),
+    "mv_rotary_positions": (_i, [_p] * 4 + [_ROTARY_P, _i, _i, _i, _i, _p]),
+    "mv_quantize_groups": (_i, [_p] * 3 + [_i64, _i, _i, _i, _p]),
+    "mv_group_linear_workspace_bytes": (_sz, [_i64, _i, _i]),
+    "mv_group_linear": (_i, [_p] * 5 + [_i64, _i, _i, _i, _i, _p, _sz, _p]),
     "mv_upload": (_i, [_p, _p, _sz, _p]),
 }
 

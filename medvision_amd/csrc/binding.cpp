@@ -886,6 +886,273 @@ Tensor block_linear(const Tensor &q_in, const Tensor &q_scales, const Tensor &we
   return y;
 }
 
+// ---- group norm with an activation ------------------------------------------------------------------------------------
+int activation_code(const std::optional<std::string> &name) {
+  static const char *const names[] = {"none", "relu", "leaky_relu", "silu", "gelu"};
+  if (!name) return MV_NO_ACTIVATION;
+  for (int i = 0; i < 5; ++i)
+    if (*name == names[i]) return i;
+  throw std::runtime_error(c10::str("activation '", *name, "': 'relu', 'leaky_relu', 'silu', 'gelu' or None are possible"));
+}
+
+struct GroupNormCall {
+  Tensor x, weight, bias;
+  int64_t cells;
+  int batch, channels, groups, code, weight_code, activation;
+  float low;
+};
+
+GroupNormCall group_norm_call(const Tensor &x, int64_t groups, const Tensor &weight, const Tensor &bias, int activation, double low) {
+  MVB_CHECK(x.is_cuda(), "group_norm_act is not implemented on CPU");
+  GroupNormCall c;
+  c.code = float_code(x, "group_norm_act");
+  MVB_CHECK(x.dim() >= 2 && x.size(-1) >= 1, "group_norm_act takes [batch, ..., channels], got shape ", shape_text(x.sizes()));
+  MVB_CHECK(groups >= 1 && x.size(-1) % groups == 0, x.size(-1), " channels in ", groups, " groups");
+  const std::pair<const Tensor *, const char *> vectors[] = {{&weight, "weight"}, {&bias, "bias"}};
+  for (const auto &[t, name] : vectors) {
+    if (!t->defined()) continue;
+    same_device(x, *t, name);
+    MVB_CHECK(t->dim() == 1 && t->size(0) == x.size(-1), name, " has shape ", shape_text(t->sizes()), ", expected (", x.size(-1), ")");
+    MVB_CHECK(t->scalar_type() == x.scalar_type() || t->scalar_type() == at::kFloat, name, " has dtype ", dtype_name(*t),
+              ", expected float32 or that of the input");
+  }
+  MVB_CHECK(!weight.defined() || !bias.defined() || weight.scalar_type() == bias.scalar_type(), "weight and bias must share one dtype");
+  c.weight_code = weight.defined() ? dtype_code(weight) : bias.defined() ? dtype_code(bias) : c.code;
+  c.x = x.contiguous();
+  c.weight = weight.defined() ? weight.contiguous() : weight;
+  c.bias = bias.defined() ? bias.contiguous() : bias;
+  c.batch = to_int(x.size(0), "the batch"), c.channels = to_int(x.size(-1), "a row"), c.groups = static_cast<int>(groups);
+  c.cells = 1;
+  for (int64_t d = 1; d + 1 < x.dim(); ++d) c.cells *= x.size(d);
+  c.activation = activation, c.low = static_cast<float>(low);
+  return c;
+}
+
+// y, and the groups' means and inverse deviations
+std::pair<Tensor, Tensor> group_norm_run(const GroupNormCall &c, double eps) {
+  const c10::DeviceGuard guard(c.x.device());
+  const Tensor y = at::empty_like(c.x), stats = at::empty({3, c.batch, c.groups}, c.x.options().dtype(at::kFloat));
+  const size_t bytes = mv_group_norm_workspace_bytes(c.batch, c.cells, c.channels, c.groups);
+  const Tensor ws = bytes_on(c.x, bytes);
+  check(mv_group_norm(ptr(c.x), ptr(c.weight), ptr(c.bias), ptr(y), ptr(stats), c.batch, c.cells, c.channels, c.groups, static_cast<float>(eps),
+                      c.activation, c.low, c.code, c.weight_code, ptr(ws), bytes, stream_of(c.x)));
+  return {y, stats};
+}
+
+// gradients of the cells, the weight and the bias, as far as they are wanted
+variable_list group_norm_grads(const GroupNormCall &c, const Tensor &stats, const Tensor &grad_in, bool for_x, bool for_weight, bool for_bias) {
+  const c10::DeviceGuard guard(c.x.device());
+  same_device(c.x, grad_in, "grad_output");
+  MVB_CHECK(grad_in.sizes() == c.x.sizes(), "grad_output has shape ", shape_text(grad_in.sizes()), ", expected ", shape_text(c.x.sizes()));
+  MVB_CHECK(stats.scalar_type() == at::kFloat && stats.is_contiguous() && stats.device() == c.x.device() &&
+            stats.numel() == int64_t{3} * c.batch * c.groups, "stats are not those of the forward pass");
+  const Tensor grad = grad_in.to(c.x.scalar_type()).contiguous();
+  Tensor gx, gw, gb;
+  if (for_x) gx = at::empty_like(c.x);
+  if (for_weight && c.weight.defined()) gw = at::empty_like(c.weight);
+  if (for_bias && c.bias.defined()) gb = at::empty_like(c.bias);
+  const size_t bytes = mv_group_norm_backward_workspace_bytes(c.batch, c.cells, c.channels, c.groups);
+  const Tensor ws = bytes_on(c.x, bytes);
+  check(mv_group_norm_backward(ptr(c.x), ptr(c.weight), ptr(c.bias), ptr(stats), ptr(grad), ptr(gx), ptr(gw), ptr(gb), c.batch, c.cells,
+                               c.channels, c.groups, c.activation, c.low, c.code, c.weight_code, ptr(ws), bytes, stream_of(c.x)));
+  return {gx, gw, gb};
+}
+
+struct GroupNormActFunction : torch::autograd::Function<GroupNormActFunction> {
+  static Tensor forward(AutogradContext *ctx, const Tensor &x, int64_t groups, const std::optional<Tensor> &weight, const std::optional<Tensor> &bias,
+                        double eps, int64_t activation, double low) {
+    const GroupNormCall c = group_norm_call(x, groups, weight.value_or(Tensor()), bias.value_or(Tensor()), static_cast<int>(activation), low);
+    const auto [y, stats] = group_norm_run(c, eps);
+    // (the copy of cells that are not in this order is not made twice)
+    ctx->save_for_backward({x.is_contiguous() ? x : c.x, weight.value_or(Tensor()), bias.value_or(Tensor()), stats});
+    ctx->saved_data["groups"] = groups;
+    ctx->saved_data["activation"] = activation;
+    ctx->saved_data["low"] = low;
+    return y;
+  }
+  static variable_list backward(AutogradContext *ctx, const variable_list &grads) {
+    variable_list out(7);
+    if (!grads[0].defined()) return out;
+    {
+      const at::NoGradGuard no_grad;
+      const auto t = ctx->get_saved_variables();
+      // (inputs that are tensors: x, the weight and the bias where there are some)
+      const bool weighted = t[1].defined(), biased = t[2].defined();
+      const bool for_x = ctx->needs_input_grad(0), for_weight = weighted && ctx->needs_input_grad(1), for_bias = biased && ctx->needs_input_grad(weighted ? 2 : 1);
+      const GroupNormCall c = group_norm_call(t[0], ctx->saved_data["groups"].toInt(), t[1], t[2], static_cast<int>(ctx->saved_data["activation"].toInt()),
+                                              ctx->saved_data["low"].toDouble());
+      const variable_list g = group_norm_grads(c, t[3], grads[0], for_x, for_weight, for_bias);
+      out[0] = g[0], out[2] = g[1], out[3] = g[2];
+    }
+    differentiable_once(grads, out);
+    return out;
+  }
+};
+
+Tensor group_norm_act(const Tensor &x, int64_t groups, const std::optional<Tensor> &weight, const std::optional<Tensor> &bias, double eps,
+                      const std::optional<std::string> &activation, double low) {
+  const Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor());
+  for (const Tensor &t : {x, w, b}) no_forward_mode(t);
+  const py::gil_scoped_release no_gil;
+  const int kind = activation_code(activation);
+  if (wants_gradient({x, w, b})) return GroupNormActFunction::apply(x, groups, weight, bias, eps, static_cast<int64_t>(kind), low);
+  const at::NoGradGuard no_grad;
+  return group_norm_run(group_norm_call(x, groups, w, b, kind, low), eps).first;
+}
+
+std::pair<Tensor, Tensor> group_norm_act_forward(const Tensor &x, int64_t groups, const std::optional<Tensor> &weight, const std::optional<Tensor> &bias,
+                                                 double eps, const std::optional<std::string> &activation, double low) {
+  const py::gil_scoped_release no_gil;
+  const at::NoGradGuard no_grad;
+  return group_norm_run(group_norm_call(x, groups, weight.value_or(Tensor()), bias.value_or(Tensor()), activation_code(activation), low), eps);
+}
+
+std::vector<std::optional<Tensor>> group_norm_act_backward(const Tensor &x, int64_t groups, const std::optional<Tensor> &weight,
+                                                           const std::optional<Tensor> &bias, const Tensor &stats, const Tensor &grad,
+                                                           const std::optional<std::string> &activation, double low, bool for_x, bool for_weight,
+                                                           bool for_bias) {
+  const py::gil_scoped_release no_gil;
+  const at::NoGradGuard no_grad;
+  const auto g = group_norm_grads(group_norm_call(x, groups, weight.value_or(Tensor()), bias.value_or(Tensor()), activation_code(activation), low), stats,
+                                  grad, for_x, for_weight, for_bias);
+  return {maybe(g[0]), maybe(g[1]), maybe(g[2])};
+}
+
+// ---- rotary positions ---------------------------------------------------------------------------------------------------
+struct RotaryCall {
+  Tensor x, places, frequencies;
+  mv_rotary_shape shape;
+  int code, place_code;
+};
+
+RotaryCall rotary_call(const Tensor &x, const Tensor &positions, const Tensor &frequencies) {
+  MVB_CHECK(x.is_cuda(), "rotary_positions is not implemented on CPU");
+  MVB_CHECK(x.dim() == 4, "rotary_positions takes [batch, rows, heads, channels], got shape ", shape_text(x.sizes()));
+  RotaryCall c;
+  c.code = float_code(x, "rotary_positions");
+  same_device(x, positions, "positions");
+  same_device(x, frequencies, "frequencies");
+  MVB_CHECK(frequencies.dim() == 2 && frequencies.size(0) >= 1 && frequencies.size(0) <= 8 && 2 * frequencies.size(1) <= x.size(3),
+            "frequencies have shape ", shape_text(frequencies.sizes()), ", expected (axes, pairs) of 1 to 8 axes and up to ", x.size(3) / 2, " pairs");
+  MVB_CHECK(x.size(3) >= 1 && x.size(3) <= 1024, "heads of ", x.size(3), " channels: 1 to 1024 are possible");
+  MVB_CHECK(frequencies.scalar_type() == at::kFloat || frequencies.scalar_type() == at::kDouble, "frequencies have to be float32 or float64, got ", dtype_name(frequencies));
+  const auto type = positions.scalar_type();
+  MVB_CHECK(type == at::kFloat || type == at::kDouble || type == at::kHalf || type == at::kBFloat16 || (at::isIntegralType(type, false) && type != at::kUInt64),
+            "positions have to be whole or floating numbers, got ", dtype_name(positions));
+  const bool shared = positions.dim() == 2;
+  MVB_CHECK((shared || (positions.dim() == 3 && positions.size(0) == x.size(0))) && positions.size(-2) == x.size(1) && positions.size(-1) == frequencies.size(0),
+            "positions have shape ", shape_text(positions.sizes()), ", expected (", x.size(0), ", ", x.size(1), ", ", frequencies.size(0), ") or (", x.size(1), ", ", frequencies.size(0), ")");
+  c.x = rows_of_heads(x);
+  c.places = type == at::kFloat || type == at::kDouble || type == at::kInt ? positions
+             : at::isIntegralType(type, false) ? positions.to(at::kDouble) : positions.to(at::kFloat);
+  c.place_code = c.places.scalar_type() == at::kInt ? static_cast<int>(MV_I32) : dtype_code(c.places);
+  c.frequencies = frequencies.to(at::kDouble).contiguous();
+  c.shape = {to_int(x.size(0), "the batch"), to_int(x.size(1), "the number of rows"), to_int(x.size(2), "the number of heads"), static_cast<int>(x.size(3)),
+             static_cast<int>(frequencies.size(0)), static_cast<int>(frequencies.size(1)), {}, {}};
+  for (int a = 0; a < 3; ++a) c.shape.x_strides[a] = c.x.stride(a), c.shape.place_strides[a] = shared ? (a ? c.places.stride(a - 1) : 0) : c.places.stride(a);
+  return c;
+}
+
+Tensor rotary_run(const RotaryCall &c, bool neighbours, bool back) {
+  const c10::DeviceGuard guard(c.x.device());
+  const Tensor y = at::empty(c.x.sizes(), c.x.options());
+  check(mv_rotary_positions(ptr(c.x), ptr(c.places), ptr(c.frequencies), ptr(y), &c.shape, neighbours, back, c.code, c.place_code, stream_of(c.x)));
+  return y;
+}
+
+struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
+  static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &positions, const Tensor &frequencies, bool neighbours) {
+    const RotaryCall c = rotary_call(x, positions, frequencies);
+    ctx->save_for_backward({positions, frequencies});
+    ctx->saved_data["neighbours"] = neighbours;
+    ctx->saved_data["dtype"] = x.scalar_type();
+    return rotary_run(c, neighbours, false);
+  }
+  static variable_list backward(AutogradContext *ctx, const variable_list &grads) {
+    variable_list out(4);
+    if (!grads[0].defined()) return out;
+    {
+      const at::NoGradGuard no_grad;
+      const auto t = ctx->get_saved_variables();
+      out[0] = rotary_run(rotary_call(grads[0].to(ctx->saved_data["dtype"].toScalarType()), t[0], t[1]), ctx->saved_data["neighbours"].toBool(), true);
+    }
+    differentiable_once(grads, out);
+    return out;
+  }
+};
+
+Tensor rotary_positions(const Tensor &x, const Tensor &positions, const Tensor &frequencies, bool neighbours) {
+  for (const Tensor &t : {x, positions, frequencies}) no_forward_mode(t);
+  MVB_CHECK(!wants_gradient({positions, frequencies}), "rotary_positions has no gradient for positions and frequencies: detach them");
+  const py::gil_scoped_release no_gil;
+  if (wants_gradient({x})) return RotaryFunction::apply(x, positions, frequencies, neighbours);
+  const at::NoGradGuard no_grad;
+  return rotary_run(rotary_call(x, positions, frequencies), neighbours, false);
+}
+
+Tensor rotary_positions_turn(const Tensor &x, const Tensor &positions, const Tensor &frequencies, bool neighbours, bool back) {
+  const py::gil_scoped_release no_gil;
+  const at::NoGradGuard no_grad;
+  return rotary_run(rotary_call(x, positions, frequencies), neighbours, back);
+}
+
+// ---- linear layers with weights in 4 bits --------------------------------------------------------------------------------
+void check_group(int64_t group) { MVB_CHECK(group == 32 || group == 64 || group == 128, "groups of ", group, " columns: 32, 64 or 128 are possible"); }
+
+std::pair<Tensor, Tensor> quantize_groups(const Tensor &given, int64_t group) {
+  no_gradient({given}, "quantize_groups");
+  const py::gil_scoped_release no_gil;
+  const at::NoGradGuard no_grad;
+  MVB_CHECK(given.is_cuda(), "quantize_groups is not implemented on CPU");
+  const int code = float_code(given, "quantize_groups");
+  check_group(group);
+  MVB_CHECK(given.dim() == 2 && given.size(1) >= 1, "quantize_groups takes a matrix of at least one column, got shape ", shape_text(given.sizes()));
+  const c10::DeviceGuard guard(given.device());
+  const Tensor w = given.contiguous();
+  const int64_t blocks = (w.size(1) + 127) / 128;
+  const Tensor q = at::empty({w.size(0), 64 * blocks}, w.options().dtype(at::kByte));
+  const Tensor scales = at::empty({w.size(0), 128 / group * blocks}, w.options().dtype(at::kFloat));
+  check(mv_quantize_groups(ptr(w), ptr(q), ptr(scales), w.size(0), to_int(w.size(1), "a row"), static_cast<int>(group), code, stream_of(w)));
+  return {q, scales};
+}
+
+Tensor group_linear(const Tensor &x_in, const Tensor &weight_in, const Tensor &scales_in, const std::optional<Tensor> &bias_in) {
+  const Tensor bias_given = bias_in.value_or(Tensor());
+  no_gradient({x_in, scales_in, bias_given}, "group_linear");
+  const py::gil_scoped_release no_gil;
+  const at::NoGradGuard no_grad;
+  MVB_CHECK(x_in.is_cuda(), "group_linear is not implemented on CPU");
+  MVB_CHECK(x_in.scalar_type() == at::kHalf || x_in.scalar_type() == at::kBFloat16, "group_linear takes float16 or bfloat16, got ", dtype_name(x_in));
+  MVB_CHECK(weight_in.scalar_type() == at::kByte && scales_in.scalar_type() == at::kFloat, "weight and scales have to be uint8 and float32, got ",
+            dtype_name(weight_in), " and ", dtype_name(scales_in));
+  same_device(x_in, weight_in, "weight");
+  same_device(x_in, scales_in, "scales");
+  same_device(x_in, bias_given, "bias");
+  MVB_CHECK(x_in.dim() >= 1 && x_in.size(-1) >= 1, "group_linear takes rows of at least one column, got shape ", shape_text(x_in.sizes()));
+  const int inputs = to_int(x_in.size(-1), "a row");
+  const int64_t blocks = (int64_t{inputs} + 127) / 128;
+  MVB_CHECK(weight_in.dim() == 2 && weight_in.size(1) == 64 * blocks, "weight has shape ", shape_text(weight_in.sizes()), ", expected (outputs, ", 64 * blocks,
+            ") for rows of ", inputs);
+  const int outputs = to_int(weight_in.size(0), "the number of outputs");
+  MVB_CHECK(scales_in.dim() == 2 && scales_in.size(0) == outputs && (scales_in.size(1) == blocks || scales_in.size(1) == 2 * blocks || scales_in.size(1) == 4 * blocks),
+            "scales have shape ", shape_text(scales_in.sizes()), ", expected (", outputs, ", ", 4 * blocks, "), (", outputs, ", ", 2 * blocks, ") or (", outputs, ", ",
+            blocks, ")");
+  MVB_CHECK(!bias_given.defined() || (bias_given.dim() == 1 && bias_given.size(0) == outputs), "bias has shape ",
+            bias_given.defined() ? shape_text(bias_given.sizes()) : "", ", expected (", outputs, ")");
+  const c10::DeviceGuard guard(x_in.device());
+  const Tensor x = x_in.contiguous(), w = aligned_rows(weight_in), scales = scales_in.contiguous();
+  const Tensor bias = bias_given.defined() ? bias_given.to(x.scalar_type()).contiguous() : bias_given;
+  const int64_t rows = x.numel() / inputs;
+  std::vector<int64_t> shape = x.sizes().vec();
+  shape.back() = outputs;
+  const Tensor y = at::empty(shape, x.options());
+  const size_t bytes = mv_group_linear_workspace_bytes(rows, inputs, outputs);
+  const Tensor work = bytes_on(x, bytes);
+  check(mv_group_linear(ptr(x), ptr(w), ptr(scales), ptr(bias), ptr(y), rows, inputs, outputs, static_cast<int>(128 * blocks / scales.size(1)), dtype_code(x),
+                        ptr(work), bytes, stream_of(x)));
+  return y;
+}
+
 // ---- helpers of the augmentation stages ----------------------------------------------------------------------------
 // A host array (rois, a control grid) on the device, without waiting for what is queued there.  float64 stays float64,
 // every other type becomes float32.
@@ -957,6 +1224,13 @@ PYBIND11_MODULE(_native, m) {
   m.def("add_rms_norm_quantized", &add_rms_norm_quantized);
   m.def("quantize_blocks", &quantize_blocks);
   m.def("block_linear", &block_linear);
+  m.def("group_norm_act", &group_norm_act);
+  m.def("group_norm_act_forward", &group_norm_act_forward);
+  m.def("group_norm_act_backward", &group_norm_act_backward);
+  m.def("rotary_positions", &rotary_positions);
+  m.def("rotary_positions_turn", &rotary_positions_turn);
+  m.def("quantize_groups", &quantize_groups);
+  m.def("group_linear", &group_linear);
   m.def("upload", &upload);
   m.def("window_roi", &window_roi);
   m.def("peak_mib", &peak_mib);

@@ -4,6 +4,7 @@
 // One v_mfma 16x16x128 takes a whole block of 128: it starts from zero, and its result is added to the sum in 32 bits with
 // the two scales' product.  The weights are its first operand, so that a lane's results lie in one row of y (one scale per
 // tile and lane, four neighbouring results).
+#include "parts.hpp"
 #include "rows.hpp"
 
 #include <algorithm>
@@ -376,30 +377,6 @@ __global__ __launch_bounds__(256) void product_rows(const unsigned char *q, cons
     }
 #pragma unroll
   for (int t = 0; t < TM; ++t) store_row(to, split, m0 + t * 16 + r16, n0 + 4 * g, acc[t]);
-}
-
-// The parts' sum, in a fixed order: `Slices` threads share the parts of a result.
-template <typename T, int Slices>
-__global__ __launch_bounds__(256) void join_parts(const float *part, const T *bias, T *y, long count, int outputs, int splits) {
-  constexpr int kWide = 256 / Slices;
-  __shared__ float sums[Slices][kWide];
-  const int in = threadIdx.x % kWide, slice = threadIdx.x / kWide;
-  const long at = static_cast<long>(linear_block()) * kWide + in;
-  float sum = 0.f;
-  if (at < count) {
-#pragma unroll 4
-    for (int s = slice; s < splits; s += Slices) sum += part[s * count + at];
-  }
-  if constexpr (Slices > 1) {
-    sums[slice][in] = sum;
-    __syncthreads();
-    if (slice) return;
-#pragma unroll
-    for (int i = 1; i < Slices; ++i) sum += sums[i][in];
-  }
-  if (at >= count) return;
-  if (bias) sum += load(bias + at % outputs);
-  y[at] = store_cast<T>(sum);
 }
 
 // ---- which kernel --------------------------------------------------------------------------------------------

@@ -1,0 +1,265 @@
+// Product of 16-bit rows with weights in 4 bits (e2m1) and a scale for each group of 32, 64 or 128 columns of a row:
+//   y[m, n] = sum over groups g of  s[n, g] sum_k x[m, k] w[n, k]  + bias[n]
+//
+// The values of 4-bit codes (0, 1/2, 1, 3/2, 2, 3, 4, 6 and their negatives) are exact in 16 bits, and so are the matrix
+// units' products; a group's sum is scaled in 32 bits when it is added.
+//
+// The weights of a row are blocks of 128 columns, 64 bytes.  The four bytes of eight neighbouring columns stay together
+// (two codes a byte, the first one in its low half); piece 4 s + g of a block's sixteen stands at place 4 g + s.  One
+// 16-byte load then brings lane group g its columns of four products of 32 columns, each within one group of a scale.
+#include "parts.hpp"
+#include "rows.hpp"
+
+#include <algorithm>
+
+namespace mv {
+namespace {
+
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+
+// Eight codes to 16 bits, two by two; their products with eight columns of 16 rows, added to `sum`
+template <typename T> struct Matrix;
+template <> struct Matrix<__half> {
+  static __device__ __forceinline__ u32x4 values(unsigned codes) {
+    return {__builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, 1.f, 0)),
+            __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, 1.f, 1)),
+            __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, 1.f, 2)),
+            __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, 1.f, 3))};
+  }
+  static __device__ __forceinline__ f32x4 product(const u32x4 &a, const u32x4 &b, const f32x4 &sum) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), sum, 0, 0, 0);
+  }
+};
+template <> struct Matrix<__hip_bfloat16> {
+  static __device__ __forceinline__ u32x4 values(unsigned codes) {
+    return {__builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, 1.f, 0)),
+            __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, 1.f, 1)),
+            __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, 1.f, 2)),
+            __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, 1.f, 3))};
+  }
+  static __device__ __forceinline__ f32x4 product(const u32x4 &a, const u32x4 &b, const f32x4 &sum) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), sum, 0, 0, 0);
+  }
+};
+
+// Eight columns of a row as they are, zeros from `left` on
+template <typename T> __device__ __forceinline__ u32x4 columns8(const T *p, int left) {
+  if (left >= 8) return reinterpret_cast<const Loose<u32x4, 2> *>(p)->v;
+  u32x4 r = {0u, 0u, 0u, 0u};
+  if (left <= 0) return r;
+  unsigned v[7];
+#pragma unroll
+  for (int i = 0; i < 7; ++i) v[i] = reinterpret_cast<const unsigned short *>(p)[min(i, left - 1)];
+#pragma unroll
+  for (int i = 0; i < 7; ++i) r[i / 2] |= i < left ? v[i] << (i % 2 * 16) : 0u;
+  return r;
+}
+
+template <typename T> struct Product {
+  const T *x;
+  const unsigned char *w;
+  const float *scales;
+  const T *bias;
+  T *y;
+  float *part;   // [splits, rows, outputs], NULL: y
+  long rows;
+  int inputs, outputs, blocks, m_tiles, n_tiles, splits;
+};
+
+// 64 outputs and 16 TM rows per workgroup, straight from memory into the operands' registers.  The four wavefronts take turns
+// at the blocks of the workgroup's share of the sum and join in LDS.
+template <typename T, int TM, int Group>
+__global__ __launch_bounds__(256) void product_rows4(const Product<T> k) {
+  constexpr int TN = 4, kScales = kBlock / Group;
+  __shared__ f32x4 part[3][TN * TM][64];
+  unsigned id = linear_block();
+  if (id >= static_cast<unsigned>(k.m_tiles) * k.n_tiles * k.splits) return;
+  const int n_tile = id % k.n_tiles;
+  id /= k.n_tiles;
+  const int split = id % k.splits, n0 = n_tile * 16 * TN;
+  const long m0 = static_cast<long>(id / k.splits) * 16 * TM;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, g = lane >> 4;
+  const int first = static_cast<int>(static_cast<long>(k.blocks) * split / k.splits), last = static_cast<int>(static_cast<long>(k.blocks) * (split + 1) / k.splits);
+  const T *x_at[TM];
+  const unsigned char *w_at[TN];
+  const float *s_at[TN];
+#pragma unroll
+  for (int t = 0; t < TM; ++t) x_at[t] = k.x + min(m0 + t * 16 + r16, k.rows - 1) * k.inputs;
+#pragma unroll
+  for (int u = 0; u < TN; ++u) {
+    const long n = min(n0 + u * 16 + r16, k.outputs - 1);
+    w_at[u] = k.w + n * k.blocks * 64 + g * 16;
+    s_at[u] = k.scales + n * k.blocks * kScales;
+  }
+  f32x4 acc[TM][TN] = {};
+  for (int b = first + wave; b < last; b += 4) {
+    u32x4 w[TN], x[TM][4];
+    float s[TN][kScales];
+#pragma unroll
+    for (int u = 0; u < TN; ++u) {
+      w[u] = *reinterpret_cast<const u32x4 *>(w_at[u] + b * 64L);
+#pragma unroll
+      for (int i = 0; i < kScales; ++i) s[u][i] = s_at[u][static_cast<long>(b) * kScales + i];
+    }
+#pragma unroll
+    for (int t = 0; t < TM; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int c = b * kBlock + i * 32 + g * 8;
+        x[t][i] = columns8(x_at[t] + c, k.inputs - c);
+      }
+#pragma unroll
+    for (int u = 0; u < TN; ++u) {
+      f32x4 d[TM];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const u32x4 v = Matrix<T>::values(w[u][i]);
+#pragma unroll
+        for (int t = 0; t < TM; ++t) {
+          if (i % (Group / 32) == 0) d[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+          d[t] = Matrix<T>::product(x[t][i], v, d[t]);
+          if ((i + 1) % (Group / 32) == 0) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[t][u][j] = fmaf(d[t][j], s[u][i / (Group / 32)], acc[t][u][j]);
+          }
+        }
+      }
+    }
+  }
+  if (wave) {
+#pragma unroll
+    for (int u = 0; u < TN; ++u)
+#pragma unroll
+      for (int t = 0; t < TM; ++t) part[wave - 1][u * TM + t][lane] = acc[t][u];
+  }
+  __syncthreads();
+  if (wave) return;
+#pragma unroll
+  for (int u = 0; u < TN; ++u) {
+    const int n = n0 + u * 16 + r16;
+    if (n >= k.outputs) continue;
+    const float add = k.bias && !k.part ? load(k.bias + n) : 0.f;
+#pragma unroll
+    for (int t = 0; t < TM; ++t) {
+#pragma unroll
+      for (int i = 0; i < 3; ++i) acc[t][u] += part[i][u * TM + t][lane];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const long m = m0 + t * 16 + 4 * g + j;
+        if (m >= k.rows) continue;
+        if (k.part) k.part[(split * k.rows + m) * k.outputs + n] = acc[t][u][j];
+        else k.y[m * k.outputs + n] = store_cast<T>(acc[t][u][j] + add);
+      }
+    }
+  }
+}
+
+// ---- weights to 4 bits ------------------------------------------------------------------------------------------
+// A thread has eight neighbouring columns; those of a group are neighbouring lanes.
+template <typename T>
+__global__ __launch_bounds__(256) void quantize_groups(const T *w, unsigned *q, float *scales, long pieces, int columns, int blocks, int group) {
+  const long at = static_cast<long>(linear_block()) * 256 + threadIdx.x;
+  if (at >= pieces) return;   // (whole blocks of sixteen lanes)
+  const int o = static_cast<int>(at & 15);
+  const long block = at >> 4, row = block / blocks;
+  const int c = static_cast<int>(block - row * blocks) * kBlock + o * 8;
+  float v[8], most = 0.f;
+  load8(w + row * columns + c, columns - c, v);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) most = max_abs(most, v[i]);
+  for (int d = 1; d < group / 8; d *= 2) most = max_abs(most, __shfl_xor(most, d));
+  const float s = most / 6.f, scale = s < kLeastScale ? kLeastScale : s, inverse = 1.f / scale;   // (NaN stays)
+  unsigned codes = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {   // to the nearest level, halves to the even code
+    const float t = v[i] * inverse, a = fabsf(t);
+    const unsigned code = (a > 0.25f) + (a >= 0.75f) + (a > 1.25f) + (a >= 1.75f) + (a > 2.5f) + (a >= 3.5f) + (a > 5.f);
+    codes |= (code + (t < 0.f ? 8u : 0u)) << (4 * i);
+  }
+  q[block * 16 + (o & 3) * 4 + (o >> 2)] = codes;
+  if (o % (group / 8) == 0) scales[at / (group / 8)] = scale;
+}
+
+// ---- which kernel --------------------------------------------------------------------------------------------------
+struct Plan {
+  int tm, m_tiles, n_tiles, splits;
+};
+
+int ceil_div(long a, long b) { return static_cast<int>((a + b - 1) / b); }
+
+Plan plan_of(long rows, int blocks, int outputs) {
+  const int tm = rows <= 16 ? 1 : rows <= 32 ? 2 : 4, n = ceil_div(outputs, 64), m = ceil_div(rows, 16 * tm);
+  return {tm, m, n, static_cast<int>(std::max(1L, std::min(blocks / 8L, 512 / (static_cast<long>(n) * m))))};
+}
+
+template <typename T, int Group> void launch(const Plan &p, const Product<T> &k, hipStream_t s) {
+  const dim3 grid = linear_grid(static_cast<long>(p.m_tiles) * p.n_tiles * p.splits, 256);
+  if (p.tm == 1) product_rows4<T, 1, Group><<<grid, 256, 0, s>>>(k);
+  else if (p.tm == 2) product_rows4<T, 2, Group><<<grid, 256, 0, s>>>(k);
+  else product_rows4<T, 4, Group><<<grid, 256, 0, s>>>(k);
+}
+
+template <typename T>
+int product(const void *x, const void *w, const void *scales, const void *bias, void *y, long rows, int inputs, int outputs, int group,
+            void *workspace, size_t workspace_bytes, hipStream_t s) {
+  const int blocks = ceil_div(inputs, kBlock);
+  Plan p = plan_of(rows, blocks, outputs);
+  if (p.splits > 1 && (!workspace || workspace_bytes < sizeof(float) * p.splits * static_cast<size_t>(rows) * outputs)) p.splits = 1;
+  const Product<T> k{static_cast<const T *>(x), static_cast<const unsigned char *>(w), static_cast<const float *>(scales), static_cast<const T *>(bias),
+                     static_cast<T *>(y), p.splits > 1 ? static_cast<float *>(workspace) : nullptr, rows, inputs, outputs, blocks, p.m_tiles, p.n_tiles, p.splits};
+  if (group == 32) launch<T, 32>(p, k, s);
+  else if (group == 64) launch<T, 64>(p, k, s);
+  else launch<T, 128>(p, k, s);
+  if (k.part) {
+    const long count = rows * outputs;
+    if (p.splits > 8) join_parts<T, 8><<<linear_grid((count + 31) / 32, 256), 256, 0, s>>>(k.part, k.bias, k.y, count, outputs, p.splits);
+    else join_parts<T, 1><<<linear_grid((count + 255) / 256, 256), 256, 0, s>>>(k.part, k.bias, k.y, count, outputs, p.splits);
+  }
+  return check_launch("group_linear");
+}
+
+}  // namespace
+}  // namespace mv
+
+using namespace mv;
+
+extern "C" {
+
+int mv_quantize_groups(const void *weight, void *q, void *scales, int64_t rows, int columns, int group, int dtype, void *stream) {
+  MV_REQUIRE(group == 32 || group == 64 || group == 128, "groups of %d columns: 32, 64 or 128 are possible", group);
+  MV_REQUIRE(rows >= 0 && rows < (1L << 31) && columns > 0 && columns <= (1 << 30), "wrong sizes: %ld rows of %d columns", static_cast<long>(rows), columns);
+  if (rows == 0) return MV_OK;
+  MV_REQUIRE(weight && q && scales, "a tensor is missing");
+  const int blocks = ceil_div(columns, kBlock);
+  const long pieces = rows * blocks * 16;
+  MV_FLOATS(dtype, {
+    quantize_groups<T><<<linear_grid((pieces + 255) / 256, 256), 256, 0, static_cast<hipStream_t>(stream)>>>(
+        static_cast<const T *>(weight), static_cast<unsigned *>(q), static_cast<float *>(scales), pieces, columns, blocks, group);
+  })
+  return check_launch("quantize_groups");
+}
+
+size_t mv_group_linear_workspace_bytes(int64_t rows, int inputs, int outputs) {
+  if (rows <= 0 || inputs <= 0 || outputs <= 0) return 0;
+  const Plan p = plan_of(rows, ceil_div(inputs, kBlock), outputs);
+  return p.splits > 1 ? sizeof(float) * p.splits * static_cast<size_t>(rows) * outputs : 0;
+}
+
+int mv_group_linear(const void *x, const void *weight, const void *scales, const void *bias, void *y, int64_t rows, int inputs, int outputs,
+                    int group, int dtype, void *workspace, size_t workspace_bytes, void *stream) {
+  MV_REQUIRE(dtype == MV_F16 || dtype == MV_BF16, "dtype %d is not float16 or bfloat16", dtype);
+  MV_REQUIRE(group == 32 || group == 64 || group == 128, "groups of %d columns: 32, 64 or 128 are possible", group);
+  MV_REQUIRE(rows >= 0 && rows < (1L << 31) - 256 && inputs > 0 && inputs <= (1 << 30) && outputs >= 0 && outputs < (1L << 31) - 256,
+             "wrong sizes: %ld rows, %d inputs, %d outputs", static_cast<long>(rows), inputs, outputs);
+  if (rows == 0 || outputs == 0) return MV_OK;
+  MV_REQUIRE(x && weight && scales && y, "a tensor is missing");
+  MV_REQUIRE(reinterpret_cast<uintptr_t>(weight) % 16 == 0, "the weight has to be 16-byte aligned");
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  return dtype == MV_F16 ? product<__half>(x, weight, scales, bias, y, rows, inputs, outputs, group, workspace, workspace_bytes, s)
+                         : product<__hip_bfloat16>(x, weight, scales, bias, y, rows, inputs, outputs, group, workspace, workspace_bytes, s);
+}
+
+}  // extern "C"

@@ -1,9 +1,9 @@
 """Linear layers in 8-bit floating point (e4m3) with a scale for each block of 128, for inference.  No counterpart in the
 reference."""
 import torch
-from torch import nn
 
 from .._lib import native
+from ._module import KeepsTypes
 
 
 def quantize_blocks(x, block_rows=1):
@@ -22,7 +22,7 @@ def block_linear(q, q_scales, weight, weight_scales, bias=None, out_dtype=torch.
     return native.block_linear(q, q_scales, weight, weight_scales, bias, out_dtype)
 
 
-class BlockScaledLinear(nn.Module):
+class BlockScaledLinear(KeepsTypes):
     """A trained ``nn.Linear`` with its weight in 8 bits.  Takes activations as they are, or ``(q, scales)`` that are in
     8 bits already (``AddRMSNorm.quantized``).
 
@@ -31,6 +31,7 @@ class BlockScaledLinear(nn.Module):
         bias (bool): whether there is a bias
         dtype (torch.dtype): of the results, float16 or bfloat16
     """
+    kept = ('weight', 'weight_scales')
 
     def __init__(self, in_features, out_features, bias=True, dtype=torch.bfloat16, device=None):
         super().__init__()
@@ -48,16 +49,6 @@ class BlockScaledLinear(nn.Module):
         if linear.bias is not None:
             layer.bias = linear.bias.detach().to(dtype)
         return layer
-
-    def _apply(self, fn, recurse=True):
-        # .half() and its like leave what is in 8 bits, and its scales, as they are; moves between devices take all
-        kept = {name: getattr(self, name) for name in ('weight', 'weight_scales')}
-        super()._apply(fn, recurse)
-        for name, tensor in kept.items():
-            now = getattr(self, name)
-            if now.dtype != tensor.dtype:
-                setattr(self, name, tensor.to(now.device))
-        return self
 
     def forward(self, x):
         if isinstance(x, tuple):
