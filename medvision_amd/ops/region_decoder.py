@@ -1,7 +1,7 @@
 """A decoder layer for the regions of a head: they look at the tokens of a feature map and go through two linear layers.
 
 ``RegionDecoderLayer`` is for training, ``RegionDecoderLayer.for_inference`` gives the same layer with its linear layers in
-8 bits: the norms then write what those read.  No counterpart in the reference."""
+8 or 4 bits: in front of layers in 8 bits the norms write what those read.  No counterpart in the reference."""
 import copy
 
 import torch
@@ -9,7 +9,9 @@ from torch import nn
 
 from .block_linear import BlockScaledLinear
 from .cross_attention import cross_attention
+from .group_linear import GroupScaledLinear
 from .rms_norm import AddRMSNorm
+from .rotary import RotaryPositions
 
 
 def map_tokens(features):
@@ -27,9 +29,11 @@ class RegionDecoderLayer(nn.Module):
         hidden (int): channels between the two linear layers, four times ``channels`` by default
         key_heads (int): of keys and values, ``heads`` by default; ``heads`` is a multiple of it
         eps (float): of the norms
+        axes (int): of the positions of regions and tokens by which queries and keys are turned; 0: they have none
+        theta (float): of the positions' frequencies (``axis_frequencies``)
     """
 
-    def __init__(self, channels, heads, hidden=None, key_heads=None, eps=1e-6):
+    def __init__(self, channels, heads, hidden=None, key_heads=None, eps=1e-6, axes=0, theta=100.0):
         super().__init__()
         key_heads = heads if key_heads is None else key_heads
         if channels % heads or heads % key_heads:
@@ -41,18 +45,24 @@ class RegionDecoderLayer(nn.Module):
         self.key_value = nn.Linear(channels, 2 * key_heads * self.head_channels, bias=False)
         self.out = nn.Linear(channels, channels)
         self.up, self.down = nn.Linear(channels, hidden), nn.Linear(hidden, channels)
+        self.register_module("place", RotaryPositions(self.head_channels, axes, theta) if axes else None)
 
-    def for_inference(self, dtype=torch.bfloat16):
-        """This layer, on the GPU, for inference: linear layers in 8 bits, their results in ``dtype``.  The norms' weights are
-        float32, which goes with regions of any type."""
+    def for_inference(self, dtype=torch.bfloat16, bits=8, group=32):
+        """This layer, on the GPU, for inference: linear layers in 8 bits, or in 4 with a scale for each ``group`` columns of a row
+        (few regions, where reading the weights takes the time); their results in ``dtype``.  The norms' weights are float32, which
+        goes with regions of any type."""
+        if bits not in (4, 8):
+            raise ValueError(f"linear layers in {bits} bits: 4 or 8 are possible")
         layer = copy.copy(self)
         for name, value in vars(self).items():   # hooks, parameters, buffers and modules of its own
             if isinstance(value, (dict, set)):
                 setattr(layer, name, value.copy())
         for name in ("query", "key_value", "out", "up", "down"):
-            layer._modules[name] = BlockScaledLinear.from_linear(getattr(self, name), dtype)
+            linear = getattr(self, name)
+            layer._modules[name] = BlockScaledLinear.from_linear(linear, dtype) if bits == 8 else GroupScaledLinear.from_linear(linear, group, dtype)
         for name in ("norm_query", "norm_hidden"):
             layer._modules[name] = copy.deepcopy(getattr(self, name)).float().requires_grad_(False)
+        layer._modules["place"] = copy.deepcopy(self.place)
         return layer.eval()
 
     def _normed(self, norm, x, residual):
@@ -62,13 +72,21 @@ class RegionDecoderLayer(nn.Module):
             return norm.quantized(x, residual)
         return norm(x, residual)
 
-    def forward(self, regions, tokens, residual=None, key_mask=None, key_lengths=None):
+    def _placed(self, x, positions, whose):
+        if (positions is None) != (self.place is None):
+            raise ValueError(f"{whose}_positions are {'missing' if positions is None else 'given'}: the layer has {'positions' if self.place else 'no axes'}")
+        return x if positions is None else self.place(x, positions)
+
+    def forward(self, regions, tokens, residual=None, key_mask=None, key_lengths=None, region_positions=None, token_positions=None):
         """``regions [batch, regions, channels]``, ``residual`` like them or None, ``tokens [batch, cells, channels]`` of
         which ``key_mask`` and ``key_lengths`` may leave some out: ``(regions, residual)`` for the next layer.  After the last
-        one the result is their sum.  The residual has the type of the one that was given, or of the regions."""
+        one the result is their sum.  The residual has the type of the one that was given, or of the regions.
+        A layer with axes takes ``region_positions [batch, regions, axes]`` and ``token_positions [batch, cells, axes]`` (either
+        without the batch where all samples share them), in one unit; they get no gradient."""
         y, residual = self._normed(self.norm_query, regions, residual)
         q = self.query(y).unflatten(-1, (self.heads, self.head_channels))
         k, v = self.key_value(tokens).unflatten(-1, (2, self.key_heads, self.head_channels)).unbind(2)
+        q, k = self._placed(q, region_positions, "region"), self._placed(k, token_positions, "token")
         seen = cross_attention(q, k, v, key_mask, key_lengths).flatten(2)
         y, residual = self._normed(self.norm_hidden, self.out(seen), residual)
         return self.down(torch.relu(self.up(y))), residual
