@@ -16,9 +16,22 @@ constexpr int kThreads = 256;
 constexpr int kMostDim = 1024, kMostAxes = 8;
 constexpr int kTable = 4096;   // angles of a workgroup at most
 
+// a / b for 0 <= a < 2^31 with a multiplication: m = floor(2^(31 + s) / b) + 1, 2^(s - 1) < b <= 2^s (exact: a m / 2^(31 + s) is off
+// by less than 1 / b)
+struct Divisor {
+  unsigned by, m;
+  int shift;
+  explicit Divisor(unsigned b) : by(b), shift(0) {
+    while ((1ul << shift) < b) ++shift;
+    m = static_cast<unsigned>((1ul << (31 + shift)) / b + 1);
+  }
+  __device__ __forceinline__ unsigned of(unsigned a) const { return static_cast<unsigned>((static_cast<unsigned long>(a) * m) >> (31 + shift)); }
+};
+
 struct Rotary {
   mv_rotary_shape of;
-  int block_rows, row_blocks;
+  int block_rows, row_blocks, pieces, kept, unit;   // pieces of eight pairs (channels) of a head; units of the channels that stay
+  Divisor by_pairs, by_pieces, by_heads, by_kept;
 };
 
 __device__ __forceinline__ double place_at(const void *p, int kind, long at) {
@@ -42,6 +55,70 @@ __device__ __forceinline__ float2 turn(double q) {
   return {quarter == 1 || quarter == 2 ? -a : a, quarter >= 2 ? -b : b};
 }
 
+template <typename T, int N> __device__ __forceinline__ void copy_unit(const T *from, T *to) {
+  typedef unsigned char bytes __attribute__((ext_vector_type(N * sizeof(T) > 16 ? 16 : N * sizeof(T))));
+#pragma unroll
+  for (unsigned i = 0; i < N * sizeof(T); i += sizeof(bytes))
+    reinterpret_cast<Loose<bytes, sizeof(T)> *>(reinterpret_cast<char *>(to) + i)->v = reinterpret_cast<const Loose<bytes, sizeof(T)> *>(reinterpret_cast<const char *>(from) + i)->v;
+}
+
+// Eight elements as they are in memory
+template <typename T> struct Raw {
+  u32x4 bits[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T *p) {
+#pragma unroll
+    for (unsigned i = 0; i < sizeof(T) / 2; ++i) bits[i] = reinterpret_cast<const Loose<u32x4, sizeof(T)> *>(p)[i].v;
+  }
+  __device__ __forceinline__ void values(float (&v)[8]) const {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(bits[i / 4][i % 4]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = Bits<T>::up(static_cast<unsigned short>(bits[0][i / 2] >> (i % 2 * 16)));
+    }
+  }
+};
+
+// Cosines and sines of a workgroup's rows
+__device__ __forceinline__ void form_table(float2 *table, const void *places, int place_kind, const double *frequencies, const Rotary &k, int b, int first,
+                                           int rows, bool back) {
+  const mv_rotary_shape &s = k.of;
+  for (int e = threadIdx.x; e < rows * s.pairs; e += kThreads) {
+    const int row = k.by_pairs.of(e), p = e - row * s.pairs;
+    const long at = b * s.place_strides[0] + (first + row) * s.place_strides[1];
+    double place[4], f[4];   // (axes that do not exist: the last one again)
+#pragma unroll
+    for (int a = 0; a < 4; ++a) {
+      const int axis = min(a, s.axes - 1);
+      place[a] = place_at(places, place_kind, at + axis * s.place_strides[2]), f[a] = frequencies[axis * s.pairs + p];
+    }
+    double angle = place[0] * f[0];
+#pragma unroll
+    for (int a = 1; a < 4; ++a) angle = a < s.axes ? fma(place[a], f[a], angle) : angle;
+    for (int a = 4; a < s.axes; ++a) angle = fma(place_at(places, place_kind, at + a * s.place_strides[2]), frequencies[a * s.pairs + p], angle);
+    float2 t = turn(angle * 0.63661977236758134);   // 2 / pi
+    if (back) t.y = -t.y;
+    table[e] = t;
+  }
+}
+
+// Up to eight pairs: (one[i], two[i]), or neighbours in one[].
+template <bool Neighbours> __device__ __forceinline__ void turn_piece(const float2 *t, int left, float (&one)[8], float (&two)[8]) {
+#pragma unroll
+  for (int i = 0; i < (Neighbours ? 4 : 8); ++i) {
+    if ((Neighbours ? 2 * i : i) >= left) break;
+    const float2 cs = t[i];
+    float &a = one[Neighbours ? 2 * i : i], &b = Neighbours ? one[2 * i + 1] : two[i];
+    const float was = a;
+    a = fmaf(was, cs.x, -(b * cs.y));
+    b = fmaf(was, cs.y, b * cs.x);
+  }
+}
+
+// Pieces are of eight pairs (neighbours: of eight channels).  The last one of a head starts earlier than its place where the pairs
+// do not fill it: what two pieces have in common is formed twice, with the same results, instead of an element at a time.
+// A thread's first piece is on its way while the angles are formed.
 template <typename T, bool Neighbours>
 __global__ __launch_bounds__(kThreads) void rotary(const T *x, const void *places, int place_kind, const double *frequencies, T *y,
                                                    const Rotary k, bool back) {
@@ -50,60 +127,60 @@ __global__ __launch_bounds__(kThreads) void rotary(const T *x, const void *place
   const unsigned id = linear_block();
   if (id >= static_cast<unsigned>(s.batch) * k.row_blocks) return;
   const int b = id / k.row_blocks;
-  const int first = (id - b * k.row_blocks) * k.block_rows, rows = min(k.block_rows, s.rows - first);
-  const int pairs = s.pairs;
-  for (int e = threadIdx.x; e < rows * pairs; e += kThreads) {
-    const int row = e / pairs, p = e - row * pairs;
-    const long at = b * s.place_strides[0] + (first + row) * s.place_strides[1];
-    double angle = 0.;
-    for (int a = 0; a < s.axes; ++a) angle = fma(place_at(places, place_kind, at + a * s.place_strides[2]), frequencies[a * pairs + p], angle);
-    float2 t = turn(angle * 0.63661977236758134);   // 2 / pi
-    if (back) t.y = -t.y;
-    table[e] = t;
-  }
-  __syncthreads();
-  const int turned = (Neighbours ? 2 * pairs + 7 : pairs + 7) / 8, kept = (s.dim - 2 * pairs + 7) / 8, pieces = turned + kept;
-  for (int e = threadIdx.x; e < rows * s.heads * pieces; e += kThreads) {
-    const int line = e / pieces, o = e - line * pieces, row = line / s.heads, head = line - row * s.heads;
-    const T *const from = x + b * s.x_strides[0] + (first + row) * s.x_strides[1] + head * s.x_strides[2];
-    T *const to = y + ((static_cast<long>(b) * s.rows + first + row) * s.heads + head) * s.dim;
-    if (o >= turned) {   // channels that stay
-      const int c = 2 * pairs + (o - turned) * 8;
-      float v[8];
-      load8(from + c, s.dim - c, v);
-      store8(to + c, s.dim - c, v);
-      continue;
+  const int first = (id - b * k.row_blocks) * k.block_rows, rows = min(k.block_rows, s.rows - first), pairs = s.pairs;
+  const T *const from = x + b * s.x_strides[0] + first * s.x_strides[1];
+  T *const to = y + (static_cast<long>(b) * s.rows + first) * s.heads * s.dim;
+  const int lines = rows * s.heads, width = Neighbours ? 2 * pairs : pairs, items = lines * k.pieces;
+  struct Piece {
+    int row, c;
+    long from, to;
+  };
+  auto piece_of = [&](int e) {
+    const int line = k.by_pieces.of(e), row = k.by_heads.of(line), c = max(0, min((e - line * k.pieces) * 8, width - 8));
+    return Piece{row, c, row * s.x_strides[1] + (line - row * s.heads) * s.x_strides[2] + c, static_cast<long>(line) * s.dim + c};
+  };
+  if (width >= 8) {
+    bool formed = false;
+    for (int e = threadIdx.x; !formed || e < items; e += kThreads) {
+      const Piece p = piece_of(min(e, items - 1));
+      Raw<T> one, two;
+      one.load(from + p.from);
+      if (!Neighbours) two.load(from + p.from + pairs);
+      if (!formed) {
+        form_table(table, places, place_kind, frequencies, k, b, first, rows, back);
+        __syncthreads();
+        formed = true;
+      }
+      if (e >= items) break;
+      float v[8], w[8];
+      one.values(v);
+      if (!Neighbours) two.values(w);
+      turn_piece<Neighbours>(table + p.row * pairs + (Neighbours ? p.c / 2 : p.c), 8, v, w);
+      store8(to + p.to, 8, v);
+      if (!Neighbours) store8(to + p.to + pairs, 8, w);
     }
-    if constexpr (Neighbours) {
-      const int c = o * 8, left = 2 * pairs - c;
-      float v[8];
-      load8(from + c, left, v);
-      const float2 *const t = table + row * pairs + o * 4;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (2 * i >= left) break;
-        const float2 cs = t[i];
-        const float one = v[2 * i], two = v[2 * i + 1];
-        v[2 * i] = fmaf(one, cs.x, -(two * cs.y));
-        v[2 * i + 1] = fmaf(one, cs.y, two * cs.x);
-      }
-      store8(to + c, left, v);
-    } else {
-      const int c = o * 8, left = pairs - c;
-      float one[8], two[8];
-      load8(from + c, left, one);
-      load8(from + pairs + c, left, two);
-      const float2 *const t = table + row * pairs + c;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (i >= left) break;
-        const float2 cs = t[i];
-        const float was = one[i];
-        one[i] = fmaf(was, cs.x, -(two[i] * cs.y));
-        two[i] = fmaf(was, cs.y, two[i] * cs.x);
-      }
-      store8(to + c, left, one);
-      store8(to + pairs + c, left, two);
+  } else {   // heads of few pairs
+    form_table(table, places, place_kind, frequencies, k, b, first, rows, back);
+    __syncthreads();
+    for (int e = threadIdx.x; e < items; e += kThreads) {
+      const Piece p = piece_of(e);
+      float v[8], w[8];
+      load8(from + p.from, width, v);
+      if (!Neighbours) load8(from + p.from + pairs, width, w);
+      turn_piece<Neighbours>(table + p.row * pairs, width, v, w);
+      store8(to + p.to, width, v);
+      if (!Neighbours) store8(to + p.to + pairs, width, w);
+    }
+  }
+  for (int e = threadIdx.x; e < lines * k.kept; e += kThreads) {   // channels that stay
+    const int line = k.by_kept.of(e), row = k.by_heads.of(line), head = line - row * s.heads, c = 2 * pairs + (e - line * k.kept) * k.unit;
+    const T *const here = from + row * s.x_strides[1] + head * s.x_strides[2] + c;
+    T *const there = to + static_cast<long>(line) * s.dim + c;
+    switch (k.unit) {
+      case 8: copy_unit<T, 8>(here, there); break;
+      case 4: copy_unit<T, 4>(here, there); break;
+      case 2: copy_unit<T, 2>(here, there); break;
+      default: *there = *here;
     }
   }
 }
@@ -124,11 +201,15 @@ extern "C" int mv_rotary_positions(const void *x, const void *places, const void
   MV_REQUIRE(s.pairs >= 0 && 2 * s.pairs <= s.dim, "%d pairs of %d channels", s.pairs, s.dim);
   if (s.batch == 0 || s.rows == 0 || s.heads == 0) return MV_OK;
   MV_REQUIRE(x && y && (s.pairs == 0 || (places && frequencies)), "a tensor is missing");
-  Rotary k{s, 0, 0};
   const long row = static_cast<long>(s.heads) * s.dim;
   MV_REQUIRE(row < (1L << 31), "rows of %d heads of %d channels are too long", s.heads, s.dim);
-  // 8192 elements a workgroup: four times eight for a thread
-  k.block_rows = static_cast<int>(std::max(1L, std::min({8192L / row, 64L, kTable / std::max(1L, static_cast<long>(s.pairs)), static_cast<long>(s.rows)})));
+  const int kept = s.dim - 2 * s.pairs, unit = kept % 8 == 0 ? 8 : kept % 4 == 0 ? 4 : kept % 2 == 0 ? 2 : 1;
+  const int pieces = ((neighbours ? 2 : 1) * s.pairs + 7) / 8;
+  Rotary k{s, 0, 0, pieces, kept / unit, unit, Divisor(std::max(1, s.pairs)), Divisor(std::max(1, pieces)), Divisor(s.heads), Divisor(std::max(1, kept / unit))};
+  // Up to 4096 elements a workgroup (2 x 32768 x 8 heads of 64 in bf16: 37 us; 8192 47, 2048 44), fewer where that would leave compute
+  // units without one
+  const long spread = static_cast<long>(s.batch) * s.rows / 1024;
+  k.block_rows = static_cast<int>(std::max(1L, std::min({4096L / row, 64L, kTable / std::max(1L, static_cast<long>(s.pairs)), static_cast<long>(s.rows), spread})));
   k.row_blocks = (s.rows + k.block_rows - 1) / k.block_rows;
   const long blocks = static_cast<long>(s.batch) * k.row_blocks;
   MV_REQUIRE(blocks < (1L << 32), "too many rows: %d in a batch of %d", s.rows, s.batch);
