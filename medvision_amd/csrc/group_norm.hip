@@ -8,8 +8,9 @@
 // Sums over the cells are kept for each channel: a thread has eight neighbouring channels and a share of the cells, a
 // workgroup joins its threads' shares, and a small kernel joins the workgroups' to those of a group.  Two kernels with a pass over
 // memory each, then; bound by memory.
-#include "rows.hpp"
 #include "activation.hpp"
+#include "group_norm.hpp"
+#include "rows.hpp"
 
 #include <algorithm>
 #include <type_traits>
@@ -25,24 +26,87 @@ struct Cells {
   int channels, groups, group_channels, tile_threads, tile_rows, chunks;
 };
 
-// Where a thread stands: channels from c on (`left` of them exist), cells first, first + step, ... below last.
+// The first channel of a piece of eight.  The last piece starts earlier than its place where it would not be whole: the channels
+// that it has in common with the one before are worked out twice, with the same results.
+__device__ __forceinline__ int first_channel(const Cells &s, int octet) { return max(0, min(octet * 8, s.channels - 8)); }
+
+// Where a thread stands: channels from c on (`left` of them exist), `cells` cells that are `stride` elements apart, the first one
+// `at` elements from the start.
 struct Place {
-  int c, left, row;
-  long first, last, step, base;   // base: of the sample's first cell, in elements
-  bool live;
+  int c, left;
+  long cells, stride, at;
 };
-__device__ __forceinline__ Place place_of(const Cells &s) {
+__device__ __forceinline__ Place place_of(const Cells &s, unsigned chunk) {
   Place p;
-  const int octet = threadIdx.x % s.tile_threads;
-  p.row = threadIdx.x / s.tile_threads;
-  p.c = (blockIdx.y * kThreads + octet) * 8;
-  p.left = s.channels - p.c;
-  p.first = blockIdx.x * s.each + p.row;
-  p.last = min(s.cells, (blockIdx.x + 1) * s.each);
-  p.step = s.tile_rows;
-  p.base = static_cast<long>(blockIdx.z) * s.cells * s.channels;
-  p.live = p.row < s.tile_rows && p.left > 0;
+  const int octet = threadIdx.x % s.tile_threads, row = threadIdx.x / s.tile_threads;
+  const int piece = blockIdx.y * kThreads + octet;
+  p.c = first_channel(s, piece);
+  p.left = s.channels - piece * 8 > 0 ? s.channels - p.c : 0;
+  const long first = chunk * s.each + row, last = min(s.cells, (chunk + 1) * s.each);
+  p.cells = row < s.tile_rows && p.left > 0 && first < last ? (last - first + s.tile_rows - 1) / s.tile_rows : 0;
+  p.stride = static_cast<long>(s.tile_rows) * s.channels;
+  p.at = (static_cast<long>(blockIdx.z) * s.cells + first) * s.channels + p.c;
   return p;
+}
+
+// How a kernel's pieces of eight channels are read and written: one element after the other (fewer than eight channels), whole, or
+// whole with results that go past the caches.
+enum Form { kParts, kWhole, kWholePast };
+
+// Eight channels of a cell: as they are in memory where all of them exist, so that several cells' loads
+// are on their way before the first is used.
+template <typename T, int F> struct Eight {
+  Raw<T> raw;
+  __device__ __forceinline__ void load(const T *p, int) { raw.load(p); }
+  __device__ __forceinline__ void values(float (&v)[8]) const { raw.values(v); }
+};
+template <typename T> struct Eight<T, kParts> {
+  float v[8];
+  __device__ __forceinline__ void load(const T *p, int left) { load8(p, left, v); }
+  __device__ __forceinline__ void values(float (&out)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) out[i] = v[i];
+  }
+};
+// Results of more than what caches hold go past them (2 x 128^3 cells of 32 channels in float16: 160 instead of 177 us, gradients 283
+// instead of 294).
+template <typename T, int F> __device__ __forceinline__ void put_eight(T *p, int left, const float (&v)[8]) {
+  if constexpr (F == kWholePast) {
+    Raw<T> raw;
+    raw.set(v);
+#pragma unroll
+    for (unsigned i = 0; i < sizeof(T) / 2; ++i) __builtin_nontemporal_store(raw.bits[i], &reinterpret_cast<Loose<u32x4, sizeof(T)> *>(p)[i].v);
+  } else {
+    store8(p, F == kWhole ? 8 : left, v);
+  }
+}
+// Pieces of kAtOnce cells, the last one again where there are fewer left.
+constexpr int kAtOnce = 4;
+template <typename T, int F>
+__device__ __forceinline__ void load_cells(Eight<T, F> (&to)[kAtOnce], const T *at, long cells, const Place &p) {
+#pragma unroll
+  for (int n = 0; n < kAtOnce; ++n) to[n].load(at + min(static_cast<long>(n), cells - 1) * p.stride, p.left);
+}
+
+// What the rows of a tile have of each of its channels, joined by teams of threads and then over the teams, in a fixed order:
+// add(row, piece, channel of it, sum), put(channel, sum).
+template <typename Sum, typename Add, typename Put> __device__ __forceinline__ void join_rows(const Cells &s, const Add &add, const Put &put) {
+  __shared__ Sum sums[kThreads];
+  const int wide = min(s.tile_threads * 8, kThreads), team = threadIdx.x / wide, teams = kThreads / wide;
+  for (int first = 0; first < s.tile_threads * 8; first += wide) {
+    const int k = first + threadIdx.x % wide, c = blockIdx.y * kThreads * 8 + k;
+    const bool mine = team < teams && k < s.tile_threads * 8 && c < s.channels;
+    Sum all = {0, 0};
+    if (mine)
+      for (int r = team; r < s.tile_rows; r += teams) add(r, k / 8, c - first_channel(s, c / 8), all);
+    if (teams > 1) {
+      sums[threadIdx.x] = all;
+      __syncthreads();
+      if (mine && team == 0)
+        for (int t = 1; t < teams; ++t) all.x += sums[t * wide + k].x, all.y += sums[t * wide + k].y;
+    }
+    if (mine && team == 0) put(c, all);
+  }
 }
 
 // ---- forward ------------------------------------------------------------------------------------------------------
@@ -52,111 +116,130 @@ struct Moments {
 };
 // partial[sample][chunk][channel].  A thread sums differences from the mean of its first cells, which keeps 32 bits enough
 // where a channel's mean is far from zero; threads are joined in 64 bits.
-template <typename T>
+template <typename T, int F>
 __global__ __launch_bounds__(kThreads) void group_sums(const T *x, Moments *partial, const Cells s) {
   __shared__ Moments shares[kThreads][8];
-  const Place p = place_of(s);
+  const Place p = place_of(s, blockIdx.x);
   float middle[8] = {}, sum[8] = {}, squares[8] = {};
-  const long mine = p.live && p.first < p.last ? (p.last - p.first + p.step - 1) / p.step : 0;
-  if (mine) {
-    constexpr int kFirst = 4;
-    float v[kFirst][8];
-    const T *const at = x + p.base + p.c;
-    const int few = static_cast<int>(min(mine, static_cast<long>(kFirst)));
+  const T *at = x + p.at;
+  for (long done = 0; done < p.cells; done += kAtOnce, at += kAtOnce * p.stride) {
+    Eight<T, F> raw[kAtOnce];
+    load_cells(raw, at, p.cells - done, p);
+    if (done == 0) {
 #pragma unroll
-    for (int i = 0; i < kFirst; ++i) load8(at + (p.first + min(i, few - 1) * p.step) * s.channels, p.left, v[i]);
+      for (int n = 0; n < kAtOnce; ++n) {
+        float v[8];
+        raw[n].values(v);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) middle[i] = ((v[0][i] + v[1][i]) + (v[2][i] + v[3][i])) * 0.25f;
-#pragma unroll
-    for (int n = 0; n < kFirst; ++n)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float d = n < few ? v[n][i] - middle[i] : 0.f;
-        sum[i] += d;
-        squares[i] = fmaf(d, d, squares[i]);
+        for (int i = 0; i < 8; ++i) middle[i] = fmaf(v[i], 1.f / kAtOnce, middle[i]);
       }
-#pragma unroll 4
-    for (long r = p.first + kFirst * p.step; r < p.last; r += p.step) {
-      float u[8];
-      load8(at + r * s.channels, p.left, u);
+    }
+#pragma unroll
+    for (int n = 0; n < kAtOnce; ++n) {
+      if (done + n >= p.cells) break;
+      float v[8];
+      raw[n].values(v);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float d = u[i] - middle[i];
+        const float d = v[i] - middle[i];
         sum[i] += d;
         squares[i] = fmaf(d, d, squares[i]);
       }
     }
-    const float each = 1.f / static_cast<float>(mine);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float off = sum[i] * each;
-      squares[i] = fmaxf(fmaf(-sum[i], off, squares[i]), 0.f) + (squares[i] - squares[i]);   // (NaN stays)
-      sum[i] = off;
-    }
   }
+  const float each = p.cells ? 1.f / static_cast<float>(p.cells) : 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) shares[threadIdx.x][i] = {middle[i], sum[i], squares[i]};
-  __syncthreads();
-  // a channel of the tile each: the rows' shares
-  for (int k = threadIdx.x; k < s.tile_threads * 8; k += kThreads) {
-    const int c = blockIdx.y * kThreads * 8 + k;
-    if (c >= s.channels) continue;
-    const long begin = blockIdx.x * s.each, all = min(s.cells, begin + s.each) - begin;
-    double total = 0., rest = 0.;
-    for (int r = 0; r < s.tile_rows; ++r) {
-      const long n = r < all ? (all - r + s.tile_rows - 1) / s.tile_rows : 0;
-      const Moments share = shares[r * s.tile_threads + k / 8][k % 8];
-      const double mean = static_cast<double>(share.mean) + share.rest;
-      if (n) total += mean * n, rest += share.squares + mean * mean * n;
-    }
-    const double mean = total / all;
-    const float high = static_cast<float>(mean);
-    partial[(static_cast<long>(blockIdx.z) * s.chunks + blockIdx.x) * s.channels + c] = {high, static_cast<float>(mean - high), static_cast<float>(rest - total * mean)};
+  for (int i = 0; i < 8; ++i) {
+    const float off = sum[i] * each;
+    shares[threadIdx.x][i] = {middle[i], off, fmaxf(fmaf(-sum[i], off, squares[i]), 0.f) + (squares[i] - squares[i])};   // (NaN stays)
   }
-}
-
-__device__ __forceinline__ double block_sum(double v, double *lds) {
-#pragma unroll
-  for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
-  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
   __syncthreads();
-  v = 0.;
-#pragma unroll
-  for (int i = 0; i < kThreads / 64; ++i) v += lds[i];
-  __syncthreads();
-  return v;
-}
-
-// A group of a sample: stats[0], [1], [2] = mean, what rounding took from it, r.
-__global__ __launch_bounds__(kThreads) void group_finish(const Moments *partial, float *stats, const Cells s, float eps, int batch) {
-  __shared__ double lds[kThreads / 64];
-  const unsigned id = linear_block();
-  if (id >= static_cast<unsigned>(batch) * s.groups) return;
-  const int b = id / s.groups, g = id % s.groups;
-  const Moments *const from = partial + static_cast<long>(b) * s.chunks * s.channels + static_cast<long>(g) * s.group_channels;
-  double total = 0., rest = 0.;
-  for (long k = threadIdx.x; k < static_cast<long>(s.chunks) * s.group_channels; k += kThreads) {
-    const long chunk = k / s.group_channels, c = k % s.group_channels;
-    const double n = static_cast<double>(min(s.cells, (chunk + 1) * s.each) - chunk * s.each);
-    const Moments share = from[chunk * s.channels + c];
+  join_rows<double2>(s, [&](int r, int o, int i, double2 &all) {
+    const long begin = blockIdx.x * s.each, cells = min(s.cells, begin + s.each) - begin;
+    const long n = r < cells ? (cells - r + s.tile_rows - 1) / s.tile_rows : 0;
+    const Moments share = shares[r * s.tile_threads + o][i];
     const double mean = static_cast<double>(share.mean) + share.rest;
-    total += n * mean;
-    rest += share.squares + n * mean * mean;
-  }
-  total = block_sum(total, lds);
-  rest = block_sum(rest, lds);
-  if (threadIdx.x) return;
-  const double all = static_cast<double>(s.cells) * s.group_channels, mean = total / all;
-  const double left = rest / all - mean * mean, var = left < 0. ? 0. : left;   // (NaN stays)
-  const long at = id, every = static_cast<long>(batch) * s.groups;
+    if (n) all.x += mean * n, all.y += share.squares + mean * mean * n;
+  }, [&](int c, const double2 &all) {
+    const long begin = blockIdx.x * s.each;
+    const double mean = all.x / static_cast<double>(min(s.cells, begin + s.each) - begin);
+    const float high = static_cast<float>(mean);
+    partial[(static_cast<long>(blockIdx.z) * s.chunks + blockIdx.x) * s.channels + c] = {high, static_cast<float>(mean - high), static_cast<float>(all.y - all.x * mean)};
+  });
+}
+
+// Two sums over the workgroup, the same for every thread
+__device__ __forceinline__ void block_sums(double &a, double &b) {
+  __shared__ double lds[2][kThreads / 64];
+#pragma unroll
+  for (int d = 32; d; d >>= 1) a += __shfl_xor(a, d), b += __shfl_xor(b, d);
+  if ((threadIdx.x & 63) == 0) lds[0][threadIdx.x >> 6] = a, lds[1][threadIdx.x >> 6] = b;
+  __syncthreads();
+  a = b = 0.;
+#pragma unroll
+  for (int i = 0; i < kThreads / 64; ++i) a += lds[0][i], b += lds[1][i];
+  __syncthreads();
+}
+
+// A group's mean in two parts and r, from sums over `all` values
+__device__ __forceinline__ void put_stats(float *stats, long at, long every, double total, double rest, double all, float eps) {
+  const double mean = total / all, left = rest / all - mean * mean, var = left < 0. ? 0. : left;   // (NaN stays)
   stats[at] = static_cast<float>(mean);
   stats[every + at] = static_cast<float>(mean - static_cast<float>(mean));
   stats[2 * every + at] = static_cast<float>(1. / sqrt(var + eps));
 }
 
+// A group of a sample: stats[0], [1], [2] = mean, what rounding took from it, r.
+__global__ __launch_bounds__(kThreads) void group_finish(const Moments *partial, float *stats, const Cells s, float eps, int batch) {
+  const unsigned id = linear_block();
+  if (id >= static_cast<unsigned>(batch) * s.groups) return;
+  const int b = id / s.groups, g = id % s.groups;
+  const Moments *const from = partial + static_cast<long>(b) * s.chunks * s.channels + static_cast<long>(g) * s.group_channels;
+  double total = 0., rest = 0.;
+  const int across = min(s.group_channels, kThreads), rows = kThreads / across, row = threadIdx.x / across;
+  const int chunks = row < rows ? s.chunks : 0;
+  for (int c = threadIdx.x % across; c < s.group_channels; c += across)
+    for (int first = row; first < chunks; first += kAtOnce * rows) {
+      Moments share[kAtOnce];
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) share[i] = from[static_cast<long>(min(first + i * rows, chunks - 1)) * s.channels + c];
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) {
+        const long chunk = first + i * rows;
+        const double n = chunk < chunks ? static_cast<double>(min(s.cells, (chunk + 1) * s.each) - chunk * s.each) : 0.;
+        const double mean = static_cast<double>(share[i].mean) + share[i].rest;
+        total += n * mean;
+        rest += (chunk < chunks ? share[i].squares : 0.) + n * mean * mean;
+      }
+    }
+  block_sums(total, rest);
+  if (threadIdx.x == 0) put_stats(stats, id, static_cast<long>(batch) * s.groups, total, rest, static_cast<double>(s.cells) * s.group_channels, eps);
+}
+
 template <typename T> __device__ __forceinline__ float vector_at(const void *w, bool wide, int c, float absent) {
   return !w ? absent : wide ? static_cast<const float *>(w)[c] : load(static_cast<const T *>(w) + c);
 }
+
+template <typename T>
+__device__ __forceinline__ void load_vector(float (&to)[8], const void *w, bool wide, const Place &p, float absent) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) to[i] = absent;
+  if (!w) return;
+  if (wide) load8(static_cast<const float *>(w) + p.c, p.left, to);
+  else load8(static_cast<const T *>(w) + p.c, p.left, to);
+}
+
+// A straight line x a + c in 32 bits, c = shift - mean a in two parts for the a that is used: exact where x is near the mean, however far
+// that is from zero.
+struct Line {
+  float a, high, low;
+  __device__ __forceinline__ void set(float mean, float rest, float by, double shift) {
+    a = by;
+    const double c = shift - (static_cast<double>(mean) + rest) * by;
+    high = static_cast<float>(c), low = static_cast<float>(c - high);
+  }
+  __device__ __forceinline__ float at(float x) const { return fmaf(x, a, high) + low; }
+};
 
 // What the channels of a thread need
 struct Channels {
@@ -168,103 +251,128 @@ __device__ __forceinline__ void load_channels(Channels &t, const Place &p, const
   const long every = static_cast<long>(gridDim.z) * s.groups, first = static_cast<long>(blockIdx.z) * s.groups;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const int c = min(p.c + i, s.channels - 1);
-    const long at = first + c / s.group_channels;
+    const long at = first + static_cast<unsigned>(min(p.c + i, s.channels - 1)) / static_cast<unsigned>(s.group_channels);
     t.mean[i] = stats[at], t.rest[i] = stats[every + at], t.r[i] = stats[2 * every + at];
-    t.w[i] = vector_at<T>(weight, wide, c, 1.f), t.b[i] = vector_at<T>(bias, wide, c, 0.f);
   }
+  load_vector<T>(t.w, weight, wide, p, 1.f);
+  load_vector<T>(t.b, bias, wide, p, 0.f);
 }
 
-template <typename T, int Kind>
+template <typename T, int Kind, int F>
 __global__ __launch_bounds__(kThreads) void group_apply(const T *x, const float *stats, const void *weight, const void *bias, bool wide, T *y,
                                                         const Cells s, float low) {
-  const Place p = place_of(s);
-  if (!p.live) return;
+  const Place p = place_of(s, blockIdx.x);
+  if (!p.cells) return;
   Channels t;
   load_channels<T>(t, p, stats, weight, bias, wide, s);
-#pragma unroll 4
-  for (long r = p.first; r < p.last; r += p.step) {
-    const long at = p.base + r * s.channels + p.c;
-    float v[8];
-    load8(x + at, p.left, v);
+  Line z[8];   // h w + b
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = Activation<Kind>::value(fmaf(((v[i] - t.mean[i]) - t.rest[i]) * t.r[i], t.w[i], t.b[i]), low);
-    store8(y + at, p.left, v);
+  for (int i = 0; i < 8; ++i) z[i].set(t.mean[i], t.rest[i], t.r[i] * t.w[i], t.b[i]);
+  const T *from = x + p.at;
+  T *to = y + p.at;
+  for (long done = 0; done < p.cells; done += kAtOnce, from += kAtOnce * p.stride, to += kAtOnce * p.stride) {
+    Eight<T, F> raw[kAtOnce];
+    load_cells(raw, from, p.cells - done, p);
+#pragma unroll
+    for (int n = 0; n < kAtOnce; ++n) {
+      if (done + n >= p.cells) break;
+      float v[8];
+      raw[n].values(v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = Activation<Kind>::value(z[i].at(v[i]), low);
+      put_eight<T, F>(to + n * p.stride, p.left, v);
+    }
   }
 }
 
 // ---- gradients ------------------------------------------------------------------------------------------------------
 // Sums of gz and gz h of each channel over a chunk's cells
-template <typename T, int Kind>
+template <typename T, int Kind, int F>
 __global__ __launch_bounds__(kThreads) void group_grad_sums(const T *x, const T *gy, const float *stats, const void *weight, const void *bias,
                                                             bool wide, float2 *partial, const Cells s, float low) {
   __shared__ float2 shares[kThreads][8 + 1];
-  const Place p = place_of(s);
+  const Place p = place_of(s, blockIdx.x);
   float sum[8] = {}, dot[8] = {};
-  if (p.live) {
+  if (p.cells) {
     Channels t;
     load_channels<T>(t, p, stats, weight, bias, wide, s);
-#pragma unroll 4
-    for (long r = p.first; r < p.last; r += p.step) {
-      const long at = p.base + r * s.channels + p.c;
-      float v[8], g[8];
-      load8(x + at, p.left, v);
-      load8(gy + at, p.left, g);
+    Line hs[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float h = ((v[i] - t.mean[i]) - t.rest[i]) * t.r[i], gz = g[i] * Activation<Kind>::slope(fmaf(h, t.w[i], t.b[i]), low);
-        sum[i] += gz;
-        dot[i] = fmaf(gz, h, dot[i]);
+    for (int i = 0; i < 8; ++i) hs[i].set(t.mean[i], t.rest[i], t.r[i], 0.);
+    const T *at = x + p.at, *gat = gy + p.at;
+    for (long done = 0; done < p.cells; done += kAtOnce, at += kAtOnce * p.stride, gat += kAtOnce * p.stride) {
+      Eight<T, F> raw[kAtOnce], graw[kAtOnce];
+      load_cells(raw, at, p.cells - done, p);
+      load_cells(graw, gat, p.cells - done, p);
+#pragma unroll
+      for (int n = 0; n < kAtOnce; ++n) {
+        if (done + n >= p.cells) break;
+        float v[8], g[8];
+        raw[n].values(v);
+        graw[n].values(g);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float h = hs[i].at(v[i]), gz = g[i] * Activation<Kind>::slope(fmaf(h, t.w[i], t.b[i]), low);
+          sum[i] += gz;
+          dot[i] = fmaf(gz, h, dot[i]);
+        }
       }
     }
   }
 #pragma unroll
   for (int i = 0; i < 8; ++i) shares[threadIdx.x][i] = {sum[i], dot[i]};
   __syncthreads();
-  for (int k = threadIdx.x; k < s.tile_threads * 8; k += kThreads) {
-    const int c = blockIdx.y * kThreads * 8 + k;
-    if (c >= s.channels) continue;
-    float2 all = {0.f, 0.f};
-    for (int r = 0; r < s.tile_rows; ++r) {
-      const float2 share = shares[r * s.tile_threads + k / 8][k % 8];
-      all.x += share.x, all.y += share.y;
-    }
-    partial[(static_cast<long>(blockIdx.z) * s.chunks + blockIdx.x) * s.channels + c] = all;
-  }
+  join_rows<float2>(s, [&](int r, int o, int i, float2 &all) {
+    const float2 share = shares[r * s.tile_threads + o][i];
+    all.x += share.x, all.y += share.y;
+  }, [&](int c, const float2 &all) { partial[(static_cast<long>(blockIdx.z) * s.chunks + blockIdx.x) * s.channels + c] = all; });
 }
 
 // A group of a sample: means[0], [1] = mean(w gz), mean(w gz h); the channels' sums over all chunks take the first one's place.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void group_grad_finish(float2 *partial, float *means, const void *weight, bool wide, const Cells s, int batch) {
-  __shared__ double lds[kThreads / 64];
+  __shared__ double2 shares[kThreads];
   const unsigned id = linear_block();
   if (id >= static_cast<unsigned>(batch) * s.groups) return;
   const int b = id / s.groups, g = id % s.groups;
   float2 *const from = partial + static_cast<long>(b) * s.chunks * s.channels + static_cast<long>(g) * s.group_channels;
   double sum = 0., dot = 0.;
-  for (int c = 0; c < s.group_channels; ++c) {
+  const int across = min(s.group_channels, kThreads), rows = kThreads / across, in = threadIdx.x % across, row = threadIdx.x / across;
+  for (int first = 0; first < s.group_channels; first += across) {   // (as many channels at a time as there are threads)
+    const int c = first + in;
     double one = 0., two = 0.;
-    for (long chunk = threadIdx.x; chunk < s.chunks; chunk += kThreads) {
-      const float2 share = from[chunk * s.channels + c];
-      one += share.x, two += share.y;
+    if (c < s.group_channels && row < rows) {
+      for (int chunk = row; chunk < s.chunks; chunk += kAtOnce * rows) {
+        float2 share[kAtOnce];
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) share[i] = from[static_cast<long>(min(chunk + i * rows, s.chunks - 1)) * s.channels + c];
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i)
+          if (chunk + i * rows < s.chunks) one += share[i].x, two += share[i].y;
+      }
     }
-    one = block_sum(one, lds);
-    two = block_sum(two, lds);
-    if (threadIdx.x == 0) from[c] = {static_cast<float>(one), static_cast<float>(two)};
-    const double w = vector_at<T>(weight, wide, g * s.group_channels + c, 1.f);
-    sum += w * one, dot += w * two;
+    shares[threadIdx.x] = {one, two};
+    __syncthreads();
+    if (row == 0 && c < s.group_channels) {
+      for (int r = 1; r < rows; ++r) one += shares[r * across + in].x, two += shares[r * across + in].y;
+      from[c] = {static_cast<float>(one), static_cast<float>(two)};
+      const double w = vector_at<T>(weight, wide, g * s.group_channels + c, 1.f);
+      sum += w * one, dot += w * two;
+    }
+    __syncthreads();
   }
+  block_sums(sum, dot);
   if (threadIdx.x) return;
   const double all = static_cast<double>(s.cells) * s.group_channels;
   means[id] = static_cast<float>(sum / all);
   means[static_cast<long>(batch) * s.groups + id] = static_cast<float>(dot / all);
 }
 
-template <typename T, int Kind>
+template <typename T, int Kind, int F>
 __global__ __launch_bounds__(kThreads) void group_grad_apply(const T *x, const T *gy, const float *stats, const float *means, const void *weight,
                                                              const void *bias, bool wide, T *gx, const Cells s, float low) {
-  const Place p = place_of(s);
-  if (!p.live) return;
+  const Place p = place_of(s, blockIdx.x);
+  if (!p.cells) return;
   Channels t;
   load_channels<T>(t, p, stats, weight, bias, wide, s);
   float one[8], two[8];
@@ -273,18 +381,28 @@ __global__ __launch_bounds__(kThreads) void group_grad_apply(const T *x, const T
     const long at = static_cast<long>(blockIdx.z) * s.groups + min(p.c + i, s.channels - 1) / s.group_channels;
     one[i] = means[at], two[i] = means[static_cast<long>(gridDim.z) * s.groups + at];
   }
-#pragma unroll 2
-  for (long r = p.first; r < p.last; r += p.step) {
-    const long at = p.base + r * s.channels + p.c;
-    float v[8], g[8];
-    load8(x + at, p.left, v);
-    load8(gy + at, p.left, g);
+  Line hs[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float h = ((v[i] - t.mean[i]) - t.rest[i]) * t.r[i], gz = g[i] * Activation<Kind>::slope(fmaf(h, t.w[i], t.b[i]), low);
-      v[i] = t.r[i] * (fmaf(gz, t.w[i], -one[i]) - h * two[i]);
+  for (int i = 0; i < 8; ++i) hs[i].set(t.mean[i], t.rest[i], t.r[i], 0.);
+  const T *at = x + p.at, *gat = gy + p.at;
+  T *to = gx + p.at;
+  for (long done = 0; done < p.cells; done += kAtOnce, at += kAtOnce * p.stride, gat += kAtOnce * p.stride, to += kAtOnce * p.stride) {
+    Eight<T, F> raw[kAtOnce], graw[kAtOnce];
+    load_cells(raw, at, p.cells - done, p);
+    load_cells(graw, gat, p.cells - done, p);
+#pragma unroll
+    for (int n = 0; n < kAtOnce; ++n) {
+      if (done + n >= p.cells) break;
+      float v[8], g[8];
+      raw[n].values(v);
+      graw[n].values(g);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float h = hs[i].at(v[i]), gz = g[i] * Activation<Kind>::slope(fmaf(h, t.w[i], t.b[i]), low);
+        v[i] = t.r[i] * (fmaf(gz, t.w[i], -one[i]) - h * two[i]);
+      }
+      put_eight<T, F>(to + n * p.stride, p.left, v);
     }
-    store8(gx + at, p.left, v);
   }
 }
 
@@ -294,6 +412,7 @@ __global__ __launch_bounds__(kThreads) void group_grad_vectors(const float2 *par
   const int c = blockIdx.x * kThreads + threadIdx.x;
   if (c >= s.channels) return;
   double sum = 0., dot = 0.;
+#pragma unroll 4
   for (int b = 0; b < batch; ++b) {
     const float2 share = partial[static_cast<long>(b) * s.chunks * s.channels + c];
     sum += share.x, dot += share.y;
@@ -308,19 +427,28 @@ __global__ __launch_bounds__(kThreads) void group_grad_vectors(const float2 *par
 }
 
 // ---- launches -------------------------------------------------------------------------------------------------------
+constexpr long kGroups = 1024;   // workgroups of a launch, about
 Cells cells_of(int batch, long cells, int channels, int groups) {
   Cells s{};
   s.cells = cells, s.channels = channels, s.groups = groups, s.group_channels = channels / groups;
   const int octets = (channels + 7) / 8, tiles = (octets + kThreads - 1) / kThreads;
   s.tile_threads = std::min(octets, kThreads), s.tile_rows = kThreads / s.tile_threads;
-  // about eight workgroups per compute unit, of eight cells a thread at least
-  const long most = std::max(1L, 2048L / std::max(1L, static_cast<long>(batch) * tiles)), rows = 8L * s.tile_rows;
+  // about four workgroups per compute unit, of four cells a thread at least
+  const long most = std::max(1L, kGroups / std::max(1L, static_cast<long>(batch) * tiles)), rows = static_cast<long>(kAtOnce) * s.tile_rows;
   s.each = std::max(rows, (cells + most - 1) / most);
   s.each = (s.each + s.tile_rows - 1) / s.tile_rows * s.tile_rows;
   s.chunks = static_cast<int>(std::max(1L, (cells + s.each - 1) / s.each));
   return s;
 }
 int tiles_of(const Cells &s) { return ((s.channels + 7) / 8 + kThreads - 1) / kThreads; }
+
+// Calls f with the form of the kernels that write `bytes`, as a constant
+constexpr size_t kCached = 128 << 20;
+template <typename F> void for_form(const Cells &s, size_t bytes, const F &f) {
+  if (s.channels < 8) f(std::integral_constant<int, kParts>());
+  else if (bytes <= kCached) f(std::integral_constant<int, kWhole>());
+  else f(std::integral_constant<int, kWholePast>());
+}
 
 int arguments(int batch, long cells, int channels, int groups, int activation, int dtype, int weight_dtype) {
   MV_REQUIRE(dtype == MV_F32 || dtype == MV_F16 || dtype == MV_BF16, "dtype %d is not float32, float16 or bfloat16", dtype);
@@ -355,16 +483,19 @@ int mv_group_norm(const void *x, const void *weight, const void *bias, void *y, 
   MV_REQUIRE(workspace && workspace_bytes >= mv_group_norm_workspace_bytes(batch, cells, channels, groups), "the workspace is too small");
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const Cells s = cells_of(batch, cells, channels, groups);
+  const size_t bytes = dtype_size(dtype) * batch * cells * channels;
   const dim3 grid(s.chunks, tiles_of(s), batch);
   const bool wide = weight_dtype == MV_F32;
   auto *const partial = static_cast<Moments *>(workspace);
   auto *const stat = static_cast<float *>(stats);
+  if (const WholePlan whole = whole_plan(cells, channels, groups, false); whole.u)
+    return group_norm_whole(whole, x, weight, bias, wide, y, stat, batch, eps, activation, low, dtype, st);
   MV_FLOATS(dtype, {
     const T *const xt = static_cast<const T *>(x);
-    group_sums<T><<<grid, kThreads, 0, st>>>(xt, partial, s);
+    for_form(s, 0, [&](auto form) { group_sums<T, form><<<grid, kThreads, 0, st>>>(xt, partial, s); });
     group_finish<<<linear_grid(static_cast<long>(batch) * groups, kThreads), kThreads, 0, st>>>(partial, stat, s, eps, batch);
     for_activation(activation, [&](auto kind) {
-      group_apply<T, kind><<<grid, kThreads, 0, st>>>(xt, stat, weight, bias, wide, static_cast<T *>(y), s, low);
+      for_form(s, bytes, [&](auto form) { group_apply<T, kind, form><<<grid, kThreads, 0, st>>>(xt, stat, weight, bias, wide, static_cast<T *>(y), s, low); });
     });
   })
   return check_launch("group_norm");
@@ -383,6 +514,7 @@ int mv_group_norm_backward(const void *x, const void *weight, const void *bias, 
   if ((empty || !grad_x) && !grad_weight && !grad_bias) return MV_OK;
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const Cells s = cells_of(batch, cells, channels, groups);
+  const size_t bytes = dtype_size(dtype) * batch * cells * channels;
   const bool wide = weight_dtype == MV_F32;
   MV_REQUIRE(empty || (x && stats && grad_y), "a tensor is missing");
   MV_REQUIRE(empty || (workspace && workspace_bytes >= mv_group_norm_backward_workspace_bytes(batch, cells, channels, groups)), "the workspace is too small");
@@ -390,20 +522,30 @@ int mv_group_norm_backward(const void *x, const void *weight, const void *bias, 
   auto *const partial = static_cast<float2 *>(workspace);
   auto *const means = reinterpret_cast<float *>(static_cast<char *>(workspace) + (empty ? 0 : partial_bytes<float2>(batch, s)));
   auto *const stat = static_cast<const float *>(stats);
+  Cells sum = s;   // where the channels' sums stand
+  const WholePlan whole = empty ? WholePlan{} : whole_plan(cells, channels, groups, true);
+  if (whole.u) {
+    sum.chunks = 1;
+    if (const int status = group_norm_whole_backward(whole, x, grad_y, stat, weight, bias, wide, grad_x, grad_weight || grad_bias ? partial : nullptr, batch,
+                                                     activation, low, dtype, st))
+      return status;
+  }
   MV_FLOATS(dtype, {
     const T *const xt = static_cast<const T *>(x), *const gy = static_cast<const T *>(grad_y);
-    if (!empty) {
+    if (!empty && !whole.u) {
       for_activation(activation, [&](auto kind) {
-        group_grad_sums<T, kind><<<grid, kThreads, 0, st>>>(xt, gy, stat, weight, bias, wide, partial, s, low);
+        for_form(s, 0, [&](auto form) { group_grad_sums<T, kind, form><<<grid, kThreads, 0, st>>>(xt, gy, stat, weight, bias, wide, partial, s, low); });
       });
       group_grad_finish<T><<<linear_grid(static_cast<long>(batch) * groups, kThreads), kThreads, 0, st>>>(partial, means, weight, wide, s, batch);
       if (grad_x)
         for_activation(activation, [&](auto kind) {
-          group_grad_apply<T, kind><<<grid, kThreads, 0, st>>>(xt, gy, stat, means, weight, bias, wide, static_cast<T *>(grad_x), s, low);
+          for_form(s, bytes, [&](auto form) {
+            group_grad_apply<T, kind, form><<<grid, kThreads, 0, st>>>(xt, gy, stat, means, weight, bias, wide, static_cast<T *>(grad_x), s, low);
+          });
         });
     }
     if (grad_weight || grad_bias)
-      group_grad_vectors<T><<<(channels + kThreads - 1) / kThreads, kThreads, 0, st>>>(partial, grad_weight, grad_bias, wide, s, empty ? 0 : batch);
+      group_grad_vectors<T><<<(channels + kThreads - 1) / kThreads, kThreads, 0, st>>>(partial, grad_weight, grad_bias, wide, sum, empty ? 0 : batch);
   })
   return check_launch("group_norm backward");
 }

@@ -62,24 +62,6 @@ template <typename T, int N> __device__ __forceinline__ void copy_unit(const T *
     reinterpret_cast<Loose<bytes, sizeof(T)> *>(reinterpret_cast<char *>(to) + i)->v = reinterpret_cast<const Loose<bytes, sizeof(T)> *>(reinterpret_cast<const char *>(from) + i)->v;
 }
 
-// Eight elements as they are in memory
-template <typename T> struct Raw {
-  u32x4 bits[sizeof(T) / 2];
-  __device__ __forceinline__ void load(const T *p) {
-#pragma unroll
-    for (unsigned i = 0; i < sizeof(T) / 2; ++i) bits[i] = reinterpret_cast<const Loose<u32x4, sizeof(T)> *>(p)[i].v;
-  }
-  __device__ __forceinline__ void values(float (&v)[8]) const {
-    if constexpr (sizeof(T) == 4) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(bits[i / 4][i % 4]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = Bits<T>::up(static_cast<unsigned short>(bits[0][i / 2] >> (i % 2 * 16)));
-    }
-  }
-};
-
 // Cosines and sines of a workgroup's rows
 __device__ __forceinline__ void form_table(float2 *table, const void *places, int place_kind, const double *frequencies, const Rotary &k, int b, int first,
                                            int rows, bool back) {

@@ -94,6 +94,33 @@ template <> __device__ __forceinline__ void store8<float>(float *p, int left, co
     if (i < left) p[i] = v[i];
 }
 
+// Eight elements as they are in memory
+template <typename T> struct Raw {
+  u32x4 bits[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T *p) {
+#pragma unroll
+    for (unsigned i = 0; i < sizeof(T) / 2; ++i) bits[i] = reinterpret_cast<const Loose<u32x4, sizeof(T)> *>(p)[i].v;
+  }
+  __device__ __forceinline__ void values(float (&v)[8]) const {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(bits[i / 4][i % 4]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = Bits<T>::up(static_cast<unsigned short>(bits[0][i / 2] >> (i % 2 * 16)));
+    }
+  }
+  __device__ __forceinline__ void set(const float (&v)[8]) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) bits[i / 4][i % 4] = __float_as_uint(v[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) bits[0][i] = pack2<T>(v[2 * i], v[2 * i + 1]);
+    }
+  }
+};
+
 // ---- 8-bit blocks --------------------------------------------------------------------------------------
 constexpr int kBlock = 128;       // columns that share a scale
 constexpr float kE4m3Max = 448.f;
