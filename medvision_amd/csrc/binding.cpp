@@ -1140,7 +1140,7 @@ Tensor group_linear(const Tensor &x_in, const Tensor &weight_in, const Tensor &s
   MVB_CHECK(!bias_given.defined() || (bias_given.dim() == 1 && bias_given.size(0) == outputs), "bias has shape ",
             bias_given.defined() ? shape_text(bias_given.sizes()) : "", ", expected (", outputs, ")");
   const c10::DeviceGuard guard(x_in.device());
-  const Tensor x = x_in.contiguous(), w = aligned_rows(weight_in), scales = scales_in.contiguous();
+  const Tensor x = aligned_rows(x_in), w = aligned_rows(weight_in), scales = scales_in.contiguous();
   const Tensor bias = bias_given.defined() ? bias_given.to(x.scalar_type()).contiguous() : bias_given;
   const int64_t rows = x.numel() / inputs;
   std::vector<int64_t> shape = x.sizes().vec();

@@ -66,9 +66,141 @@ template <typename T> struct Product {
   T *y;
   float *part;   // [splits, rows, outputs], NULL: y
   long rows;
+  long stride;   // of x's rows, in elements
   int inputs, outputs, blocks, m_tiles, n_tiles, splits;
 };
 
+// ---- tiles ---------------------------------------------------------------------------------------------------------
+// A workgroup takes BM rows and BN outputs, each of its WM x WN wavefronts 64 x 64 of them.  Rows and weights of a block of 128
+// columns go through LDS, without registers on the way (x: rows in whole pieces of 16 bytes), the next block's while this one is multiplied;
+// scales go to the lanes that want them.  A row of x is 256 bytes there, sixteen pieces, piece c of row r at c ^ (r & 7); a row of weights four, piece g
+// of row r at g ^ (r / 2 & 3): reads of 16 rows side by side spread over all banks.
+// Outputs are the wider side of a tile: their bytes are a quarter of the rows'.
+template <int BM, int BN> struct Tile {
+  static constexpr int kWaves = BM / 64 * (BN / 64), kRows = BM * 256, kStage = kRows + BN * 64;
+};
+
+template <typename T, int Group, int BM, int BN>
+__global__ __launch_bounds__(BM / 64 * (BN / 64) * 64, 2) void product_tiles4(const Product<T> k) {
+  using S = Tile<BM, BN>;
+  constexpr int kScales = kBlock / Group, kThreads = 64 * S::kWaves;
+  __shared__ __attribute__((aligned(16))) unsigned char lds[2 * S::kStage];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, g = lane >> 4;
+  const int wm = wave % (BM / 64), wn = wave / (BM / 64);
+  // tiles in an order in which neighbouring workgroups of a die share rows and weights: eight rows of tiles at a time
+  const int tiles = k.m_tiles * k.n_tiles;
+  unsigned id = linear_block();
+  if (id >= static_cast<unsigned>(tiles) * k.splits) return;
+  const int split = id / tiles;
+  id = xcd_contiguous(id % tiles, tiles);
+  const int band = id / (8 * k.n_tiles), in_band = id % (8 * k.n_tiles), tall = min(8, k.m_tiles - 8 * band);
+  const long m0 = (8L * band + in_band % tall) * BM;
+  const int n0 = in_band / tall * BN;
+  const int first = static_cast<int>(static_cast<long>(k.blocks) * split / k.splits), last = static_cast<int>(static_cast<long>(k.blocks) * (split + 1) / k.splits);
+
+  // What a thread brings of a block: pieces of 16 bytes, in the order in which they stand in LDS
+  constexpr int kPiecesX = BM * 16 / kThreads, kPiecesW = BN * 4 / kThreads;
+  static_assert(BM * 16 % kThreads == 0 && BN * 4 % kThreads == 0, "");
+  const T *x_from[kPiecesX];
+  int x_column[kPiecesX];
+  const unsigned char *w_from[kPiecesW];
+#pragma unroll
+  for (int i = 0; i < kPiecesX; ++i) {
+    const int at = i * kThreads + threadIdx.x, row = at / 16;
+    x_column[i] = ((at % 16) ^ (row & 7)) * 8;
+    x_from[i] = k.x + min(m0 + row, k.rows - 1) * k.stride + x_column[i];
+  }
+#pragma unroll
+  for (int i = 0; i < kPiecesW; ++i) {
+    const int at = i * kThreads + threadIdx.x, row = at / 4;
+    w_from[i] = k.w + static_cast<long>(min(n0 + row, k.outputs - 1)) * k.blocks * 64 + ((at % 4) ^ (row / 2 & 3)) * 16;
+  }
+  const float *s_from[4];
+#pragma unroll
+  for (int u = 0; u < 4; ++u) s_from[u] = k.scales + static_cast<long>(min(n0 + wn * 64 + u * 16 + r16, k.outputs - 1)) * k.blocks * kScales;
+
+  float scale[4][kScales];
+  auto bring = [&](int b) {
+    unsigned char *const to = lds + (b & 1) * S::kStage + wave * 1024;
+#pragma unroll
+    for (int i = 0; i < kPiecesX; ++i) {   // (of a piece behind the row's end: the row's first one, which zeros take the place of)
+      const T *const from = b * kBlock + x_column[i] < k.inputs ? x_from[i] + b * kBlock : x_from[i] - x_column[i];
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)from,
+                                       (__attribute__((address_space(3))) void *)(to + i * kThreads * 16), 16, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < kPiecesW; ++i)
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(w_from[i] + b * 64L),
+                                       (__attribute__((address_space(3))) void *)(to + S::kRows + i * kThreads * 16), 16, 0, 0);
+  };
+  f32x4 acc[4][4] = {};
+  bring(first);
+  for (int b = first; b < last; ++b) {
+    __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0): what this wavefront brought has arrived (a barrier alone does not promise that)
+    __syncthreads();   // this block's operands are there, and nobody reads the place of the next ones
+    unsigned char *const here = lds + (b & 1) * S::kStage;
+    if ((b + 1) * kBlock > k.inputs) {   // the columns behind the rows' ends
+#pragma unroll
+      for (int i = 0; i < kPiecesX; ++i)
+        if (b * kBlock + x_column[i] >= k.inputs) *reinterpret_cast<u32x4 *>(here + (i * kThreads + threadIdx.x) * 16) = u32x4{0u, 0u, 0u, 0u};
+      __syncthreads();
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int i = 0; i < kScales; ++i) scale[u][i] = s_from[u][b * kScales + i];
+    if (b + 1 < last) bring(b + 1);
+    u32x4 x[4][4], w[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int row = wn * 64 + u * 16 + r16;
+      w[u] = *reinterpret_cast<const u32x4 *>(here + S::kRows + row * 64 + (g ^ (row / 2 & 3)) * 16);
+    }
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = wm * 64 + t * 16 + r16;
+        x[t][i] = *reinterpret_cast<const u32x4 *>(here + row * 256 + ((4 * i + g) ^ (row & 7)) * 16);
+      }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      f32x4 d[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const u32x4 v = Matrix<T>::values(w[u][i]);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          if (i % (Group / 32) == 0) d[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+          d[t] = Matrix<T>::product(x[t][i], v, d[t]);
+        }
+        if ((i + 1) % (Group / 32) == 0) {
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[t][u][j] = fmaf(d[t][j], scale[u][i / (Group / 32)], acc[t][u][j]);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const int n = n0 + wn * 64 + u * 16 + r16;
+    if (n >= k.outputs) continue;
+    const float add = k.bias && !k.part ? load(k.bias + n) : 0.f;
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const long m = m0 + wm * 64 + t * 16 + 4 * g + j;
+        if (m >= k.rows) continue;
+        if (k.part) k.part[(split * k.rows + m) * k.outputs + n] = acc[t][u][j];
+        else k.y[m * k.outputs + n] = store_cast<T>(acc[t][u][j] + add);
+      }
+  }
+}
+
+// ---- few rows -------------------------------------------------------------------------------------------------------
 // 64 outputs and 16 TM rows per workgroup, straight from memory into the operands' registers.  The four wavefronts take turns
 // at the blocks of the workgroup's share of the sum and join in LDS.
 template <typename T, int TM, int Group>
@@ -87,7 +219,7 @@ __global__ __launch_bounds__(256) void product_rows4(const Product<T> k) {
   const unsigned char *w_at[TN];
   const float *s_at[TN];
 #pragma unroll
-  for (int t = 0; t < TM; ++t) x_at[t] = k.x + min(m0 + t * 16 + r16, k.rows - 1) * k.inputs;
+  for (int t = 0; t < TM; ++t) x_at[t] = k.x + min(m0 + t * 16 + r16, k.rows - 1) * k.stride;
 #pragma unroll
   for (int u = 0; u < TN; ++u) {
     const long n = min(n0 + u * 16 + r16, k.outputs - 1);
@@ -184,32 +316,66 @@ __global__ __launch_bounds__(256) void quantize_groups(const T *w, unsigned *q, 
 }
 
 // ---- which kernel --------------------------------------------------------------------------------------------------
+enum Kind { kFew1, kFew2, kFew4, kTiles, kWideTiles };
 struct Plan {
-  int tm, m_tiles, n_tiles, splits;
+  int kind, m_tiles, n_tiles, splits;
 };
 
 int ceil_div(long a, long b) { return static_cast<int>((a + b - 1) / b); }
 
 Plan plan_of(long rows, int blocks, int outputs) {
-  const int tm = rows <= 16 ? 1 : rows <= 32 ? 2 : 4, n = ceil_div(outputs, 64), m = ceil_div(rows, 16 * tm);
-  return {tm, m, n, static_cast<int>(std::max(1L, std::min(blocks / 8L, 512 / (static_cast<long>(n) * m))))};
+  if (rows <= 64) {
+    const int kind = rows <= 16 ? kFew1 : rows <= 32 ? kFew2 : kFew4, n = ceil_div(outputs, 64);
+    return {kind, 1, n, std::max(1, std::min(blocks / 8, 512 / n))};
+  }
+  const int m = ceil_div(rows, 128), wide = ceil_div(outputs, 256), n = ceil_div(outputs, 128);
+  if (outputs > 128) return {kWideTiles, m, wide, static_cast<int>(std::max(1L, std::min(blocks / 8L, 256 / (static_cast<long>(m) * wide))))};
+  return {kTiles, m, n, static_cast<int>(std::max(1L, std::min(blocks / 8L, 512 / (static_cast<long>(m) * n))))};
 }
 
 template <typename T, int Group> void launch(const Plan &p, const Product<T> &k, hipStream_t s) {
-  const dim3 grid = linear_grid(static_cast<long>(p.m_tiles) * p.n_tiles * p.splits, 256);
-  if (p.tm == 1) product_rows4<T, 1, Group><<<grid, 256, 0, s>>>(k);
-  else if (p.tm == 2) product_rows4<T, 2, Group><<<grid, 256, 0, s>>>(k);
-  else product_rows4<T, 4, Group><<<grid, 256, 0, s>>>(k);
+  const long groups = static_cast<long>(p.m_tiles) * p.n_tiles * p.splits;
+  switch (p.kind) {
+    case kFew1: product_rows4<T, 1, Group><<<linear_grid(groups, 256), 256, 0, s>>>(k); break;
+    case kFew2: product_rows4<T, 2, Group><<<linear_grid(groups, 256), 256, 0, s>>>(k); break;
+    case kFew4: product_rows4<T, 4, Group><<<linear_grid(groups, 256), 256, 0, s>>>(k); break;
+    case kTiles: product_tiles4<T, Group, 128, 128><<<linear_grid(groups, 256), 256, 0, s>>>(k); break;
+    default: product_tiles4<T, Group, 128, 256><<<linear_grid(groups, 512), 512, 0, s>>>(k);
+  }
 }
+
+// Rows as tiles read them: with zeros up to whole blocks, 16-byte aligned.  A thread has eight columns.
+template <typename T> __global__ __launch_bounds__(256) void pad_rows(const T *x, u32x4 *to, long pieces, int inputs, int blocks) {
+  const long at = static_cast<long>(linear_block()) * 256 + threadIdx.x;
+  if (at >= pieces) return;
+  const long row = at / (blocks * 16L);
+  const int c = static_cast<int>(at - row * (blocks * 16L)) * 8;
+  to[at] = columns8(x + row * inputs + min(c, inputs - 1), inputs - c);
+}
+size_t padded_bytes(long rows, int blocks) { return static_cast<size_t>(rows) * blocks * kBlock * 2; }
+size_t part_bytes(const Plan &p, long rows, int outputs) { return p.splits > 1 ? sizeof(float) * p.splits * static_cast<size_t>(rows) * outputs : 0; }
 
 template <typename T>
 int product(const void *x, const void *w, const void *scales, const void *bias, void *y, long rows, int inputs, int outputs, int group,
             void *workspace, size_t workspace_bytes, hipStream_t s) {
   const int blocks = ceil_div(inputs, kBlock);
   Plan p = plan_of(rows, blocks, outputs);
-  if (p.splits > 1 && (!workspace || workspace_bytes < sizeof(float) * p.splits * static_cast<size_t>(rows) * outputs)) p.splits = 1;
-  const Product<T> k{static_cast<const T *>(x), static_cast<const unsigned char *>(w), static_cast<const float *>(scales), static_cast<const T *>(bias),
-                     static_cast<T *>(y), p.splits > 1 ? static_cast<float *>(workspace) : nullptr, rows, inputs, outputs, blocks, p.m_tiles, p.n_tiles, p.splits};
+  // Rows that tiles cannot read are copied first; where there is no room for that, they go straight to registers.
+  const bool tiles = p.kind == kTiles || p.kind == kWideTiles, odd = tiles && (inputs % 8 || reinterpret_cast<uintptr_t>(x) % 16);
+  const size_t pad = odd ? padded_bytes(rows, blocks) : 0;
+  if (!workspace) workspace_bytes = 0;
+  const bool pads = odd && pad <= workspace_bytes && reinterpret_cast<uintptr_t>(workspace) % 16 == 0;
+  if (odd && !pads) p = {kFew4, ceil_div(rows, 64), ceil_div(outputs, 64), 1};
+  const size_t at = pads ? pad : 0;
+  if (workspace_bytes - at < part_bytes(p, rows, outputs)) p.splits = 1;
+  Product<T> k{static_cast<const T *>(x), static_cast<const unsigned char *>(w), static_cast<const float *>(scales), static_cast<const T *>(bias),
+               static_cast<T *>(y), p.splits > 1 ? reinterpret_cast<float *>(static_cast<char *>(workspace) + at) : nullptr, rows, inputs, inputs, outputs, blocks,
+               p.m_tiles, p.n_tiles, p.splits};
+  if (pads) {
+    const long pieces = rows * blocks * 16;
+    pad_rows<<<linear_grid((pieces + 255) / 256, 256), 256, 0, s>>>(k.x, static_cast<u32x4 *>(workspace), pieces, inputs, blocks);
+    k.x = static_cast<const T *>(workspace), k.stride = static_cast<long>(blocks) * kBlock, k.inputs = blocks * kBlock;
+  }
   if (group == 32) launch<T, 32>(p, k, s);
   else if (group == 64) launch<T, 64>(p, k, s);
   else launch<T, 128>(p, k, s);
@@ -244,8 +410,9 @@ int mv_quantize_groups(const void *weight, void *q, void *scales, int64_t rows, 
 
 size_t mv_group_linear_workspace_bytes(int64_t rows, int inputs, int outputs) {
   if (rows <= 0 || inputs <= 0 || outputs <= 0) return 0;
-  const Plan p = plan_of(rows, ceil_div(inputs, kBlock), outputs);
-  return p.splits > 1 ? sizeof(float) * p.splits * static_cast<size_t>(rows) * outputs : 0;
+  const int blocks = ceil_div(inputs, kBlock);
+  const Plan p = plan_of(rows, blocks, outputs);
+  return part_bytes(p, rows, outputs) + ((p.kind == kTiles || p.kind == kWideTiles) && inputs % 8 ? padded_bytes(rows, blocks) : 0);
 }
 
 int mv_group_linear(const void *x, const void *weight, const void *scales, const void *bias, void *y, int64_t rows, int inputs, int outputs,
