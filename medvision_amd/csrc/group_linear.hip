@@ -19,6 +19,7 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 // Eight codes to 16 bits, two by two; their products with eight columns of 16 rows, added to `sum`
 template <typename T> struct Matrix;
@@ -71,22 +72,22 @@ template <typename T> struct Product {
 };
 
 // ---- tiles ---------------------------------------------------------------------------------------------------------
-// A workgroup takes BM rows and BN outputs, each of its WM x WN wavefronts 64 x 64 of them.  Rows and weights of a block of 128
-// columns go through LDS, without registers on the way (x: rows in whole pieces of 16 bytes), the next block's while this one is multiplied;
-// scales go to the lanes that want them.  A row of x is 256 bytes there, sixteen pieces, piece c of row r at c ^ (r & 7); a row of weights four, piece g
-// of row r at g ^ (r / 2 & 3): reads of 16 rows side by side spread over all banks.
-// Outputs are the wider side of a tile: their bytes are a quarter of the rows'.
-template <int BM, int BN> struct Tile {
-  static constexpr int kWaves = BM / 64 * (BN / 64), kRows = BM * 256, kStage = kRows + BN * 64;
-};
+// A workgroup takes 128 rows and 128 outputs, each of its 2 x 2 wavefronts 64 x 64 of them.  Rows and weights of a block of 128
+// columns go through LDS, without registers on the way (x: rows in whole pieces of 16 bytes), the next block's while this one is
+// multiplied; scales go to the lanes that want them.  A row of x is 256 bytes there, sixteen pieces, piece c of row r at c ^ (r & 15); a row of
+// weights four, piece g at g ^ turned(r): reads of 16 rows side by side spread over all banks.
+// 4000 x 4096 x 4096 in bf16 with groups of 128, 64, 32: 128, 141, 168 us = 1.05, 0.95, 0.80 PFLOP/s (a plain product of the library: 1.21;
+// this kernel without its scales: 1.17).  What the scales take is the additions of the scaled sums, an instruction for each result and
+// group, beside the matrix units' own; decoding takes nothing.  Two workgroups share a compute unit, so that one multiplies while
+// the other waits for its operands: tiles of 128 x 256, of which one fits, took 145 us with groups of 128.
+constexpr int kTile = 128, kTileThreads = 256, kTileRows = kTile * 256, kStage = kTileRows + kTile * 64;   // bytes of the rows, of a block
+__device__ __forceinline__ int turned(int row) { return (row / 2 & 3) ^ (row / 8 & 1); }
 
-template <typename T, int Group, int BM, int BN>
-__global__ __launch_bounds__(BM / 64 * (BN / 64) * 64, 2) void product_tiles4(const Product<T> k) {
-  using S = Tile<BM, BN>;
-  constexpr int kScales = kBlock / Group, kThreads = 64 * S::kWaves;
-  __shared__ __attribute__((aligned(16))) unsigned char lds[2 * S::kStage];
+template <typename T, int Group> __global__ __launch_bounds__(kTileThreads, 2) void product_tiles4(const Product<T> k) {
+  constexpr int kScales = kBlock / Group;
+  __shared__ __attribute__((aligned(16))) unsigned char lds[2 * kStage];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, g = lane >> 4;
-  const int wm = wave % (BM / 64), wn = wave / (BM / 64);
+  const int wm = wave % 2, wn = wave / 2;
   // tiles in an order in which neighbouring workgroups of a die share rows and weights: eight rows of tiles at a time
   const int tiles = k.m_tiles * k.n_tiles;
   unsigned id = linear_block();
@@ -94,26 +95,26 @@ __global__ __launch_bounds__(BM / 64 * (BN / 64) * 64, 2) void product_tiles4(co
   const int split = id / tiles;
   id = xcd_contiguous(id % tiles, tiles);
   const int band = id / (8 * k.n_tiles), in_band = id % (8 * k.n_tiles), tall = min(8, k.m_tiles - 8 * band);
-  const long m0 = (8L * band + in_band % tall) * BM;
-  const int n0 = in_band / tall * BN;
+  const long m0 = (8L * band + in_band % tall) * kTile;
+  const int n0 = in_band / tall * kTile;
   const int first = static_cast<int>(static_cast<long>(k.blocks) * split / k.splits), last = static_cast<int>(static_cast<long>(k.blocks) * (split + 1) / k.splits);
 
   // What a thread brings of a block: pieces of 16 bytes, in the order in which they stand in LDS
-  constexpr int kPiecesX = BM * 16 / kThreads, kPiecesW = BN * 4 / kThreads;
-  static_assert(BM * 16 % kThreads == 0 && BN * 4 % kThreads == 0, "");
+  constexpr int kPiecesX = kTile * 16 / kTileThreads, kPiecesW = kTile * 4 / kTileThreads;
+  static_assert(kTile * 16 % kTileThreads == 0 && kTile * 4 % kTileThreads == 0, "");
   const T *x_from[kPiecesX];
   int x_column[kPiecesX];
   const unsigned char *w_from[kPiecesW];
 #pragma unroll
   for (int i = 0; i < kPiecesX; ++i) {
-    const int at = i * kThreads + threadIdx.x, row = at / 16;
-    x_column[i] = ((at % 16) ^ (row & 7)) * 8;
+    const int at = i * kTileThreads + threadIdx.x, row = at / 16;
+    x_column[i] = ((at % 16) ^ (row & 15)) * 8;
     x_from[i] = k.x + min(m0 + row, k.rows - 1) * k.stride + x_column[i];
   }
 #pragma unroll
   for (int i = 0; i < kPiecesW; ++i) {
-    const int at = i * kThreads + threadIdx.x, row = at / 4;
-    w_from[i] = k.w + static_cast<long>(min(n0 + row, k.outputs - 1)) * k.blocks * 64 + ((at % 4) ^ (row / 2 & 3)) * 16;
+    const int at = i * kTileThreads + threadIdx.x, row = at / 4;
+    w_from[i] = k.w + static_cast<long>(min(n0 + row, k.outputs - 1)) * k.blocks * 64 + ((at % 4) ^ turned(row)) * 16;
   }
   const float *s_from[4];
 #pragma unroll
@@ -121,28 +122,28 @@ __global__ __launch_bounds__(BM / 64 * (BN / 64) * 64, 2) void product_tiles4(co
 
   float scale[4][kScales];
   auto bring = [&](int b) {
-    unsigned char *const to = lds + (b & 1) * S::kStage + wave * 1024;
+    unsigned char *const to = lds + (b & 1) * kStage + wave * 1024;
 #pragma unroll
     for (int i = 0; i < kPiecesX; ++i) {   // (of a piece behind the row's end: the row's first one, which zeros take the place of)
       const T *const from = b * kBlock + x_column[i] < k.inputs ? x_from[i] + b * kBlock : x_from[i] - x_column[i];
       __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)from,
-                                       (__attribute__((address_space(3))) void *)(to + i * kThreads * 16), 16, 0, 0);
+                                       (__attribute__((address_space(3))) void *)(to + i * kTileThreads * 16), 16, 0, 0);
     }
 #pragma unroll
     for (int i = 0; i < kPiecesW; ++i)
       __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(w_from[i] + b * 64L),
-                                       (__attribute__((address_space(3))) void *)(to + S::kRows + i * kThreads * 16), 16, 0, 0);
+                                       (__attribute__((address_space(3))) void *)(to + kTileRows + i * kTileThreads * 16), 16, 0, 0);
   };
   f32x4 acc[4][4] = {};
   bring(first);
   for (int b = first; b < last; ++b) {
     __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0): what this wavefront brought has arrived (a barrier alone does not promise that)
     __syncthreads();   // this block's operands are there, and nobody reads the place of the next ones
-    unsigned char *const here = lds + (b & 1) * S::kStage;
+    unsigned char *const here = lds + (b & 1) * kStage;
     if ((b + 1) * kBlock > k.inputs) {   // the columns behind the rows' ends
 #pragma unroll
       for (int i = 0; i < kPiecesX; ++i)
-        if (b * kBlock + x_column[i] >= k.inputs) *reinterpret_cast<u32x4 *>(here + (i * kThreads + threadIdx.x) * 16) = u32x4{0u, 0u, 0u, 0u};
+        if (b * kBlock + x_column[i] >= k.inputs) *reinterpret_cast<u32x4 *>(here + (i * kTileThreads + threadIdx.x) * 16) = u32x4{0u, 0u, 0u, 0u};
       __syncthreads();
     }
 #pragma unroll
@@ -154,14 +155,14 @@ __global__ __launch_bounds__(BM / 64 * (BN / 64) * 64, 2) void product_tiles4(co
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const int row = wn * 64 + u * 16 + r16;
-      w[u] = *reinterpret_cast<const u32x4 *>(here + S::kRows + row * 64 + (g ^ (row / 2 & 3)) * 16);
+      w[u] = *reinterpret_cast<const u32x4 *>(here + kTileRows + row * 64 + (g ^ turned(row)) * 16);
     }
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int row = wm * 64 + t * 16 + r16;
-        x[t][i] = *reinterpret_cast<const u32x4 *>(here + row * 256 + ((4 * i + g) ^ (row & 7)) * 16);
+        x[t][i] = *reinterpret_cast<const u32x4 *>(here + row * 256 + ((4 * i + g) ^ (row & 15)) * 16);
       }
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
@@ -200,13 +201,109 @@ __global__ __launch_bounds__(BM / 64 * (BN / 64) * 64, 2) void product_tiles4(co
   }
 }
 
+// ---- a row or two ------------------------------------------------------------------------------------------------------
+// Bound by reading the weights once, in vector instructions (a matrix instruction would have fifteen rows of nothing): a wavefront
+// has four outputs and sixteen blocks of them at a time, 1024 neighbouring bytes of each; a lane has a quarter of a block, the columns
+// 32 s + 8 g .. + 7 of lane group g.  `along` wavefronts of a workgroup share the blocks and join in LDS.
+constexpr int kDotOutputs = 4, kDotBlocks = 16, kMostAlong = 8;
+
+template <typename T, int M, int Group> __global__ __launch_bounds__(64 * kMostAlong) void product_dots(const Product<T> k, int along) {
+  constexpr int kScales = kBlock / Group;
+  __shared__ float part[kMostAlong][M][kDotOutputs];
+  unsigned id = linear_block();
+  if (id >= static_cast<unsigned>(k.n_tiles) * k.splits) return;
+  const int split = id / k.n_tiles, waves = blockDim.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane & 3;
+  const int n0 = ((id - split * k.n_tiles) * (waves / along) + wave / along) * kDotOutputs;
+  const int chunks = (k.blocks + kDotBlocks - 1) / kDotBlocks;
+  const int first = static_cast<int>(static_cast<long>(chunks) * split / k.splits) + wave % along, last = static_cast<int>(static_cast<long>(chunks) * (split + 1) / k.splits);
+  const unsigned char *w_at[kDotOutputs];
+  const float *s_at[kDotOutputs];
+#pragma unroll
+  for (int u = 0; u < kDotOutputs; ++u) {
+    const long n = min(n0 + u, k.outputs - 1);
+    w_at[u] = k.w + n * k.blocks * 64 + g * 16;
+    s_at[u] = k.scales + n * k.blocks * kScales;
+  }
+  struct Operands {
+    u32x4 w[kDotOutputs], x[M][4];
+    float s[kDotOutputs][kScales];
+  };
+  auto bring = [&](Operands &o, int chunk) {
+    const int at = chunk * kDotBlocks + (lane >> 2), b = min(at, k.blocks - 1);   // (behind the last one: that one, times zero)
+#pragma unroll
+    for (int u = 0; u < kDotOutputs; ++u) {
+      o.w[u] = *reinterpret_cast<const u32x4 *>(w_at[u] + b * 64L);
+#pragma unroll
+      for (int i = 0; i < kScales; ++i) o.s[u][i] = s_at[u][static_cast<long>(b) * kScales + i];
+    }
+#pragma unroll
+    for (int m = 0; m < M; ++m)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int c = b * kBlock + i * 32 + g * 8;
+        o.x[m][i] = columns8(k.x + m * k.stride + c, at < k.blocks ? k.inputs - c : 0);
+      }
+  };
+  float acc[M][kDotOutputs] = {};
+  Operands next;
+  if (first < last) bring(next, first);
+  for (int chunk = first; chunk < last; chunk += along) {
+    const Operands o = next;
+    if (chunk + along < last) bring(next, chunk + along);
+    const bool there = chunk * kDotBlocks + (lane >> 2) < k.blocks;
+    float sum[M][kDotOutputs] = {};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float x[M][8];
+#pragma unroll
+      for (int m = 0; m < M; ++m)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[m][j] = Bits<T>::up(static_cast<unsigned short>(o.x[m][i][j / 2] >> (j % 2 * 16)));
+#pragma unroll
+      for (int u = 0; u < kDotOutputs; ++u) {
+        const f32x2 v[4] = {__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(o.w[u][i], 1.f, 0), __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(o.w[u][i], 1.f, 1),
+                            __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(o.w[u][i], 1.f, 2), __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(o.w[u][i], 1.f, 3)};
+#pragma unroll
+        for (int m = 0; m < M; ++m) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) sum[m][u] = fmaf(x[m][j], v[j / 2][j % 2], sum[m][u]);
+          if ((i + 1) % (Group / 32) == 0) {
+            acc[m][u] = there ? fmaf(sum[m][u], o.s[u][i / (Group / 32)], acc[m][u]) : acc[m][u];
+            sum[m][u] = 0.f;
+          }
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int m = 0; m < M; ++m)
+#pragma unroll
+    for (int u = 0; u < kDotOutputs; ++u) {
+#pragma unroll
+      for (int d = 32; d; d >>= 1) acc[m][u] += __shfl_xor(acc[m][u], d);
+      if (lane == 0) part[wave][m][u] = acc[m][u];
+    }
+  __syncthreads();
+  if (wave % along || lane >= M * kDotOutputs) return;
+  const int m = lane / kDotOutputs, n = n0 + lane % kDotOutputs;
+  float y = 0.f;
+  for (int i = 0; i < along; ++i) y += part[wave + i][m][lane % kDotOutputs];
+  if (n >= k.outputs) return;
+  if (k.part) k.part[(split * k.rows + m) * k.outputs + n] = y;
+  else k.y[m * k.outputs + n] = store_cast<T>(k.bias ? y + load(k.bias + n) : y);
+}
+
 // ---- few rows -------------------------------------------------------------------------------------------------------
-// 64 outputs and 16 TM rows per workgroup, straight from memory into the operands' registers.  The four wavefronts take turns
+// 16 TN outputs and 16 TM rows per workgroup, straight from memory into the operands' registers.  The wavefronts take turns
 // at the blocks of the workgroup's share of the sum and join in LDS.
+constexpr int waves_of(int tm) { return tm <= 1 ? 8 : 4; }
+constexpr int tiles_wide(int tm) { return tm <= 1 ? 2 : 4; }
+
 template <typename T, int TM, int Group>
-__global__ __launch_bounds__(256) void product_rows4(const Product<T> k) {
-  constexpr int TN = 4, kScales = kBlock / Group;
-  __shared__ f32x4 part[3][TN * TM][64];
+__global__ __launch_bounds__(64 * waves_of(TM), 2) void product_rows4(const Product<T> k) {
+  constexpr int TN = tiles_wide(TM), kScales = kBlock / Group, kWaves = waves_of(TM);
+  __shared__ f32x4 part[kWaves - 1][TN * TM][64];
   unsigned id = linear_block();
   if (id >= static_cast<unsigned>(k.m_tiles) * k.n_tiles * k.splits) return;
   const int n_tile = id % k.n_tiles;
@@ -226,36 +323,55 @@ __global__ __launch_bounds__(256) void product_rows4(const Product<T> k) {
     w_at[u] = k.w + n * k.blocks * 64 + g * 16;
     s_at[u] = k.scales + n * k.blocks * kScales;
   }
-  f32x4 acc[TM][TN] = {};
-  for (int b = first + wave; b < last; b += 4) {
+  struct Operands {
     u32x4 w[TN], x[TM][4];
     float s[TN][kScales];
+  };
+  auto bring_weights = [&](Operands &o, int b) {
 #pragma unroll
     for (int u = 0; u < TN; ++u) {
-      w[u] = *reinterpret_cast<const u32x4 *>(w_at[u] + b * 64L);
+      o.w[u] = *reinterpret_cast<const u32x4 *>(w_at[u] + b * 64L);
 #pragma unroll
-      for (int i = 0; i < kScales; ++i) s[u][i] = s_at[u][static_cast<long>(b) * kScales + i];
+      for (int i = 0; i < kScales; ++i) o.s[u][i] = s_at[u][static_cast<long>(b) * kScales + i];
     }
+  };
+  auto bring_rows = [&](Operands &o, int b) {
 #pragma unroll
     for (int t = 0; t < TM; ++t)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int c = b * kBlock + i * 32 + g * 8;
-        x[t][i] = columns8(x_at[t] + c, k.inputs - c);
+        o.x[t][i] = columns8(x_at[t] + c, k.inputs - c);
       }
+  };
+  f32x4 acc[TM][TN] = {};
+  // The next block's weights are on their way while these are multiplied, and its rows as far as there are registers for them.
+  constexpr bool kRowsAhead = TM <= 2;
+  Operands next;
+  if (first + wave < last) {
+    bring_weights(next, first + wave);
+    if (kRowsAhead) bring_rows(next, first + wave);
+  }
+  for (int b = first + wave; b < last; b += kWaves) {
+    Operands o = next;
+    if (!kRowsAhead) bring_rows(o, b);
+    if (b + kWaves < last) {
+      bring_weights(next, b + kWaves);
+      if (kRowsAhead) bring_rows(next, b + kWaves);
+    }
 #pragma unroll
     for (int u = 0; u < TN; ++u) {
       f32x4 d[TM];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const u32x4 v = Matrix<T>::values(w[u][i]);
+        const u32x4 v = Matrix<T>::values(o.w[u][i]);
 #pragma unroll
         for (int t = 0; t < TM; ++t) {
           if (i % (Group / 32) == 0) d[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-          d[t] = Matrix<T>::product(x[t][i], v, d[t]);
+          d[t] = Matrix<T>::product(o.x[t][i], v, d[t]);
           if ((i + 1) % (Group / 32) == 0) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) acc[t][u][j] = fmaf(d[t][j], s[u][i / (Group / 32)], acc[t][u][j]);
+            for (int j = 0; j < 4; ++j) acc[t][u][j] = fmaf(d[t][j], o.s[u][i / (Group / 32)], acc[t][u][j]);
           }
         }
       }
@@ -277,7 +393,7 @@ __global__ __launch_bounds__(256) void product_rows4(const Product<T> k) {
 #pragma unroll
     for (int t = 0; t < TM; ++t) {
 #pragma unroll
-      for (int i = 0; i < 3; ++i) acc[t][u] += part[i][u * TM + t][lane];
+      for (int i = 0; i < kWaves - 1; ++i) acc[t][u] += part[i][u * TM + t][lane];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const long m = m0 + t * 16 + 4 * g + j;
@@ -316,31 +432,43 @@ __global__ __launch_bounds__(256) void quantize_groups(const T *w, unsigned *q, 
 }
 
 // ---- which kernel --------------------------------------------------------------------------------------------------
-enum Kind { kFew1, kFew2, kFew4, kTiles, kWideTiles };
+enum Kind { kDots, kFew1, kFew2, kFew4, kTiles };
 struct Plan {
   int kind, m_tiles, n_tiles, splits;
+  int along = 1, waves = 4;   // of kDots
 };
 
+constexpr int kDotRows = 2;
 int ceil_div(long a, long b) { return static_cast<int>((a + b - 1) / b); }
 
 Plan plan_of(long rows, int blocks, int outputs) {
-  if (rows <= 64) {
-    const int kind = rows <= 16 ? kFew1 : rows <= 32 ? kFew2 : kFew4, n = ceil_div(outputs, 64);
-    return {kind, 1, n, std::max(1, std::min(blocks / 8, 512 / n))};
+  if (rows <= kDotRows) {
+    const int chunks = ceil_div(blocks, kDotBlocks);
+    int along = 1;
+    while (along < kMostAlong && along < chunks) along *= 2;
+    const int waves = std::max(4, along), n = ceil_div(outputs, waves / along * kDotOutputs);
+    return {kDots, 1, n, std::max(1, std::min(chunks / along, 256 / n)), along, waves};
   }
-  const int m = ceil_div(rows, 128), wide = ceil_div(outputs, 256), n = ceil_div(outputs, 128);
-  if (outputs > 128) return {kWideTiles, m, wide, static_cast<int>(std::max(1L, std::min(blocks / 8L, 256 / (static_cast<long>(m) * wide))))};
-  return {kTiles, m, n, static_cast<int>(std::max(1L, std::min(blocks / 8L, 512 / (static_cast<long>(m) * n))))};
+  if (rows <= 64) {
+    const int kind = rows <= 16 ? kFew1 : rows <= 32 ? kFew2 : kFew4, tm = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+    const int n = ceil_div(outputs, 16 * tiles_wide(tm)), waves = waves_of(tm);
+    return {kind, 1, n, std::max(1, std::min(blocks / (2 * waves), 256 * 8 / waves / n))};
+  }
+  const int m = ceil_div(rows, 128), n = ceil_div(outputs, 128);
+  return {kTiles, m, n, static_cast<int>(std::max(1L, std::min(blocks / 4L, 512 / (static_cast<long>(m) * n))))};
 }
 
 template <typename T, int Group> void launch(const Plan &p, const Product<T> &k, hipStream_t s) {
   const long groups = static_cast<long>(p.m_tiles) * p.n_tiles * p.splits;
   switch (p.kind) {
-    case kFew1: product_rows4<T, 1, Group><<<linear_grid(groups, 256), 256, 0, s>>>(k); break;
-    case kFew2: product_rows4<T, 2, Group><<<linear_grid(groups, 256), 256, 0, s>>>(k); break;
-    case kFew4: product_rows4<T, 4, Group><<<linear_grid(groups, 256), 256, 0, s>>>(k); break;
-    case kTiles: product_tiles4<T, Group, 128, 128><<<linear_grid(groups, 256), 256, 0, s>>>(k); break;
-    default: product_tiles4<T, Group, 128, 256><<<linear_grid(groups, 512), 512, 0, s>>>(k);
+    case kDots:
+      if (k.rows == 1) product_dots<T, 1, Group><<<linear_grid(groups, 64 * p.waves), 64 * p.waves, 0, s>>>(k, p.along);
+      else product_dots<T, 2, Group><<<linear_grid(groups, 64 * p.waves), 64 * p.waves, 0, s>>>(k, p.along);
+      break;
+    case kFew1: product_rows4<T, 1, Group><<<linear_grid(groups, 64 * waves_of(1)), 64 * waves_of(1), 0, s>>>(k); break;
+    case kFew2: product_rows4<T, 2, Group><<<linear_grid(groups, 64 * waves_of(2)), 64 * waves_of(2), 0, s>>>(k); break;
+    case kFew4: product_rows4<T, 4, Group><<<linear_grid(groups, 64 * waves_of(4)), 64 * waves_of(4), 0, s>>>(k); break;
+    default: product_tiles4<T, Group><<<linear_grid(groups, 256), 256, 0, s>>>(k);
   }
 }
 
@@ -361,11 +489,11 @@ int product(const void *x, const void *w, const void *scales, const void *bias, 
   const int blocks = ceil_div(inputs, kBlock);
   Plan p = plan_of(rows, blocks, outputs);
   // Rows that tiles cannot read are copied first; where there is no room for that, they go straight to registers.
-  const bool tiles = p.kind == kTiles || p.kind == kWideTiles, odd = tiles && (inputs % 8 || reinterpret_cast<uintptr_t>(x) % 16);
+  const bool tiles = p.kind == kTiles, odd = tiles && (inputs % 8 || reinterpret_cast<uintptr_t>(x) % 16);
   const size_t pad = odd ? padded_bytes(rows, blocks) : 0;
   if (!workspace) workspace_bytes = 0;
   const bool pads = odd && pad <= workspace_bytes && reinterpret_cast<uintptr_t>(workspace) % 16 == 0;
-  if (odd && !pads) p = {kFew4, ceil_div(rows, 64), ceil_div(outputs, 64), 1};
+  if (odd && !pads) p = {kFew4, ceil_div(rows, 64), ceil_div(outputs, 16 * tiles_wide(4)), 1};
   const size_t at = pads ? pad : 0;
   if (workspace_bytes - at < part_bytes(p, rows, outputs)) p.splits = 1;
   Product<T> k{static_cast<const T *>(x), static_cast<const unsigned char *>(w), static_cast<const float *>(scales), static_cast<const T *>(bias),
@@ -412,7 +540,7 @@ size_t mv_group_linear_workspace_bytes(int64_t rows, int inputs, int outputs) {
   if (rows <= 0 || inputs <= 0 || outputs <= 0) return 0;
   const int blocks = ceil_div(inputs, kBlock);
   const Plan p = plan_of(rows, blocks, outputs);
-  return part_bytes(p, rows, outputs) + ((p.kind == kTiles || p.kind == kWideTiles) && inputs % 8 ? padded_bytes(rows, blocks) : 0);
+  return part_bytes(p, rows, outputs) + (p.kind == kTiles && inputs % 8 ? padded_bytes(rows, blocks) : 0);
 }
 
 int mv_group_linear(const void *x, const void *weight, const void *scales, const void *bias, void *y, int64_t rows, int inputs, int outputs,
