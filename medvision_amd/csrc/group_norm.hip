@@ -368,9 +368,54 @@ __global__ __launch_bounds__(kThreads) void group_grad_finish(float2 *partial, f
   means[static_cast<long>(batch) * s.groups + id] = static_cast<float>(dot / all);
 }
 
+// Sums of a tile's channels over the samples, in their order: the gradients of weight and bias
+struct Vectors {
+  const float2 *sums;   // of a sample's channels, `every` from one sample to the next
+  void *weight, *bias;
+  long every;
+  int batch;
+};
+template <typename T> __device__ __forceinline__ void put_vectors(const Vectors &v, bool wide, int first, int last) {
+  __shared__ double2 shares[kThreads];
+  const int across = min(last - first, kThreads), in = threadIdx.x % across, team = threadIdx.x / across, teams = kThreads / across;
+  for (int c = first + in; c - in < last; c += across) {   // (teams of threads share the samples where there are few channels)
+    double sum = 0., dot = 0.;
+    if (team < teams && c < last) {
+#pragma unroll 4
+      for (int b = team; b < v.batch; b += teams) {
+        const float2 share = v.sums[b * v.every + c];
+        sum += share.x, dot += share.y;
+      }
+    }
+    if (teams > 1) {
+      shares[threadIdx.x] = {sum, dot};
+      __syncthreads();
+      if (team == 0)
+        for (int t = 1; t < teams; ++t) sum += shares[t * across + in].x, dot += shares[t * across + in].y;
+    }
+    if (team || c >= last) continue;
+    auto put = [&](void *to, double value) {
+      if (!to) return;
+      if (wide) static_cast<float *>(to)[c] = static_cast<float>(value);
+      else static_cast<T *>(to)[c] = store_cast<T>(static_cast<float>(value));
+    };
+    put(v.bias, sum);
+    put(v.weight, dot);
+  }
+}
+constexpr int kVectorChannels = 16;   // of a workgroup
+template <typename T> __global__ __launch_bounds__(kThreads) void group_grad_vectors(const Vectors v, bool wide, int channels) {
+  const int first = blockIdx.x * kVectorChannels;
+  put_vectors<T>(v, wide, first, min(channels, first + kVectorChannels));
+}
+
 template <typename T, int Kind, int F>
 __global__ __launch_bounds__(kThreads) void group_grad_apply(const T *x, const T *gy, const float *stats, const float *means, const void *weight,
-                                                             const void *bias, bool wide, T *gx, const Cells s, float low) {
+                                                             const void *bias, bool wide, T *gx, const Vectors sums, const Cells s, float low) {
+  if (static_cast<int>(blockIdx.x) == s.chunks) {   // behind the last chunk: a tile's gradients of weight and bias
+    if (blockIdx.z == 0) put_vectors<T>(sums, wide, blockIdx.y * kThreads * 8, min(s.channels, static_cast<int>(blockIdx.y + 1) * kThreads * 8));
+    return;
+  }
   const Place p = place_of(s, blockIdx.x);
   if (!p.cells) return;
   Channels t;
@@ -404,26 +449,6 @@ __global__ __launch_bounds__(kThreads) void group_grad_apply(const T *x, const T
       put_eight<T, F>(to + n * p.stride, p.left, v);
     }
   }
-}
-
-// Sums of the channels over the samples, in their order
-template <typename T>
-__global__ __launch_bounds__(kThreads) void group_grad_vectors(const float2 *partial, void *gw, void *gb, bool wide, const Cells s, int batch) {
-  const int c = blockIdx.x * kThreads + threadIdx.x;
-  if (c >= s.channels) return;
-  double sum = 0., dot = 0.;
-#pragma unroll 4
-  for (int b = 0; b < batch; ++b) {
-    const float2 share = partial[static_cast<long>(b) * s.chunks * s.channels + c];
-    sum += share.x, dot += share.y;
-  }
-  auto put = [&](void *to, double v) {
-    if (!to) return;
-    if (wide) static_cast<float *>(to)[c] = static_cast<float>(v);
-    else static_cast<T *>(to)[c] = store_cast<T>(static_cast<float>(v));
-  };
-  put(gb, sum);
-  put(gw, dot);
 }
 
 // ---- launches -------------------------------------------------------------------------------------------------------
@@ -488,7 +513,7 @@ int mv_group_norm(const void *x, const void *weight, const void *bias, void *y, 
   const bool wide = weight_dtype == MV_F32;
   auto *const partial = static_cast<Moments *>(workspace);
   auto *const stat = static_cast<float *>(stats);
-  if (const WholePlan whole = whole_plan(cells, channels, groups, false); whole.u)
+  if (const WholePlan whole = whole_plan(batch, cells, channels, groups, false); whole.u)
     return group_norm_whole(whole, x, weight, bias, wide, y, stat, batch, eps, activation, low, dtype, st);
   MV_FLOATS(dtype, {
     const T *const xt = static_cast<const T *>(x);
@@ -522,12 +547,11 @@ int mv_group_norm_backward(const void *x, const void *weight, const void *bias, 
   auto *const partial = static_cast<float2 *>(workspace);
   auto *const means = reinterpret_cast<float *>(static_cast<char *>(workspace) + (empty ? 0 : partial_bytes<float2>(batch, s)));
   auto *const stat = static_cast<const float *>(stats);
-  Cells sum = s;   // where the channels' sums stand
-  const WholePlan whole = empty ? WholePlan{} : whole_plan(cells, channels, groups, true);
+  const WholePlan whole = empty ? WholePlan{} : whole_plan(batch, cells, channels, groups, true);
+  const Vectors vectors{partial, grad_weight, grad_bias, (whole.u ? 1L : s.chunks) * channels, empty ? 0 : batch};
+  const bool wanted = grad_weight || grad_bias;
   if (whole.u) {
-    sum.chunks = 1;
-    if (const int status = group_norm_whole_backward(whole, x, grad_y, stat, weight, bias, wide, grad_x, grad_weight || grad_bias ? partial : nullptr, batch,
-                                                     activation, low, dtype, st))
+    if (const int status = group_norm_whole_backward(whole, x, grad_y, stat, weight, bias, wide, grad_x, wanted ? partial : nullptr, batch, activation, low, dtype, st))
       return status;
   }
   MV_FLOATS(dtype, {
@@ -540,12 +564,12 @@ int mv_group_norm_backward(const void *x, const void *weight, const void *bias, 
       if (grad_x)
         for_activation(activation, [&](auto kind) {
           for_form(s, bytes, [&](auto form) {
-            group_grad_apply<T, kind, form><<<grid, kThreads, 0, st>>>(xt, gy, stat, means, weight, bias, wide, static_cast<T *>(grad_x), s, low);
+            group_grad_apply<T, kind, form><<<dim3(s.chunks + (wanted ? 1 : 0), grid.y, batch), kThreads, 0, st>>>(xt, gy, stat, means, weight, bias, wide,
+                                                                                                               static_cast<T *>(grad_x), vectors, s, low);
           });
         });
     }
-    if (grad_weight || grad_bias)
-      group_grad_vectors<T><<<(channels + kThreads - 1) / kThreads, kThreads, 0, st>>>(partial, grad_weight, grad_bias, wide, sum, empty ? 0 : batch);
+    if (wanted && (empty || whole.u || !grad_x)) group_grad_vectors<T><<<(channels + kVectorChannels - 1) / kVectorChannels, kThreads, 0, st>>>(vectors, wide, channels);
   })
   return check_launch("group_norm backward");
 }

@@ -12,7 +12,7 @@ struct WholePlan {
   Whole s;
   int threads, v, u;   // u: cells of a thread, 0: the sample is too large
 };
-WholePlan whole_plan(long cells, int channels, int groups, bool gradients);
+WholePlan whole_plan(int batch, long cells, int channels, int groups, bool gradients);
 
 // y and stats; gx (NULL: not wanted) and the channels' sums of gz and gz h, sums[sample][channel] (NULL: not wanted)
 int group_norm_whole(const WholePlan &plan, const void *x, const void *weight, const void *bias, bool wide, void *y, float *stats, int batch, float eps,

@@ -216,9 +216,13 @@ template <bool Gradients, typename F> void for_plan(const WholePlan &p, const F 
 
 }  // namespace
 
-// V is the largest power of two up to 8 that divides a group's channels.
-WholePlan whole_plan(long cells, int channels, int groups, bool gradients) {
+// V is the largest power of two up to 8 that divides a group's channels.  A workgroup reads as many cache lines as there are cells, by itself:
+// 8 x 5000 cells of 20 channels in groups of 4 8.9 us (12.3 in the three kernels of large samples), 8000 of 32 in groups of 8 16.4
+// (13.4).  Gradients read two tensors, and keep the chip's other workgroups waiting where there are many: 4 x 2000 of 64 in groups of 4
+// 11 us (16), 1 x 4000 of 256 in groups of 8 18 (15), 64 x 343 of 256 29 (26).
+WholePlan whole_plan(int batch, long cells, int channels, int groups, bool gradients) {
   WholePlan p{};
+  if (cells > (gradients ? 3000 : 5000) || (gradients && batch * cells * channels > (4L << 20))) return p;
   const int each = channels / groups;
   p.v = each % 8 == 0 ? 8 : each % 4 == 0 ? 4 : each % 2 == 0 ? 2 : 1;
   p.s = {0, channels, groups, each, each / p.v, 0};
