@@ -150,8 +150,8 @@ __global__ __launch_bounds__(kThreads) void group_sums(const T *x, Moments *part
   const float each = p.cells ? 1.f / static_cast<float>(p.cells) : 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float off = sum[i] * each;
-    shares[threadIdx.x][i] = {middle[i], off, fmaxf(fmaf(-sum[i], off, squares[i]), 0.f) + (squares[i] - squares[i])};   // (NaN stays)
+    const float off = sum[i] * each, left = fmaf(-sum[i], off, squares[i]);
+    shares[threadIdx.x][i] = {middle[i], off, left < 0.f ? 0.f : left};   // (NaN stays)
   }
   __syncthreads();
   join_rows<double2>(s, [&](int r, int o, int i, double2 &all) {
@@ -458,9 +458,9 @@ Cells cells_of(int batch, long cells, int channels, int groups) {
   s.cells = cells, s.channels = channels, s.groups = groups, s.group_channels = channels / groups;
   const int octets = (channels + 7) / 8, tiles = (octets + kThreads - 1) / kThreads;
   s.tile_threads = std::min(octets, kThreads), s.tile_rows = kThreads / s.tile_threads;
-  // about four workgroups per compute unit, of four cells a thread at least
+  // about four workgroups per compute unit, of four cells a thread at least, and no more than 256: longer sums in 32 bits lose bits
   const long most = std::max(1L, kGroups / std::max(1L, static_cast<long>(batch) * tiles)), rows = static_cast<long>(kAtOnce) * s.tile_rows;
-  s.each = std::max(rows, (cells + most - 1) / most);
+  s.each = std::max(rows, std::min(256L * s.tile_rows, (cells + most - 1) / most));
   s.each = (s.each + s.tile_rows - 1) / s.tile_rows * s.tile_rows;
   s.chunks = static_cast<int>(std::max(1L, (cells + s.each - 1) / s.each));
   return s;
@@ -475,10 +475,11 @@ template <typename F> void for_form(const Cells &s, size_t bytes, const F &f) {
   else f(std::integral_constant<int, kWholePast>());
 }
 
+constexpr int kMostBatch = 65536;   // (a grid's third dimension)
 int arguments(int batch, long cells, int channels, int groups, int activation, int dtype, int weight_dtype) {
   MV_REQUIRE(dtype == MV_F32 || dtype == MV_F16 || dtype == MV_BF16, "dtype %d is not float32, float16 or bfloat16", dtype);
   MV_REQUIRE(weight_dtype == dtype || weight_dtype == MV_F32, "weight and bias have dtype %d, expected %d or float32", weight_dtype, dtype);
-  MV_REQUIRE(batch >= 0 && batch < 65536 && cells >= 0 && cells < (1L << 40) && channels > 0 && channels <= (1 << 24), "wrong sizes: a batch of %d, %ld cells of %d channels", batch, cells, channels);
+  MV_REQUIRE(batch >= 0 && cells >= 0 && cells <= (1L << 36) && channels > 0 && channels <= (1 << 24), "wrong sizes: a batch of %d, %ld cells of %d channels", batch, cells, channels);
   MV_REQUIRE(groups > 0 && channels % groups == 0, "%d channels in %d groups", channels, groups);
   MV_REQUIRE(static_cast<long>(batch) * groups < (1L << 31), "too many groups: %d in a batch of %d", groups, batch);
   MV_REQUIRE(activation >= MV_NO_ACTIVATION && activation <= MV_GELU, "unknown activation %d", activation);
@@ -515,6 +516,7 @@ int mv_group_norm(const void *x, const void *weight, const void *bias, void *y, 
   auto *const stat = static_cast<float *>(stats);
   if (const WholePlan whole = whole_plan(batch, cells, channels, groups, false); whole.u)
     return group_norm_whole(whole, x, weight, bias, wide, y, stat, batch, eps, activation, low, dtype, st);
+  MV_REQUIRE(batch < kMostBatch, "a batch of %d is too large for samples of %ld cells", batch, static_cast<long>(cells));
   MV_FLOATS(dtype, {
     const T *const xt = static_cast<const T *>(x);
     for_form(s, 0, [&](auto form) { group_sums<T, form><<<grid, kThreads, 0, st>>>(xt, partial, s); });
@@ -554,6 +556,7 @@ int mv_group_norm_backward(const void *x, const void *weight, const void *bias, 
     if (const int status = group_norm_whole_backward(whole, x, grad_y, stat, weight, bias, wide, grad_x, wanted ? partial : nullptr, batch, activation, low, dtype, st))
       return status;
   }
+  MV_REQUIRE(empty || whole.u || batch < kMostBatch, "a batch of %d is too large for samples of %ld cells", batch, static_cast<long>(cells));
   MV_FLOATS(dtype, {
     const T *const xt = static_cast<const T *>(x), *const gy = static_cast<const T *>(grad_y);
     if (!empty && !whole.u) {

@@ -3,7 +3,7 @@
 // from one sum over the workgroup to the next.
 //
 // A thread has V neighbouring channels (V divides those of the group, so that all its values are of one group) of up to U
-// cells: 64 / V, and half as many where gradients are read beside them.
+// cells: 64 / V and no more than 16; for gradients 32 / V.
 #include "activation.hpp"
 #include "group_norm.hpp"
 #include "rows.hpp"
@@ -195,7 +195,7 @@ __global__ __launch_bounds__(1024) void group_grad_whole(const T *x, const T *gy
 }
 
 constexpr int forward_cells(int v) { return 64 / v > 16 ? 16 : 64 / v; }
-constexpr int grad_cells(int v) { return forward_cells(v) / 2; }
+constexpr int grad_cells(int v) { return v <= 2 ? 16 : forward_cells(v) / 2; }
 bool folds(const Whole &s) { return s.units < 64 && (s.units & (s.units - 1)) == 0; }
 
 // Calls f with V and U of a plan, as constants
@@ -219,14 +219,14 @@ template <bool Gradients, typename F> void for_plan(const WholePlan &p, const F 
 // V is the largest power of two up to 8 that divides a group's channels.  A workgroup reads as many cache lines as there are cells, by itself:
 // 8 x 5000 cells of 20 channels in groups of 4 8.9 us (12.3 in the three kernels of large samples), 8000 of 32 in groups of 8 16.4
 // (13.4).  Gradients read two tensors, and keep the chip's other workgroups waiting where there are many: 4 x 2000 of 64 in groups of 4
-// 11 us (16), 1 x 4000 of 256 in groups of 8 18 (15), 64 x 343 of 256 29 (26).
+// 11 us (16), 1 x 4000 of 256 in groups of 8 18 (15), 64 x 343 of 256 29 (26).  (The three kernels take batches of less than 65536.)
 WholePlan whole_plan(int batch, long cells, int channels, int groups, bool gradients) {
   WholePlan p{};
-  if (cells > (gradients ? 3000 : 5000) || (gradients && batch * cells * channels > (4L << 20))) return p;
+  if (cells > (gradients ? 3000 : 5000) || (gradients && batch * cells * channels > (4L << 20) && batch < 65536)) return p;
   const int each = channels / groups;
   p.v = each % 8 == 0 ? 8 : each % 4 == 0 ? 4 : each % 2 == 0 ? 2 : 1;
   p.s = {0, channels, groups, each, each / p.v, 0};
-  const int most = gradients ? grad_cells(p.v) : forward_cells(p.v), most_threads = gradients && !folds(p.s) ? 512 : 1024;   // (sums of each row in LDS)
+  const int most = gradients ? grad_cells(p.v) : forward_cells(p.v), most_threads = gradients && !folds(p.s) && p.v == 8 ? 512 : 1024;   // (sums of each row in LDS: 32 KB)
   if (p.s.units > most_threads || cells > static_cast<long>(most_threads / p.s.units) * most) return p;
   p.threads = 64;   // two cells a thread while there are threads
   while (p.threads < most_threads && cells > 2L * (p.threads / p.s.units)) p.threads *= 2;

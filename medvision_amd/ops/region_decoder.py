@@ -62,7 +62,7 @@ class RegionDecoderLayer(nn.Module):
             layer._modules[name] = BlockScaledLinear.from_linear(linear, dtype) if bits == 8 else GroupScaledLinear.from_linear(linear, group, dtype)
         for name in ("norm_query", "norm_hidden"):
             layer._modules[name] = copy.deepcopy(getattr(self, name)).float().requires_grad_(False)
-        layer._modules["place"] = copy.deepcopy(self.place)
+        layer._modules["place"] = copy.deepcopy(self._modules.get("place"))
         return layer.eval()
 
     def _normed(self, norm, x, residual):
@@ -73,9 +73,10 @@ class RegionDecoderLayer(nn.Module):
         return norm(x, residual)
 
     def _placed(self, x, positions, whose):
-        if (positions is None) != (self.place is None):
-            raise ValueError(f"{whose}_positions are {'missing' if positions is None else 'given'}: the layer has {'positions' if self.place else 'no axes'}")
-        return x if positions is None else self.place(x, positions)
+        place = self._modules.get("place")   # (layers that were stored before there were positions have no such entry)
+        if (positions is None) != (place is None):
+            raise ValueError(f"{whose}_positions are {'missing' if positions is None else 'given'}: the layer has {'no axes' if place is None else 'axes'}")
+        return x if positions is None else place(x, positions)
 
     def forward(self, regions, tokens, residual=None, key_mask=None, key_lengths=None, region_positions=None, token_positions=None):
         """``regions [batch, regions, channels]``, ``residual`` like them or None, ``tokens [batch, cells, channels]`` of

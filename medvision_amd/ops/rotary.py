@@ -27,16 +27,16 @@ class RotaryPositionsFunction(NativeFunction):
 
 
 def axis_frequencies(channels, axes=3, theta=100.0, device=None):
-    """Frequencies that give each axis a share of a head's pairs: float64 ``[axes, pairs]`` for ``rotary_positions``.
+    """Frequencies that give each axis a share of a head's pairs: float64 ``[axes, channels // 2]`` for ``rotary_positions``.
 
-    Of ``channels // 2`` pairs each axis has ``n = channels // 2 // axes``, which turn by ``theta ** (-i / n)``, ``i = 0 .. n - 1``,
-    per unit of the position; what is left over does not turn.  Whole positions over a few hundred cells go well with the
-    default ``theta``."""
+    Of the ``channels // 2`` pairs each axis has ``n = channels // 2 // axes``, which turn by ``theta ** (-i / n)``, ``i = 0 .. n - 1``,
+    per unit of the position; the pairs that are left over, the last ones, do not turn.  Whole positions over a few hundred cells go
+    well with the default ``theta``."""
     each = channels // 2 // axes if axes > 0 else 0
     if each < 1:
         raise ValueError(f"{channels} channels for {axes} axes: at least one pair for each is needed")
     turn = float(theta) ** (-torch.arange(each, dtype=torch.float64, device=device) / each)
-    return torch.block_diag(*[turn[None]] * axes)
+    return torch.nn.functional.pad(torch.block_diag(*[turn[None]] * axes), (0, channels // 2 - axes * each))
 
 
 def rotary_positions(x, positions, frequencies, neighbours=False):

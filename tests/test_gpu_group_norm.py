@@ -97,6 +97,31 @@ def test_empty_inputs():
     assert torch.allclose(ops.group_norm_act(x, 2), torch.nn.functional.group_norm(x, 2), atol=1e-5)
 
 
+@pytest.mark.parametrize("N", [1, 3])
+def test_large_batches(N):
+    """More samples than a grid's third dimension has places; the same as a part of them."""
+    import medvision_amd.ops as ops
+    B, C = 70000, 40
+    x, go, w = rand(1, B, N, C).to(DEV).requires_grad_(True), rand(2, B, N, C).to(DEV), rand(3, C).to(DEV).requires_grad_(True)
+    y = ops.group_norm_act(x, 4, w, None, activation="silu")
+    gx, gw = torch.autograd.grad(y, (x, w), go)
+    part = x.detach()[-100:].requires_grad_(True)
+    want = ops.group_norm_act(part, 4, w, None, activation="silu")
+    wx, = torch.autograd.grad(want, part, go[-100:])
+    assert torch.equal(y[-100:], want) and torch.equal(gx[-100:], wx)
+    _, _, (dw, bound), _ = ref.group_norm(x, 4, w, None, 1e-5, "silu", grad=go)
+    check(gw, dw, bound, "dw")
+
+
+def test_values_whose_squares_are_too_large():
+    """A variance that 32 bits do not hold: its group's cells are the bias, as the formula has it for an infinite variance."""
+    import medvision_amd.ops as ops
+    for N in (100, 20000):
+        x = 1e25 * rand(1, 1, N, 16)
+        y = ops.group_norm_act(x.to(DEV), 2, None, rand(2, 16).to(DEV))
+        assert torch.isfinite(y).all()
+
+
 def test_maps_in_either_order():
     """Tokens of a map: in channels-last order they are read as they are, others are copied; the same bits."""
     import medvision_amd.ops as ops
@@ -207,7 +232,7 @@ def test_refusals():
                        (lambda: ops.group_norm_act(x, 3, w.half()), "weight has dtype"), (lambda: ops.group_norm_act(x.double(), 3), "float32, float16 or bfloat16"),
                        (lambda: ops.group_norm_act(x, 3, w.cpu()), "weight is on cpu"), (lambda: ops.group_norm_act(x[0, 0], 3), "batch, ..., channels"),
                        (lambda: ops.group_norm_act(x, 3, activation="elu"), "activation 'elu'"),
-                       (lambda: ops.group_norm_act(torch.zeros(65536, 1, 4, device=DEV), 1), "wrong sizes")]:
+                       (lambda: ops.group_norm_act(torch.zeros(65536, 6000, 1, device=DEV, dtype=torch.float16), 1), "a batch of 65536")]:
         with pytest.raises(RuntimeError, match=text):
             call()
     y = ops.group_norm_act(x.requires_grad_(True), 3)

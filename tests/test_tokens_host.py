@@ -36,7 +36,7 @@ def test_group_norm_entry_points_refuse_on_the_host():
                                           None, 0, None)
 
     for call in (forward, backward):
-        for wrong in (dict(batch=-1), dict(batch=65536), dict(cells=-1), dict(channels=0), dict(groups=0), dict(groups=3), dict(activation=5), dict(activation=-1),
+        for wrong in (dict(batch=-1), dict(cells=-1), dict(cells=2 ** 37), dict(channels=0), dict(groups=0), dict(groups=3), dict(activation=5), dict(activation=-1),
                       dict(dtype=_lib.MV_F64), dict(weight_dtype=_lib.MV_BF16)):
             assert call(**wrong) == 1 and lib.mv_last_error()
         assert call(batch=0) == 0 and call(cells=0) == 0
@@ -46,6 +46,10 @@ def test_group_norm_entry_points_refuse_on_the_host():
     p = ctypes.c_void_p(16)
     assert lib.mv_group_norm(p, None, None, p, p, 2, 3, 8, 2, 1e-5, 0, 0.0, _lib.MV_F16, _lib.MV_F16, None, 0, None) == 1
     assert b"workspace" in lib.mv_last_error()
+    assert lib.mv_group_norm(p, None, None, p, p, 65536, 6000, 8, 2, 1e-5, 0, 0.0, _lib.MV_F16, _lib.MV_F16, p, 1 << 40, None) == 1
+    assert b"a batch of 65536" in lib.mv_last_error()
+    assert lib.mv_group_norm_backward(p, None, None, p, p, p, None, None, 65536, 6000, 8, 2, 0, 0.0, _lib.MV_F16, _lib.MV_F16, p, 1 << 40, None) == 1
+    assert b"a batch of 65536" in lib.mv_last_error()
     assert lib.mv_group_norm_workspace_bytes(2, 3, 8, 2) > 0 and lib.mv_group_norm_backward_workspace_bytes(2, 3, 8, 2) > 0
     for wrong in ((0, 3, 8, 2), (2, 0, 8, 2), (2, 3, 8, 3), (2, 3, 0, 1), (2, -1, 8, 2)):
         assert lib.mv_group_norm_workspace_bytes(*wrong) == 0 and lib.mv_group_norm_backward_workspace_bytes(*wrong) == 0
@@ -125,7 +129,7 @@ def test_plain_rotary_turns_and_turns_back(neighbours):
 def test_frequencies_of_axes():
     import medvision_amd.ops as ops
     f = ops.axis_frequencies(32, 3, 100.0)
-    assert f.shape == (3, 15) and f.dtype == torch.float64
+    assert f.shape == (3, 16) and f.dtype == torch.float64 and f[:, 15].abs().sum() == 0
     assert torch.allclose(f[1, 5:10], 100.0 ** (-torch.arange(5, dtype=torch.float64) / 5)) and f[1, :5].abs().sum() == 0 and f[1, 10:].abs().sum() == 0
     assert ops.axis_frequencies(9, 1).shape == (1, 4)
     for wrong in ((5, 3), (16, 0), (1, 1)):
@@ -194,14 +198,14 @@ def test_modules():
     was = r.frequencies.clone()
     for cast in (lambda t: t.half(), lambda t: t.float(), lambda t: t.to(torch.bfloat16)):
         assert cast(r).frequencies.dtype == torch.float64 and torch.equal(r.frequencies, was)
-    assert "RotaryPositions((3, 15)" in repr(r)
+    assert "RotaryPositions((3, 16)" in repr(r)
 
 
 def test_layer_with_axes_wants_positions():
     import medvision_amd.ops as ops
     x, tokens = torch.zeros(1, 2, 96), torch.zeros(1, 3, 96)
     layer, plain = ops.RegionDecoderLayer(96, 6, axes=3), ops.RegionDecoderLayer(96, 6)
-    assert layer.place.frequencies.shape == (3, 6) and plain.place is None and "place.frequencies" not in plain.state_dict()
+    assert layer.place.frequencies.shape == (3, 8) and plain.place is None and "place.frequencies" not in plain.state_dict()
     assert set(plain.state_dict()) | {"place.frequencies"} == set(layer.state_dict())
     q = torch.zeros(1, 2, 6, 16)
     with pytest.raises(ValueError, match="region_positions are missing"):
