@@ -76,10 +76,12 @@ template <typename T> struct Product {
 // columns go through LDS, without registers on the way (x: rows in whole pieces of 16 bytes), the next block's while this one is
 // multiplied; scales go to the lanes that want them.  A row of x is 256 bytes there, sixteen pieces, piece c of row r at c ^ (r & 15); a row of
 // weights four, piece g at g ^ turned(r): reads of 16 rows side by side spread over all banks.
-// 4000 x 4096 x 4096 in bf16 with groups of 128, 64, 32: 128, 141, 168 us = 1.05, 0.95, 0.80 PFLOP/s (a plain product of the library: 1.21;
-// this kernel without its scales: 1.17).  What the scales take is the additions of the scaled sums, an instruction for each result and
-// group, beside the matrix units' own; decoding takes nothing.  Two workgroups share a compute unit, so that one multiplies while
-// the other waits for its operands: tiles of 128 x 256, of which one fits, took 145 us with groups of 128.
+// 4000 x 4096 x 4096 in bf16 with groups of 128, 64, 32: 130, 147, 172 us = 1.03, 0.91, 0.78 PFLOP/s (a plain product of the library: 1.21;
+// this kernel without its scales: 1.17); 2000 x 12544 x 1024 with groups of 64 62 us and 8 for the join: its loads alone take 52, its
+// reads and products alone 48.  What the scales take is the additions of the scaled sums, an instruction for each result and group;
+// decoding takes nothing.  Two workgroups share a compute unit, so that one multiplies while the other waits for its operands:
+// tiles of 128 x 256, of which one fits, took 145 us with groups of 128.  Without gain: products of 32 x 32, matrix instructions with the
+// additions of the group before in between, scales brought a block ahead.
 constexpr int kTile = 128, kTileThreads = 256, kTileRows = kTile * 256, kStage = kTileRows + kTile * 64;   // bytes of the rows, of a block
 __device__ __forceinline__ int turned(int row) { return (row / 2 & 3) ^ (row / 8 & 1); }
 
@@ -88,14 +90,15 @@ template <typename T, int Group> __global__ __launch_bounds__(kTileThreads, 2) v
   __shared__ __attribute__((aligned(16))) unsigned char lds[2 * kStage];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, g = lane >> 4;
   const int wm = wave % 2, wn = wave / 2;
-  // tiles in an order in which neighbouring workgroups of a die share rows and weights: eight rows of tiles at a time
+  // tiles in an order in which neighbouring workgroups of a die share rows and weights: four rows of tiles at a time, for rows are four
+  // times as many bytes as weights (1000 x 12544 x 1024: 44 us, of eight 50)
   const int tiles = k.m_tiles * k.n_tiles;
   unsigned id = linear_block();
   if (id >= static_cast<unsigned>(tiles) * k.splits) return;
   const int split = id / tiles;
   id = xcd_contiguous(id % tiles, tiles);
-  const int band = id / (8 * k.n_tiles), in_band = id % (8 * k.n_tiles), tall = min(8, k.m_tiles - 8 * band);
-  const long m0 = (8L * band + in_band % tall) * kTile;
+  const int band = id / (4 * k.n_tiles), in_band = id % (4 * k.n_tiles), tall = min(4, k.m_tiles - 4 * band);
+  const long m0 = (4L * band + in_band % tall) * kTile;
   const int n0 = in_band / tall * kTile;
   const int first = static_cast<int>(static_cast<long>(k.blocks) * split / k.splits), last = static_cast<int>(static_cast<long>(k.blocks) * (split + 1) / k.splits);
 
