@@ -29,27 +29,27 @@ template <> struct Activation<MV_SILU> {
   }
 };
 // z P(z), P the normal distribution's: P(-a) = 2^(-a^2 log2(e) / 2) g(a) for a >= 0, g(a) = erfcx(a / sqrt 2) / 2, which
-// has no cancellation.  g is a polynomial of degree 9 in t = 3 / (a + 3), without constant term, fitted to the least
-// relative error over 0 <= a <= 14 (5e-8; in 32 bits 4e-7); beyond that the exponential is zero.
+// has no cancellation; z P(z) = max(z, 0) - |z| P(-|z|).  g is a polynomial of degree 9 in t = 1 / (a + 3), without constant
+// term, fitted to the least relative error over 0 <= a <= 14 (5e-8; in 32 bits 4e-7); beyond that the exponential is zero.
 template <> struct Activation<MV_GELU> {
   static __device__ __forceinline__ float tail(float z, float &bell) {   // P(-|z|); bell = 2^(-z^2 log2(e) / 2)
-    const float t = 3.f * __builtin_amdgcn_rcpf(fabsf(z) + 3.f);
-    float g = -2.276401745e-2f;
-    g = fmaf(g, t, 1.295948172e-1f);
-    g = fmaf(g, t, -2.712782945e-1f);
-    g = fmaf(g, t, 2.189550510e-1f);
-    g = fmaf(g, t, -5.337175970e-2f);
-    g = fmaf(g, t, 1.199162648e-1f);
-    g = fmaf(g, t, 1.124179544e-1f);
-    g = fmaf(g, t, 1.335751283e-1f);
-    g = fmaf(g, t, 1.329548793e-1f);
+    const float t = __builtin_amdgcn_rcpf(fabsf(z) + 3.f);
+    float g = -4.480641555e+02f;
+    g = fmaf(g, t, 8.502715956e+02f);
+    g = fmaf(g, t, -5.932856301e+02f);
+    g = fmaf(g, t, 1.596182322e+02f);
+    g = fmaf(g, t, -1.296933761e+01f);
+    g = fmaf(g, t, 9.713217449e+00f);
+    g = fmaf(g, t, 3.035284769e+00f);
+    g = fmaf(g, t, 1.202176155e+00f);
+    g = fmaf(g, t, 3.988646379e-01f);
     bell = __builtin_amdgcn_exp2f(-0.721347520f * z * z);
-    return bell * (g * t);
+    return bell * t * g;
   }
   static __device__ __forceinline__ float value(float z, float) {
     float bell;
     const float p = tail(z, bell);
-    return z * (z > 0.f ? 1.f - p : p);
+    return fmaf(-fabsf(z), p, z > 0.f ? z : 0.f);   // (NaN: the product's)
   }
   static __device__ __forceinline__ float slope(float z, float) {
     float bell;

@@ -7,7 +7,9 @@
 //
 // Sums over the cells are kept for each channel: a thread has eight neighbouring channels and a share of the cells, a
 // workgroup joins its threads' shares, and a small kernel joins the workgroups' to those of a group.  Two kernels with a pass over
-// memory each, then; bound by memory.
+// memory each, then; bound by memory: 2 x 128^3 cells of 32 channels in float16 (268 MB a pass) 60 us the sums, 5 the join, 95 the second
+// pass; gradients 109 and 159 us, 7 the join (4.5 - 5.6 TB/s, about a copy's 4.9).  2 x 27648 cells of 256 channels in bf16, which caches
+// hold: 10.5, 4, and 12 us with SiLU; the exact GELU's instructions make it 17.
 #include "activation.hpp"
 #include "group_norm.hpp"
 #include "rows.hpp"

