@@ -373,7 +373,8 @@ int mv_block_linear(const void *q, const void *q_scales, const void *weight, con
  * weight, bias: [channels] of `weight_dtype`, `dtype` or MV_F32 (NULL: ones, zeros).  low: the slope of MV_LEAKY_RELU below
  * zero.  MV_GELU is z times the normal distribution's value.  stats [3, batch, groups] float32 receives each group's mean,
  * what rounding took from it, and 1 / sqrt(var + eps).
- * ..._backward WRITES grad_x, grad_weight and grad_bias (of weight_dtype); each may be NULL where nobody wants it.  At the
+ * Results do not overlap what is read.  ..._backward WRITES grad_x, grad_weight and grad_bias (of weight_dtype); each may be NULL
+ * where nobody wants it.  At the
  * border of two branches the derivative is the lower one's.  Sums are formed in a fixed order.  Batches of 65536 and more
  * are taken for small samples only (a group whose values fit into a workgroup's registers), others are refused. */
 typedef enum { MV_NO_ACTIVATION = 0, MV_RELU = 1, MV_LEAKY_RELU = 2, MV_SILU = 3, MV_GELU = 4 } mv_activation;
@@ -390,7 +391,8 @@ int mv_group_norm_backward(const void *x, const void *weight, const void *bias, 
  * sum over a of places[batch, row, a] * frequencies[a, p] (radians; formed in 64 bits).  A pair is (p, pairs + p), or
  * (2p, 2p + 1) where `neighbours` is not 0; channels behind 2 * pairs stay.  back != 0 turns the other way, which is the
  * gradient.  x is read through strides (elements; the channels of a head are neighbours; dim 1..1024), places (`place_dtype`
- * MV_F32, MV_F64 or MV_I32; axes 1..8) too (0: shared by a batch); frequencies [axes, pairs] are float64 and dense, y is dense. */
+ * MV_F32, MV_F64 or MV_I32; axes 1..8) too (0: shared by a batch); frequencies [axes, pairs] are float64 and dense, y is
+ * dense and does not overlap x. */
 typedef struct {
   int batch, rows, heads, dim, axes, pairs;
   int64_t x_strides[3];     /* batch, row, head */

@@ -33,6 +33,7 @@ struct Divisor {
 struct Rotary {
   mv_rotary_shape of;
   int block_rows, row_blocks, pieces, kept, unit;   // pieces of eight pairs (channels) of a head; units of the channels that stay
+  int kept_here;   // units that go with a head's first pieces (0: by themselves)
   Divisor by_pairs, by_pieces, by_heads, by_kept;
 };
 
@@ -63,6 +64,29 @@ template <typename T, int N> __device__ __forceinline__ void copy_unit(const T *
   for (unsigned i = 0; i < N * sizeof(T); i += sizeof(bytes))
     reinterpret_cast<Loose<bytes, sizeof(T)> *>(reinterpret_cast<char *>(to) + i)->v = reinterpret_cast<const Loose<bytes, sizeof(T)> *>(reinterpret_cast<const char *>(from) + i)->v;
 }
+
+// Up to 16 bytes of channels that stay
+template <typename T> struct Stays {
+  u32x4 bits;
+  template <typename V> static __device__ __forceinline__ Loose<V, sizeof(T)> *at(T *p) { return reinterpret_cast<Loose<V, sizeof(T)> *>(p); }
+  template <typename V> static __device__ __forceinline__ const Loose<V, sizeof(T)> *at(const T *p) { return reinterpret_cast<const Loose<V, sizeof(T)> *>(p); }
+  __device__ __forceinline__ void load(int unit, const T *p) {
+    switch (unit * sizeof(T)) {
+      case 16: bits = at<u32x4>(p)->v; break;
+      case 8: { const u32x2 v = at<u32x2>(p)->v; bits = {v[0], v[1], 0u, 0u}; break; }
+      case 4: bits = {at<unsigned>(p)->v, 0u, 0u, 0u}; break;
+      default: bits = {at<unsigned short>(p)->v, 0u, 0u, 0u};
+    }
+  }
+  __device__ __forceinline__ void store(int unit, T *p) const {
+    switch (unit * sizeof(T)) {
+      case 16: at<u32x4>(p)->v = bits; break;
+      case 8: at<u32x2>(p)->v = u32x2{bits[0], bits[1]}; break;
+      case 4: at<unsigned>(p)->v = bits[0]; break;
+      default: at<unsigned short>(p)->v = static_cast<unsigned short>(bits[0]);
+    }
+  }
+};
 
 // Cosines and sines of a workgroup's rows
 __device__ __forceinline__ void form_table(float2 *table, const void *places, int place_kind, const double *frequencies, const Rotary &k, int b, int first,
@@ -101,7 +125,8 @@ template <bool Neighbours> __device__ __forceinline__ void turn_piece(const floa
 }
 
 // Pieces are of eight pairs (neighbours: of eight channels).  The last one of a head starts earlier than its place where the pairs
-// do not fill it: what two pieces have in common is formed twice, with the same results, instead of an element at a time.
+// do not fill it: what two pieces have in common is formed twice, with the same results, instead of an element at a time.  Channels
+// that stay go with a head's first pieces where there are no more units of them: by themselves, later, they cost 37 instead of 31 us.
 // A thread's first piece is on its way while the angles are formed.
 template <typename T, bool Neighbours>
 __global__ __launch_bounds__(kThreads) void rotary(const T *x, const void *places, int place_kind, const double *frequencies, T *y,
@@ -116,12 +141,12 @@ __global__ __launch_bounds__(kThreads) void rotary(const T *x, const void *place
   T *const to = y + (static_cast<long>(b) * s.rows + first) * s.heads * s.dim;
   const int lines = rows * s.heads, width = Neighbours ? 2 * pairs : pairs, items = lines * k.pieces;
   struct Piece {
-    int row, c;
+    int row, c, own;
     long from, to;
   };
   auto piece_of = [&](int e) {
-    const int line = k.by_pieces.of(e), row = k.by_heads.of(line), c = max(0, min((e - line * k.pieces) * 8, width - 8));
-    return Piece{row, c, row * s.x_strides[1] + (line - row * s.heads) * s.x_strides[2] + c, static_cast<long>(line) * s.dim + c};
+    const int line = k.by_pieces.of(e), row = k.by_heads.of(line), own = e - line * k.pieces, c = max(0, min(own * 8, width - 8));
+    return Piece{row, c, own, row * s.x_strides[1] + (line - row * s.heads) * s.x_strides[2] + c, static_cast<long>(line) * s.dim + c};
   };
   if (width >= 8) {
     bool formed = false;
@@ -130,6 +155,10 @@ __global__ __launch_bounds__(kThreads) void rotary(const T *x, const void *place
       Raw<T> one, two;
       one.load(from + p.from);
       if (!Neighbours) two.load(from + p.from + pairs);
+      const bool keeps = p.own < k.kept_here;
+      const int after = 2 * pairs - p.c + p.own * k.unit;   // from the piece to its unit of the channels that stay
+      Stays<T> stays;
+      if (keeps) stays.load(k.unit, from + p.from + after);
       if (!formed) {
         form_table(table, places, place_kind, frequencies, k, b, first, rows, back);
         __syncthreads();
@@ -142,7 +171,9 @@ __global__ __launch_bounds__(kThreads) void rotary(const T *x, const void *place
       turn_piece<Neighbours>(table + p.row * pairs + (Neighbours ? p.c / 2 : p.c), 8, v, w);
       store8(to + p.to, 8, v);
       if (!Neighbours) store8(to + p.to + pairs, 8, w);
+      if (keeps) stays.store(k.unit, to + p.to + after);
     }
+    if (k.kept_here) return;
   } else {   // heads of few pairs
     form_table(table, places, place_kind, frequencies, k, b, first, rows, back);
     __syncthreads();
@@ -189,7 +220,7 @@ extern "C" int mv_rotary_positions(const void *x, const void *places, const void
   MV_REQUIRE(row < (1L << 31), "rows of %d heads of %d channels are too long", s.heads, s.dim);
   const int kept = s.dim - 2 * s.pairs, unit = kept % 8 == 0 ? 8 : kept % 4 == 0 ? 4 : kept % 2 == 0 ? 2 : 1;
   const int pieces = ((neighbours ? 2 : 1) * s.pairs + 7) / 8;
-  Rotary k{s, 0, 0, pieces, kept / unit, unit, Divisor(std::max(1, s.pairs)), Divisor(std::max(1, pieces)), Divisor(s.heads), Divisor(std::max(1, kept / unit))};
+  Rotary k{s, 0, 0, pieces, kept / unit, unit, unit * dtype_size(dtype) <= 16 && kept / unit <= pieces ? kept / unit : 0, Divisor(std::max(1, s.pairs)), Divisor(std::max(1, pieces)), Divisor(s.heads), Divisor(std::max(1, kept / unit))};
   // Up to 4096 elements a workgroup (2 x 32768 x 8 heads of 64 in bf16: 37 us; 8192 47, 2048 44), fewer where that would leave compute
   // units without one
   const long spread = static_cast<long>(s.batch) * s.rows / 1024;

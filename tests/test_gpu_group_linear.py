@@ -129,7 +129,7 @@ def test_without_a_workspace():
 
 def test_streams_and_replays():
     import medvision_amd.ops as ops
-    sizes = [(1, 9000, 64), (40, 2048, 256), (300, 512, 128)]
+    sizes = [(1, 9000, 64), (40, 2048, 256), (300, 512, 128), (200, 4099, 100)]
     layers = [tuple(t.to(DEV) for t in ref.quantize_groups(rand(n, size[2], size[1]), 32)) for n, size in enumerate(sizes)]
     xs = [rand(9 + n, size[0], size[1], dtype=torch.float16).to(DEV) for n, size in enumerate(sizes)]
     step = lambda: [ops.group_linear(x, *w) for x, w in zip(xs, layers)]   # noqa: E731

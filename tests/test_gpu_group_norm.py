@@ -141,8 +141,8 @@ def test_maps_in_either_order():
     assert torch.equal(ops.group_norm_act(flat, 3), ops.group_norm_act(flat.clone(), 3))
 
 
-@pytest.mark.parametrize("kind", [None, "gelu"])
-def test_gradients_of_some_inputs_and_both_forms_of_the_node(kind):
+@pytest.mark.parametrize("kind,cells", [(None, 90), ("gelu", 90), ("silu", 7000)])
+def test_gradients_of_some_inputs_and_both_forms_of_the_node(kind, cells):
     from medvision_amd.ops.group_norm import GroupNormActFunction
 
     class Python(GroupNormActFunction):
@@ -150,7 +150,7 @@ def test_gradients_of_some_inputs_and_both_forms_of_the_node(kind):
         def backward(ctx, grad):
             return GroupNormActFunction.backward(ctx, grad)
 
-    tensors, go = (rand(1, 3, 90, 20), rand(2, 20), rand(3, 20)), rand(4, 3, 90, 20).to(DEV)
+    tensors, go = (rand(1, 3, cells, 20), rand(2, 20), rand(3, 20)), rand(4, 3, cells, 20).to(DEV)
 
     def grads(function, wanted):
         ins = [t.to(DEV).requires_grad_(w) for t, w in zip(tensors, wanted)]
