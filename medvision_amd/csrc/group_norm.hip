@@ -9,7 +9,7 @@
 // workgroup joins its threads' shares, and a small kernel joins the workgroups' to those of a group.  Two kernels with a pass over
 // memory each, then; bound by memory: 2 x 128^3 cells of 32 channels in float16 (268 MB a pass) 60 us the sums, 5 the join, 95 the second
 // pass; gradients 109 and 159 us, 7 the join (4.5 - 5.6 TB/s, about a copy's 4.9).  2 x 27648 cells of 256 channels in bf16, which caches
-// hold: 10.5, 4, and 12 us with SiLU; the exact GELU's instructions make it 17.
+// hold: 10.5, 4, and 12 us with SiLU; the exact GELU's instructions make it 16.
 #include "activation.hpp"
 #include "group_norm.hpp"
 #include "rows.hpp"
@@ -55,8 +55,8 @@ __device__ __forceinline__ Place place_of(const Cells &s, unsigned chunk) {
 // whole with results that go past the caches.
 enum Form { kParts, kWhole, kWholePast };
 
-// Eight channels of a cell: as they are in memory where all of them exist, so that several cells' loads
-// are on their way before the first is used.
+// Eight channels of a cell: as they are in memory where all of them exist, so that several cells' loads are on their way before the
+// first is used.
 template <typename T, int F> struct Eight {
   Raw<T> raw;
   __device__ __forceinline__ void load(const T *p, int) { raw.load(p); }

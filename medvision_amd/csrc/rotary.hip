@@ -5,8 +5,8 @@
 // A pair is (p, pairs + p), or (2p, 2p + 1).  Angles are formed in 64 bits (32 would lose the turn of far places) in
 // quarters of a turn, whose whole part swaps sine and cosine and whose rest goes through a polynomial in 32 bits.  A
 // workgroup forms the angles of its rows once for all heads, in LDS.  Bound by memory, one pass over it: 2 x 32768 rows of 8 heads of 64 in
-// bf16 with 30 pairs 30 - 35 us (134 MB, 3.9 - 4.4 TB/s; with 32 pairs, which start at whole pieces, 31 where 30 take 37), 2 x 27648 of 8 heads
-// of 32 in float16, neighbours, 15.5 us a way (57 MB).
+// bf16 with 30 pairs 29 - 32 us (134 MB, 4.2 - 4.6 TB/s; with 32 pairs 31), 2 x 27648 of 8 heads
+// of 32 in float16, neighbours, 15 us a way (57 MB).
 #include "rows.hpp"
 
 #include <algorithm>
@@ -213,21 +213,21 @@ extern "C" int mv_rotary_positions(const void *x, const void *places, const void
   MV_REQUIRE(place_dtype == MV_F32 || place_dtype == MV_F64 || place_dtype == MV_I32, "places have dtype %d, expected float32, float64 or int32", place_dtype);
   MV_REQUIRE(s.batch >= 0 && s.rows >= 0 && s.heads >= 0 && s.dim >= 1 && s.dim <= kMostDim && s.axes >= 1 && s.axes <= kMostAxes,
              "wrong sizes: a batch of %d, %d rows, %d heads of %d channels (1 to %d), %d axes (1 to %d)", s.batch, s.rows, s.heads, s.dim, kMostDim, s.axes, kMostAxes);
-  MV_REQUIRE(s.pairs >= 0 && 2 * s.pairs <= s.dim, "%d pairs of %d channels", s.pairs, s.dim);
+  MV_REQUIRE(s.pairs >= 0 && s.pairs <= s.dim / 2, "%d pairs of %d channels", s.pairs, s.dim);
   if (s.batch == 0 || s.rows == 0 || s.heads == 0) return MV_OK;
   MV_REQUIRE(x && y && (s.pairs == 0 || (places && frequencies)), "a tensor is missing");
   const long row = static_cast<long>(s.heads) * s.dim;
-  MV_REQUIRE(row < (1L << 31), "rows of %d heads of %d channels are too long", s.heads, s.dim);
+  MV_REQUIRE(row <= (1L << 30), "rows of %d heads of %d channels are too long", s.heads, s.dim);
   const int kept = s.dim - 2 * s.pairs, unit = kept % 8 == 0 ? 8 : kept % 4 == 0 ? 4 : kept % 2 == 0 ? 2 : 1;
   const int pieces = ((neighbours ? 2 : 1) * s.pairs + 7) / 8;
   Rotary k{s, 0, 0, pieces, kept / unit, unit, unit * dtype_size(dtype) <= 16 && kept / unit <= pieces ? kept / unit : 0, Divisor(std::max(1, s.pairs)), Divisor(std::max(1, pieces)), Divisor(s.heads), Divisor(std::max(1, kept / unit))};
-  // Up to 4096 elements a workgroup (2 x 32768 x 8 heads of 64 in bf16: 37 us; 8192 47, 2048 44), fewer where that would leave compute
+  // Up to 4096 elements a workgroup (2 x 32768 x 8 heads of 64 in bf16: 37 us, with 8192 47, with 2048 44), fewer where that would leave compute
   // units without one
   const long spread = static_cast<long>(s.batch) * s.rows / 1024;
   k.block_rows = static_cast<int>(std::max(1L, std::min({4096L / row, 64L, kTable / std::max(1L, static_cast<long>(s.pairs)), static_cast<long>(s.rows), spread})));
   k.row_blocks = (s.rows + k.block_rows - 1) / k.block_rows;
   const long blocks = static_cast<long>(s.batch) * k.row_blocks;
-  MV_REQUIRE(blocks < (1L << 32), "too many rows: %d in a batch of %d", s.rows, s.batch);
+  MV_REQUIRE(blocks < (1L << 31), "too many rows: %d in a batch of %d", s.rows, s.batch);
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const size_t lds = sizeof(float2) * k.block_rows * s.pairs;
   MV_FLOATS(dtype, {

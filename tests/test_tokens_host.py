@@ -63,8 +63,8 @@ def test_rotary_entry_point_refuses_on_the_host():
         s = _lib.RotaryShape(batch, rows, heads, dim, axes, pairs)
         return lib.mv_rotary_positions(*[None] * 4, ctypes.byref(s), 0, 0, dtype, place, None)
 
-    for wrong in (dict(batch=-1), dict(dim=0), dict(dim=1025), dict(axes=0), dict(axes=9), dict(pairs=5), dict(pairs=-1), dict(dtype=_lib.MV_F64),
-                  dict(place=_lib.MV_F16), dict(heads=2 ** 28, dim=512)):
+    for wrong in (dict(batch=-1), dict(dim=0), dict(dim=1025), dict(axes=0), dict(axes=9), dict(pairs=5), dict(pairs=-1), dict(pairs=2 ** 30 + 1), dict(dtype=_lib.MV_F64),
+                  dict(place=_lib.MV_F16), dict(heads=2 ** 28, dim=512), dict(heads=2 ** 21 + 1, dim=512)):
         assert call(**wrong) == 1 and lib.mv_last_error()
     assert call() == 1 and b"missing" in lib.mv_last_error()
     assert call(rows=0) == 0 and call(heads=0) == 0 and call(batch=0) == 0
