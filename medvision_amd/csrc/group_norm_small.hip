@@ -187,10 +187,10 @@ __global__ __launch_bounds__(1024) void group_grad_whole(const T *x, const T *gy
   }
   __syncthreads();
   for (int c = threadIdx.x; c < s.group_channels; c += blockDim.x) {
-    float2 t = {0.f, 0.f};
+    double t = 0., u = 0.;   // (up to a thousand rows one after the other)
 #pragma unroll 4
-    for (int k = 0; k < lines; ++k) t.x += rows[k * s.group_channels + c].x, t.y += rows[k * s.group_channels + c].y;
-    sums[static_cast<long>(p.b) * s.channels + p.g * s.group_channels + c] = t;
+    for (int k = 0; k < lines; ++k) t += rows[k * s.group_channels + c].x, u += rows[k * s.group_channels + c].y;
+    sums[static_cast<long>(p.b) * s.channels + p.g * s.group_channels + c] = {static_cast<float>(t), static_cast<float>(u)};
   }
 }
 
