@@ -122,6 +122,14 @@ __global__ __launch_bounds__(1024) void group_whole(const T *x, const void *weig
     }
 }
 
+// Every step-th of the rows from the first, in 64 bits
+__device__ __forceinline__ float2 join_rows(const float2 *column, int first, int step, int lines, int channels) {
+  double t = 0., u = 0.;
+#pragma unroll 4
+  for (int k = first; k < lines; k += step) t += column[k * channels].x, u += column[k * channels].y;
+  return {static_cast<float>(t), static_cast<float>(u)};
+}
+
 // The gradients of a group of a sample: gx, and the sums of its channels, sums[sample][channel].
 template <typename T, int V, int U, int Kind>
 __global__ __launch_bounds__(1024) void group_grad_whole(const T *x, const T *gy, const float *stats, const void *weight, const void *bias, bool wide, T *gx,
@@ -186,12 +194,17 @@ __global__ __launch_bounds__(1024) void group_grad_whole(const T *x, const T *gy
     for (int i = 0; i < V; ++i) rows[line * s.group_channels + unit % s.units * V + i] = {one[i], two[i]};
   }
   __syncthreads();
-  for (int c = threadIdx.x; c < s.group_channels; c += blockDim.x) {
-    double t = 0., u = 0.;   // (up to a thousand rows one after the other)
-#pragma unroll 4
-    for (int k = 0; k < lines; ++k) t += rows[k * s.group_channels + c].x, u += rows[k * s.group_channels + c].y;
-    sums[static_cast<long>(p.b) * s.channels + p.g * s.group_channels + c] = {static_cast<float>(t), static_cast<float>(u)};
+  // Then sixteen threads to a channel (each leaves its sum in the first row that it reads, which no other reads), and one over their sums:
+  // 3 x 1955 x 60 in 6 groups 15.4 us, with one thread to a channel 18
+  const int strides = min(16, static_cast<int>(blockDim.x) / s.group_channels);
+  if (strides > 1 && lines > strides) {
+    const int c = threadIdx.x % s.group_channels, first = threadIdx.x / s.group_channels;
+    if (first < strides) rows[first * s.group_channels + c] = join_rows(rows + c, first, strides, lines, s.group_channels);
+    __syncthreads();
+    lines = strides;
   }
+  for (int c = threadIdx.x; c < s.group_channels; c += blockDim.x)
+    sums[static_cast<long>(p.b) * s.channels + p.g * s.group_channels + c] = join_rows(rows + c, 0, 1, lines, s.group_channels);
 }
 
 constexpr int forward_cells(int v) { return 64 / v > 16 ? 16 : 64 / v; }
