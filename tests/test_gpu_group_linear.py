@@ -97,6 +97,17 @@ def test_what_is_not_finite_stays_in_its_row(rows, inputs):
     assert torch.equal(y[keep], want[keep])
 
 
+@pytest.mark.parametrize("rows", [1, 2, 13, 40, 200])
+def test_small_values(rows):
+    """float16 below its least normal value counts in full: whole multiples of 2^-24, and sums that are exact in 32 bits."""
+    import medvision_amd.ops as ops
+    codes, scales = ref.quantize_groups(rand(3, 70, 200), 32)
+    scales = torch.full_like(scales, 2.0 ** 12)
+    x = torch.randint(-15, 16, (rows, 200), generator=torch.Generator().manual_seed(5)).double() * 2.0 ** -24
+    y = ops.group_linear(x.half().to(DEV), codes.to(DEV), scales.to(DEV))
+    assert torch.equal(y.cpu(), (x @ ref.group_values(codes, scales, 200).t()).half())
+
+
 def test_layouts():
     import medvision_amd.ops as ops
     codes, scales = (t.to(DEV) for t in ref.quantize_groups(rand(3, 70, 300), 64))
