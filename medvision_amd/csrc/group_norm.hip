@@ -9,7 +9,7 @@
 // workgroup joins its threads' shares, and a small kernel joins the workgroups' to those of a group.  Two kernels with a pass over
 // memory each, then; bound by memory: 2 x 128^3 cells of 32 channels in float16 (268 MB a pass) 60 us the sums, 5 the join, 95 the second
 // pass; gradients 109 and 159 us, 7 the join (4.5 - 5.6 TB/s, about a copy's 4.9).  2 x 27648 cells of 256 channels in bf16, which caches
-// hold: 10.5, 4, and 12 us with SiLU; the exact GELU's instructions make it 16.
+// hold: 9, 4, and 12 us with SiLU; the exact GELU's instructions make it 16.
 #include "activation.hpp"
 #include "group_norm.hpp"
 #include "rows.hpp"
@@ -32,11 +32,20 @@ struct Cells {
 // that it has in common with the one before are worked out twice, with the same results.
 __device__ __forceinline__ int first_channel(const Cells &s, int octet) { return max(0, min(octet * 8, s.channels - 8)); }
 
+// Cells of a chunk, and those of them that a row of a tile takes.  (In 32 bits, and divided once for a workgroup: divisions in 64 bits by
+// each thread and row took the sums of 2 x 27648 cells of 256 channels from 9.2 to 11.4 us.)
+__device__ __forceinline__ int cells_in(const Cells &s, unsigned chunk) { return static_cast<int>(min(s.each, s.cells - chunk * s.each)); }
+struct Rows {
+  int each, more;
+  __device__ __forceinline__ Rows(const Cells &s, int cells) : each(cells / s.tile_rows), more(cells % s.tile_rows) {}
+  __device__ __forceinline__ int of(int row) const { return each + (row < more ? 1 : 0); }
+};
+
 // Where a thread stands: channels from c on (`left` of them exist), `cells` cells that are `stride` elements apart, the first one
 // `at` elements from the start.
 struct Place {
-  int c, left;
-  long cells, stride, at;
+  int c, left, cells;
+  long stride, at;
 };
 __device__ __forceinline__ Place place_of(const Cells &s, unsigned chunk) {
   Place p;
@@ -44,10 +53,9 @@ __device__ __forceinline__ Place place_of(const Cells &s, unsigned chunk) {
   const int piece = blockIdx.y * kThreads + octet;
   p.c = first_channel(s, piece);
   p.left = s.channels - piece * 8 > 0 ? s.channels - p.c : 0;
-  const long first = chunk * s.each + row, last = min(s.cells, (chunk + 1) * s.each);
-  p.cells = row < s.tile_rows && p.left > 0 && first < last ? (last - first + s.tile_rows - 1) / s.tile_rows : 0;
+  p.cells = row < s.tile_rows && p.left > 0 ? Rows(s, cells_in(s, chunk)).of(row) : 0;
   p.stride = static_cast<long>(s.tile_rows) * s.channels;
-  p.at = (static_cast<long>(blockIdx.z) * s.cells + first) * s.channels + p.c;
+  p.at = (static_cast<long>(blockIdx.z) * s.cells + chunk * s.each + row) * s.channels + p.c;
   return p;
 }
 
@@ -85,9 +93,9 @@ template <typename T, int F> __device__ __forceinline__ void put_eight(T *p, int
 // Pieces of kAtOnce cells, the last one again where there are fewer left.
 constexpr int kAtOnce = 4;
 template <typename T, int F>
-__device__ __forceinline__ void load_cells(Eight<T, F> (&to)[kAtOnce], const T *at, long cells, const Place &p) {
+__device__ __forceinline__ void load_cells(Eight<T, F> (&to)[kAtOnce], const T *at, int cells, const Place &p) {
 #pragma unroll
-  for (int n = 0; n < kAtOnce; ++n) to[n].load(at + min(static_cast<long>(n), cells - 1) * p.stride, p.left);
+  for (int n = 0; n < kAtOnce; ++n) to[n].load(at + min(n, cells - 1) * p.stride, p.left);
 }
 
 // What the rows of a tile have of each of its channels, joined by teams of threads and then over the teams, in a fixed order:
@@ -124,7 +132,7 @@ __global__ __launch_bounds__(kThreads) void group_sums(const T *x, Moments *part
   const Place p = place_of(s, blockIdx.x);
   float middle[8] = {}, sum[8] = {}, squares[8] = {};
   const T *at = x + p.at;
-  for (long done = 0; done < p.cells; done += kAtOnce, at += kAtOnce * p.stride) {
+  for (int done = 0; done < p.cells; done += kAtOnce, at += kAtOnce * p.stride) {
     Eight<T, F> raw[kAtOnce];
     load_cells(raw, at, p.cells - done, p);
     if (done == 0) {
@@ -156,15 +164,15 @@ __global__ __launch_bounds__(kThreads) void group_sums(const T *x, Moments *part
     shares[threadIdx.x][i] = {middle[i], off, left < 0.f ? 0.f : left};   // (NaN stays)
   }
   __syncthreads();
+  const int cells = cells_in(s, blockIdx.x);
+  const Rows count(s, cells);
   join_rows<double2>(s, [&](int r, int o, int i, double2 &all) {
-    const long begin = blockIdx.x * s.each, cells = min(s.cells, begin + s.each) - begin;
-    const long n = r < cells ? (cells - r + s.tile_rows - 1) / s.tile_rows : 0;
+    const int n = count.of(r);
     const Moments share = shares[r * s.tile_threads + o][i];
     const double mean = static_cast<double>(share.mean) + share.rest;
     if (n) all.x += mean * n, all.y += share.squares + mean * mean * n;
   }, [&](int c, const double2 &all) {
-    const long begin = blockIdx.x * s.each;
-    const double mean = all.x / static_cast<double>(min(s.cells, begin + s.each) - begin);
+    const double mean = all.x / cells;
     const float high = static_cast<float>(mean);
     partial[(static_cast<long>(blockIdx.z) * s.chunks + blockIdx.x) * s.channels + c] = {high, static_cast<float>(mean - high), static_cast<float>(all.y - all.x * mean)};
   });
@@ -272,7 +280,7 @@ __global__ __launch_bounds__(kThreads) void group_apply(const T *x, const float 
   for (int i = 0; i < 8; ++i) z[i].set(t.mean[i], t.rest[i], t.r[i] * t.w[i], t.b[i]);
   const T *from = x + p.at;
   T *to = y + p.at;
-  for (long done = 0; done < p.cells; done += kAtOnce, from += kAtOnce * p.stride, to += kAtOnce * p.stride) {
+  for (int done = 0; done < p.cells; done += kAtOnce, from += kAtOnce * p.stride, to += kAtOnce * p.stride) {
     Eight<T, F> raw[kAtOnce];
     load_cells(raw, from, p.cells - done, p);
 #pragma unroll
@@ -302,7 +310,7 @@ __global__ __launch_bounds__(kThreads) void group_grad_sums(const T *x, const T 
 #pragma unroll
     for (int i = 0; i < 8; ++i) hs[i].set(t.mean[i], t.rest[i], t.r[i], 0.);
     const T *at = x + p.at, *gat = gy + p.at;
-    for (long done = 0; done < p.cells; done += kAtOnce, at += kAtOnce * p.stride, gat += kAtOnce * p.stride) {
+    for (int done = 0; done < p.cells; done += kAtOnce, at += kAtOnce * p.stride, gat += kAtOnce * p.stride) {
       Eight<T, F> raw[kAtOnce], graw[kAtOnce];
       load_cells(raw, at, p.cells - done, p);
       load_cells(graw, gat, p.cells - done, p);
@@ -433,7 +441,7 @@ __global__ __launch_bounds__(kThreads) void group_grad_apply(const T *x, const T
   for (int i = 0; i < 8; ++i) hs[i].set(t.mean[i], t.rest[i], t.r[i], 0.);
   const T *at = x + p.at, *gat = gy + p.at;
   T *to = gx + p.at;
-  for (long done = 0; done < p.cells; done += kAtOnce, at += kAtOnce * p.stride, gat += kAtOnce * p.stride, to += kAtOnce * p.stride) {
+  for (int done = 0; done < p.cells; done += kAtOnce, at += kAtOnce * p.stride, gat += kAtOnce * p.stride, to += kAtOnce * p.stride) {
     Eight<T, F> raw[kAtOnce], graw[kAtOnce];
     load_cells(raw, at, p.cells - done, p);
     load_cells(graw, gat, p.cells - done, p);
