@@ -77,11 +77,12 @@ template <typename T> struct Product {
 // multiplied; scales go to the lanes that want them.  A row of x is 256 bytes there, sixteen pieces, piece c of row r at c ^ (r & 15); a row of
 // weights four, piece g at g ^ turned(r): reads of 16 rows side by side spread over all banks.
 // 4000 x 4096 x 4096 in bf16 with groups of 128, 64, 32: 130, 147, 172 us = 1.03, 0.91, 0.78 PFLOP/s (a plain product of the library: 1.21;
-// this kernel without its scales: 1.17); 2000 x 12544 x 1024 with groups of 64 62 us and 8 for the join: its loads alone take 52, its
-// reads and products alone 48.  What the scales take is the additions of the scaled sums, an instruction for each result and group;
-// decoding takes nothing.  Two workgroups share a compute unit, so that one multiplies while the other waits for its operands:
-// tiles of 128 x 256, of which one fits, took 145 us with groups of 128.  Without gain: products of 32 x 32, matrix instructions with the
-// additions of the group before in between, scales brought a block ahead.
+// this kernel without its scales: 1.17); 2000 x 12544 x 1024 with groups of 64 60 us and 8 for the join.  No one thing bounds it: of the first
+// 128 us its matrix instructions alone take 70, with the additions of scaled sums (an instruction for each result and group) 80, with reads
+// of LDS 95, its loads alone 68.  Two workgroups share a compute unit, so that one multiplies while the other waits for its operands:
+// tiles of 128 x 256, of which one fits, took 145 us, and two teams of wavefronts in one workgroup, which join in LDS, 172.  Without gain:
+// products of 32 x 32, matrix instructions with the additions of the group before in between, scales brought a block ahead, two blocks
+// under way at once.
 constexpr int kTile = 128, kTileThreads = 256, kTileRows = kTile * 256, kStage = kTileRows + kTile * 64;   // bytes of the rows, of a block
 __device__ __forceinline__ int turned(int row) { return (row / 2 & 3) ^ (row / 8 & 1); }
 
