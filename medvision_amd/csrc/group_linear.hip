@@ -11,6 +11,7 @@
 #include "rows.hpp"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace mv {
 namespace {
@@ -303,8 +304,9 @@ template <typename T, int M, int Group> __global__ __launch_bounds__(64 * kMostA
 // ---- few rows -------------------------------------------------------------------------------------------------------
 // 16 TN outputs and 16 TM rows per workgroup, straight from memory into the operands' registers.  The wavefronts take turns
 // at the blocks of the workgroup's share of the sum and join in LDS.  Bound by memory, and by loads of rows that every workgroup repeats:
-// 13 rows of 8100 x 8190 in float16 with groups of 32 13.7 us (42 MB, 3.1 TB/s); with four wavefronts 16.0, with four tiles of outputs 16.6.
-// From 17 rows on four wavefronts with four tiles: 32 x 4096 x 4096 12.1 us (15.9 with eight), 64 x 12544 x 1024 17.6.
+// 13 rows of 8100 x 8190 in float16 with groups of 32 13.4 us (42 MB, 3.1 TB/s); with four wavefronts 16.0, with four tiles of outputs 16.6.
+// From 17 rows on four wavefronts with four tiles: 32 x 4096 x 4096 with groups of 64 11.6 us (with eight
+// 15.3, eight of two tiles 12.1; these take 16.8 instead of 19 for 20 x 8100 x 8190, but 24 instead of 18.5 for 17 x 1024 x 50000), 64 x 12544 x 1024 17.7.
 constexpr int waves_of(int tm) { return tm <= 1 ? 8 : 4; }
 constexpr int tiles_wide(int tm) { return tm <= 1 ? 2 : 4; }
 
@@ -343,30 +345,18 @@ __global__ __launch_bounds__(64 * waves_of(TM), 2) void product_rows4(const Prod
       for (int i = 0; i < kScales; ++i) o.s[u][i] = s_at[u][static_cast<long>(b) * kScales + i];
     }
   };
-  auto bring_rows = [&](Operands &o, int b) {
+  auto bring_rows = [&](Operands &o, int b, auto whole) {
 #pragma unroll
     for (int t = 0; t < TM; ++t)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int c = b * kBlock + i * 32 + g * 8;
-        o.x[t][i] = columns8(x_at[t] + c, k.inputs - c);
+        if constexpr (whole) o.x[t][i] = reinterpret_cast<const Loose<u32x4, 2> *>(x_at[t] + c)->v;
+        else o.x[t][i] = columns8(x_at[t] + c, k.inputs - c);
       }
   };
   f32x4 acc[TM][TN] = {};
-  // The next block's weights are on their way while these are multiplied, and its rows as far as there are registers for them.
-  constexpr bool kRowsAhead = TM <= 2;
-  Operands next;
-  if (first + wave < last) {
-    bring_weights(next, first + wave);
-    if (kRowsAhead) bring_rows(next, first + wave);
-  }
-  for (int b = first + wave; b < last; b += kWaves) {
-    Operands o = next;
-    if (!kRowsAhead) bring_rows(o, b);
-    if (b + kWaves < last) {
-      bring_weights(next, b + kWaves);
-      if (kRowsAhead) bring_rows(next, b + kWaves);
-    }
+  auto multiply = [&](const Operands &o) {
 #pragma unroll
     for (int u = 0; u < TN; ++u) {
       f32x4 d[TM];
@@ -384,6 +374,48 @@ __global__ __launch_bounds__(64 * waves_of(TM), 2) void product_rows4(const Prod
         }
       }
     }
+  };
+  // Whole blocks with nothing to ask on the way, so that another one is under way whole while one is multiplied (where there are
+  // registers for that: else the next one's weights); then the one that ends with the rows.  20 x 8100 x 8190 with groups of 32: 19 us, where each
+  // load asks whether the row is long enough 21.5; 13 rows 13.4 and 13.8.
+  const int whole = min(last, k.inputs / kBlock), mine = max(0, (whole - first - wave + kWaves - 1) / kWaves), b0 = first + wave;
+  const std::true_type all;
+  int n = 0;
+  if constexpr (TM == 1 || (TM == 2 && Group > 32)) {
+    auto bring = [&](Operands &o, int n) { bring_weights(o, b0 + n * kWaves), bring_rows(o, b0 + n * kWaves, all), __builtin_amdgcn_sched_barrier(0); };   // (stays where it is)
+    Operands one, two;
+    if (mine > 1) {
+      bring(one, 0);
+      bring(two, 1);
+      for (; n + 3 < mine; n += 2) {
+        multiply(one);
+        bring(one, n + 2);
+        multiply(two);
+        bring(two, n + 3);
+      }
+      multiply(one);   // (two or three are left)
+      if (n + 2 < mine) bring(one, n + 2);
+      multiply(two);
+      if (n + 2 < mine) multiply(one);
+    } else if (mine == 1) {
+      bring(one, 0);
+      multiply(one);
+    }
+  } else {
+    Operands next;
+    if (mine > 0) bring_weights(next, b0);
+    for (; n < mine; ++n) {
+      Operands o = next;
+      bring_rows(o, b0 + n * kWaves, all);
+      if (n + 1 < mine) bring_weights(next, b0 + (n + 1) * kWaves);
+      multiply(o);
+    }
+  }
+  if (whole < last && (whole - first) % kWaves == wave) {
+    Operands o;
+    bring_weights(o, whole);
+    bring_rows(o, whole, std::false_type());
+    multiply(o);
   }
   if (wave) {
 #pragma unroll
