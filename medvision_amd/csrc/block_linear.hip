@@ -426,11 +426,7 @@ int product(const void *q, const void *qs, const void *w, const void *ws, const 
   float *const part = p.splits > 1 ? static_cast<float *>(workspace) : nullptr;
   const Results<T> to{static_cast<T *>(y), static_cast<const T *>(bias), part, rows, outputs};
   launch(p, q, qs, w, ws, to, static_cast<int>(rows), inputs, outputs, s);
-  if (part) {
-    const long count = rows * outputs;
-    if (p.splits > 8) join_parts<T, 8><<<linear_grid((count + 31) / 32, 256), 256, 0, s>>>(part, to.bias, to.y, count, outputs, p.splits);
-    else join_parts<T, 1><<<linear_grid((count + 255) / 256, 256), 256, 0, s>>>(part, to.bias, to.y, count, outputs, p.splits);
-  }
+  if (part) launch_join(part, to.bias, to.y, rows * outputs, outputs, p.splits, s);
   return check_launch("block_linear");
 }
 

@@ -78,7 +78,7 @@ template <typename T> struct Product {
 // multiplied; scales go to the lanes that want them.  A row of x is 256 bytes there, sixteen pieces, piece c of row r at c ^ (r & 15); a row of
 // weights four, piece g at g ^ turned(r): reads of 16 rows side by side spread over all banks.
 // 4000 x 4096 x 4096 in bf16 with groups of 128, 64, 32: 130, 147, 172 us = 1.03, 0.91, 0.78 PFLOP/s (a plain product of the library: 1.21;
-// this kernel without its scales: 1.17); 2000 x 12544 x 1024 with groups of 64 60 us and 8 for the join.  No one thing bounds it: of the first
+// this kernel without its scales: 1.17); 2000 x 12544 x 1024 with groups of 64 60 us and 7 for the join.  No one thing bounds it: of the first
 // 128 us its matrix instructions alone take 70, with the additions of scaled sums (an instruction for each result and group) 80, with reads
 // of LDS 95, its loads alone 68.  Two workgroups share a compute unit, so that one multiplies while the other waits for its operands:
 // tiles of 128 x 256, of which one fits, took 145 us, and two teams of wavefronts in one workgroup, which join in LDS, 172.  Without gain:
@@ -550,11 +550,7 @@ int product(const void *x, const void *w, const void *scales, const void *bias, 
   if (group == 32) launch<T, 32>(p, k, s);
   else if (group == 64) launch<T, 64>(p, k, s);
   else launch<T, 128>(p, k, s);
-  if (k.part) {
-    const long count = rows * outputs;
-    if (p.splits > 8) join_parts<T, 8><<<linear_grid((count + 31) / 32, 256), 256, 0, s>>>(k.part, k.bias, k.y, count, outputs, p.splits);
-    else join_parts<T, 1><<<linear_grid((count + 255) / 256, 256), 256, 0, s>>>(k.part, k.bias, k.y, count, outputs, p.splits);
-  }
+  if (k.part) launch_join(k.part, k.bias, k.y, rows * outputs, outputs, p.splits, s);
   return check_launch("group_linear");
 }
 
