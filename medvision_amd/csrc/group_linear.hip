@@ -212,23 +212,25 @@ template <typename T, int Group> __global__ __launch_bounds__(kTileThreads, 2) v
 // 32 s + 8 g .. + 7 of lane group g.  `along` wavefronts of a workgroup share the blocks and join in LDS.  Codes go to 32 bits (two in an
 // instruction), so that small float16 values count in full.  One row of 87808 x 1024 in bf16 with groups of 128: 11.5 us (48 MB, 4.2 TB/s);
 // sixteen rows' form takes 16 with its join, and 4096 x 4096 9.3 instead of 5.0 us (two rows: 9 and 6.3).
-constexpr int kDotOutputs = 4, kDotBlocks = 16, kMostAlong = 8;
+// A wavefront whose row of weights has no more than half its blocks takes other outputs beside them (Sides): one row of 1024 x 87808 with
+// groups of 64 13.7 us, without 23.5, of 256 x 87808 5.4 and 23.
+constexpr int kDotOutputs = 4, kDotBlocks = 16, kMostAlong = 8, kMostSides = 8;
 
-template <typename T, int M, int Group> __global__ __launch_bounds__(64 * kMostAlong) void product_dots(const Product<T> k, int along) {
-  constexpr int kScales = kBlock / Group;
-  __shared__ float part[kMostAlong][M][kDotOutputs];
+template <typename T, int M, int Group, int Sides> __global__ __launch_bounds__(64 * kMostAlong) void product_dots(const Product<T> k, int along) {
+  constexpr int kScales = kBlock / Group, kWidth = 64 / Sides, kSpan = kDotBlocks / Sides, kWide = kDotOutputs * Sides;
+  __shared__ float part[kMostAlong][M][kDotOutputs * Sides];
   unsigned id = linear_block();
   if (id >= static_cast<unsigned>(k.n_tiles) * k.splits) return;
   const int split = id / k.n_tiles, waves = blockDim.x >> 6;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane & 3;
-  const int n0 = ((id - split * k.n_tiles) * (waves / along) + wave / along) * kDotOutputs;
-  const int chunks = (k.blocks + kDotBlocks - 1) / kDotBlocks;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane & 3, side = lane / kWidth, in = lane % kWidth >> 2;
+  const int n0 = ((id - split * k.n_tiles) * (waves / along) + wave / along) * kWide;
+  const int chunks = (k.blocks + kSpan - 1) / kSpan;
   const int first = static_cast<int>(static_cast<long>(chunks) * split / k.splits) + wave % along, last = static_cast<int>(static_cast<long>(chunks) * (split + 1) / k.splits);
   const unsigned char *w_at[kDotOutputs];
   const float *s_at[kDotOutputs];
 #pragma unroll
   for (int u = 0; u < kDotOutputs; ++u) {
-    const long n = min(n0 + u, k.outputs - 1);
+    const long n = min(n0 + side * kDotOutputs + u, k.outputs - 1);
     w_at[u] = k.w + n * k.blocks * 64 + g * 16;
     s_at[u] = k.scales + n * k.blocks * kScales;
   }
@@ -237,7 +239,7 @@ template <typename T, int M, int Group> __global__ __launch_bounds__(64 * kMostA
     float s[kDotOutputs][kScales];
   };
   auto bring = [&](Operands &o, int chunk) {
-    const int at = chunk * kDotBlocks + (lane >> 2), b = min(at, k.blocks - 1);   // (behind the last one: that one, times zero)
+    const int at = chunk * kSpan + in, b = min(at, k.blocks - 1);   // (behind the last one: that one, times zero)
 #pragma unroll
     for (int u = 0; u < kDotOutputs; ++u) {
       o.w[u] = *reinterpret_cast<const u32x4 *>(w_at[u] + b * 64L);
@@ -258,7 +260,7 @@ template <typename T, int M, int Group> __global__ __launch_bounds__(64 * kMostA
   for (int chunk = first; chunk < last; chunk += along) {
     const Operands o = next;
     if (chunk + along < last) bring(next, chunk + along);
-    const bool there = chunk * kDotBlocks + (lane >> 2) < k.blocks;
+    const bool there = chunk * kSpan + in < k.blocks;
     float sum[M][kDotOutputs] = {};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -288,14 +290,14 @@ template <typename T, int M, int Group> __global__ __launch_bounds__(64 * kMostA
 #pragma unroll
     for (int u = 0; u < kDotOutputs; ++u) {
 #pragma unroll
-      for (int d = 32; d; d >>= 1) acc[m][u] += __shfl_xor(acc[m][u], d);
-      if (lane == 0) part[wave][m][u] = acc[m][u];
+      for (int d = kWidth / 2; d; d >>= 1) acc[m][u] += __shfl_xor(acc[m][u], d);
+      if (lane % kWidth == 0) part[wave][m][side * kDotOutputs + u] = acc[m][u];
     }
   __syncthreads();
-  if (wave % along || lane >= M * kDotOutputs) return;
-  const int m = lane / kDotOutputs, n = n0 + lane % kDotOutputs;
+  if (wave % along || lane >= M * kWide) return;
+  const int m = lane / kWide, n = n0 + lane % kWide;
   float y = 0.f;
-  for (int i = 0; i < along; ++i) y += part[wave + i][m][lane % kDotOutputs];
+  for (int i = 0; i < along; ++i) y += part[wave + i][m][lane % kWide];
   if (n >= k.outputs) return;
   if (k.part) k.part[(split * k.rows + m) * k.outputs + n] = y;
   else k.y[m * k.outputs + n] = store_cast<T>(k.bias ? y + load(k.bias + n) : y);
@@ -475,7 +477,7 @@ __global__ __launch_bounds__(256) void quantize_groups(const T *w, unsigned *q, 
 enum Kind { kDots, kFew1, kFew2, kFew4, kTiles };
 struct Plan {
   int kind, m_tiles, n_tiles, splits;
-  int along = 1, waves = 4;   // of kDots
+  int along = 1, waves = 4, sides = 1;   // of kDots
 };
 
 constexpr int kDotRows = 2;
@@ -487,10 +489,12 @@ int ceil_div(long a, long b) { return static_cast<int>((a + b - 1) / b); }
 Plan plan_of(long rows, int blocks, int outputs) {
   if (rows <= kDotRows) {
     const int chunks = ceil_div(blocks, kDotBlocks);
-    int along = 1;
+    int along = 1, sides = 1;
     while (along < kMostAlong && along < chunks) along *= 2;
-    const int waves = std::max(4, along), n = ceil_div(outputs, waves / along * kDotOutputs);
-    return {kDots, 1, n, std::max(1, std::min(chunks / along, 256 / n)), along, waves};
+    // (as many outputs side by side as leave a thousand workgroups: 1024 x 16384 4.9 us, without 5.9, of 8192 outputs 4.9 both ways)
+    while (sides < kMostSides && 2 * sides * blocks <= kDotBlocks && outputs >= 1024L * 4 * kDotOutputs * sides) sides *= 2;
+    const int waves = std::max(4, along), n = ceil_div(outputs, waves / along * kDotOutputs * sides);
+    return {kDots, 1, n, std::max(1, std::min(chunks / along, 256 / n)), along, waves, sides};
   }
   if (rows <= 64) {
     const int kind = rows <= 16 ? kFew1 : rows <= 32 ? kFew2 : kFew4, tm = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
@@ -501,12 +505,19 @@ Plan plan_of(long rows, int blocks, int outputs) {
   return {kTiles, m, n, static_cast<int>(std::max(1L, std::min(blocks / 4L, 512 / (static_cast<long>(m) * n))))};
 }
 
+template <typename T, int Group, int Sides> void dots(const Plan &p, const Product<T> &k, long groups, hipStream_t s) {
+  if (k.rows == 1) product_dots<T, 1, Group, Sides><<<linear_grid(groups, 64 * p.waves), 64 * p.waves, 0, s>>>(k, p.along);
+  else product_dots<T, 2, Group, Sides><<<linear_grid(groups, 64 * p.waves), 64 * p.waves, 0, s>>>(k, p.along);
+}
+
 template <typename T, int Group> void launch(const Plan &p, const Product<T> &k, hipStream_t s) {
   const long groups = static_cast<long>(p.m_tiles) * p.n_tiles * p.splits;
   switch (p.kind) {
     case kDots:
-      if (k.rows == 1) product_dots<T, 1, Group><<<linear_grid(groups, 64 * p.waves), 64 * p.waves, 0, s>>>(k, p.along);
-      else product_dots<T, 2, Group><<<linear_grid(groups, 64 * p.waves), 64 * p.waves, 0, s>>>(k, p.along);
+      if (p.sides == 1) dots<T, Group, 1>(p, k, groups, s);
+      else if (p.sides == 2) dots<T, Group, 2>(p, k, groups, s);
+      else if (p.sides == 4) dots<T, Group, 4>(p, k, groups, s);
+      else dots<T, Group, 8>(p, k, groups, s);
       break;
     case kFew1: product_rows4<T, 1, Group><<<linear_grid(groups, 64 * waves_of(1)), 64 * waves_of(1), 0, s>>>(k); break;
     case kFew2: product_rows4<T, 2, Group><<<linear_grid(groups, 64 * waves_of(2)), 64 * waves_of(2), 0, s>>>(k); break;

@@ -65,6 +65,18 @@ def test_products(shape, dtype, group):
     assert torch.equal(got, again)
 
 
+@pytest.mark.parametrize("shape", [(1000, 20011), (1024, 16384), (640, 50000), (500, 33333), (384, 40002), (200, 70001), (128, 66000)])
+@pytest.mark.parametrize("rows", [1, 2])
+def test_many_outputs_of_short_rows(rows, shape):
+    import medvision_amd.ops as ops
+    K, N = shape
+    dtype, group = (torch.float16, torch.bfloat16)[K % 3 % 2], (32, 64, 128)[(K + rows) % 3]
+    x, bias = rand(1, rows, K, dtype=dtype), rand(2, N, dtype=dtype)
+    codes, scales = (t.cpu() for t in ops.quantize_groups(rand(3, N, K).to(DEV), group))
+    got = ops.group_linear(x.to(DEV), codes.to(DEV), scales.to(DEV), bias.to(DEV))
+    check(got, *ref.group_linear(x, codes, scales, bias), shape)
+
+
 def test_every_code_and_place():
     """A row of x with a single one picks a column; every column of a block, with all sixteen codes."""
     import medvision_amd.ops as ops
