@@ -304,15 +304,15 @@ template <typename T, int M, int Group, int Sides> __global__ __launch_bounds__(
 }
 
 // ---- few rows -------------------------------------------------------------------------------------------------------
-// 16 TN outputs and 16 TM rows per workgroup, straight from memory into the operands' registers.  The wavefronts take turns
-// at the blocks of the workgroup's share of the sum and join in LDS.  Bound by memory, and by loads of rows that every workgroup repeats:
+// 16 TN outputs and 16 TM rows, straight from memory into the operands' registers.  `Along` wavefronts (all of a workgroup's, or two)
+// take turns at the blocks of their share of the sum and join in LDS.  Bound by memory, and by loads of rows that every workgroup repeats:
 // 13 rows of 8100 x 8190 in float16 with groups of 32 13.4 us (42 MB, 3.1 TB/s); with four wavefronts 16.0, with four tiles of outputs 16.6.
 // From 17 rows on four wavefronts with four tiles: 32 x 4096 x 4096 with groups of 64 11.6 us (with eight
-// 15.3, eight of two tiles 12.1; these take 16.8 instead of 19 for 20 x 8100 x 8190, but 24 instead of 18.5 for 17 x 1024 x 50000), 64 x 12544 x 1024 17.7.
+// 15.3, eight of two tiles 12.1), 64 x 12544 x 1024 17.7.
 constexpr int waves_of(int tm) { return tm <= 1 ? 8 : 4; }
 constexpr int tiles_wide(int tm) { return tm <= 1 ? 2 : 4; }
 
-template <typename T, int TM, int Group>
+template <typename T, int TM, int Group, int Along>
 __global__ __launch_bounds__(64 * waves_of(TM), 2) void product_rows4(const Product<T> k) {
   constexpr int TN = tiles_wide(TM), kScales = kBlock / Group, kWaves = waves_of(TM);
   __shared__ f32x4 part[kWaves - 1][TN * TM][64];
@@ -320,9 +320,10 @@ __global__ __launch_bounds__(64 * waves_of(TM), 2) void product_rows4(const Prod
   if (id >= static_cast<unsigned>(k.m_tiles) * k.n_tiles * k.splits) return;
   const int n_tile = id % k.n_tiles;
   id /= k.n_tiles;
-  const int split = id % k.splits, n0 = n_tile * 16 * TN;
+  const int split = id % k.splits;
   const long m0 = static_cast<long>(id / k.splits) * 16 * TM;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, g = lane >> 4;
+  const int own = wave % Along, n0 = (n_tile * (kWaves / Along) + wave / Along) * 16 * TN;   // (its place among those that share the blocks)
   const int first = static_cast<int>(static_cast<long>(k.blocks) * split / k.splits), last = static_cast<int>(static_cast<long>(k.blocks) * (split + 1) / k.splits);
   const T *x_at[TM];
   const unsigned char *w_at[TN];
@@ -380,11 +381,11 @@ __global__ __launch_bounds__(64 * waves_of(TM), 2) void product_rows4(const Prod
   // Whole blocks with nothing to ask on the way, so that another one is under way whole while one is multiplied (where there are
   // registers for that: else the next one's weights); then the one that ends with the rows.  20 x 8100 x 8190 with groups of 32: 19 us, where each
   // load asks whether the row is long enough 21.5; 13 rows 13.4 and 13.8.
-  const int whole = min(last, k.inputs / kBlock), mine = max(0, (whole - first - wave + kWaves - 1) / kWaves), b0 = first + wave;
+  const int whole = min(last, k.inputs / kBlock), mine = max(0, (whole - first - own + Along - 1) / Along), b0 = first + own;
   const std::true_type all;
   int n = 0;
   if constexpr (TM == 1 || (TM == 2 && Group > 32)) {
-    auto bring = [&](Operands &o, int n) { bring_weights(o, b0 + n * kWaves), bring_rows(o, b0 + n * kWaves, all), __builtin_amdgcn_sched_barrier(0); };   // (stays where it is)
+    auto bring = [&](Operands &o, int n) { bring_weights(o, b0 + n * Along), bring_rows(o, b0 + n * Along, all), __builtin_amdgcn_sched_barrier(0); };   // (stays where it is)
     Operands one, two;
     if (mine > 1) {
       bring(one, 0);
@@ -408,25 +409,25 @@ __global__ __launch_bounds__(64 * waves_of(TM), 2) void product_rows4(const Prod
     if (mine > 0) bring_weights(next, b0);
     for (; n < mine; ++n) {
       Operands o = next;
-      bring_rows(o, b0 + n * kWaves, all);
-      if (n + 1 < mine) bring_weights(next, b0 + (n + 1) * kWaves);
+      bring_rows(o, b0 + n * Along, all);
+      if (n + 1 < mine) bring_weights(next, b0 + (n + 1) * Along);
       multiply(o);
     }
   }
-  if (whole < last && (whole - first) % kWaves == wave) {
+  if (whole < last && (whole - first) % Along == own) {
     Operands o;
     bring_weights(o, whole);
     bring_rows(o, whole, std::false_type());
     multiply(o);
   }
-  if (wave) {
+  if (own) {
 #pragma unroll
     for (int u = 0; u < TN; ++u)
 #pragma unroll
       for (int t = 0; t < TM; ++t) part[wave - 1][u * TM + t][lane] = acc[t][u];
   }
   __syncthreads();
-  if (wave) return;
+  if (own) return;
 #pragma unroll
   for (int u = 0; u < TN; ++u) {
     const int n = n0 + u * 16 + r16;
@@ -435,7 +436,7 @@ __global__ __launch_bounds__(64 * waves_of(TM), 2) void product_rows4(const Prod
 #pragma unroll
     for (int t = 0; t < TM; ++t) {
 #pragma unroll
-      for (int i = 0; i < kWaves - 1; ++i) acc[t][u] += part[i][u * TM + t][lane];
+      for (int i = 0; i < Along - 1; ++i) acc[t][u] += part[wave + i][u * TM + t][lane];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const long m = m0 + t * 16 + 4 * g + j;
@@ -477,7 +478,7 @@ __global__ __launch_bounds__(256) void quantize_groups(const T *w, unsigned *q, 
 enum Kind { kDots, kFew1, kFew2, kFew4, kTiles };
 struct Plan {
   int kind, m_tiles, n_tiles, splits;
-  int along = 1, waves = 4, sides = 1;   // of kDots
+  int along = 1, waves = 4, sides = 1;   // of kDots; of kFew the first two
 };
 
 constexpr int kDotRows = 2;
@@ -498,8 +499,11 @@ Plan plan_of(long rows, int blocks, int outputs) {
   }
   if (rows <= 64) {
     const int kind = rows <= 16 ? kFew1 : rows <= 32 ? kFew2 : kFew4, tm = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-    const int n = ceil_div(outputs, 16 * tiles_wide(tm)), waves = waves_of(tm);
-    return {kind, 1, n, std::max(1, std::min(blocks / (2 * waves), 256 * 8 / waves / n))};
+    // (two wavefronts on few blocks while there is a workgroup for every compute unit: 13 x 256 x 50000 5.8 us, all eight 9.1, 13 x 1024 x 50000 16
+    // and 18.2; 13 x 2048 x 50000 28.4 and 26.9)
+    const int waves = waves_of(tm), along = blocks <= 8 && outputs >= 256L * 16 * tiles_wide(tm) * (waves / 2) ? 2 : waves;
+    const int n = ceil_div(outputs, 16 * tiles_wide(tm) * (waves / along));
+    return {kind, 1, n, std::max(1, std::min(blocks / (2 * waves), 256 * 8 / waves / n)), along, waves};
   }
   const int m = ceil_div(rows, 128), n = ceil_div(outputs, 128);
   return {kTiles, m, n, static_cast<int>(std::max(1L, std::min(blocks / 4L, 512 / (static_cast<long>(m) * n))))};
@@ -508,6 +512,12 @@ Plan plan_of(long rows, int blocks, int outputs) {
 template <typename T, int Group, int Sides> void dots(const Plan &p, const Product<T> &k, long groups, hipStream_t s) {
   if (k.rows == 1) product_dots<T, 1, Group, Sides><<<linear_grid(groups, 64 * p.waves), 64 * p.waves, 0, s>>>(k, p.along);
   else product_dots<T, 2, Group, Sides><<<linear_grid(groups, 64 * p.waves), 64 * p.waves, 0, s>>>(k, p.along);
+}
+
+template <typename T, int TM, int Group> void few(const Plan &p, const Product<T> &k, long groups, hipStream_t s) {
+  constexpr int kWaves = waves_of(TM);
+  if (p.along == kWaves) product_rows4<T, TM, Group, kWaves><<<linear_grid(groups, 64 * kWaves), 64 * kWaves, 0, s>>>(k);
+  else product_rows4<T, TM, Group, 2><<<linear_grid(groups, 64 * kWaves), 64 * kWaves, 0, s>>>(k);
 }
 
 template <typename T, int Group> void launch(const Plan &p, const Product<T> &k, hipStream_t s) {
@@ -519,9 +529,9 @@ template <typename T, int Group> void launch(const Plan &p, const Product<T> &k,
       else if (p.sides == 4) dots<T, Group, 4>(p, k, groups, s);
       else dots<T, Group, 8>(p, k, groups, s);
       break;
-    case kFew1: product_rows4<T, 1, Group><<<linear_grid(groups, 64 * waves_of(1)), 64 * waves_of(1), 0, s>>>(k); break;
-    case kFew2: product_rows4<T, 2, Group><<<linear_grid(groups, 64 * waves_of(2)), 64 * waves_of(2), 0, s>>>(k); break;
-    case kFew4: product_rows4<T, 4, Group><<<linear_grid(groups, 64 * waves_of(4)), 64 * waves_of(4), 0, s>>>(k); break;
+    case kFew1: few<T, 1, Group>(p, k, groups, s); break;
+    case kFew2: few<T, 2, Group>(p, k, groups, s); break;
+    case kFew4: few<T, 4, Group>(p, k, groups, s); break;
     default: product_tiles4<T, Group><<<linear_grid(groups, 256), 256, 0, s>>>(k);
   }
 }
@@ -547,7 +557,7 @@ int product(const void *x, const void *w, const void *scales, const void *bias, 
   const size_t pad = odd ? padded_bytes(rows, blocks) : 0;
   if (!workspace) workspace_bytes = 0;
   const bool pads = odd && pad <= workspace_bytes && reinterpret_cast<uintptr_t>(workspace) % 16 == 0;
-  if (odd && !pads) p = {kFew4, ceil_div(rows, 64), ceil_div(outputs, 16 * tiles_wide(4)), 1};
+  if (odd && !pads) p = {kFew4, ceil_div(rows, 64), ceil_div(outputs, 16 * tiles_wide(4)), 1, waves_of(4), waves_of(4)};
   const size_t at = pads ? pad : 0;
   if (workspace_bytes - at < part_bytes(p, rows, outputs)) p.splits = 1;
   Product<T> k{static_cast<const T *>(x), static_cast<const unsigned char *>(w), static_cast<const float *>(scales), static_cast<const T *>(bias),

@@ -66,7 +66,7 @@ def test_products(shape, dtype, group):
 
 
 @pytest.mark.parametrize("shape", [(1000, 20011), (1024, 16384), (640, 50000), (500, 33333), (384, 40002), (200, 70001), (128, 66000)])
-@pytest.mark.parametrize("rows", [1, 2])
+@pytest.mark.parametrize("rows", [1, 2, 13, 20, 64])
 def test_many_outputs_of_short_rows(rows, shape):
     import medvision_amd.ops as ops
     K, N = shape
