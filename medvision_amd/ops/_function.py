@@ -23,3 +23,22 @@ class NativeFunction(Function):
         if cls._direct and _tracing() is None:
             return cls.native(*args, **kwargs)
         return super().apply(*args, **kwargs)
+
+
+class RecordedFunction(NativeFunction):
+    """The node of an operator without a gradient.  Outside of traces ``apply`` is ``native``; ``torch.jit.trace``, which
+    would record nothing of that call but the allocation of its result, gets a Python function that runs it."""
+    refuses = None   # the operator's name, where it refuses tensors that want a gradient (others give results without one)
+
+    @classmethod
+    def apply(cls, *args):
+        if _tracing() is None:
+            return cls.native(*args)
+        if cls.refuses and torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in args):
+            raise RuntimeError(f"{cls.refuses} has no gradient: call it under torch.no_grad()")
+        with torch.no_grad():
+            return super().apply(*args)
+
+    @classmethod
+    def forward(cls, ctx, *args):
+        return cls.native(*args)

@@ -3,7 +3,24 @@ reference."""
 import torch
 
 from .._lib import native
+from ._function import RecordedFunction
 from ._module import KeepsTypes
+
+
+class QuantizeBlocksFunction(RecordedFunction):
+    refuses = 'quantize_blocks'
+
+    @staticmethod
+    def native(x, block_rows):
+        return native.quantize_blocks(x, block_rows)
+
+
+class BlockLinearFunction(RecordedFunction):
+    refuses = 'block_linear'
+
+    @staticmethod
+    def native(q, q_scales, weight, weight_scales, bias, out_dtype):
+        return native.block_linear(q, q_scales, weight, weight_scales, bias, out_dtype)
 
 
 def quantize_blocks(x, block_rows=1):
@@ -12,14 +29,14 @@ def quantize_blocks(x, block_rows=1):
     ``q`` is float8_e4m3fn with the columns padded with zeros to whole blocks of 128, ``scales`` float32: one for each row
     and block of 128 columns (activations, ``block_rows=1``) or for each 128 x 128 block of a matrix (weights,
     ``block_rows=128``).  ``scale = max(max|x| / 448, 2 ** -126)``, ``q = e4m3(x * (1 / scale))``.  No gradient."""
-    return native.quantize_blocks(x, block_rows)
+    return QuantizeBlocksFunction.apply(x, block_rows)
 
 
 def block_linear(q, q_scales, weight, weight_scales, bias=None, out_dtype=torch.bfloat16):
     """``(q * q_scales) @ (weight * weight_scales).T + bias`` of 8-bit activations ``[..., inputs]`` and weights
     ``[outputs, inputs]`` as ``quantize_blocks`` gives them (``block_rows`` 1 and 128); float16 or bfloat16
     ``[..., outputs]``.  No gradient."""
-    return native.block_linear(q, q_scales, weight, weight_scales, bias, out_dtype)
+    return BlockLinearFunction.apply(q, q_scales, weight, weight_scales, bias, out_dtype)
 
 
 class BlockScaledLinear(KeepsTypes):

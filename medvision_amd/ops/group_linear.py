@@ -3,7 +3,24 @@ reference."""
 import torch
 
 from .._lib import native
+from ._function import RecordedFunction
 from ._module import KeepsTypes
+
+
+class QuantizeGroupsFunction(RecordedFunction):
+    refuses = 'quantize_groups'
+
+    @staticmethod
+    def native(weight, group):
+        return native.quantize_groups(weight, group)
+
+
+class GroupLinearFunction(RecordedFunction):
+    refuses = 'group_linear'
+
+    @staticmethod
+    def native(x, weight, scales, bias):
+        return native.group_linear(x, weight, scales, bias)
 
 
 def quantize_groups(weight, group=32):
@@ -14,13 +31,13 @@ def quantize_groups(weight, group=32):
     4, 6 (codes 0 .. 7, halves to even codes) or their negatives (8 .. 15).  ``codes [outputs, 64 * blocks]`` is uint8: two codes a
     byte, the first one in its low half; the four bytes of eight neighbouring columns together; of a block's sixteen
     such pieces number ``4 s + g`` at place ``4 g + s``.  No gradient."""
-    return native.quantize_groups(weight, group)
+    return QuantizeGroupsFunction.apply(weight, group)
 
 
 def group_linear(x, weight, scales, bias=None):
     """``x @ values.T + bias`` of float16 or bfloat16 rows ``[..., inputs]`` and the values of weights ``[outputs, inputs]`` as
     ``quantize_groups`` gives them, in the type of ``x``.  Values and products are exact, sums are in 32 bits.  No gradient."""
-    return native.group_linear(x, weight, scales, bias)
+    return GroupLinearFunction.apply(x, weight, scales, bias)
 
 
 class GroupScaledLinear(KeepsTypes):

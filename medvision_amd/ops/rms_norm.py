@@ -5,7 +5,7 @@ from torch import nn
 from torch.autograd.function import once_differentiable
 
 from .._lib import native
-from ._function import NativeFunction
+from ._function import NativeFunction, RecordedFunction
 
 
 class AddRMSNormFunction(NativeFunction):
@@ -32,6 +32,14 @@ class AddRMSNormFunction(NativeFunction):
         return grad_h if for_x else None, grad_h if for_residual else None, grad_weight, None
 
 
+class AddRMSNormQuantizedFunction(RecordedFunction):
+    refuses = 'add_rms_norm_quantized'
+
+    @staticmethod
+    def native(x, residual, weight, eps):
+        return native.add_rms_norm_quantized(x, residual, weight, eps)
+
+
 def add_rms_norm(x, residual, weight, eps=1e-6):
     """``h = x + residual`` and its norm ``y = h / sqrt(mean(h ** 2) + eps) * weight`` over the last dimension: ``(y, h)``.
 
@@ -43,7 +51,7 @@ def add_rms_norm(x, residual, weight, eps=1e-6):
 
 def add_rms_norm_quantized(x, residual, weight, eps=1e-6):
     """``add_rms_norm`` whose ``y`` is in 8 bits, as ``quantize_blocks`` gives them: ``(q, scales, h)``.  No gradient."""
-    return native.add_rms_norm_quantized(x, residual, weight, eps)
+    return AddRMSNormQuantizedFunction.apply(x, residual, weight, eps)
 
 
 class AddRMSNorm(nn.Module):
