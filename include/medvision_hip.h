@@ -374,9 +374,9 @@ int mv_block_linear(const void *q, const void *q_scales, const void *weight, con
  * zero.  MV_GELU is z times the normal distribution's value.  stats [3, batch, groups] float32 receives each group's mean,
  * what rounding took from it, and 1 / sqrt(var + eps).
  * Results do not overlap what is read.  ..._backward WRITES grad_x, grad_weight and grad_bias (of weight_dtype); each may be NULL
- * where nobody wants it.  At the
- * border of two branches the derivative is the lower one's.  Sums are formed in a fixed order.  Batches of 65536 and more
- * are taken for small samples only (a group whose values fit into a workgroup's registers), others are refused. */
+ * where nobody wants it.  At the border of two branches the derivative is the lower one's.  Sums are formed in a fixed
+ * order.  Batches of 65536 and more are taken for small samples only (a group whose values fit into a workgroup's registers in
+ * the forward pass), by both; others are refused by both. */
 typedef enum { MV_NO_ACTIVATION = 0, MV_RELU = 1, MV_LEAKY_RELU = 2, MV_SILU = 3, MV_GELU = 4 } mv_activation;
 size_t mv_group_norm_workspace_bytes(int batch, int64_t cells, int channels, int groups);
 int mv_group_norm(const void *x, const void *weight, const void *bias, void *y, void *stats, int batch, int64_t cells, int channels,

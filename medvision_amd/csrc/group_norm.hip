@@ -26,7 +26,9 @@ constexpr int kThreads = 256;
 struct Cells {
   long cells, each;   // of a sample, of a chunk
   int channels, groups, group_channels, tile_threads, tile_rows, chunks;
+  int batch, first;   // all samples, the launch's first one
 };
+__device__ __forceinline__ long sample_of(const Cells &s) { return static_cast<long>(s.first) + blockIdx.z; }
 
 // The first channel of a piece of eight.  The last piece starts earlier than its place where it would not be whole: the channels
 // that it has in common with the one before are worked out twice, with the same results.
@@ -55,7 +57,7 @@ __device__ __forceinline__ Place place_of(const Cells &s, unsigned chunk) {
   p.left = s.channels - piece * 8 > 0 ? s.channels - p.c : 0;
   p.cells = row < s.tile_rows && p.left > 0 ? Rows(s, cells_in(s, chunk)).of(row) : 0;
   p.stride = static_cast<long>(s.tile_rows) * s.channels;
-  p.at = (static_cast<long>(blockIdx.z) * s.cells + chunk * s.each + row) * s.channels + p.c;
+  p.at = (sample_of(s) * s.cells + chunk * s.each + row) * s.channels + p.c;
   return p;
 }
 
@@ -174,7 +176,7 @@ __global__ __launch_bounds__(kThreads) void group_sums(const T *x, Moments *part
   }, [&](int c, const double2 &all) {
     const double mean = all.x / cells;
     const float high = static_cast<float>(mean);
-    partial[(static_cast<long>(blockIdx.z) * s.chunks + blockIdx.x) * s.channels + c] = {high, static_cast<float>(mean - high), static_cast<float>(all.y - all.x * mean)};
+    partial[(sample_of(s) * s.chunks + blockIdx.x) * s.channels + c] = {high, static_cast<float>(mean - high), static_cast<float>(all.y - all.x * mean)};
   });
 }
 
@@ -258,7 +260,7 @@ struct Channels {
 template <typename T>
 __device__ __forceinline__ void load_channels(Channels &t, const Place &p, const float *stats, const void *weight, const void *bias, bool wide,
                                               const Cells &s) {
-  const long every = static_cast<long>(gridDim.z) * s.groups, first = static_cast<long>(blockIdx.z) * s.groups;
+  const long every = static_cast<long>(s.batch) * s.groups, first = sample_of(s) * s.groups;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const long at = first + static_cast<unsigned>(min(p.c + i, s.channels - 1)) / static_cast<unsigned>(s.group_channels);
@@ -335,7 +337,7 @@ __global__ __launch_bounds__(kThreads) void group_grad_sums(const T *x, const T 
   join_rows<float2>(s, [&](int r, int o, int i, float2 &all) {
     const float2 share = shares[r * s.tile_threads + o][i];
     all.x += share.x, all.y += share.y;
-  }, [&](int c, const float2 &all) { partial[(static_cast<long>(blockIdx.z) * s.chunks + blockIdx.x) * s.channels + c] = all; });
+  }, [&](int c, const float2 &all) { partial[(sample_of(s) * s.chunks + blockIdx.x) * s.channels + c] = all; });
 }
 
 // A group of a sample: means[0], [1] = mean(w gz), mean(w gz h); the channels' sums over all chunks take the first one's place.
@@ -433,8 +435,8 @@ __global__ __launch_bounds__(kThreads) void group_grad_apply(const T *x, const T
   float one[8], two[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const long at = static_cast<long>(blockIdx.z) * s.groups + min(p.c + i, s.channels - 1) / s.group_channels;
-    one[i] = means[at], two[i] = means[static_cast<long>(gridDim.z) * s.groups + at];
+    const long at = sample_of(s) * s.groups + min(p.c + i, s.channels - 1) / s.group_channels;
+    one[i] = means[at], two[i] = means[static_cast<long>(s.batch) * s.groups + at];
   }
   Line hs[8];
 #pragma unroll
@@ -465,7 +467,7 @@ __global__ __launch_bounds__(kThreads) void group_grad_apply(const T *x, const T
 constexpr long kGroups = 1024;   // workgroups of a launch, about
 Cells cells_of(int batch, long cells, int channels, int groups) {
   Cells s{};
-  s.cells = cells, s.channels = channels, s.groups = groups, s.group_channels = channels / groups;
+  s.cells = cells, s.channels = channels, s.groups = groups, s.group_channels = channels / groups, s.batch = batch;
   const int octets = (channels + 7) / 8, tiles = (octets + kThreads - 1) / kThreads;
   s.tile_threads = std::min(octets, kThreads), s.tile_rows = kThreads / s.tile_threads;
   // about four workgroups per compute unit, of four cells a thread at least, and no more than 256: longer sums in 32 bits lose bits
@@ -486,6 +488,18 @@ template <typename F> void for_form(const Cells &s, size_t bytes, const F &f) {
 }
 
 constexpr int kMostBatch = 65536;   // (a grid's third dimension)
+// Larger batches are taken where the forward pass has the form for small samples.  Its gradients need more registers: where they do not fit,
+// the kernels of large samples take a slice of the batch at a time.
+int too_many(int batch, long cells, int channels, int groups) {
+  MV_REQUIRE(batch < kMostBatch || whole_plan(batch, cells, channels, groups, false).u, "a batch of %d is too large for samples of %ld cells", batch, cells);
+  return MV_OK;
+}
+template <typename F> void for_slices(Cells s, const F &f) {
+  for (long first = 0; first < s.batch; first += kMostBatch - 1) {
+    s.first = static_cast<int>(first);
+    f(s, static_cast<unsigned>(std::min(kMostBatch - 1L, s.batch - first)));
+  }
+}
 int arguments(int batch, long cells, int channels, int groups, int activation, int dtype, int weight_dtype) {
   MV_REQUIRE(dtype == MV_F32 || dtype == MV_F16 || dtype == MV_BF16, "dtype %d is not float32, float16 or bfloat16", dtype);
   MV_REQUIRE(weight_dtype == dtype || weight_dtype == MV_F32, "weight and bias have dtype %d, expected %d or float32", weight_dtype, dtype);
@@ -526,7 +540,7 @@ int mv_group_norm(const void *x, const void *weight, const void *bias, void *y, 
   auto *const stat = static_cast<float *>(stats);
   if (const WholePlan whole = whole_plan(batch, cells, channels, groups, false); whole.u)
     return group_norm_whole(whole, x, weight, bias, wide, y, stat, batch, eps, activation, low, dtype, st);
-  MV_REQUIRE(batch < kMostBatch, "a batch of %d is too large for samples of %ld cells", batch, static_cast<long>(cells));
+  if (const int status = too_many(batch, cells, channels, groups)) return status;
   MV_FLOATS(dtype, {
     const T *const xt = static_cast<const T *>(x);
     for_form(s, 0, [&](auto form) { group_sums<T, form><<<grid, kThreads, 0, st>>>(xt, partial, s); });
@@ -555,34 +569,41 @@ int mv_group_norm_backward(const void *x, const void *weight, const void *bias, 
   const bool wide = weight_dtype == MV_F32;
   MV_REQUIRE(empty || (x && stats && grad_y), "a tensor is missing");
   MV_REQUIRE(empty || (workspace && workspace_bytes >= mv_group_norm_backward_workspace_bytes(batch, cells, channels, groups)), "the workspace is too small");
-  const dim3 grid(s.chunks, tiles_of(s), batch);
+  const unsigned tiles = tiles_of(s);
   auto *const partial = static_cast<float2 *>(workspace);
   auto *const means = reinterpret_cast<float *>(static_cast<char *>(workspace) + (empty ? 0 : partial_bytes<float2>(batch, s)));
   auto *const stat = static_cast<const float *>(stats);
   const WholePlan whole = empty ? WholePlan{} : whole_plan(batch, cells, channels, groups, true);
   const Vectors vectors{partial, grad_weight, grad_bias, (whole.u ? 1L : s.chunks) * channels, empty ? 0 : batch};
-  const bool wanted = grad_weight || grad_bias;
+  const bool wanted = grad_weight || grad_bias, behind = wanted && grad_x && !whole.u && !empty && batch < kMostBatch;   // behind the last chunk
   if (whole.u) {
     if (const int status = group_norm_whole_backward(whole, x, grad_y, stat, weight, bias, wide, grad_x, wanted ? partial : nullptr, batch, activation, low, dtype, st))
       return status;
+  } else if (!empty) {
+    if (const int status = too_many(batch, cells, channels, groups)) return status;
   }
-  MV_REQUIRE(empty || whole.u || batch < kMostBatch, "a batch of %d is too large for samples of %ld cells", batch, static_cast<long>(cells));
   MV_FLOATS(dtype, {
     const T *const xt = static_cast<const T *>(x), *const gy = static_cast<const T *>(grad_y);
     if (!empty && !whole.u) {
       for_activation(activation, [&](auto kind) {
-        for_form(s, 0, [&](auto form) { group_grad_sums<T, kind, form><<<grid, kThreads, 0, st>>>(xt, gy, stat, weight, bias, wide, partial, s, low); });
+        for_form(s, 0, [&](auto form) {
+          for_slices(s, [&](const Cells &part, unsigned samples) {
+            group_grad_sums<T, kind, form><<<dim3(s.chunks, tiles, samples), kThreads, 0, st>>>(xt, gy, stat, weight, bias, wide, partial, part, low);
+          });
+        });
       });
       group_grad_finish<T><<<linear_grid(static_cast<long>(batch) * groups, kThreads), kThreads, 0, st>>>(partial, means, weight, wide, s, batch);
       if (grad_x)
         for_activation(activation, [&](auto kind) {
           for_form(s, bytes, [&](auto form) {
-            group_grad_apply<T, kind, form><<<dim3(s.chunks + (wanted ? 1 : 0), grid.y, batch), kThreads, 0, st>>>(xt, gy, stat, means, weight, bias, wide,
-                                                                                                               static_cast<T *>(grad_x), vectors, s, low);
+            for_slices(s, [&](const Cells &part, unsigned samples) {
+              group_grad_apply<T, kind, form><<<dim3(s.chunks + (behind ? 1 : 0), tiles, samples), kThreads, 0, st>>>(xt, gy, stat, means, weight, bias, wide,
+                                                                                                                    static_cast<T *>(grad_x), vectors, part, low);
+            });
           });
         });
     }
-    if (wanted && (empty || whole.u || !grad_x)) group_grad_vectors<T><<<(channels + kVectorChannels - 1) / kVectorChannels, kThreads, 0, st>>>(vectors, wide, channels);
+    if (wanted && !behind) group_grad_vectors<T><<<(channels + kVectorChannels - 1) / kVectorChannels, kThreads, 0, st>>>(vectors, wide, channels);
   })
   return check_launch("group_norm backward");
 }
