@@ -101,7 +101,7 @@ __device__ __forceinline__ void load_cells(Eight<T, F> (&to)[kAtOnce], const T *
 }
 
 // What the rows of a tile have of each of its channels, joined by teams of threads and then over the teams, in a fixed order:
-// add(row, piece, channel of it, sum), put(channel, sum).
+// add(first row, step, piece, channel of it, sum), put(channel, sum).
 template <typename Sum, typename Add, typename Put> __device__ __forceinline__ void join_rows(const Cells &s, const Add &add, const Put &put) {
   __shared__ Sum sums[kThreads];
   const int wide = min(s.tile_threads * 8, kThreads), team = threadIdx.x / wide, teams = kThreads / wide;
@@ -109,8 +109,7 @@ template <typename Sum, typename Add, typename Put> __device__ __forceinline__ v
     const int k = first + threadIdx.x % wide, c = blockIdx.y * kThreads * 8 + k;
     const bool mine = team < teams && k < s.tile_threads * 8 && c < s.channels;
     Sum all = {0, 0};
-    if (mine)
-      for (int r = team; r < s.tile_rows; r += teams) add(r, k / 8, c - first_channel(s, c / 8), all);
+    if (mine) add(team, teams, k / 8, c - first_channel(s, c / 8), all);
     if (teams > 1) {
       sums[threadIdx.x] = all;
       __syncthreads();
@@ -122,61 +121,98 @@ template <typename Sum, typename Add, typename Put> __device__ __forceinline__ v
 }
 
 // ---- forward ------------------------------------------------------------------------------------------------------
-// Of a channel over a chunk's cells: its mean in two parts and the sum of squared differences from it.
+// Of a channel over a chunk's cells: its mean in two parts and the sum of squared differences from it.  A sum that 32 bits do
+// not hold is kept negative, 2^-200 of it.
 struct Moments {
   float mean, rest, squares;
 };
+__device__ __forceinline__ double mean_of(const Moments &m) { return static_cast<double>(m.mean) + m.rest; }
+// Sums over moments take squares as they are and keep their signs: where one is negative they start again (`Again`).
+template <bool Again> __device__ __forceinline__ double squares_of(const Moments &m, int &signs) {
+  if constexpr (!Again) signs |= __float_as_int(m.squares);
+  return Again && m.squares < 0.f ? static_cast<double>(m.squares) * -0x1p200 : m.squares;
+}
 // partial[sample][chunk][channel].  A thread sums differences from the mean of its first cells, which keeps 32 bits enough
 // where a channel's mean is far from zero; threads are joined in 64 bits.
 template <typename T, int F>
 __global__ __launch_bounds__(kThreads) void group_sums(const T *x, Moments *partial, const Cells s) {
   __shared__ Moments shares[kThreads][8];
   const Place p = place_of(s, blockIdx.x);
-  float middle[8] = {}, sum[8] = {}, squares[8] = {};
-  const T *at = x + p.at;
-  for (int done = 0; done < p.cells; done += kAtOnce, at += kAtOnce * p.stride) {
-    Eight<T, F> raw[kAtOnce];
-    load_cells(raw, at, p.cells - done, p);
-    if (done == 0) {
+  float middle[8] = {}, sum[8] = {}, squares[8] = {}, by[8];
+  auto add_up = [&](auto again) {
+    const T *at = x + p.at;
+    for (int done = 0; done < p.cells; done += kAtOnce, at += kAtOnce * p.stride) {
+      Eight<T, F> raw[kAtOnce];
+      load_cells(raw, at, p.cells - done, p);
+      if (!again && done == 0) {
+#pragma unroll
+        for (int n = 0; n < kAtOnce; ++n) {
+          float v[8];
+          raw[n].values(v);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) middle[i] = fmaf(v[i], 1.f / kAtOnce, middle[i]);
+        }
+      }
 #pragma unroll
       for (int n = 0; n < kAtOnce; ++n) {
+        if (done + n >= p.cells) break;
         float v[8];
         raw[n].values(v);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) middle[i] = fmaf(v[i], 1.f / kAtOnce, middle[i]);
+        for (int i = 0; i < 8; ++i) {
+          const float d = again ? fmaf(v[i], by[i], -middle[i]) : v[i] - middle[i];
+          sum[i] += d;
+          squares[i] = fmaf(d, d, squares[i]);
+        }
       }
     }
-#pragma unroll
-    for (int n = 0; n < kAtOnce; ++n) {
-      if (done + n >= p.cells) break;
-      float v[8];
-      raw[n].values(v);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float d = v[i] - middle[i];
-        sum[i] += d;
-        squares[i] = fmaf(d, d, squares[i]);
-      }
-    }
-  }
+  };
+  add_up(std::false_type());
   const float each = p.cells ? 1.f / static_cast<float>(p.cells) : 0.f;
+  float most = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const float off = sum[i] * each, left = fmaf(-sum[i], off, squares[i]);
-    shares[threadIdx.x][i] = {middle[i], off, left < 0.f ? 0.f : left};   // (NaN stays)
+    shares[threadIdx.x][i] = {middle[i], off, left <= 0.f ? 0.f : left};   // (NaN stays)
+    most = fmaxf(most, squares[i]);
+  }
+  if (kFar<T> && !held(most)) {   // channels whose squares are too large once more, values times kDown
+    unsigned far = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      by[i] = held(squares[i]) ? 1.f : kDown;
+      far |= held(squares[i]) ? 0u : 1u << i;
+      middle[i] *= by[i], sum[i] = squares[i] = 0.f;
+    }
+    add_up(std::true_type());
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (!(far >> i & 1)) continue;
+      const float off = sum[i] * each, left = fmaf(-sum[i], off, squares[i]), mean = middle[i] + off;
+      shares[threadIdx.x][i] = {mean * 0x1p100f, (middle[i] - mean + off) * 0x1p100f, left < 1e-37f ? -1e-37f : -left};
+    }
   }
   __syncthreads();
   const int cells = cells_in(s, blockIdx.x);
   const Rows count(s, cells);
-  join_rows<double2>(s, [&](int r, int o, int i, double2 &all) {
-    const int n = count.of(r);
-    const Moments share = shares[r * s.tile_threads + o][i];
-    const double mean = static_cast<double>(share.mean) + share.rest;
-    if (n) all.x += mean * n, all.y += share.squares + mean * mean * n;
+  join_rows<double2>(s, [&](int first, int step, int o, int i, double2 &all) {
+    int signs = 0;
+    auto add_up = [&](auto again) {
+      all = {0., 0.};
+      for (int r = first; r < s.tile_rows; r += step) {
+        const int n = count.of(r);
+        const Moments share = shares[r * s.tile_threads + o][i];
+        const double mean = mean_of(share), squares = squares_of<again>(share, signs);
+        if (n) all.x += mean * n, all.y += squares + mean * mean * n;
+      }
+    };
+    add_up(std::false_type());
+    if (kFar<T> && signs < 0) add_up(std::true_type());
   }, [&](int c, const double2 &all) {
-    const double mean = all.x / cells;
+    const double mean = all.x / cells, squares = all.y - all.x * mean;
     const float high = static_cast<float>(mean);
-    partial[(sample_of(s) * s.chunks + blockIdx.x) * s.channels + c] = {high, static_cast<float>(mean - high), static_cast<float>(all.y - all.x * mean)};
+    partial[(sample_of(s) * s.chunks + blockIdx.x) * s.channels + c] = {
+        high, static_cast<float>(mean - high), squares > 3.4e38 ? static_cast<float>(squares * -0x1p-200) : squares < 0. ? 0.f : static_cast<float>(squares)};
   });
 }
 
@@ -210,20 +246,26 @@ __global__ __launch_bounds__(kThreads) void group_finish(const Moments *partial,
   double total = 0., rest = 0.;
   const int across = min(s.group_channels, kThreads), rows = kThreads / across, row = threadIdx.x / across;
   const int chunks = row < rows ? s.chunks : 0;
-  for (int c = threadIdx.x % across; c < s.group_channels; c += across)
-    for (int first = row; first < chunks; first += kAtOnce * rows) {
-      Moments share[kAtOnce];
+  int signs = 0;
+  auto add_up = [&](auto again) {
+    total = rest = 0.;
+    for (int c = threadIdx.x % across; c < s.group_channels; c += across)
+      for (int first = row; first < chunks; first += kAtOnce * rows) {
+        Moments share[kAtOnce];
 #pragma unroll
-      for (int i = 0; i < kAtOnce; ++i) share[i] = from[static_cast<long>(min(first + i * rows, chunks - 1)) * s.channels + c];
+        for (int i = 0; i < kAtOnce; ++i) share[i] = from[static_cast<long>(min(first + i * rows, chunks - 1)) * s.channels + c];
 #pragma unroll
-      for (int i = 0; i < kAtOnce; ++i) {
-        const long chunk = first + i * rows;
-        const double n = chunk < chunks ? static_cast<double>(min(s.cells, (chunk + 1) * s.each) - chunk * s.each) : 0.;
-        const double mean = static_cast<double>(share[i].mean) + share[i].rest;
-        total += n * mean;
-        rest += (chunk < chunks ? share[i].squares : 0.) + n * mean * mean;
+        for (int i = 0; i < kAtOnce; ++i) {
+          const long chunk = first + i * rows;
+          const double n = chunk < chunks ? static_cast<double>(min(s.cells, (chunk + 1) * s.each) - chunk * s.each) : 0.;
+          const double mean = mean_of(share[i]), squares = squares_of<again>(share[i], signs);
+          total += n * mean;
+          rest += (chunk < chunks ? squares : 0.) + n * mean * mean;
+        }
       }
-    }
+  };
+  add_up(std::false_type());
+  if (signs < 0) add_up(std::true_type());
   block_sums(total, rest);
   if (threadIdx.x == 0) put_stats(stats, id, static_cast<long>(batch) * s.groups, total, rest, static_cast<double>(s.cells) * s.group_channels, eps);
 }
@@ -334,9 +376,11 @@ __global__ __launch_bounds__(kThreads) void group_grad_sums(const T *x, const T 
 #pragma unroll
   for (int i = 0; i < 8; ++i) shares[threadIdx.x][i] = {sum[i], dot[i]};
   __syncthreads();
-  join_rows<float2>(s, [&](int r, int o, int i, float2 &all) {
-    const float2 share = shares[r * s.tile_threads + o][i];
-    all.x += share.x, all.y += share.y;
+  join_rows<float2>(s, [&](int first, int step, int o, int i, float2 &all) {
+    for (int r = first; r < s.tile_rows; r += step) {
+      const float2 share = shares[r * s.tile_threads + o][i];
+      all.x += share.x, all.y += share.y;
+    }
   }, [&](int c, const float2 &all) { partial[(sample_of(s) * s.chunks + blockIdx.x) * s.channels + c] = all; });
 }
 

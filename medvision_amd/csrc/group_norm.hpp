@@ -4,6 +4,13 @@
 
 namespace mv {
 
+// Values whose squares 32 bits do not hold (float16 has none) are scaled by this in front of their sums.
+constexpr float kDown = 0x1p-100f;
+constexpr double kUp = 0x1p100;
+template <typename T> inline constexpr bool kFar = true;
+template <> inline constexpr bool kFar<__half> = false;
+__device__ __forceinline__ bool held(float v) { return v <= 3.402823466e38f; }   // (of a sum of squares; not NaN)
+
 // A workgroup for a group of a sample, whose values stay in its registers.
 struct Whole {
   int cells, channels, groups, group_channels, units, rows;   // units of V channels of a group, rows of cells at a time

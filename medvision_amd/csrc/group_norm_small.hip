@@ -89,28 +89,39 @@ __global__ __launch_bounds__(1024) void group_whole(const T *x, const void *weig
   few_at<T, V>(w, weight, wide, p.c, 1.f);
   few_at<T, V>(b, bias, wide, p.c, 0.f);
   const int mine = p.live ? (s.cells - p.row + s.rows - 1) / s.rows : 0;   // (0 or less: none)
-  float sum = 0.f;
-#pragma unroll
-  for (int n = 0; n < U; ++n)
-    if (n < mine) {
-#pragma unroll
-      for (int i = 0; i < V; ++i) sum += raw[n].value(i);
-    }
   const double all = static_cast<double>(s.cells) * s.group_channels;
-  const float middle = static_cast<float>(group_sum(sum) / all);   // about the mean: differences from it are small
-  float off = 0.f, squares = 0.f;
+  double mean, var;
+  auto moments = [&](auto scaled) {   // of the values, or of them times kDown
+    float sum = 0.f;
 #pragma unroll
-  for (int n = 0; n < U; ++n)
-    if (n < mine) {
+    for (int n = 0; n < U; ++n)
+      if (n < mine) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float d = raw[n].value(i) - middle;
-        off += d;
-        squares = fmaf(d, d, squares);
+        for (int i = 0; i < V; ++i) sum += scaled ? raw[n].value(i) * kDown : raw[n].value(i);
       }
+    const float middle = static_cast<float>(group_sum(sum) / all);   // about the mean: differences from it are small
+    float off = 0.f, squares = 0.f;
+#pragma unroll
+    for (int n = 0; n < U; ++n)
+      if (n < mine) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const float d = scaled ? fmaf(raw[n].value(i), kDown, -middle) : raw[n].value(i) - middle;
+          off += d;
+          squares = fmaf(d, d, squares);
+        }
+      }
+    const double total = group_sum(static_cast<double>(off)), rest = group_sum(static_cast<double>(squares));
+    const double shift = total / all, left = rest / all - shift * shift;
+    mean = middle + shift, var = left < 0. ? 0. : left;   // (NaN stays)
+  };
+  moments(std::false_type());
+  if constexpr (kFar<T>) {
+    if (!(var < 1e300)) {   // squares that 32 bits do not hold (the same for every thread)
+      moments(std::true_type());
+      mean *= kUp, var *= kUp * kUp;
     }
-  const double total = group_sum(static_cast<double>(off)), rest = group_sum(static_cast<double>(squares));
-  const double shift = total / all, mean = middle + shift, left = rest / all - shift * shift, var = left < 0. ? 0. : left;   // (NaN stays)
+  }
   const float high = static_cast<float>(mean), small = static_cast<float>(mean - high), r = static_cast<float>(1. / sqrt(var + eps));
   if (threadIdx.x == 0) stats[id] = high, stats[count + id] = small, stats[2L * count + id] = r;
 #pragma unroll
