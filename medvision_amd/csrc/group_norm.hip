@@ -565,6 +565,7 @@ extern "C" {
 
 size_t mv_group_norm_workspace_bytes(int batch, int64_t cells, int channels, int groups) {
   if (batch <= 0 || cells <= 0 || channels <= 0 || groups <= 0 || channels % groups) return 0;
+  if (whole_plan(batch, cells, channels, groups, false).u) return sizeof(Moments);   // (nothing is put there)
   return partial_bytes<Moments>(batch, cells_of(batch, cells, channels, groups));
 }
 
@@ -598,6 +599,7 @@ int mv_group_norm(const void *x, const void *weight, const void *bias, void *y, 
 
 size_t mv_group_norm_backward_workspace_bytes(int batch, int64_t cells, int channels, int groups) {
   if (batch <= 0 || cells <= 0 || channels <= 0 || groups <= 0 || channels % groups) return 0;
+  if (whole_plan(batch, cells, channels, groups, true).u) return sizeof(float2) * batch * static_cast<size_t>(channels);   // a sum of each sample's channels
   return partial_bytes<float2>(batch, cells_of(batch, cells, channels, groups)) + sizeof(float) * 2 * batch * groups;
 }
 
