@@ -2,7 +2,7 @@
 import torch
 from torch.autograd import Function
 
-_tracing = torch._C._get_tracing_state     # None outside of torch.jit.trace
+tracing = torch._C._get_tracing_state     # None outside of torch.jit.trace
 
 
 class NativeFunction(Function):
@@ -20,19 +20,19 @@ class NativeFunction(Function):
 
     @classmethod
     def apply(cls, *args, **kwargs):
-        if cls._direct and _tracing() is None:
+        if cls._direct and tracing() is None:
             return cls.native(*args, **kwargs)
         return super().apply(*args, **kwargs)
 
 
 class RecordedFunction(NativeFunction):
-    """The node of an operator without a gradient.  Outside of traces ``apply`` is ``native``; ``torch.jit.trace``, which
-    would record nothing of that call but the allocation of its result, gets a Python function that runs it."""
+    """What a trace records of an operator without a gradient, which outside of traces is a call of the native function: of
+    that ``torch.jit.trace`` would record nothing but the allocation of its result."""
     refuses = None   # the operator's name, where it refuses tensors that want a gradient (others give results without one)
 
     @classmethod
     def apply(cls, *args):
-        if _tracing() is None:
+        if tracing() is None:
             return cls.native(*args)
         if cls.refuses and torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in args):
             raise RuntimeError(f"{cls.refuses} has no gradient: call it under torch.no_grad()")

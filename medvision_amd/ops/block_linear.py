@@ -3,7 +3,7 @@ reference."""
 import torch
 
 from .._lib import native
-from ._function import RecordedFunction
+from ._function import RecordedFunction, tracing
 from ._module import KeepsTypes
 
 
@@ -29,6 +29,8 @@ def quantize_blocks(x, block_rows=1):
     ``q`` is float8_e4m3fn with the columns padded with zeros to whole blocks of 128, ``scales`` float32: one for each row
     and block of 128 columns (activations, ``block_rows=1``) or for each 128 x 128 block of a matrix (weights,
     ``block_rows=128``).  ``scale = max(max|x| / 448, 2 ** -126)``, ``q = e4m3(x * (1 / scale))``.  No gradient."""
+    if tracing() is None:
+        return native.quantize_blocks(x, block_rows)
     return QuantizeBlocksFunction.apply(x, block_rows)
 
 
@@ -36,6 +38,8 @@ def block_linear(q, q_scales, weight, weight_scales, bias=None, out_dtype=torch.
     """``(q * q_scales) @ (weight * weight_scales).T + bias`` of 8-bit activations ``[..., inputs]`` and weights
     ``[outputs, inputs]`` as ``quantize_blocks`` gives them (``block_rows`` 1 and 128); float16 or bfloat16
     ``[..., outputs]``.  No gradient."""
+    if tracing() is None:
+        return native.block_linear(q, q_scales, weight, weight_scales, bias, out_dtype)
     return BlockLinearFunction.apply(q, q_scales, weight, weight_scales, bias, out_dtype)
 
 

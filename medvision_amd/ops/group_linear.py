@@ -3,7 +3,7 @@ reference."""
 import torch
 
 from .._lib import native
-from ._function import RecordedFunction
+from ._function import RecordedFunction, tracing
 from ._module import KeepsTypes
 
 
@@ -31,12 +31,16 @@ def quantize_groups(weight, group=32):
     4, 6 (codes 0 .. 7, halves to even codes) or their negatives (8 .. 15).  ``codes [outputs, 64 * blocks]`` is uint8: two codes a
     byte, the first one in its low half; the four bytes of eight neighbouring columns together; of a block's sixteen
     such pieces number ``4 s + g`` at place ``4 g + s``.  No gradient."""
+    if tracing() is None:
+        return native.quantize_groups(weight, group)
     return QuantizeGroupsFunction.apply(weight, group)
 
 
 def group_linear(x, weight, scales, bias=None):
     """``x @ values.T + bias`` of float16 or bfloat16 rows ``[..., inputs]`` and the values of weights ``[outputs, inputs]`` as
     ``quantize_groups`` gives them, in the type of ``x``.  Values and products are exact, sums are in 32 bits.  No gradient."""
+    if tracing() is None:
+        return native.group_linear(x, weight, scales, bias)
     return GroupLinearFunction.apply(x, weight, scales, bias)
 
 

@@ -5,7 +5,7 @@ from torch import nn
 from torch.autograd.function import once_differentiable
 
 from .._lib import native
-from ._function import NativeFunction, RecordedFunction
+from ._function import NativeFunction, RecordedFunction, tracing
 
 
 class AddRMSNormFunction(NativeFunction):
@@ -51,6 +51,8 @@ def add_rms_norm(x, residual, weight, eps=1e-6):
 
 def add_rms_norm_quantized(x, residual, weight, eps=1e-6):
     """``add_rms_norm`` whose ``y`` is in 8 bits, as ``quantize_blocks`` gives them: ``(q, scales, h)``.  No gradient."""
+    if tracing() is None:
+        return native.add_rms_norm_quantized(x, residual, weight, eps)
     return AddRMSNormQuantizedFunction.apply(x, residual, weight, eps)
 
 
