@@ -243,7 +243,8 @@ template <bool Gradients, typename F> void for_plan(const WholePlan &p, const F 
 // V is the largest power of two up to 8 that divides a group's channels.  A workgroup reads as many cache lines as there are cells, by itself:
 // 8 x 5000 cells of 20 channels in groups of 4 8.9 us (12.3 in the three kernels of large samples), 8000 of 32 in groups of 8 16.4
 // (13.4).  Gradients read two tensors, and keep the chip's other workgroups waiting where there are many: 4 x 2000 of 64 in groups of 4
-// 11 us (16), 1 x 4000 of 256 in groups of 8 18 (15), 64 x 343 of 256 29 (26).  (Batches of 65536 and more are taken for the sake of this form: they have it for gradients too where it holds them.)
+// 11 us (16), 1 x 4000 of 256 in groups of 8 18 (15), 64 x 343 of 256 29 (26).  (Batches of 65536 and more, which are
+// taken for the sake of this form, have it for gradients wherever it holds them.)
 WholePlan whole_plan(int batch, long cells, int channels, int groups, bool gradients) {
   WholePlan p{};
   if (cells > (gradients ? 3000 : 5000) || (gradients && batch * cells * channels > (4L << 20) && batch < 65536)) return p;

@@ -44,7 +44,9 @@ def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, activation=None,
         slope (float): of ``'leaky_relu'`` below zero
 
     Gradients flow to ``x``, ``weight`` and ``bias``; at zero the activations with two branches have the lower one's.  Statistics
-    and sums are in 32 bits or more, each result is rounded once."""
+    and sums are in 32 bits or more, each result is rounded once.  Batches of 65536 and more are taken where a group of a sample
+    fits into a workgroup's registers (up to 5000 cells, and about 16384 values of an odd number of channels to 65536 of a
+    multiple of four)."""
     return GroupNormActFunction.apply(x, groups, weight, bias, eps, activation, slope)
 
 

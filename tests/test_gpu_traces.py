@@ -54,6 +54,7 @@ def test_layers_for_inference(bits, axes):
         compare(lambda r, h, t, p, c: layer(r, t, h, region_positions=p, token_positions=c), regions, residual, tokens, rand(5, 2, 33, 3), rand(6, 50, 3))
     else:
         compare(lambda r, h, t: layer(r, t, h), regions, residual, tokens)
+        compare(lambda r, t: layer(r, t), regions, tokens)   # (the first layer: no residual)
 
 
 def test_resampling():
