@@ -289,7 +289,8 @@ struct Line {
   float a, high, low;
   __device__ __forceinline__ void set(float mean, float rest, float by, double shift) {
     a = by;
-    const double c = shift - (static_cast<double>(mean) + rest) * by;
+    double c = shift - (static_cast<double>(mean) + rest) * by;
+    if (fabs(c) > 3.4e38) a = 0.f, c = shift;   // (values that far from zero beside their deviation are all the same: masked ones; NaN stays)
     high = static_cast<float>(c), low = static_cast<float>(c - high);
   }
   __device__ __forceinline__ float at(float x) const { return fmaf(x, a, high) + low; }

@@ -68,3 +68,15 @@ def test_small_channels_beside_large_ones(cells):
     plain[..., [1, 3, 5]] = rand(9, 1, cells, 3)
     want = ops.group_norm_act(plain.to(DEV), 8).cpu()
     assert torch.equal(y[..., [0, 2, 4, 6, 7]], want[..., [0, 2, 4, 6, 7]])
+
+
+@pytest.mark.parametrize("cells", [50, 8000])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_groups_that_are_masked_throughout(cells, dtype):
+    """Every cell of a group at the type's lowest or highest value: no variance, so that its cells are the bias."""
+    import medvision_amd.ops as ops
+    x = rand(1, 2, cells, 24).to(dtype)
+    x[0, :, :8], x[1, :, 8:16] = torch.finfo(dtype).min, torch.finfo(dtype).max
+    compare(x, 3, None)
+    y = ops.group_norm_act(x.to(DEV), 3, None, torch.ones(24, device=DEV))
+    assert (y[0, :, :8] == 1).all() and (y[1, :, 8:16] == 1).all()
